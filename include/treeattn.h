@@ -78,6 +78,98 @@ typedef struct ta_leaf_store_out {
 } ta_leaf_store_out;
 
 /*
+ * A decode cache in 8 bits (engine.py:26-27 keeps it in the model's type; no counterpart in the reference).
+ * pool (num_pages, 2, leaf, D) e4m3 bytes: page p holds the K rows and then the V rows of one leaf block of one
+ * (sequence, head); its values are the e4m3 numbers times scale[2p] (keys) and scale[2p + 1] (values), powers of two.
+ * table[b*sb + h*sh + j] is the page of leaf block j (outside [0, num_pages): no page).  The block being filled stands
+ * unrounded, in the model's type, in tail: K rows at tail + b*tail_sb + h*tail_sh, V rows leaf * D elements after them;
+ * tail_block[b*tb_sb + h] is its index (-1: the tail holds nothing).  A block is rounded into its page when its last
+ * row arrives, with the smallest power-of-two scale that brings its largest finite magnitude to 448 or less (1 for
+ * all zeros); what is not finite is stored as NaN.  The block the tail holds is read from the tail.
+ * D 16, 32, 64 or 128; the dtype of a call is that of q, the new rows and the tail.
+ */
+typedef struct ta_kv8 {
+  void* pool;              /* 16-byte aligned */
+  float* scale;            /* (num_pages, 2), 8-byte aligned */
+  const int32_t* table;
+  int64_t sb, sh;          /* element strides of the table for sequence and head */
+  int64_t num_pages;
+  void* tail;              /* 16-byte aligned, as are its strides in bytes */
+  int64_t tail_sb, tail_sh;
+  int32_t* tail_block;
+  int64_t tb_sb;           /* element stride of tail_block for the sequence (1 for the head) */
+  int block_log2;          /* rows per page = 2^block_log2 = the leaf block of the tree (2 to 16384) */
+  int tcap;                /* positions a sequence may have; the table covers them */
+} ta_kv8;
+
+/*
+ * Append of one position of every (sequence, head) to an 8-bit cache (engine.py:41-55, SegState.add): k_new, v_new
+ * (B, H, D) with strides nsb, nsh / vnsb, vnsh become row t_pos[b] of the tail; when they end a leaf block the block
+ * is rounded into its page, and the nodes ending there are formed from the unrounded keys as ta_kv_append forms them
+ * (tree level j of n_levels, leaf * arity^j positions per node).  A position outside [0, tcap) or in a block without a
+ * page is not stored.  Going back to a position inside an earlier block restores that block's rows before it from its
+ * page.
+ */
+int ta_kv8_append(const void* k_new, const void* v_new, int dtype, int64_t nsb, int64_t nsh, int64_t vnsb,
+                  int64_t vnsh, const ta_kv8* cache, int B, int H, int D, const int32_t* t_pos, int n_levels,
+                  float* const* lv_ptr, const int64_t* lv_sb, const int64_t* lv_sh, int arity_log2, void* stream);
+
+/*
+ * Positions 0 .. lengths[b]-1 of k, v (B, H, T, D; 16-byte aligned rows) into an 8-bit cache (engine.py:57-71,
+ * SegState.fill): whole leaf blocks into their pages, the rows of the last partial block into the tail (tail_block -1
+ * when there is none).  lengths (B,) int32, clamped to [0, T]; NULL: T for every sequence.  Rows, pages and tails past a
+ * sequence's length are not touched; node sums are ta_level_sums's.
+ */
+int ta_kv8_fill(const void* k, const void* v, int dtype, int64_t ksb, int64_t ksh, int64_t kst, int64_t vsb,
+                int64_t vsh, int64_t vst, const ta_kv8* cache, int B, int H, int T, int D, const int32_t* lengths,
+                void* stream);
+
+/*
+ * ta_seg_attn_fwd / ta_seg_attn_nb_fwd over an 8-bit cache: attention of q (B, H, Nq, D) at positions tq over the first
+ * min(valid ids, n_tree) selected leaf blocks (distinct, before the own block), the matched neighbour leaves (nb_S
+ * slots; 0: none), the own block up to the position and the static keys.  At most 512 leaves; ids outside the table and
+ * blocks without a page contribute nothing; a query at a position outside [0, tcap), or with no key, gives zeros and
+ * lse -1e30.  nsplit and ws as for ta_seg_attn_fwd (ta_seg_attn_workspace_size; zero-filled once, calls that share it
+ * must not overlap in time).  lse (B, H, Nq) and keys (B, H, Nq; the number of keys) may be NULL.
+ */
+int ta_seg_attn8_fwd(const void* q, int dtype, int64_t qsb, int64_t qsh, int64_t qsn, const ta_kv8* cache, int B, int H,
+                     int Nq, int D, const int32_t* tq, int64_t tq_sb, const int32_t* ids, const uint8_t* vld,
+                     const int32_t* n_tree, int wl, int local, float scale, const int32_t* nb_id, const uint8_t* nb_ok,
+                     int nb_S, void* out, int64_t osb, int64_t osh, int64_t osn, float* lse, float* keys, int nsplit,
+                     float* ws, int64_t ws_bytes, void* stream);
+
+/*
+ * Rows of microscaled 4-bit floats (the OCP MX format, e2m1 values): blocks of 32 along a row share a scale
+ * 2^(byte - 127); packed (rows, Kp / 2) bytes hold two values each, the lower index in the low half, and scale
+ * (rows, Kp / 32) one byte per block, with Kp = K rounded up to a multiple of 128 (values past K are 0, and the scale
+ * byte of a block that lies wholly past K is 0).
+ *
+ * ta_mx4_quant rounds x (rows, K; row stride ldx) to that form: byte - 127 = floor(log2 of the block's largest
+ * magnitude) - 2, at least -127; values to nearest, ties to even, saturating at 6; byte 255 (NaN) for a block that
+ * holds anything not finite.  values (row stride ldv, x's dtype; may be NULL) receives what the rounded form stands
+ * for.
+ */
+int ta_mx4_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int K, void* packed, uint8_t* scale, void* values,
+                 int64_t ldv, void* stream);
+
+/*
+ * Y[M, N] = epilogue(LN(X) . W^T), bf16, for weights W (N, K) in 4 bits (packed and scale as above, contiguous, packed
+ * 16-byte and scale 4-byte aligned): the weights are exact in bf16, products are summed in float32, and the result is
+ * rounded once, after the epilogue (0 none, 1 GELU in the erf form, 2 R + product).  ln_w (K bf16; M at most 64): the
+ * rows of X are normalised first (as ta_rowmm does, rounded to bf16).  K a multiple of 32, X 16-byte aligned with rows
+ * of a multiple of 8 elements.  Y may be R, not X.
+ */
+int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,
+                int64_t ldr, const void* ln_w, float ln_eps, int M, int N, int K, int epilogue, void* stream);
+
+/*
+ * The same product of two matrices in 4 bits, X (M, K) and W (N, K), on the scaled matrix instructions; any K of at
+ * least 1.
+ */
+int ta_mx4_both(const void* Xp, const uint8_t* Xs, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,
+                int64_t ldr, int M, int N, int K, int epilogue, void* stream);
+
+/*
  * Level-sum pyramid of a key tensor (replaces seg.py:26-41 level_sums, fastseg.py:238-251 level_sums_min
  * without the gate, and the index-key preparation seg.py:128-130 / fastseg.py:306-308).
  *

@@ -28,6 +28,13 @@ class KvPages(ctypes.Structure):
                 ('block_log2', c_i32)]
 
 
+class Kv8(ctypes.Structure):
+    """ta_kv8"""
+    _fields_ = [('pool', c_vp), ('scale', c_vp), ('table', c_vp), ('sb', c_i64), ('sh', c_i64), ('num_pages', c_i64),
+                ('tail', c_vp), ('tail_sb', c_i64), ('tail_sh', c_i64), ('tail_block', c_vp), ('tb_sb', c_i64),
+                ('block_log2', c_i32), ('tcap', c_i32)]
+
+
 class LeafStoreOut(ctypes.Structure):
     """ta_leaf_store_out (include/treeattn.h)."""
     _fields_ = [('leaf', c_vp), ('score', c_vp), ('ok', c_vp), ('sb', c_i64), ('sh', c_i64), ('st', c_i64),
@@ -120,6 +127,16 @@ SIGNATURES = {
     'ta_kv_append': (c_i32, [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
                              c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, _P(c_vp), _P(c_i64), _P(c_i64), c_i32,
                              c_i32, _P(KvPages), c_vp]),
+    'ta_kv8_append': (c_i32, [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, _P(Kv8), c_i32, c_i32, c_i32, c_vp, c_i32,
+                              _P(c_vp), _P(c_i64), _P(c_i64), c_i32, c_vp]),
+    'ta_kv8_fill': (c_i32, [c_vp, c_vp, c_i32] + [c_i64] * 6 + [_P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]),
+    'ta_seg_attn8_fwd': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, _P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp,
+                                 c_vp, c_vp, c_i32, c_i32, c_f32, c_vp, c_vp, c_i32, c_vp, c_i64, c_i64, c_i64, c_vp,
+                                 c_vp, c_i32, c_vp, c_i64, c_vp]),
+    'ta_mx4_quant': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    'ta_mx4_rows': (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_f32, c_i32, c_i32, c_i32, c_i32,
+                            c_vp]),
+    'ta_mx4_both': (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp]),
     'ta_argmax_rows': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp]),
     'ta_embed': (c_i32, [c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i64, c_i64, c_vp,
                          c_i64, c_vp, c_vp, c_f32, c_vp, c_i64, c_vp]),
@@ -226,6 +243,16 @@ def require_gpu(*tensors):
                 if lib().ta_device_supported() != 1:
                     raise RuntimeError('treeattn_amd: device %d is not a gfx950 (MI355X)' % dev)
             _checked_devices.add(dev)
+
+
+def call_on(dev, name, *args):
+    """call(name, *args, stream) with dev as the current device and its current stream, whatever device is current
+    outside."""
+    if dev.index == torch.cuda.current_device():
+        check(getattr(lib(), name)(*args, stream()), name)
+    else:
+        with torch.cuda.device(dev):
+            check(getattr(lib(), name)(*args, stream()), name)
 
 
 def stream():

@@ -37,6 +37,11 @@ SOURCES = {
     'gate.hip': [],
     'forest.hip': [],
     'lanetree.hip': [],
+    'kv8.hip': [],
+    'attend8.hip': [],
+    'mx4.hip': [],
+    'mx4_rows.hip': [],
+    'mx4_gemm.hip': [],
 }
 
 COMMON = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function',

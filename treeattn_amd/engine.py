@@ -317,6 +317,11 @@ def decode_nsplit(B, H, wl, leaf):
     return 4 * g
 
 
+def decode_nsplit8(B, H, Nq, wl, leaf):
+    """decode_nsplit for a cache of 8-bit pages (kernels.seg_attn8) and Nq queries per (sequence, head)."""
+    return decode_nsplit(B, H * Nq, wl, leaf)
+
+
 def _budget_weights(state, pw):
     """The budget head's weights as ta_budget_head takes them (float32, W1 transposed, classes int32), prepared
     once per layer state and kept while the same weight dict is passed."""

@@ -927,6 +927,250 @@ def bf16_round(x):
     return out
 
 
+# ----------------------------------------------------------------------------------------------- 8-bit cache
+def _same_device(name, dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError('%s: every tensor must be on %s (got one on %s)' % (name, dev, t.device))
+
+
+class Cache8:
+    """One layer's decode cache in 8 bits.  pool (P, 2, leaf, D) float8_e4m3fn: page p holds the K rows (pool[p, 0]) and
+    the V rows (pool[p, 1]) of one leaf block of one (sequence, head), their values being the numbers times
+    scale[p, 0] and scale[p, 1] ((P, 2) float32, powers of two); table (B, H, n_blocks) int32 maps leaf block j of
+    (b, h) to its page (-1: none) and may be shared by several layers.  The block being filled stands unrounded in
+    tail (B, H, 2, leaf, D), in the model's type, and tail_block (B, H) int32 says which it is (-1: none); it is
+    rounded into its page when its last row arrives.  tcap: positions per sequence.  The tensors are the caller's;
+    a new cache is pool of zeros, scale of ones, tail_block of -1."""
+
+    def __init__(self, pool, scale, table, tail, tail_block, tcap):
+        P, two, leaf, D = pool.shape
+        B, H, nblk = table.shape
+        if two != 2 or not pool.is_contiguous() or pool.dtype != torch.float8_e4m3fn:
+            raise ValueError('Cache8: pool (P, 2, leaf, D) float8_e4m3fn, contiguous')
+        if scale.dtype != torch.float32 or scale.shape != (P, 2) or not scale.is_contiguous():
+            raise ValueError('Cache8: scale (P, 2) float32, contiguous')
+        if table.dtype != torch.int32 or table.stride(2) != 1 or nblk * leaf < tcap or tcap < 1:
+            raise ValueError('Cache8: table (B, H, n_blocks) int32 that covers tcap positions')
+        if tail.shape != (B, H, 2, leaf, D) or not tail[0, 0].is_contiguous() or tail.dtype not in L._DT:
+            raise ValueError('Cache8: tail (B, H, 2, leaf, D) in the model dtype, each (sequence, head) contiguous')
+        if tail_block.dtype != torch.int32 or tail_block.shape != (B, H) or (H > 1 and tail_block.stride(1) != 1):
+            raise ValueError('Cache8: tail_block (B, H) int32')
+        _same_device('Cache8', pool.device, scale, table, tail, tail_block)
+        self.pool, self.scale, self.table, self.tail, self.tail_block = pool, scale, table, tail, tail_block
+        self.B, self.H, self.leaf, self.D, self.tcap = B, H, leaf, D, int(tcap)
+        self.dtype, self.device = tail.dtype, pool.device
+        self.desc = L.Kv8(pool.data_ptr(), scale.data_ptr(), table.data_ptr(), table.stride(0), table.stride(1), P,
+                          tail.data_ptr(), tail.stride(0), tail.stride(1), tail_block.data_ptr(), tail_block.stride(0),
+                          _ilog2(leaf), self.tcap)
+        self.ref = ctypes.byref(self.desc)
+
+    def rows(self, b0, b1):
+        """The same cache seen from sequences b0..b1-1."""
+        return Cache8(self.pool, self.scale, self.table[b0:b1], self.tail[b0:b1], self.tail_block[b0:b1], self.tcap)
+
+    def dense(self, b, t_end=None):
+        """Contiguous (1, H, t_end, D) copies of K and V of sequence b in the model's type (rows without a page are
+        zero)."""
+        t_end = self.tcap if t_end is None else int(t_end)
+        nb = (t_end + self.leaf - 1) // self.leaf
+        pg = self.table[b, :, :nb].long()
+        ok = ((pg >= 0) & (pg < self.pool.shape[0])).view(self.H, nb, 1, 1, 1)
+        pg = torch.where(ok.view(self.H, nb), pg, 0)
+        kv = self.pool.view(torch.uint8)[pg].view(torch.float8_e4m3fn).float() * self.scale[pg].view(self.H, nb, 2, 1, 1)
+        kv = torch.where(ok, kv, 0.0).to(self.dtype)
+        mine = torch.arange(nb, device=self.device) == self.tail_block[b].view(self.H, 1)
+        kv = torch.where(mine.view(self.H, nb, 1, 1, 1), self.tail[b].unsqueeze(1), kv)
+        kv = kv.transpose(1, 2).reshape(self.H, 2, nb * self.leaf, self.D)[:, :, :t_end]
+        return kv[:, 0].unsqueeze(0).contiguous(), kv[:, 1].unsqueeze(0).contiguous()
+
+
+def _cache8_rows(name, cache, *rows):
+    """Checks new rows (B, H, ..., D) against the cache."""
+    L.require_gpu(cache.pool, *rows)
+    _same_device(name, cache.device, *rows)
+    for t in rows:
+        if t.shape[:2] != (cache.B, cache.H) or t.shape[-1] != cache.D or t.shape != rows[0].shape:
+            raise ValueError('%s: rows of %d sequences, %d heads and head size %d, got %s'
+                             % (name, cache.B, cache.H, cache.D, tuple(t.shape)))
+        if t.dtype != cache.dtype:
+            raise TypeError('%s: rows must have the cache dtype %s' % (name, cache.dtype))
+        if t.stride(-1) != 1:
+            raise ValueError('%s: the last dimension must be contiguous' % name)
+
+
+def kv8_append(k_new, v_new, cache, t_pos, levels, arity):
+    """Append one position of every (sequence, head) to a Cache8: k_new, v_new (B,H,D) at t_pos (B,) int32, forming the
+    tree nodes that end there in `levels` (tree levels 0.. of (B,H,nodes,D) float32, arity children per node) from the
+    unrounded keys.  The block a token ends is rounded into its page.  A position outside [0, tcap), or in a block
+    without a page, is not stored.  Going back to an earlier block restores its rows from its page."""
+    _cache8_rows('kv8_append', cache, k_new, v_new)
+    if k_new.dim() != 3:
+        raise ValueError('kv8_append: one row (B, H, D) per (sequence, head)')
+    if t_pos.dtype != torch.int32 or t_pos.shape != (cache.B,) or not t_pos.is_contiguous():
+        raise ValueError('kv8_append: contiguous int32 positions (B,)')
+    _same_device('kv8_append', cache.device, t_pos, *levels)
+    s, l = _ilog2(arity), cache.desc.block_log2
+    for t in levels:
+        if (t.dtype != torch.float32 or t.shape[:2] != (cache.B, cache.H) or t.shape[3] != cache.D
+                or t.shape[2] < cache.tcap >> l or t.stride(3) != 1 or t.stride(2) != cache.D):
+            raise ValueError('kv8_append: levels (B, H, nodes, D) float32 with contiguous node rows for every whole '
+                             'node of tcap positions')
+        l += s
+    L.call_on(cache.device, 'ta_kv8_append', L.ptr(k_new), L.ptr(v_new), L._DT[cache.dtype], k_new.stride(0),
+              k_new.stride(1), v_new.stride(0), v_new.stride(1), cache.ref, cache.B, cache.H, cache.D, L.ptr(t_pos),
+              len(levels), L.ptr_array(levels), L.i64_array([t.stride(0) for t in levels]),
+              L.i64_array([t.stride(1) for t in levels]), s)
+
+
+def kv8_fill(k, v, cache, lengths=None):
+    """Positions 0 .. lengths[b]-1 of k, v (B,H,T,D; lengths (B,) int32, all T by default) into a Cache8: whole leaf blocks
+    rounded into their pages, the rest of a sequence into its tail.  What lies past a sequence's length stays as it is."""
+    _cache8_rows('kv8_fill', cache, k, v)
+    if k.dim() != 4 or k.shape[2] > cache.tcap:
+        raise ValueError('kv8_fill: rows (B, H, T, D) of at most tcap positions')
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.shape != (cache.B,) or not lengths.is_contiguous():
+            raise ValueError('kv8_fill: contiguous int32 lengths (B,)')
+        _same_device('kv8_fill', cache.device, lengths)
+    L.call_on(cache.device, 'ta_kv8_fill', L.ptr(k), L.ptr(v), L._DT[cache.dtype], *L.rows3(k), *L.rows3(v), cache.ref,
+              cache.B, cache.H, k.shape[2], cache.D, L.ptr(lengths))
+
+
+def seg_attn8_workspace(B, H, Nq, D, nsplit, device):
+    """Zero-filled workspace for seg_attn8 with `nsplit` (None when none is needed); as seg_attn_workspace."""
+    return seg_attn_workspace(B, H, Nq, D, nsplit, device)
+
+
+def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, keys=None, nsplit=1, ws=None, nb=None):
+    """seg_attn over a Cache8: attention of q (B,H,Nq,D; the cache's dtype) at positions tq ((Nq,) or (B,Nq)) over the
+    first min(valid, n_tree) selected leaf blocks ids / vld (B,H,Nq,wl; distinct blocks before the own one, at most
+    512), the own block and the static keys; nb = (nid, match) as for seg_attn.  Keys of the block in the tail are read
+    unrounded.  Returns (out, lse, keys)."""
+    B, H, Nq, D = q.shape
+    _cache8_rows('seg_attn8', cache, q)
+    wl = ids.shape[-1]
+    tq32 = (tq if tq.dtype == torch.int32 else tq.to(torch.int32)).contiguous()
+    if tq32.shape not in ((Nq,), (B, Nq)):
+        raise ValueError('seg_attn8: positions (Nq,) or (B, Nq)')
+    if (ids.dtype != torch.int32 or vld.dtype not in (torch.uint8, torch.bool) or ids.shape != (B, H, Nq, wl)
+            or vld.shape != ids.shape or not ids.is_contiguous() or not vld.is_contiguous()):
+        raise ValueError('seg_attn8: contiguous ids int32 and vld uint8 or bool, (B, H, Nq, wl)')
+    nt = None
+    if n_tree is not None:
+        if n_tree.shape != (B, H, Nq):
+            raise ValueError('seg_attn8: n_tree (B, H, Nq)')
+        nt = n_tree if (n_tree.dtype == torch.int32 and n_tree.is_contiguous()) else n_tree.to(torch.int32).contiguous()
+    if out is None:
+        out = torch.empty(B, H, Nq, D, device=q.device, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+        raise ValueError('seg_attn8: out must have the shape and dtype of q, the last dimension contiguous')
+    for t in (lse, keys):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (B, H, Nq) or not t.is_contiguous()):
+            raise ValueError('seg_attn8: lse and keys (B, H, Nq) float32, contiguous')
+    nid = nmatch = None
+    nS = 0
+    if nb is not None:
+        nid, nmatch = nb
+        nS = nid.shape[-1]
+        if (nid.dtype != torch.int32 or nmatch.dtype != torch.bool or not nid.is_contiguous() or
+                not nmatch.is_contiguous() or nid.shape[:3] != (B, H, Nq) or nmatch.shape != nid.shape):
+            raise ValueError('seg_attn8: nb must be contiguous (nid int32, match bool) of shape (B, H, Nq, S)')
+    if ws is None and nsplit > 1:
+        ws = seg_attn8_workspace(B, H, Nq, D, nsplit, q.device)
+    _same_device('seg_attn8', cache.device, tq32, ids, vld, nt, out, lse, keys, nid, nmatch, ws)
+    L.call_on(cache.device, 'ta_seg_attn8_fwd', L.ptr(q), L._DT[cache.dtype], *L.rows3(q), cache.ref, B, H, Nq, D,
+              L.ptr(tq32), 0 if tq32.dim() == 1 else tq32.stride(0), L.ptr(ids), L.ptr(vld), L.ptr(nt), wl, int(local),
+              float(scale), L.ptr(nid), L.ptr(nmatch), nS, L.ptr(out), out.stride(0), out.stride(1), out.stride(2),
+              L.ptr(lse), L.ptr(keys), int(nsplit), L.ptr(ws),
+              ws.numel() * ws.element_size() if ws is not None else 0)
+    return out, lse, keys
+
+
+# ----------------------------------------------------------------------------------------------- 4-bit rows
+class Mx4:
+    """Rows of microscaled 4-bit floats (the OCP MX format with e2m1 values): blocks of 32 along a row share a scale
+    2^(byte - 127), byte 255 meaning NaN.  packed (rows, Kp / 2) uint8, the value of the lower index in the low half;
+    scale (rows, Kp / 32) uint8; Kp is K rounded up to a multiple of 128, the values past K being 0."""
+
+    def __init__(self, packed, scale, K):
+        Kp = (int(K) + 127) // 128 * 128
+        if (K < 1 or packed.dtype != torch.uint8 or scale.dtype != torch.uint8 or packed.dim() != 2
+                or packed.shape[1] != Kp // 2 or scale.shape != (packed.shape[0], Kp // 32)
+                or not packed.is_contiguous() or not scale.is_contiguous()):
+            raise ValueError('Mx4: contiguous uint8 packed (rows, Kp / 2) and scale (rows, Kp / 32), Kp = K rounded up to '
+                             'a multiple of 128')
+        _same_device('Mx4', packed.device, scale)
+        self.packed, self.scale, self.K = packed, scale, int(K)
+        self.shape, self.device = (packed.shape[0], int(K)), packed.device
+
+    def values(self, dtype=torch.float32):
+        """What the rows stand for, (rows, K)."""
+        grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], device=self.device)
+        code = torch.stack((self.packed & 15, self.packed >> 4), -1).flatten(-2)
+        v = grid[(code & 7).long()]
+        v = torch.where(code >= 8, -v, v).view(self.shape[0], -1, 32)
+        e = self.scale.long() - 127
+        s = torch.where(self.scale == 255, float('nan'), ((e + 1023) << 52).view(torch.float64))
+        return (v * s.unsqueeze(-1)).flatten(-2)[:, :self.K].to(dtype)
+
+
+def mx4_quant(x, values=False):
+    """x (rows, K) float32 / float16 / bfloat16 rounded to Mx4: per block of 32 the scale 2^(floor(log2 of the largest
+    magnitude) - 2), values to the nearest (ties to even) and at most 6; a block with anything not finite becomes NaN.
+    With values: (Mx4, the values it stands for in x's dtype)."""
+    L.require_gpu(x)
+    if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError('mx4_quant: rows (M, K) with contiguous rows, K at least 1')
+    M, K = x.shape
+    Kp = (K + 127) // 128 * 128
+    packed = torch.empty(M, Kp // 2, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(M, Kp // 32, dtype=torch.uint8, device=x.device)
+    v = torch.empty(M, K, dtype=x.dtype, device=x.device) if values else None
+    L.call_on(x.device, 'ta_mx4_quant', L.ptr(x), L.dtype_code(x), x.stride(0), M, K, L.ptr(packed), L.ptr(scale), L.ptr(v),
+              K)
+    return (Mx4(packed, scale, K), v) if values else Mx4(packed, scale, K)
+
+
+def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
+    """epilogue(LN(x) @ w.T) in bf16 for weights w (Mx4, (N,K)): x (M,K) bf16, K a multiple of 32 -- the weights are exact in
+    bf16 -- or x an Mx4 (M,K), whose product runs on the 4-bit matrix instructions.  ln_w (K,) bf16: a LayerNorm of x's
+    rows first (bf16 x, M at most 64).  epilogue None | 'gelu' | 'residual' (adds `residual`, (M,N) bf16); sums are
+    float32, rounded once at the end.  `out` may be `residual` (not x)."""
+    if not isinstance(w, Mx4):
+        raise TypeError('mx4_mm: w must be an Mx4')
+    both = isinstance(x, Mx4)
+    (M, K), N = x.shape, w.shape[0]
+    if w.K != K:
+        raise ValueError('mx4_mm: x has rows of %d values, w of %d' % (K, w.K))
+    if epilogue not in _EPI:
+        raise ValueError('mx4_mm: epilogue None, gelu or residual')
+    if out is None:
+        out = torch.empty(M, N, device=w.device, dtype=torch.bfloat16)
+    r = residual if epilogue == 'residual' else None
+    if epilogue == 'residual' and r is None:
+        raise ValueError('mx4_mm: the residual epilogue needs residual')
+    for t in (out, r):
+        if t is not None and (t.shape != (M, N) or t.dtype != torch.bfloat16 or (N > 1 and t.stride(1) != 1)):
+            raise ValueError('mx4_mm: out and residual (M, N) bf16 with contiguous rows')
+    L.require_gpu(w.packed, out)
+    _same_device('mx4_mm', w.device, x.packed if both else x, out, r, ln_w)
+    tail = (L.ptr(out), out.stride(0), L.ptr(r), r.stride(0) if r is not None else 0)
+    if both:
+        if ln_w is not None:
+            raise ValueError('mx4_mm: the LayerNorm prologue takes bf16 rows')
+        L.call_on(w.device, 'ta_mx4_both', L.ptr(x.packed), L.ptr(x.scale), L.ptr(w.packed), L.ptr(w.scale), *tail, M, N, K,
+                  _EPI[epilogue])
+        return out
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError('mx4_mm: x (M, K) bf16 with contiguous rows, or an Mx4')
+    if ln_w is not None and (ln_w.dtype != torch.bfloat16 or ln_w.shape != (K,) or not ln_w.is_contiguous()):
+        raise ValueError('mx4_mm: ln_w (K,) bf16, contiguous')
+    L.call_on(w.device, 'ta_mx4_rows', L.ptr(x), x.stride(0), L.ptr(w.packed), L.ptr(w.scale), *tail, L.ptr(ln_w),
+              float(eps), M, N, K, _EPI[epilogue])
+    return out
+
+
 # ----------------------------------------------------------------------------------------------- sampling
 def argmax_rows(x, out=None):
     """First index of the maximum of every row of x (R, n) -> (R,) int64."""
