@@ -128,7 +128,7 @@ SIGNATURES = {
                              c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, _P(c_vp), _P(c_i64), _P(c_i64), c_i32,
                              c_i32, _P(KvPages), c_vp]),
     'ta_kv8_append': (c_i32, [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, _P(Kv8), c_i32, c_i32, c_i32, c_vp, c_i32,
-                              _P(c_vp), _P(c_i64), _P(c_i64), c_i32, c_vp]),
+                              c_vp, c_vp, c_vp, c_i32, c_vp]),
     'ta_kv8_fill': (c_i32, [c_vp, c_vp, c_i32] + [c_i64] * 6 + [_P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]),
     'ta_seg_attn8_fwd': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, _P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp,
                                  c_vp, c_vp, c_i32, c_i32, c_f32, c_vp, c_vp, c_i32, c_vp, c_i64, c_i64, c_i64, c_vp,
@@ -245,14 +245,32 @@ def require_gpu(*tensors):
             _checked_devices.add(dev)
 
 
-def call_on(dev, name, *args):
-    """call(name, *args, stream) with dev as the current device and its current stream, whatever device is current
-    outside."""
-    if dev.index == torch.cuda.current_device():
-        check(getattr(lib(), name)(*args, stream()), name)
-    else:
-        with torch.cuda.device(dev):
-            check(getattr(lib(), name)(*args, stream()), name)
+def device_index(t):
+    """The index of t's device, checked on first use to be a supported GPU (require_gpu)."""
+    dev = t.get_device()
+    if dev not in _checked_devices:
+        require_gpu(t)
+    return dev
+
+
+def entry(name):
+    """The library's function `name` as fn(dev, *args): called with torch's current stream of device dev appended and dev
+    as the current device, whatever is current outside; a non-zero status raises.  (Resolved on first use: the library
+    is loaded lazily.)"""
+    fn = None
+
+    def run(dev, *args):
+        nonlocal fn
+        if fn is None:
+            fn = getattr(lib(), name)
+        if dev == torch._C._cuda_getDevice():
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if rc:
+            check(rc, name)
+    return run
 
 
 def stream():

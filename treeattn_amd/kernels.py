@@ -5,6 +5,7 @@ allocates) unless the caller passes them in.  Work goes on torch's current strea
 """
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -928,12 +929,6 @@ def bf16_round(x):
 
 
 # ----------------------------------------------------------------------------------------------- 8-bit cache
-def _same_device(name, dev, *tensors):
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError('%s: every tensor must be on %s (got one on %s)' % (name, dev, t.device))
-
-
 class Cache8:
     """One layer's decode cache in 8 bits.  pool (P, 2, leaf, D) float8_e4m3fn: page p holds the K rows (pool[p, 0]) and
     the V rows (pool[p, 1]) of one leaf block of one (sequence, head), their values being the numbers times
@@ -956,13 +951,14 @@ class Cache8:
             raise ValueError('Cache8: tail (B, H, 2, leaf, D) in the model dtype, each (sequence, head) contiguous')
         if tail_block.dtype != torch.int32 or tail_block.shape != (B, H) or (H > 1 and tail_block.stride(1) != 1):
             raise ValueError('Cache8: tail_block (B, H) int32')
-        _same_device('Cache8', pool.device, scale, table, tail, tail_block)
+        self.index = L.device_index(pool)
+        _on('Cache8', self.index, scale, table, tail, tail_block)
         self.pool, self.scale, self.table, self.tail, self.tail_block = pool, scale, table, tail, tail_block
         self.B, self.H, self.leaf, self.D, self.tcap = B, H, leaf, D, int(tcap)
-        self.dtype, self.device = tail.dtype, pool.device
+        self.dtype, self.device, self.code, self.block_log2 = tail.dtype, pool.device, L._DT[tail.dtype], _ilog2(leaf)
         self.desc = L.Kv8(pool.data_ptr(), scale.data_ptr(), table.data_ptr(), table.stride(0), table.stride(1), P,
                           tail.data_ptr(), tail.stride(0), tail.stride(1), tail_block.data_ptr(), tail_block.stride(0),
-                          _ilog2(leaf), self.tcap)
+                          self.block_log2, self.tcap)
         self.ref = ctypes.byref(self.desc)
 
     def rows(self, b0, b1):
@@ -985,18 +981,32 @@ class Cache8:
         return kv[:, 0].unsqueeze(0).contiguous(), kv[:, 1].unsqueeze(0).contiguous()
 
 
-def _cache8_rows(name, cache, *rows):
-    """Checks new rows (B, H, ..., D) against the cache."""
-    L.require_gpu(cache.pool, *rows)
-    _same_device(name, cache.device, *rows)
-    for t in rows:
-        if t.shape[:2] != (cache.B, cache.H) or t.shape[-1] != cache.D or t.shape != rows[0].shape:
-            raise ValueError('%s: rows of %d sequences, %d heads and head size %d, got %s'
-                             % (name, cache.B, cache.H, cache.D, tuple(t.shape)))
-        if t.dtype != cache.dtype:
-            raise TypeError('%s: rows must have the cache dtype %s' % (name, cache.dtype))
-        if t.stride(-1) != 1:
-            raise ValueError('%s: the last dimension must be contiguous' % name)
+_kv8_append = L.entry('ta_kv8_append')
+_kv8_fill = L.entry('ta_kv8_fill')
+_seg_attn8_fwd = L.entry('ta_seg_attn8_fwd')
+
+
+def _cache8_rows(name, cache, k, v, dims):
+    """Checks new rows k, v (B, H, [T,] D) against the cache; returns their strides."""
+    ks, vs = k.shape, v.shape
+    if len(ks) != dims or ks != vs or ks[0] != cache.B or ks[1] != cache.H or ks[-1] != cache.D:
+        raise ValueError('%s: rows of %d sequences, %d heads and head size %d as (B, H%s, D), got %s and %s'
+                         % (name, cache.B, cache.H, cache.D, ', T' if dims == 4 else '', tuple(ks), tuple(vs)))
+    if k.dtype != cache.dtype or v.dtype != cache.dtype:
+        raise TypeError('%s: rows must have the cache dtype %s' % (name, cache.dtype))
+    kt, vt = k.stride(), v.stride()
+    if kt[-1] != 1 or vt[-1] != 1:
+        raise ValueError('%s: the last dimension must be contiguous' % name)
+    return kt, vt
+
+
+def _on(name, dev, *tensors):
+    """Every tensor (None: left out) is on GPU `dev`."""
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            L.require_gpu(t)
+            raise ValueError('%s: every tensor must be on the device of the first (cuda:%d), got one on %s'
+                             % (name, dev, t.device))
 
 
 def kv8_append(k_new, v_new, cache, t_pos, levels, arity):
@@ -1004,37 +1014,42 @@ def kv8_append(k_new, v_new, cache, t_pos, levels, arity):
     tree nodes that end there in `levels` (tree levels 0.. of (B,H,nodes,D) float32, arity children per node) from the
     unrounded keys.  The block a token ends is rounded into its page.  A position outside [0, tcap), or in a block
     without a page, is not stored.  Going back to an earlier block restores its rows from its page."""
-    _cache8_rows('kv8_append', cache, k_new, v_new)
-    if k_new.dim() != 3:
-        raise ValueError('kv8_append: one row (B, H, D) per (sequence, head)')
-    if t_pos.dtype != torch.int32 or t_pos.shape != (cache.B,) or not t_pos.is_contiguous():
+    dev = cache.index
+    kt, vt = _cache8_rows('kv8_append', cache, k_new, v_new, 3)
+    if t_pos.dtype != torch.int32 or t_pos.dim() != 1 or t_pos.shape[0] != cache.B or not t_pos.is_contiguous():
         raise ValueError('kv8_append: contiguous int32 positions (B,)')
-    _same_device('kv8_append', cache.device, t_pos, *levels)
-    s, l = _ilog2(arity), cache.desc.block_log2
+    _on('kv8_append', dev, k_new, v_new, t_pos)
+    s, l = _ilog2(arity), cache.block_log2
+    B, H, D, tcap = cache.B, cache.H, cache.D, cache.tcap
+    at = []
     for t in levels:
-        if (t.dtype != torch.float32 or t.shape[:2] != (cache.B, cache.H) or t.shape[3] != cache.D
-                or t.shape[2] < cache.tcap >> l or t.stride(3) != 1 or t.stride(2) != cache.D):
+        b, h, n, d = t.shape
+        sb, sh, sn, sd = t.stride()
+        if (t.dtype != torch.float32 or b != B or h != H or d != D or n < tcap >> l or sd != 1 or sn != D
+                or t.get_device() != dev):
             raise ValueError('kv8_append: levels (B, H, nodes, D) float32 with contiguous node rows for every whole '
-                             'node of tcap positions')
+                             'node of tcap positions, on the cache device')
+        at += t.data_ptr(), sb, sh
         l += s
-    L.call_on(cache.device, 'ta_kv8_append', L.ptr(k_new), L.ptr(v_new), L._DT[cache.dtype], k_new.stride(0),
-              k_new.stride(1), v_new.stride(0), v_new.stride(1), cache.ref, cache.B, cache.H, cache.D, L.ptr(t_pos),
-              len(levels), L.ptr_array(levels), L.i64_array([t.stride(0) for t in levels]),
-              L.i64_array([t.stride(1) for t in levels]), s)
+    n = len(levels)
+    pack = struct.Struct('%dq' % n).pack if n else bytes
+    _kv8_append(dev, k_new.data_ptr(), v_new.data_ptr(), cache.code, kt[0], kt[1], vt[0], vt[1], cache.ref, B, H, D,
+                t_pos.data_ptr(), n, pack(*at[::3]), pack(*at[1::3]), pack(*at[2::3]), s)
 
 
 def kv8_fill(k, v, cache, lengths=None):
     """Positions 0 .. lengths[b]-1 of k, v (B,H,T,D; lengths (B,) int32, all T by default) into a Cache8: whole leaf blocks
     rounded into their pages, the rest of a sequence into its tail.  What lies past a sequence's length stays as it is."""
-    _cache8_rows('kv8_fill', cache, k, v)
-    if k.dim() != 4 or k.shape[2] > cache.tcap:
+    dev = cache.index
+    kt, vt = _cache8_rows('kv8_fill', cache, k, v, 4)
+    if k.shape[2] > cache.tcap:
         raise ValueError('kv8_fill: rows (B, H, T, D) of at most tcap positions')
-    if lengths is not None:
-        if lengths.dtype != torch.int32 or lengths.shape != (cache.B,) or not lengths.is_contiguous():
-            raise ValueError('kv8_fill: contiguous int32 lengths (B,)')
-        _same_device('kv8_fill', cache.device, lengths)
-    L.call_on(cache.device, 'ta_kv8_fill', L.ptr(k), L.ptr(v), L._DT[cache.dtype], *L.rows3(k), *L.rows3(v), cache.ref,
-              cache.B, cache.H, k.shape[2], cache.D, L.ptr(lengths))
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (cache.B,)
+                                or not lengths.is_contiguous()):
+        raise ValueError('kv8_fill: contiguous int32 lengths (B,)')
+    _on('kv8_fill', dev, k, v, lengths)
+    _kv8_fill(dev, k.data_ptr(), v.data_ptr(), cache.code, kt[0], kt[1], kt[2], vt[0], vt[1], vt[2], cache.ref, cache.B,
+              cache.H, k.shape[2], cache.D, lengths.data_ptr() if lengths is not None else None)
 
 
 def seg_attn8_workspace(B, H, Nq, D, nsplit, device):
@@ -1047,26 +1062,38 @@ def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, 
     first min(valid, n_tree) selected leaf blocks ids / vld (B,H,Nq,wl; distinct blocks before the own one, at most
     512), the own block and the static keys; nb = (nid, match) as for seg_attn.  Keys of the block in the tail are read
     unrounded.  Returns (out, lse, keys)."""
-    B, H, Nq, D = q.shape
-    _cache8_rows('seg_attn8', cache, q)
+    dev = cache.index
+    qt, _ = _cache8_rows('seg_attn8', cache, q, q, 4)
+    B, H, Nq, D = shape = q.shape
     wl = ids.shape[-1]
-    tq32 = (tq if tq.dtype == torch.int32 else tq.to(torch.int32)).contiguous()
-    if tq32.shape not in ((Nq,), (B, Nq)):
+    per = (B, H, Nq)
+    if tq.dtype != torch.int32 or not tq.is_contiguous():
+        tq = tq.to(torch.int32).contiguous()
+    if tq.shape == (B, Nq):
+        tq_sb = Nq
+    elif tq.shape == (Nq,):
+        tq_sb = 0
+    else:
         raise ValueError('seg_attn8: positions (Nq,) or (B, Nq)')
-    if (ids.dtype != torch.int32 or vld.dtype not in (torch.uint8, torch.bool) or ids.shape != (B, H, Nq, wl)
-            or vld.shape != ids.shape or not ids.is_contiguous() or not vld.is_contiguous()):
+    want = (B, H, Nq, wl)
+    if (ids.dtype != torch.int32 or (vld.dtype != torch.uint8 and vld.dtype != torch.bool) or ids.shape != want
+            or vld.shape != want or not ids.is_contiguous() or not vld.is_contiguous()):
         raise ValueError('seg_attn8: contiguous ids int32 and vld uint8 or bool, (B, H, Nq, wl)')
-    nt = None
     if n_tree is not None:
-        if n_tree.shape != (B, H, Nq):
+        if n_tree.shape != per:
             raise ValueError('seg_attn8: n_tree (B, H, Nq)')
-        nt = n_tree if (n_tree.dtype == torch.int32 and n_tree.is_contiguous()) else n_tree.to(torch.int32).contiguous()
+        if n_tree.dtype != torch.int32 or not n_tree.is_contiguous():
+            n_tree = n_tree.to(torch.int32).contiguous()
     if out is None:
-        out = torch.empty(B, H, Nq, D, device=q.device, dtype=q.dtype)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
-        raise ValueError('seg_attn8: out must have the shape and dtype of q, the last dimension contiguous')
+        out = torch.empty(shape, device=q.device, dtype=q.dtype)
+        ot = (H * Nq * D, Nq * D, D)
+    else:
+        ot = out.stride()
+        if out.shape != shape or out.dtype != q.dtype or ot[3] != 1:
+            raise ValueError('seg_attn8: out must have the shape and dtype of q, the last dimension contiguous')
+        _on('seg_attn8', dev, out)
     for t in (lse, keys):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (B, H, Nq) or not t.is_contiguous()):
+        if t is not None and (t.dtype != torch.float32 or t.shape != per or not t.is_contiguous()):
             raise ValueError('seg_attn8: lse and keys (B, H, Nq) float32, contiguous')
     nid = nmatch = None
     nS = 0
@@ -1074,16 +1101,17 @@ def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, 
         nid, nmatch = nb
         nS = nid.shape[-1]
         if (nid.dtype != torch.int32 or nmatch.dtype != torch.bool or not nid.is_contiguous() or
-                not nmatch.is_contiguous() or nid.shape[:3] != (B, H, Nq) or nmatch.shape != nid.shape):
+                not nmatch.is_contiguous() or nid.shape[:3] != per or nmatch.shape != nid.shape):
             raise ValueError('seg_attn8: nb must be contiguous (nid int32, match bool) of shape (B, H, Nq, S)')
+        _on('seg_attn8', dev, nid, nmatch)
     if ws is None and nsplit > 1:
         ws = seg_attn8_workspace(B, H, Nq, D, nsplit, q.device)
-    _same_device('seg_attn8', cache.device, tq32, ids, vld, nt, out, lse, keys, nid, nmatch, ws)
-    L.call_on(cache.device, 'ta_seg_attn8_fwd', L.ptr(q), L._DT[cache.dtype], *L.rows3(q), cache.ref, B, H, Nq, D,
-              L.ptr(tq32), 0 if tq32.dim() == 1 else tq32.stride(0), L.ptr(ids), L.ptr(vld), L.ptr(nt), wl, int(local),
-              float(scale), L.ptr(nid), L.ptr(nmatch), nS, L.ptr(out), out.stride(0), out.stride(1), out.stride(2),
-              L.ptr(lse), L.ptr(keys), int(nsplit), L.ptr(ws),
-              ws.numel() * ws.element_size() if ws is not None else 0)
+    _on('seg_attn8', dev, q, tq, ids, vld, n_tree, lse, keys, ws)
+    _seg_attn8_fwd(dev, q.data_ptr(), cache.code, qt[0], qt[1], qt[2], cache.ref, B, H, Nq, D, tq.data_ptr(), tq_sb,
+                   ids.data_ptr(), vld.data_ptr(), n_tree.data_ptr() if n_tree is not None else None, wl, int(local), scale,
+                   nid.data_ptr() if nS else None, nmatch.data_ptr() if nS else None, nS, out.data_ptr(), ot[0], ot[1],
+                   ot[2], lse.data_ptr() if lse is not None else None, keys.data_ptr() if keys is not None else None, nsplit,
+                   ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0)
     return out, lse, keys
 
 
@@ -1100,9 +1128,17 @@ class Mx4:
                 or not packed.is_contiguous() or not scale.is_contiguous()):
             raise ValueError('Mx4: contiguous uint8 packed (rows, Kp / 2) and scale (rows, Kp / 32), Kp = K rounded up to '
                              'a multiple of 128')
-        _same_device('Mx4', packed.device, scale)
+        self.index = L.device_index(packed)
+        _on('Mx4', self.index, scale)
         self.packed, self.scale, self.K = packed, scale, int(K)
         self.shape, self.device = (packed.shape[0], int(K)), packed.device
+
+    @classmethod
+    def _of(cls, packed, scale, rows, K, index):
+        """An Mx4 of tensors made here, without the checks."""
+        w = object.__new__(cls)
+        w.packed, w.scale, w.K, w.shape, w.device, w.index = packed, scale, K, (rows, K), packed.device, index
+        return w
 
     def values(self, dtype=torch.float32):
         """What the rows stand for, (rows, K)."""
@@ -1115,21 +1151,32 @@ class Mx4:
         return (v * s.unsqueeze(-1)).flatten(-2)[:, :self.K].to(dtype)
 
 
+_mx4_quant = L.entry('ta_mx4_quant')
+_mx4_rows = L.entry('ta_mx4_rows')
+_mx4_both = L.entry('ta_mx4_both')
+
+
 def mx4_quant(x, values=False):
     """x (rows, K) float32 / float16 / bfloat16 rounded to Mx4: per block of 32 the scale 2^(floor(log2 of the largest
     magnitude) - 2), values to the nearest (ties to even) and at most 6; a block with anything not finite becomes NaN.
     With values: (Mx4, the values it stands for in x's dtype)."""
-    L.require_gpu(x)
-    if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+    dev = L.device_index(x)
+    if x.dim() != 2:
         raise ValueError('mx4_quant: rows (M, K) with contiguous rows, K at least 1')
     M, K = x.shape
+    ld, one = x.stride()
+    if K < 1 or (K > 1 and one != 1):
+        raise ValueError('mx4_quant: rows (M, K) with contiguous rows, K at least 1')
     Kp = (K + 127) // 128 * 128
-    packed = torch.empty(M, Kp // 2, dtype=torch.uint8, device=x.device)
-    scale = torch.empty(M, Kp // 32, dtype=torch.uint8, device=x.device)
+    # one allocation: the packed rows, then their scales
+    buf = torch.empty(M * (Kp // 2 + Kp // 32), dtype=torch.uint8, device=x.device)
+    packed = buf.as_strided((M, Kp // 2), (Kp // 2, 1))
+    scale = buf.as_strided((M, Kp // 32), (Kp // 32, 1), M * (Kp // 2))
     v = torch.empty(M, K, dtype=x.dtype, device=x.device) if values else None
-    L.call_on(x.device, 'ta_mx4_quant', L.ptr(x), L.dtype_code(x), x.stride(0), M, K, L.ptr(packed), L.ptr(scale), L.ptr(v),
-              K)
-    return (Mx4(packed, scale, K), v) if values else Mx4(packed, scale, K)
+    _mx4_quant(dev, x.data_ptr(), L.dtype_code(x), ld, M, K, packed.data_ptr(), scale.data_ptr(),
+               v.data_ptr() if values else None, K)
+    w = Mx4._of(packed, scale, M, K, dev)
+    return (w, v) if values else w
 
 
 def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
@@ -1139,36 +1186,48 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     float32, rounded once at the end.  `out` may be `residual` (not x)."""
     if not isinstance(w, Mx4):
         raise TypeError('mx4_mm: w must be an Mx4')
-    both = isinstance(x, Mx4)
-    (M, K), N = x.shape, w.shape[0]
+    dev = w.index
+    M, K = x.shape
+    N = w.shape[0]
     if w.K != K:
         raise ValueError('mx4_mm: x has rows of %d values, w of %d' % (K, w.K))
-    if epilogue not in _EPI:
+    epi = _EPI.get(epilogue)
+    if epi is None:
         raise ValueError('mx4_mm: epilogue None, gelu or residual')
     if out is None:
-        out = torch.empty(M, N, device=w.device, dtype=torch.bfloat16)
-    r = residual if epilogue == 'residual' else None
-    if epilogue == 'residual' and r is None:
-        raise ValueError('mx4_mm: the residual epilogue needs residual')
-    for t in (out, r):
-        if t is not None and (t.shape != (M, N) or t.dtype != torch.bfloat16 or (N > 1 and t.stride(1) != 1)):
-            raise ValueError('mx4_mm: out and residual (M, N) bf16 with contiguous rows')
-    L.require_gpu(w.packed, out)
-    _same_device('mx4_mm', w.device, x.packed if both else x, out, r, ln_w)
-    tail = (L.ptr(out), out.stride(0), L.ptr(r), r.stride(0) if r is not None else 0)
-    if both:
+        out = torch.empty((M, N), device=w.device, dtype=torch.bfloat16)
+        ldo = N
+    else:
+        _mx4_out(dev, out, M, N)
+        ldo = out.stride(0)
+    rp, ldr = None, 0
+    if epi == 2:
+        if residual is None:
+            raise ValueError('mx4_mm: the residual epilogue needs residual')
+        _mx4_out(dev, residual, M, N)
+        rp, ldr = residual.data_ptr(), residual.stride(0)
+    if isinstance(x, Mx4):
         if ln_w is not None:
             raise ValueError('mx4_mm: the LayerNorm prologue takes bf16 rows')
-        L.call_on(w.device, 'ta_mx4_both', L.ptr(x.packed), L.ptr(x.scale), L.ptr(w.packed), L.ptr(w.scale), *tail, M, N, K,
-                  _EPI[epilogue])
+        _on('mx4_mm', dev, x.packed)
+        _mx4_both(dev, x.packed.data_ptr(), x.scale.data_ptr(), w.packed.data_ptr(), w.scale.data_ptr(), out.data_ptr(),
+                  ldo, rp, ldr, M, N, K, epi)
         return out
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+    ldx, one = x.stride()
+    if x.dtype != torch.bfloat16 or one != 1:
         raise ValueError('mx4_mm: x (M, K) bf16 with contiguous rows, or an Mx4')
     if ln_w is not None and (ln_w.dtype != torch.bfloat16 or ln_w.shape != (K,) or not ln_w.is_contiguous()):
         raise ValueError('mx4_mm: ln_w (K,) bf16, contiguous')
-    L.call_on(w.device, 'ta_mx4_rows', L.ptr(x), x.stride(0), L.ptr(w.packed), L.ptr(w.scale), *tail, L.ptr(ln_w),
-              float(eps), M, N, K, _EPI[epilogue])
+    _on('mx4_mm', dev, x, ln_w)
+    _mx4_rows(dev, x.data_ptr(), ldx, w.packed.data_ptr(), w.scale.data_ptr(), out.data_ptr(), ldo, rp, ldr,
+              ln_w.data_ptr() if ln_w is not None else None, eps, M, N, K, epi)
     return out
+
+
+def _mx4_out(dev, t, M, N):
+    if t.shape != (M, N) or t.dtype != torch.bfloat16 or (N > 1 and t.stride(1) != 1):
+        raise ValueError('mx4_mm: out and residual (M, N) bf16 with contiguous rows')
+    _on('mx4_mm', dev, t)
 
 
 # ----------------------------------------------------------------------------------------------- sampling
