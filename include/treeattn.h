@@ -155,12 +155,15 @@ int ta_mx4_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int K, voi
 /*
  * Y[M, N] = epilogue(LN(X) . W^T), bf16, for weights W (N, K) in 4 bits (packed and scale as above, contiguous, packed
  * 16-byte and scale 4-byte aligned): the weights are exact in bf16, products are summed in float32, and the result is
- * rounded once, after the epilogue (0 none, 1 GELU in the erf form, 2 R + product).  ln_w (K bf16; M at most 64): the
- * rows of X are normalised first (as ta_rowmm does, rounded to bf16).  K a multiple of 32, X 16-byte aligned with rows
- * of a multiple of 8 elements.  Y may be R, not X.
+ * rounded once, after the epilogue (0 none, 1 GELU in the erf form, 2 R + product).  ln_w (K bf16): the rows of X are
+ * normalised first (as ta_rowmm does, rounded to bf16); where that is not part of the product's launch it needs ws, 16-byte
+ * aligned, of ta_mx4_rows_workspace_size bytes (0: none).  K a multiple of 32, X 16-byte aligned with rows of a multiple of
+ * 8 elements.  Y may be R, not X.
  */
+int64_t ta_mx4_rows_workspace_size(int M, int K, int layernorm);
 int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,
-                int64_t ldr, const void* ln_w, float ln_eps, int M, int N, int K, int epilogue, void* stream);
+                int64_t ldr, const void* ln_w, float ln_eps, int M, int N, int K, int epilogue, void* ws,
+                int64_t ws_bytes, void* stream);
 
 /*
  * The same product of two matrices in 4 bits, X (M, K) and W (N, K), on the scaled matrix instructions; any K of at

@@ -134,8 +134,9 @@ SIGNATURES = {
                                  c_vp, c_vp, c_i32, c_i32, c_f32, c_vp, c_vp, c_i32, c_vp, c_i64, c_i64, c_i64, c_vp,
                                  c_vp, c_i32, c_vp, c_i64, c_vp]),
     'ta_mx4_quant': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    'ta_mx4_rows_workspace_size': (c_i64, [c_i32, c_i32, c_i32]),
     'ta_mx4_rows': (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_f32, c_i32, c_i32, c_i32, c_i32,
-                            c_vp]),
+                            c_vp, c_i64, c_vp]),
     'ta_mx4_both': (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp]),
     'ta_argmax_rows': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp]),
     'ta_embed': (c_i32, [c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i64, c_i64, c_vp,

@@ -7,10 +7,15 @@
 // 128 is thus (i, lane / 16, 8): X is read from LDS in the same order.  Dequantised weights are exact in bf16, so the
 // product is that of the bf16 rows with the values the 4 bits stand for, summed in float32.
 //
-// A workgroup of eight wavefronts computes 16 * CT * WN columns: WN wavefronts side by side, 8 / WN of them over K.  X
-// passes through LDS in pieces of kPiece values of K (normalised on the way in when there is a LayerNorm); the weights
-// of the next piece are requested before a piece is multiplied.  The partial sums of the wavefronts over K are added in
-// LDS in wavefront order.
+// A workgroup of eight wavefronts computes 16 * CT columns of up to 32 rows, each wavefront a run of steps of 128 of K.
+// Each value of X is thus used by one wavefront of the workgroup: it reads the step's slice of X by rows and turns it round
+// in LDS of its own, without a barrier.  The slices and weights of the next steps are in flight in registers meanwhile;
+// loads return in order, so they are issued in the order they are used.  The wavefronts' partial sums are added in LDS in
+// wavefront order.
+//
+// A LayerNorm of short rows (kFused values in all) happens on the way: the workgroup reads X once, 16 or 32 lanes a row,
+// and leaves it normalised in LDS for its wavefronts.  Every workgroup does that for itself, so longer rows are normalised
+// once by a kernel of their own, into the workspace.
 #include "mx4.hpp"
 
 namespace ta {
@@ -36,81 +41,163 @@ struct RowsArgs {
 
 constexpr int kThreads = 512;
 constexpr int kWaves8 = 8;
+constexpr int kFused = 32768;   // values of X, rows and K rounded up to whole tiles and steps, that a workgroup normalises
 
-// MT 16-row tiles of X, CT 16-column tiles per wavefront, WN wavefronts side by side; PC: steps of 128 of K per piece
-// and wavefront.
-template <int MT, int CT, int WN, int PC, bool LN, int EPI>
-__global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a) {
-  constexpr int WK = kWaves8 / WN;
-  constexpr int kPiece = 128 * PC * WK;          // of K
-  constexpr int RS = kPiece + 8;                 // LDS row stride in elements: 16 bytes more, off the banks
+// Sum over the G lanes (16 or 32, aligned) of a row.
+template <int G>
+__device__ __forceinline__ float row_sum(float x) { return group_sum<G>(x); }
+
+// (x - mean) * rstd * g of eight values, as bf16.
+__device__ __forceinline__ uint4 normalised(const uint4& x, const uint4& g, float mean, float rstd) {
+  const bf16_t* e = reinterpret_cast<const bf16_t*>(&x);
+  const bf16_t* ge = reinterpret_cast<const bf16_t*>(&g);
+  float f[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) f[u] = (to_f32(e[u]) - mean) * rstd * to_f32(ge[u]);
+  return make_uint4(bf16_pack2(f[0], f[1]), bf16_pack2(f[2], f[3]), bf16_pack2(f[4], f[5]), bf16_pack2(f[6], f[7]));
+}
+__device__ __forceinline__ float sum8(const uint4& x) {
+  const bf16_t* e = reinterpret_cast<const bf16_t*>(&x);
+  float s = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) s += to_f32(e[u]);
+  return s;
+}
+__device__ __forceinline__ float squares8(const uint4& x, float mean) {
+  const bf16_t* e = reinterpret_cast<const bf16_t*>(&x);
+  float q = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const float d = to_f32(e[u]) - mean;
+    q = fmaf(d, d, q);
+  }
+  return q;
+}
+
+// Scales of a workgroup's columns that fit this many dwords are read once, whole rows at a time, into LDS (a lane's own
+// dword per step and column is a cache line's visit each: 2.3 of 16.5 us at 32 x 4096 x 16384); longer rows' are not.
+constexpr int kScales = 4096;
+
+// The slot of 16-byte vector c (of 16) of row r of a step's slice of X in LDS: the 16 lanes that read one vector of 16
+// rows touch all banks.
+__device__ __forceinline__ int x_slot(int r, int c) { return r * 256 + (c ^ (r & 15)) * 16; }
+
+// MT 16-row tiles of X, CT 16-column tiles; LN: normalised on the way, SL: scales through LDS.
+template <int MT, int CT, bool LN, bool SL, int EPI>
+__global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) {
   constexpr int R = MT * 16;
-  constexpr int COLS = 16 * CT * WN;
+  constexpr int COLS = 16 * CT;
+  constexpr int XB = R * 256;                    // bytes of a step's slice of X
   extern __shared__ __align__(16) char lds[];
-  bf16_t* xs = reinterpret_cast<bf16_t*>(lds);   // [R][RS]
-  float* stat = reinterpret_cast<float*>(lds + (size_t)R * RS * 2);   // mean, rstd of each row
-  const int tid = threadIdx.x, lane = lane_id(), w = wave_id();
-  const int wn = w % WN, wk = w / WN;
+  const int tid = threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
   const int li = lane & 15, lg = lane >> 4;
-  const int n0 = blockIdx.x * COLS + wn * 16 * CT;
-  const int kb = a.Kp / 32, ks = a.Kp / 128;     // blocks, steps of a row
+  const int n0 = (int)(blockIdx.x / ny) * COLS, m0 = (int)(blockIdx.x % ny) * R;
+  const int ks = a.Kp / 128;                     // steps of a row: dwords of scales, groups of four blocks
+  const int per = (ks + kWaves8 - 1) / kWaves8;
+  const int st0 = w * per;                       // this wavefront's steps: st0 .. st0 + mine - 1
+  const int mine = ks - st0 < per ? (ks > st0 ? ks - st0 : 0) : per;
 
-  const uint4* wp[CT];
-  const uint32_t* sp[CT];
+  // Byte offsets from the workgroup's first column and row (what lies past the last repeats it and is not stored); a
+  // step's are 64 bytes of a weight row, 256 of a row of X.
+  const char* wbase = reinterpret_cast<const char*>(a.W) + (int64_t)n0 * ks * 64;
+  const uint32_t* sbase = a.S + (int64_t)n0 * ks;
+  const char* xbase = reinterpret_cast<const char*>(a.X) + (int64_t)m0 * a.ldx * 2;
+  uint32_t so[CT], wo[CT], xo[MT * 4];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const int n = n0 + c * 16 + li;
-    const int nc = n < a.N ? n : a.N - 1;        // columns past the last repeat it and are not stored
-    wp[c] = a.W + (int64_t)nc * kb + lg;
-    sp[c] = a.S + (int64_t)nc * ks;
+    so[c] = (uint32_t)(n0 + c * 16 + li < a.N ? c * 16 + li : a.N - 1 - n0) * (uint32_t)ks;
+    wo[c] = so[c] * 64 + lg * 16;
   }
-  struct Wt {
-    uint4 q[PC][CT];
-    uint32_t s[PC][CT];
+#pragma unroll
+  for (int t = 0; t < MT * 4; ++t) {
+    const int r = t * 4 + lg;
+    xo[t] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (uint32_t)(a.ldx * 2) + li * 16;
+  }
+  const bool ragged = (a.K & 127) != 0;
+  // this wavefront's step i: column li of each tile of the weights, block lg of the step's four; rows lg, lg + 4, ... of
+  // X's slice, vector li of each
+  struct Step {
+    uint4 x[LN ? 1 : MT * 4];
+    uint4 q[CT];
+    uint32_t s[CT];
   };
-  // the weights of a piece for this wavefront (steps past K repeat the last one; its X is zero)
-  auto load_w = [&](int piece, Wt& x) {
+  auto load = [&](int i, Step& v) {
+    const int st = st0 + i;
+    if constexpr (!LN) {
+      const char* xs = xbase + (int64_t)st * 256;
+      if (ragged && st == ks - 1) {              // what lies past K is zero
+        const bool in = st * 128 + li * 8 < a.K;
 #pragma unroll
-    for (int i = 0; i < PC; ++i) {
-      int st = (piece * PC + i) * WK + wk;
-      st = st < ks ? st : ks - 1;
+        for (int t = 0; t < MT * 4; ++t) {
+          v.x[t] = ldg16(in ? xs + xo[t] : xbase + xo[t] - li * 16);
+          if (!in) v.x[t] = make_uint4(0, 0, 0, 0);
+        }
+      } else {
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        x.q[i][c] = ldg16(wp[c] + st * 4);
-        x.s[i][c] = sp[c][st];
+        for (int t = 0; t < MT * 4; ++t) v.x[t] = ldg16(xs + xo[t]);
       }
     }
+    const char* ws = wbase + (int64_t)st * 64;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      v.q[c] = ldg16(ws + wo[c]);
+      if constexpr (!SL) v.s[c] = sbase[so[c] + st];
+    }
   };
-  Wt cur;
-  load_w(0, cur);
 
+  uint32_t* s_sc = reinterpret_cast<uint32_t*>(lds + (LN ? kFused * 2 : kWaves8 * XB));
+  constexpr int NS = kScales / kThreads;
+  uint32_t sv[NS];
+  const int ns = (a.N - n0 < COLS ? a.N - n0 : COLS) * ks;
+  if constexpr (SL) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (i * kThreads < ns) sv[i] = sbase[i * kThreads + tid < ns ? i * kThreads + tid : ns - 1];
+  }
+  auto keep_scales = [&]() {
+    if constexpr (SL) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (i * kThreads < ns) s_sc[i * kThreads + tid] = sv[i];
+    }
+  };
+  Step va, vb;
   if constexpr (LN) {
-    // a row's mean and variance by one wavefront, in two passes over values it holds or reads again
-    for (int r = w; r < R; r += kWaves8) {
-      const bf16_t* xr = a.X + (int64_t)(r < a.M ? r : 0) * a.ldx;
-      float s = 0.0f;
-      for (int k = lane * 8; k < a.K; k += kWave * 8) {
-        float f[8];
-        load_row_g<bf16_t, 8>(xr + k, f);
+    // row r of the workgroup's by G lanes, eight vectors each at most
+    constexpr int G = kThreads / R, NV = kFused / R / 8 / G;
+    const int r = tid / G, j = tid % G;
+    const bf16_t* xr = a.X + (int64_t)(m0 + r < a.M ? m0 + r : a.M - 1) * a.ldx;
+    uint4 x[NV], g[NV];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s += f[u];
-      }
-      const float mean = wave_sum(s) / (float)a.K;
-      float v = 0.0f;
-      for (int k = lane * 8; k < a.K; k += kWave * 8) {
-        float f[8];
-        load_row_g<bf16_t, 8>(xr + k, f);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v += (f[u] - mean) * (f[u] - mean);
-      }
-      v = wave_sum(v) / (float)a.K;
-      if (lane == 0) {
-        stat[2 * r] = mean;
-        stat[2 * r + 1] = rsqrtf(v + a.eps);
+    for (int i = 0; i < NV; ++i) {
+      const int k = (i * G + j) * 8;
+      x[i] = g[i] = make_uint4(0, 0, 0, 0);
+      if (k < a.K) {
+        x[i] = ldg16(xr + k);
+        g[i] = ldg16(a.gam + k);
       }
     }
-    __syncthreads();
+    if (mine > 0) load(0, va);
+    if (mine > 1) load(1, vb);
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s += sum8(x[i]);
+    const float mean = row_sum<G>(s) / (float)a.K;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * G + j) * 8 < a.K) q += squares8(x[i], mean);
+    const float rstd = rsqrtf(row_sum<G>(q) / (float)a.K + a.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = i * G + j;                   // vector of the row (past K: weight 0, value 0)
+      if (v * 8 < a.Kp) *reinterpret_cast<uint4*>(lds + (v / 16) * XB + x_slot(r, v % 16)) = normalised(x[i], g[i], mean, rstd);
+    }
+  } else {
+    if (mine > 0) load(0, va);
+    if (mine > 1) load(1, vb);
   }
+  keep_scales();
+  if constexpr (LN || SL) lds_barrier();
 
   f32x4_t acc[MT][CT];
 #pragma unroll
@@ -118,126 +205,147 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[m][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int pieces = (a.K + kPiece - 1) / kPiece;
-  constexpr int VR = kPiece / 8;                  // vectors of a row
-  constexpr int VT = (R * VR + kThreads - 1) / kThreads;
-  for (int p = 0; p < pieces; ++p) {
-    // X's piece, vector i of it by thread i mod 512
-    uint4 xv[VT];
+  auto multiply = [&](int i, Step& v) {
+    const char* xs = lds + (LN ? st0 + i : w) * XB;
+    if constexpr (!LN) {
+      wave_sync();                               // the previous step's slice has been read
 #pragma unroll
-    for (int j = 0; j < VT; ++j) {
-      const int i = j * kThreads + tid;
-      const int r = i / VR, k = p * kPiece + (i % VR) * 8;
-      xv[j] = make_uint4(0, 0, 0, 0);
-      if (i < R * VR && r < a.M && k < a.K) xv[j] = ldg16(a.X + (int64_t)r * a.ldx + k);
+      for (int t = 0; t < MT * 4; ++t) *reinterpret_cast<uint4*>(lds + w * XB + x_slot(t * 4 + lg, li)) = v.x[t];
+      wave_sync();
     }
-    if (p > 0) __syncthreads();                   // the previous piece has been multiplied
+    float sc[CT];
 #pragma unroll
-    for (int j = 0; j < VT; ++j) {
-      const int i = j * kThreads + tid;
-      if (i < R * VR) {
-        const int r = i / VR, kk = (i % VR) * 8;
-        uint4 o = xv[j];
-        if constexpr (LN) {
-          const int k = p * kPiece + kk;
-          if (k < a.K) {
-            float f[8], gm[8];
-            const bf16_t* e = reinterpret_cast<const bf16_t*>(&xv[j]);
+    for (int c = 0; c < CT; ++c) {
+      if constexpr (SL) sc[c] = mx4_scale(reinterpret_cast<const uint8_t*>(s_sc + so[c] + st0 + i)[lg]);
+      else sc[c] = mx4_scale((v.s[c] >> (8 * lg)) & 255u);
+    }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) f[u] = to_f32(e[u]);
-            load_row_g<bf16_t, 8>(a.gam + k, gm);
-            const float mean = stat[2 * r], rstd = stat[2 * r + 1];
+    for (int u = 0; u < 4; ++u) {
+      bf16x8_t ax[MT];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) f[u] = (f[u] - mean) * rstd * gm[u];
-            o = make_uint4(bf16_pack2(f[0], f[1]), bf16_pack2(f[2], f[3]), bf16_pack2(f[4], f[5]),
-                           bf16_pack2(f[6], f[7]));
-            if (r >= a.M) o = make_uint4(0, 0, 0, 0);
-          }
-        }
-        *reinterpret_cast<uint4*>(xs + r * RS + kk) = o;
+      for (int m = 0; m < MT; ++m) ax[m] = *reinterpret_cast<const bf16x8_t*>(xs + x_slot(m * 16 + li, lg * 4 + u));
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const bf16x8_t bw = mx4_bf16x8(u == 0 ? v.q[c].x : u == 1 ? v.q[c].y : u == 2 ? v.q[c].z : v.q[c].w, sc[c]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ax[m], bw, acc[m][c], 0, 0, 0);
       }
     }
-    __syncthreads();
-    Wt nxt;
-    load_w(p + 1 < pieces ? p + 1 : p, nxt);
-#pragma unroll
-    for (int i = 0; i < PC; ++i) {
-      const int k0 = (i * WK + wk) * 128 + lg * 32;
-      float sc[CT];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) sc[c] = mx4_scale((cur.s[i][c] >> (8 * lg)) & 255u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        bf16x8_t bw[CT];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const uint32_t q = u == 0 ? cur.q[i][c].x : u == 1 ? cur.q[i][c].y : u == 2 ? cur.q[i][c].z : cur.q[i][c].w;
-          bw[c] = mx4_bf16x8(q, sc[c]);
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const bf16x8_t ax = *reinterpret_cast<const bf16x8_t*>(xs + (m * 16 + li) * RS + k0 + u * 8);
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ax, bw[c], acc[m][c], 0, 0, 0);
-        }
-      }
-    }
-    cur = nxt;
+    if (i + 2 < mine) load(i + 2, v);
+  };
+#pragma unroll 1
+  for (int i = 0; i < mine; i += 2) {
+    multiply(i, va);
+    if (i + 1 < mine) multiply(i + 1, vb);
   }
 
-  // sums over the wavefronts along K, then the epilogue: element (row, col) of a tile is register row % 4 of lane
+  // sums over the wavefronts, then the epilogue: element (row, col) of a tile is register row % 4 of lane
   // (row / 4) * 16 + col
-  float* red = reinterpret_cast<float*>(lds);     // [WK][R][COLS + 1]
+  float* red = reinterpret_cast<float*>(lds);     // [8][R][COLS + 1]
   __syncthreads();
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[(wk * R + m * 16 + lg * 4 + i) * (COLS + 1) + wn * 16 * CT + c * 16 + li] = acc[m][c][i];
+      for (int i = 0; i < 4; ++i) red[(w * R + m * 16 + lg * 4 + i) * (COLS + 1) + c * 16 + li] = acc[m][c][i];
   __syncthreads();
   for (int i = tid; i < R * COLS; i += kThreads) {
     const int r = i / COLS, cc = i % COLS;
-    const int n = blockIdx.x * COLS + cc;
-    if (r >= a.M || n >= a.N) continue;
+    const int n = n0 + cc;
+    if (m0 + r >= a.M || n >= a.N) continue;
     float s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < WK; ++k) s += red[(k * R + r) * (COLS + 1) + cc];
+    for (int k = 0; k < kWaves8; ++k) s += red[(k * R + r) * (COLS + 1) + cc];
     if constexpr (EPI == MX_EPI_GELU) s = mx4_gelu(s);
-    if constexpr (EPI == MX_EPI_RESIDUAL) s += to_f32(a.R[(int64_t)r * a.ldr + n]);
-    a.Y[(int64_t)r * a.ldy + n] = bf16_from(s);
+    if constexpr (EPI == MX_EPI_RESIDUAL) s += to_f32(a.R[(int64_t)(m0 + r) * a.ldr + n]);
+    a.Y[(int64_t)(m0 + r) * a.ldy + n] = bf16_from(s);
   }
 }
 
-template <int MT, int CT, int WN, int PC>
-int launch_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
-  constexpr int WK = kWaves8 / WN, R = MT * 16, COLS = 16 * CT * WN;
-  const size_t x = (size_t)R * (128 * PC * WK + 8) * 2 + R * 8;
-  const size_t red = (size_t)WK * R * (COLS + 1) * 4;
-  const size_t lds = x > red ? x : red;
-  const dim3 grid((a.N + COLS - 1) / COLS), blk(kThreads);
-#define TA_MXR(L, E) hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, WN, PC, L, E>), grid, blk, lds, st, a)
-#define TA_MXL(E)                      \
-  if (a.gam != nullptr) TA_MXR(true, E); \
-  else TA_MXR(false, E)
-  switch (epilogue) {
-    case MX_EPI_NONE: TA_MXL(MX_EPI_NONE); break;
-    case MX_EPI_GELU: TA_MXL(MX_EPI_GELU); break;
-    default: TA_MXL(MX_EPI_RESIDUAL); break;
+// LayerNorm of one row per workgroup, from X to Y (rows of K, contiguous); up to 16384 values are held in registers, longer
+// rows read again.
+__global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, bf16_t* __restrict__ Y) {
+  __shared__ float s_red[2][kWaves8];
+  const int tid = threadIdx.x;
+  const bf16_t* xr = a.X + (int64_t)blockIdx.x * a.ldx;
+  bf16_t* yr = Y + (int64_t)blockIdx.x * a.K;
+  const int nv = a.K / 8;
+  auto total = [&](float x, int which) {
+    x = group_sum<64>(x);
+    if (lane_id() == 0) s_red[which][wave_id()] = x;
+    __syncthreads();
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves8; ++i) t += s_red[which][i];
+    return t;
+  };
+  constexpr int NV = 4;
+  uint4 x[NV], g[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = i * kThreads + tid;
+    x[i] = g[i] = make_uint4(0, 0, 0, 0);
+    if (v < nv) {
+      x[i] = ldg16(xr + v * 8);
+      g[i] = ldg16(a.gam + v * 8);
+    }
   }
-#undef TA_MXL
-#undef TA_MXR
+  float s = 0.0f, q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) s += sum8(x[i]);
+  for (int v = NV * kThreads + tid; v < nv; v += kThreads) s += sum8(ldg16(xr + (int64_t)v * 8));
+  const float mean = total(s, 0) / (float)a.K;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * kThreads + tid < nv) q += squares8(x[i], mean);
+  for (int v = NV * kThreads + tid; v < nv; v += kThreads) q += squares8(ldg16(xr + (int64_t)v * 8), mean);
+  const float rstd = rsqrtf(total(q, 1) / (float)a.K + a.eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = i * kThreads + tid;
+    if (v < nv) *reinterpret_cast<uint4*>(yr + v * 8) = normalised(x[i], g[i], mean, rstd);
+  }
+  for (int v = NV * kThreads + tid; v < nv; v += kThreads)
+    *reinterpret_cast<uint4*>(yr + (int64_t)v * 8) =
+        normalised(ldg16(xr + (int64_t)v * 8), ldg16(a.gam + (int64_t)v * 8), mean, rstd);
+}
+
+// Whether ta_mx4_rows normalises M rows of K values within the product.
+bool norm_fused(int M, int K) { return M <= 64 && (int64_t)(M <= 16 ? 16 : 32) * mx4_padded(K) <= kFused; }
+
+template <int MT, int CT, bool LN, int EPI>
+int launch_one(const RowsArgs& a, hipStream_t st) {
+  constexpr int R = MT * 16, COLS = 16 * CT;
+  constexpr int x = LN ? kFused * 2 : kWaves8 * R * 256, red = kWaves8 * R * (COLS + 1) * 4;
+  const int ny = (a.M + R - 1) / R;
+  const dim3 grid((unsigned)((a.N + COLS - 1) / COLS * ny)), blk(kThreads);
+  if (COLS * (a.Kp / 128) <= kScales)
+    hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, LN, true, EPI>), grid, blk, x + kScales * 4 > red ? x + kScales * 4 : red,
+                       st, a, ny);
+  else
+    hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, LN, false, EPI>), grid, blk, x > red ? x : red, st, a, ny);
   return check_launch("mx4_rows_kernel");
 }
 
-// 64 columns per workgroup where that still leaves every compute unit one, else 16 (32 for more than 32 rows, whose X
-// would not fit the LDS of a workgroup with eight wavefronts over K).
+template <int MT, int CT>
+int launch_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
+  const bool ln = a.gam != nullptr;
+  switch (epilogue) {
+    case MX_EPI_NONE: return ln ? launch_one<MT, CT, true, MX_EPI_NONE>(a, st) : launch_one<MT, CT, false, MX_EPI_NONE>(a, st);
+    case MX_EPI_GELU: return ln ? launch_one<MT, CT, true, MX_EPI_GELU>(a, st) : launch_one<MT, CT, false, MX_EPI_GELU>(a, st);
+    default:
+      return ln ? launch_one<MT, CT, true, MX_EPI_RESIDUAL>(a, st) : launch_one<MT, CT, false, MX_EPI_RESIDUAL>(a, st);
+  }
+}
+
+// The widest workgroup (of 16, 32 or 64 columns) that still leaves every compute unit one: X is read once per workgroup.
 template <int MT>
 int pick_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
-  if ((a.N + 63) / 64 >= device_cus()) return launch_rows<MT, 2, 2, MT == 4 ? 1 : 2>(a, epilogue, st);
-  return launch_rows<MT, 1, MT == 4 ? 2 : 1, 1>(a, epilogue, st);
+  const int cus = device_cus();
+  if ((a.N + 63) / 64 >= cus) return launch_rows<MT, 4>(a, epilogue, st);
+  if ((a.N + 31) / 32 >= cus) return launch_rows<MT, 2>(a, epilogue, st);
+  return launch_rows<MT, 1>(a, epilogue, st);
 }
 
 }  // namespace
@@ -245,30 +353,45 @@ int pick_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
 
 using namespace ta;
 
+extern "C" int64_t ta_mx4_rows_workspace_size(int M, int K, int layernorm) {
+  return !layernorm || M <= 0 || K <= 0 || norm_fused(M, K) ? 0 : (int64_t)M * K * 2;
+}
+
 extern "C" int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy,
                            const void* R, int64_t ldr, const void* ln_w, float ln_eps, int M, int N, int K,
-                           int epilogue, void* stream) {
+                           int epilogue, void* ws, int64_t ws_bytes, void* stream) {
   if (M < 0 || N < 1 || K < 32 || K % 32 || K > 0x7fffff00 || (M > 1 && (ldx < K || ldy < N)) || epilogue < 0 ||
       epilogue > 2 || (epilogue == MX_EPI_RESIDUAL && (R == nullptr || (M > 1 && ldr < N)))) {
     set_error("ta_mx4_rows: bad sizes (K a multiple of 32; a residual needs its rows)");
     return TA_ERR_ARG;
   }
   if (M == 0) return TA_OK;
+  if (M > 1 && ldx > (1 << 25)) {
+    set_error("ta_mx4_rows: rows of X of at most 2^25 elements apart");
+    return TA_ERR_UNSUPPORTED;
+  }
   if (X == nullptr || Wp == nullptr || Ws == nullptr || Y == nullptr || ((uintptr_t)X | (uintptr_t)Wp) % 16 ||
       (uintptr_t)Ws % 4 || (ldx * 2) % 16 || (uintptr_t)ln_w % 16 || (uintptr_t)Y % 2) {
     set_error("ta_mx4_rows: X, the packed weights and the LayerNorm weight must be 16-byte aligned with X's row stride "
               "a multiple of 8, the scales 4-byte aligned");
     return TA_ERR_ARG;
   }
-  if (ln_w != nullptr && M > 64) {
-    set_error("ta_mx4_rows: the LayerNorm prologue takes at most 64 rows");
-    return TA_ERR_UNSUPPORTED;
-  }
   hipStream_t st = (hipStream_t)stream;
-  if (M > 64) return mx4_gemm_bf16(X, ldx, Wp, Ws, Y, ldy, R, ldr, M, N, K, epilogue, st);
   RowsArgs a{(const bf16_t*)X, ldx, (const uint4*)Wp, (const uint32_t*)Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr,
              (const bf16_t*)ln_w, ln_eps, M, N, K, mx4_padded(K)};
-  if (M <= 16) return pick_rows<1>(a, epilogue, st);
-  if (M <= 32) return pick_rows<2>(a, epilogue, st);
-  return pick_rows<4>(a, epilogue, st);
+  if (ln_w != nullptr && !norm_fused(M, K)) {
+    const int64_t need = ta_mx4_rows_workspace_size(M, K, 1);
+    if (ws == nullptr || ws_bytes < need || (uintptr_t)ws % 16) {
+      set_error("ta_mx4_rows: workspace missing, too small or not 16-byte aligned");
+      return TA_ERR_WORKSPACE;
+    }
+    hipLaunchKernelGGL(mx4_norm_kernel, dim3((unsigned)M), dim3(kThreads), 0, st, a, (bf16_t*)ws);
+    const int rc = check_launch("mx4_norm_kernel");
+    if (rc != TA_OK) return rc;
+    a.X = (const bf16_t*)ws;
+    a.ldx = K;
+    a.gam = nullptr;
+  }
+  if (M > 64) return mx4_gemm_bf16(a.X, a.ldx, Wp, Ws, Y, ldy, R, ldr, M, N, K, epilogue, st);
+  return M <= 16 ? pick_rows<1>(a, epilogue, st) : pick_rows<2>(a, epilogue, st);
 }

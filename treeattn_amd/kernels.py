@@ -1182,7 +1182,7 @@ def mx4_quant(x, values=False):
 def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     """epilogue(LN(x) @ w.T) in bf16 for weights w (Mx4, (N,K)): x (M,K) bf16, K a multiple of 32 -- the weights are exact in
     bf16 -- or x an Mx4 (M,K), whose product runs on the 4-bit matrix instructions.  ln_w (K,) bf16: a LayerNorm of x's
-    rows first (bf16 x, M at most 64).  epilogue None | 'gelu' | 'residual' (adds `residual`, (M,N) bf16); sums are
+    rows first (bf16 x).  epilogue None | 'gelu' | 'residual' (adds `residual`, (M,N) bf16); sums are
     float32, rounded once at the end.  `out` may be `residual` (not x)."""
     if not isinstance(w, Mx4):
         raise TypeError('mx4_mm: w must be an Mx4')
@@ -1219,8 +1219,15 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     if ln_w is not None and (ln_w.dtype != torch.bfloat16 or ln_w.shape != (K,) or not ln_w.is_contiguous()):
         raise ValueError('mx4_mm: ln_w (K,) bf16, contiguous')
     _on('mx4_mm', dev, x, ln_w)
-    _mx4_rows(dev, x.data_ptr(), ldx, w.packed.data_ptr(), w.scale.data_ptr(), out.data_ptr(), ldo, rp, ldr,
-              ln_w.data_ptr() if ln_w is not None else None, eps, M, N, K, epi)
+    ws = gp = None
+    nbytes = 0
+    if ln_w is not None:
+        gp = ln_w.data_ptr()
+        nbytes = L.lib().ta_mx4_rows_workspace_size(M, K, 1)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+    _mx4_rows(dev, x.data_ptr(), ldx, w.packed.data_ptr(), w.scale.data_ptr(), out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K,
+              epi, ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
