@@ -35,17 +35,40 @@ constexpr int kGemmThreads = 512;
 // What copies past the end of a row read.
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 
-// Slot of 16-byte vector c of row r in an LDS array of rows of eight: rotated so that the 16 lanes that read one vector
-// of 16 consecutive rows touch all banks.
-__device__ __forceinline__ int slot8(int r, int c) { return r * 8 + (c ^ ((r >> 1) & 7)); }
-// The same for rows of two vectors read in halves.
+// Slot of 16-byte vector c of row r in an LDS array of rows of eight.  A 16-byte read is served 16 lanes at a time: lanes
+// 0-3 and 12-15 of one group of 16 with lanes 4-11 of the next; the groups read vectors two apart of rows that lie two to
+// a line of banks.  With this turn those 16 lanes touch every bank once.
+__device__ __forceinline__ int turn8(int r) { return ((r >> 1) & 1) | ((r >> 3) & 1) * 6; }
+__device__ __forceinline__ int slot8(int r, int c) { return r * 8 + (c ^ turn8(r)); }
+// Slot of vector c of row r in an array of rows of two, read in halves.
 __device__ __forceinline__ int slot2(int r, int c) { return r * 2 + (c ^ ((r >> 3) & 1)); }
 
-__device__ __forceinline__ void to_lds16(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void*)dst, 16, 0, 0);
+// Copies of 16 or 4 bytes a lane, from a uniform base plus a lane's byte offset (or a lane's own address) to consecutive
+// places in LDS.  Written as instructions because the compiler waits for every such copy before the next read of LDS, also
+// of another buffer: here copies are in flight while LDS is read, and are waited for by count.  They have no result
+// registers, and their operands are read when they issue.
+__device__ __forceinline__ void copy16(const void* base, uint32_t off, const void* dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(off),
+               "s"(base)
+               : "memory");
 }
-__device__ __forceinline__ void to_lds4(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void*)dst, 4, 0, 0);
+__device__ __forceinline__ void copy16(const void* src, const void* dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(const void* base, uint32_t off, const void* dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(off),
+               "s"(base)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(const void* src, const void* dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(src)
+               : "memory");
+}
+
+// 32 codes as the instruction's operand (which reads its first four registers for 4-bit values).
+__device__ __forceinline__ i32x8_t codes(const uint4& q) {
+  return i32x8_t{(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
 }
 
 template <bool BOTH, int MT, int NT>
@@ -55,7 +78,8 @@ struct GemmTile {
   static constexpr int XB = BM * 128;                         // LDS bytes of X a step
   static constexpr int WB = BOTH ? BN * 128 : BN * 32;        // of W
   static constexpr int SB = BOTH ? (BM + BN) * 8 : BN * 4;    // of scales (bf16 X: of two steps)
-  static constexpr int LDS = 2 * (XB + WB + SB);
+  static constexpr int BUFS = BOTH ? 2 : 3;                   // steps in LDS
+  static constexpr int LDS = BUFS * (XB + WB) + 2 * SB;
 };
 
 template <bool BOTH, int MT, int NT, int EPI>
@@ -63,7 +87,7 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
   using G = GemmTile<BOTH, MT, NT>;
   constexpr int BM = G::BM, BN = G::BN;
   extern __shared__ __align__(16) char lds[];
-  const int lane = lane_id(), w = wave_id();
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
   const int li = lane & 15, lg = lane >> 4;
   const int wm = (w & 1) * 16 * MT, wn = (w >> 1) * 16 * NT;
   // Workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles, in groups of eight rows of tiles,
@@ -90,63 +114,68 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < NX; ++i) {
     const int s = (i * 8 + w) * 64 + lane, r = s / 8;
-    xc[i] = (s % 8) ^ ((r >> 1) & 7);
+    xc[i] = (s % 8) ^ turn8(r);
     xo[i] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (uint32_t)a.xb + xc[i] * 16;
   }
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
     const int s = (i * 8 + w) * 64 + lane;
     const int r = BOTH ? s / 8 : s / 2;
-    wc[i] = BOTH ? (s % 8) ^ ((r >> 1) & 7) : (s % 2) ^ ((r >> 3) & 1);
+    wc[i] = BOTH ? (s % 8) ^ turn8(r) : (s % 2) ^ ((r >> 3) & 1);
     wo[i] = (uint32_t)(n0 + r < a.N ? r : a.N - 1 - n0) * (uint32_t)(a.Kp / 2) + wc[i] * 16;
   }
-  const uint32_t* sp[NS];
+  const char* xsc = reinterpret_cast<const char*>(a.XS) + (int64_t)m0 * kd * 4;   // scales, from the tile's first row
+  const char* wsc = reinterpret_cast<const char*>(a.S) + (int64_t)n0 * kd * 4;
+  uint32_t so[NS];
   int sd[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     const int s = (i * 8 + w) * 64 + lane;
-    if constexpr (BOTH) {
-      const int r = s / 2;
-      sd[i] = s & 1;
-      sp[i] = r < BM ? a.XS + (int64_t)(m0 + r < a.M ? m0 + r : a.M - 1) * kd + sd[i]
-                     : a.S + (int64_t)(n0 + r - BM < a.N ? n0 + r - BM : a.N - 1) * kd + sd[i];
-    } else {
-      sd[i] = 0;
-      sp[i] = a.S + (int64_t)(n0 + s < a.N ? n0 + s : a.N - 1) * kd;
-    }
+    const int r = BOTH ? (s / 2 < BM ? s / 2 : s / 2 - BM) : s;
+    sd[i] = BOTH ? s & 1 : 0;
+    const int rr = BOTH && s / 2 < BM ? (m0 + r < a.M ? r : a.M - 1 - m0) : (n0 + r < a.N ? r : a.N - 1 - n0);
+    so[i] = (uint32_t)(rr * kd + sd[i]) * 4;
   }
   const bool ragged = BOTH ? (a.Kp & 255) != 0 : (a.K & 63) != 0;
 
+  constexpr int BUFS = G::BUFS;
   auto lx = [&](int buf) { return lds + buf * G::XB; };
-  auto lw = [&](int buf) { return lds + 2 * G::XB + buf * G::WB; };
-  auto ls = [&](int buf) { return lds + 2 * (G::XB + G::WB) + buf * G::SB; };
+  auto lw = [&](int buf) { return lds + BUFS * G::XB + buf * G::WB; };
+  auto ls = [&](int buf) { return lds + BUFS * (G::XB + G::WB) + buf * G::SB; };
 
   auto stage = [&](int s, int buf) {
-    const bool last = ragged && s == steps - 1;
     const char* xs = xbase + (int64_t)s * 128;
     const char* ws = wbase + (int64_t)s * (BOTH ? 128 : 32);
+    if (ragged && s == steps - 1) {
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const void* src = xs + xo[i];
-      if (last && (BOTH ? s * 8 + xc[i] >= kd * 4 : s * 64 + xc[i] * 8 >= a.K)) src = &kZeros;
-      to_lds16(src, lx(buf) + (i * 8 + w) * 1024);
-    }
-    if constexpr (BOTH) {
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        const void* src = ws + wo[i];
-        if (last && s * 8 + wc[i] >= kd * 4) src = &kZeros;
-        to_lds16(src, lw(buf) + (i * 8 + w) * 1024);
+      for (int i = 0; i < NX; ++i) {
+        const bool in = BOTH ? s * 8 + xc[i] < kd * 4 : s * 64 + xc[i] * 8 < a.K;
+        copy16(in ? (const void*)(xs + xo[i]) : (const void*)&kZeros, lx(buf) + (i * 8 + w) * 1024);
       }
+      if constexpr (BOTH) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const void* src = sp[i] + s * 2;
-        if (last && s * 2 + sd[i] >= kd) src = &kZeros;
-        to_lds4(src, ls(buf) + (i * 8 + w) * 256);
+        for (int i = 0; i < NW; ++i)
+          copy16(s * 8 + wc[i] < kd * 4 ? (const void*)(ws + wo[i]) : (const void*)&kZeros, lw(buf) + (i * 8 + w) * 1024);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const char* sb = (i * 8 + w) * 32 < BM ? xsc : wsc;
+          copy4(s * 2 + sd[i] < kd ? (const void*)(sb + s * 8 + so[i]) : (const void*)&kZeros, ls(buf) + (i * 8 + w) * 256);
+        }
       }
     } else {
-      if (w < BN / 32) to_lds16(ws + wo[0], lw(buf) + w * 1024);
-      if ((s & 1) == 0 && w < BN / 64) to_lds4(sp[0] + (s >> 1), ls((s >> 1) & 1) + w * 256);
+#pragma unroll
+      for (int i = 0; i < NX; ++i) copy16(xs, xo[i], lx(buf) + (i * 8 + w) * 1024);
+      if constexpr (BOTH) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) copy16(ws, wo[i], lw(buf) + (i * 8 + w) * 1024);
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          copy4(((i * 8 + w) * 32 < BM ? xsc : wsc) + s * 8, so[i], ls(buf) + (i * 8 + w) * 256);
+      }
+    }
+    if constexpr (!BOTH) {
+      if (w < BN / 32) copy16(ws, wo[0], lw(buf) + w * 1024);
+      if ((s & 1) == 0 && w < BN / 64) copy4(wsc + (s >> 1) * 4, so[0], ls((s >> 1) & 1) + w * 256);
     }
   };
 
@@ -156,72 +185,103 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int c = 0; c < NT; ++c) acc[m][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // The operands of row tile m + 1 are read while the instructions of row tile m run.
   auto multiply = [&](int s, int buf) {
     const uint4* x = reinterpret_cast<const uint4*>(lx(buf));
     if constexpr (BOTH) {
       const uint4* wl = reinterpret_cast<const uint4*>(lw(buf));
       const uint16_t* sc = reinterpret_cast<const uint16_t*>(ls(buf));
-      uint4 wq[NT][2];
+      i32x8_t wq[2][NT];
       int sw[NT];
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         const int r = wn + c * 16 + li;
         sw[c] = sc[(BM + r) * 4 + lg];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) wq[c][k] = wl[slot8(r, lg * 2 + k)];
+        for (int k = 0; k < 2; ++k) wq[k][c] = codes(wl[slot8(r, lg * 2 + k)]);
       }
+      i32x8_t xq[2][2];
+      int sx[2];
+      auto read = [&](int m, int j) {
+        const int r = wm + m * 16 + li;
+        sx[j] = sc[r * 4 + lg];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) xq[j][k] = codes(x[slot8(r, lg * 2 + k)]);
+      };
+      read(0, 0);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const int r = wm + m * 16 + li;
-        const int sx = sc[r * 4 + lg];
-        uint4 xq[2];
+        if (m + 1 < MT) read(m + 1, (m + 1) & 1);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) xq[k] = x[slot8(r, lg * 2 + k)];
-        const i32x8_t x0 = {(int)xq[0].x, (int)xq[0].y, (int)xq[0].z, (int)xq[0].w, 0, 0, 0, 0};
-        const i32x8_t x1 = {(int)xq[1].x, (int)xq[1].y, (int)xq[1].z, (int)xq[1].w, 0, 0, 0, 0};
+        for (int c = 0; c < NT; ++c)
+          acc[m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wq[0][c], xq[m & 1][0], acc[m][c], 4, 4, 0, sw[c], 0,
+                                                                       sx[m & 1]);
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const i32x8_t w0 = {(int)wq[c][0].x, (int)wq[c][0].y, (int)wq[c][0].z, (int)wq[c][0].w, 0, 0, 0, 0};
-          acc[m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w0, x0, acc[m][c], 4, 4, 0, sw[c], 0, sx);
-        }
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const i32x8_t w1 = {(int)wq[c][1].x, (int)wq[c][1].y, (int)wq[c][1].z, (int)wq[c][1].w, 0, 0, 0, 0};
-          acc[m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w1, x1, acc[m][c], 4, 4, 1, sw[c], 1, sx);
-        }
+        for (int c = 0; c < NT; ++c)
+          acc[m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wq[1][c], xq[m & 1][1], acc[m][c], 4, 4, 1, sw[c], 1,
+                                                                       sx[m & 1]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 0);
       }
     } else {
       const uint2* wl = reinterpret_cast<const uint2*>(lw(buf));
       const uint8_t* sc = reinterpret_cast<const uint8_t*>(ls((s >> 1) & 1)) + 2 * (s & 1) + (lg >> 1);
-      bf16x8_t wv[NT][2];
+      bf16x8_t xv[2][2];
+      auto read = [&](int m, int j) {
+        const int r = wm + m * 16 + li;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) xv[j][k] = __builtin_bit_cast(bf16x8_t, x[slot8(r, lg * 2 + k)]);
+      };
+      uint2 q[NT];
+      uint32_t sb[NT];
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         const int r = wn + c * 16 + li;
-        const uint2 q = wl[slot2(r, lg >> 1) * 2 + (lg & 1)];
-        const float f = mx4_scale(sc[r * 4]);
-        wv[c][0] = mx4_bf16x8(q.x, f);
-        wv[c][1] = mx4_bf16x8(q.y, f);
+        q[c] = wl[slot2(r, lg >> 1) * 2 + (lg & 1)];
+        sb[c] = sc[r * 4];
+      }
+      read(0, 0);
+      bf16x8_t wv[NT][2];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const float f = mx4_scale(sb[c]);
+        wv[c][0] = mx4_bf16x8(q[c].x, f);
+        wv[c][1] = mx4_bf16x8(q[c].y, f);
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const int r = wm + m * 16 + li;
+        if (m + 1 < MT) read(m + 1, (m + 1) & 1);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bf16x8_t xv = __builtin_bit_cast(bf16x8_t, x[slot8(r, lg * 2 + k)]);
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int c = 0; c < NT; ++c)
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[c][k], xv, acc[m][c], 0, 0, 0);
-        }
+            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[c][k], xv[m & 1][k], acc[m][c], 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 0);
       }
     }
   };
 
+  // Step s + BUFS - 1 is requested when step s begins, into the buffer of step s - 1, which everyone has left by then.
   stage(0, 0);
+  if (BUFS == 3 && steps > 1) stage(1, 1);
+  int buf = 0;
   for (int s = 0; s < steps; ++s) {
-    wait_vmcnt_n<0>();   // this wavefront's copies of step s have landed
-    __syncthreads();     // everyone's have, and everyone is done with the buffer the next copies fill
-    if (s + 1 < steps) stage(s + 1, (s + 1) & 1);
-    multiply(s, s & 1);
+    // this wavefront's copies of step s have landed; with three buffers those of step s + 1 may be on their way
+    if constexpr (BOTH) {
+      wait_vmcnt_n<0>();
+    } else {
+      const int later = s + 1 < steps ? NX + (w < BN / 32) + ((s & 1) && w < BN / 64) : 0;
+      if (later == NX + 2) wait_vmcnt_n<NX + 2>();
+      else if (later == NX + 1) wait_vmcnt_n<NX + 1>();
+      else if (later == NX) wait_vmcnt_n<NX>();
+      else wait_vmcnt_n<0>();
+    }
+    lds_barrier();       // everyone's have
+    const int next = buf == 0 ? BUFS - 1 : buf - 1;
+    if (s + BUFS - 1 < steps) stage(s + BUFS - 1, next);
+    multiply(s, buf);
+    buf = buf == BUFS - 1 ? 0 : buf + 1;
   }
 
   // element (row n, col m) of an instruction tile is register n % 4 of lane (n / 4) * 16 + m

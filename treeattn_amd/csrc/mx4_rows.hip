@@ -78,9 +78,10 @@ __device__ __forceinline__ float squares8(const uint4& x, float mean) {
 // dword per step and column is a cache line's visit each: 2.3 of 16.5 us at 32 x 4096 x 16384); longer rows' are not.
 constexpr int kScales = 4096;
 
-// The slot of 16-byte vector c (of 16) of row r of a step's slice of X in LDS: the 16 lanes that read one vector of 16
-// rows touch all banks.
-__device__ __forceinline__ int x_slot(int r, int c) { return r * 256 + (c ^ (r & 15)) * 16; }
+// The slot of 16-byte vector c (of 16) of row r of a step's slice of X in LDS.  A 16-byte read is served 16 lanes at a time:
+// lanes 0-3 and 12-15 of one group of 16 with lanes 4-11 of the next; the groups read vectors four apart.  With rows 4-7
+// turned like 0-3 and rows 8-11 like 12-15 those 16 lanes touch every bank once.
+__device__ __forceinline__ int x_slot(int r, int c) { return r * 256 + (c ^ ((r & 3) | ((r >> 3) & 1) * 12)) * 16; }
 
 // MT 16-row tiles of X, CT 16-column tiles; LN: normalised on the way, SL: scales through LDS.
 template <int MT, int CT, bool LN, bool SL, int EPI>
