@@ -140,21 +140,23 @@ int ta_seg_attn8_fwd(const void* q, int dtype, int64_t qsb, int64_t qsh, int64_t
 
 /*
  * Rows of microscaled 4-bit floats (the OCP MX format, e2m1 values): blocks of 32 along a row share a scale
- * 2^(byte - 127); packed (rows, Kp / 2) bytes hold two values each, the lower index in the low half, and scale
- * (rows, Kp / 32) one byte per block, with Kp = K rounded up to a multiple of 128 (values past K are 0, and the scale
- * byte of a block that lies wholly past K is 0).
+ * 2^(byte - 127), two values a byte, the lower index in the low half.  Rows are kept as tiles of 16 rows by 128 values:
+ * with steps = ceil(K / 128), tile t * steps + s holds rows 16t .. 16t + 15 and values 128s .. 128s + 127 as 64 blocks of 16
+ * bytes, block l = 16g + r being values 128s + 32g .. of row 16t + r: packed has 1024 bytes a tile, ceil(rows / 16) * steps
+ * tiles.  The scale of that block is byte 256 * (t / 4 * steps + s) + 4 * l + t % 4 of scale, 256 bytes for each of
+ * ceil(rows / 64) * steps groups of four tiles.  Values past K and rows past the last are 0 with scale 0.
  *
  * ta_mx4_quant rounds x (rows, K; row stride ldx) to that form: byte - 127 = floor(log2 of the block's largest
  * magnitude) - 2, at least -127; values to nearest, ties to even, saturating at 6; byte 255 (NaN) for a block that
  * holds anything not finite.  values (row stride ldv, x's dtype; may be NULL) receives what the rounded form stands
- * for.
+ * for.  packed 16-byte, scale 4-byte aligned.
  */
 int ta_mx4_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int K, void* packed, uint8_t* scale, void* values,
                  int64_t ldv, void* stream);
 
 /*
- * Y[M, N] = epilogue(LN(X) . W^T), bf16, for weights W (N, K) in 4 bits (packed and scale as above, contiguous, packed
- * 16-byte and scale 4-byte aligned): the weights are exact in bf16, products are summed in float32, and the result is
+ * Y[M, N] = epilogue(LN(X) . W^T), bf16, for weights W (N, K) in 4 bits (packed and scale as above, packed 16-byte
+ * and scale 4-byte aligned): the weights are exact in bf16, products are summed in float32, and the result is
  * rounded once, after the epilogue (0 none, 1 GELU in the erf form, 2 R + product).  ln_w (K bf16): the rows of X are
  * normalised first (as ta_rowmm does, rounded to bf16); where that is not part of the product's launch it needs ws, 16-byte
  * aligned, of ta_mx4_rows_workspace_size bytes (0: none).  K a multiple of 32, X 16-byte aligned with rows of a multiple of

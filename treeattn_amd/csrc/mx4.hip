@@ -8,25 +8,25 @@
 namespace ta {
 namespace {
 
-// Eight consecutive values of a row per lane, four lanes per block.
+// A workgroup takes a tile after another: thread i eight values (i % 16) of row i / 16, four threads a block.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void mx4_quant_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int K,
-                                                        uint32_t* __restrict__ packed, uint8_t* __restrict__ scale,
-                                                        T* __restrict__ values, int64_t ldv) {
-  const int per = mx4_padded(K) / 8;   // groups of eight in a row
-  const int64_t total = rows * per;
-  const int64_t step = (int64_t)gridDim.x * 256;
-  // (total is a multiple of 16, so the four lanes of a block leave the loop together)
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += step) {
-    const int64_t row = i / per;
-    const int c0 = (int)(i - row * per) * 8;
-    const T* xr = x + row * ldx + c0;
+__global__ __launch_bounds__(256) void mx4_quant_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int steps,
+                                                        int64_t tiles, uint32_t* __restrict__ packed,
+                                                        uint8_t* __restrict__ scale, T* __restrict__ values, int64_t ldv) {
+  const int li = threadIdx.x / 16, j = threadIdx.x % 16;
+  const int64_t last = (rows - 1) / 16;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t rt = steps == 1 ? t : t / steps;
+    const int64_t row = rt * 16 + li;
+    const int c0 = (int)(t - rt * steps) * 128 + j * 8;
+    const bool in = row < rows;
+    const T* xr = x + (in ? row : 0) * ldx + c0;
     float f[8];
-    if (VEC && c0 + 8 <= K) {
+    if (VEC && in && c0 + 8 <= K) {
       load_row_g<T, 8>(xr, f);
     } else {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) f[u] = c0 + u < K ? to_f32(xr[u]) : 0.0f;
+      for (int u = 0; u < 8; ++u) f[u] = in && c0 + u < K ? to_f32(xr[u]) : 0.0f;
     }
     float a = 0.0f;
     bool bad = false;
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void mx4_quant_kernel(const T* __restrict__ x,
       bad |= !(fabsf(f[u]) < INFINITY);
     }
     a = bad ? INFINITY : a;
-    a = fmaxf(a, dpp_f<0xB1>(a));   // the four lanes of the block
+    a = fmaxf(a, dpp_f<0xB1>(a));   // the four threads of the block
     a = fmaxf(a, dpp_f<0x4E>(a));
     bad = !(a < INFINITY);
     int e = -127;
@@ -54,9 +54,15 @@ __global__ __launch_bounds__(256) void mx4_quant_kernel(const T* __restrict__ x,
       w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6] * inv, f[7] * inv, 1.0f, 3);
     }
     const uint32_t byte = bad ? 255u : (uint32_t)(e + 127);
-    packed[i] = w;
-    if ((i & 3) == 0) scale[i >> 2] = (uint8_t)byte;
-    if (values != nullptr) {
+    const int l = (j / 4) * 16 + li;   // the lane whose block this is
+    packed[t * 256 + l * 4 + j % 4] = w;
+    if (j % 4 == 0) {
+      uint8_t* sc = scale + ((rt >> 2) * steps + (t - rt * steps)) * 256 + l * 4;
+      sc[rt & 3] = (uint8_t)byte;
+      if (rt == last)
+        for (int i = (int)(rt & 3) + 1; i < 4; ++i) sc[i] = 0;   // the rest of the last group
+    }
+    if (values != nullptr && in) {
       const float s = mx4_scale(byte);
       f32x2_t v[4];
       v[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
@@ -83,17 +89,17 @@ __global__ __launch_bounds__(256) void mx4_quant_kernel(const T* __restrict__ x,
 template <typename T>
 int launch_quant(const void* x, int64_t ldx, int64_t rows, int K, void* packed, uint8_t* scale, void* values,
                  int64_t ldv, hipStream_t st) {
-  const int64_t groups = rows * (mx4_padded(K) / 8);
-  const int64_t want = (groups + 255) / 256;
-  const unsigned grid = (unsigned)(want < (1 << 20) ? want : (1 << 20));
+  const int steps = mx4_padded(K) / 128;
+  const int64_t tiles = (rows + 15) / 16 * steps;
+  const unsigned grid = (unsigned)(tiles < (1 << 20) ? tiles : (1 << 20));
   const int sz = (int)sizeof(T);
   const bool vec = (uintptr_t)x % 16 == 0 && (ldx * sz) % 16 == 0 &&
                    (values == nullptr || ((uintptr_t)values % 16 == 0 && (ldv * sz) % 16 == 0));
   if (vec)
-    hipLaunchKernelGGL((mx4_quant_kernel<T, true>), dim3(grid), dim3(256), 0, st, (const T*)x, ldx, rows, K,
+    hipLaunchKernelGGL((mx4_quant_kernel<T, true>), dim3(grid), dim3(256), 0, st, (const T*)x, ldx, rows, K, steps, tiles,
                        (uint32_t*)packed, scale, (T*)values, ldv);
   else
-    hipLaunchKernelGGL((mx4_quant_kernel<T, false>), dim3(grid), dim3(256), 0, st, (const T*)x, ldx, rows, K,
+    hipLaunchKernelGGL((mx4_quant_kernel<T, false>), dim3(grid), dim3(256), 0, st, (const T*)x, ldx, rows, K, steps, tiles,
                        (uint32_t*)packed, scale, (T*)values, ldv);
   return check_launch("mx4_quant_kernel");
 }

@@ -3,30 +3,30 @@
 // codes and scales as they are).  Sums are float32, the result is rounded once after the epilogue.
 //
 // A workgroup of eight wavefronts, two along M by four along N, computes a (32 MT) x (64 NT) tile; a wavefront MT x NT
-// instruction tiles of it.  K goes through LDS in steps of 256 (both in 4 bits) or 64 (bf16 X): 128 bytes a row of X,
-// copied straight from memory to LDS, the next step's copies in flight while a step is multiplied.  The weights are the
+// instruction tiles of it.  K goes through LDS in steps of 128 (both in 4 bits) or 64 (bf16 X), copied there straight from
+// memory, the copies of the next BUFS - 1 steps in flight.  Tiles of 4-bit rows are copied and read as they are, lane by
+// lane; of bf16 X the rows are, 128 bytes a step, turned so that LDS reads touch every bank once.  The weights are the
 // instructions' first operand, so a lane ends with four consecutive columns of one row.
 //
-// k inside a step is dealt so that a lane's operands lie together: with both in 4 bits, lane group g = lane / 16 takes
-// blocks 2g and 2g + 1 of the step's eight, so two scale bytes that lie together serve its two instructions; with bf16 X
-// it takes k = 16g .. 16g + 15, half a block (eight bytes of codes, one scale).  X and W agree, so any order is right.
-// Rows and columns past the last repeat it and are not stored; what a step has past K is read as zeros.
+// With bf16 X a lane takes half a block of weights a step (k = 16g .. 16g + 15 of the step's 64 for lane group g): eight
+// bytes of codes and one scale serve its two instructions.  Rows and tiles past the last repeat it and are not stored; what
+// a step has past K is read as zeros.
 #include "mx4.hpp"
 
 namespace ta {
 namespace {
 
 struct GemmArgs {
-  const char* X;         // rows of xb bytes
+  const char* X;         // bf16: rows of xb bytes; 4 bits: tiles
   int64_t xb;
-  const uint32_t* XS;    // 4-bit X: its scales, Kp / 128 dwords a row
-  const char* W;         // rows of Kp / 2 bytes
-  const uint32_t* S;
+  const uint8_t* XS;     // 4-bit X: its scales
+  const char* W;
+  const uint8_t* S;
   bf16_t* Y;
   int64_t ldy;
   const bf16_t* R;
   int64_t ldr;
-  int M, N, K, Kp;
+  int M, N, K, ks;       // ks: steps of 128 in a row
   int tm, tn;            // tiles along M and N
   int vec;               // Y and R take 8-byte accesses
 };
@@ -39,9 +39,6 @@ __device__ const uint4 kZeros = {0, 0, 0, 0};
 // 0-3 and 12-15 of one group of 16 with lanes 4-11 of the next; the groups read vectors two apart of rows that lie two to
 // a line of banks.  With this turn those 16 lanes touch every bank once.
 __device__ __forceinline__ int turn8(int r) { return ((r >> 1) & 1) | ((r >> 3) & 1) * 6; }
-__device__ __forceinline__ int slot8(int r, int c) { return r * 8 + (c ^ turn8(r)); }
-// Slot of vector c of row r in an array of rows of two, read in halves.
-__device__ __forceinline__ int slot2(int r, int c) { return r * 2 + (c ^ ((r >> 3) & 1)); }
 
 // Copies of 16 or 4 bytes a lane, from a uniform base plus a lane's byte offset (or a lane's own address) to consecutive
 // places in LDS.  Written as instructions because the compiler waits for every such copy before the next read of LDS, also
@@ -61,9 +58,84 @@ __device__ __forceinline__ void copy4(const void* base, uint32_t off, const void
                "s"(base)
                : "memory");
 }
-__device__ __forceinline__ void copy4(const void* src, const void* dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(src)
-               : "memory");
+
+// Workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles, in groups of eight rows of tiles, so
+// that what its workgroups share stays in its L2.
+__device__ __forceinline__ void tile_of(const GemmArgs& a, int& tm, int& tn) {
+  const int T = a.tm * a.tn, id = blockIdx.x, x = id & 7, q = T >> 3, r = T & 7;
+  const int t = x * q + (x < r ? x : r) + (id >> 3);
+  const int per = 8 * a.tn, g = t / per, gm = a.tm - g * 8 < 8 ? a.tm - g * 8 : 8;
+  tm = g * 8 + (t - g * per) % gm;
+  tn = (t - g * per) / gm;
+}
+
+// The epilogue of a wavefront's MT x NT instruction tiles from row m0 and column n0: element (column n, row m) of a tile is
+// register n % 4 of lane (n / 4) * 16 + m.  Rows go through LDS of the wavefront's own (16 of them at a time, 8 bytes more
+// apart than they are long) so that they are stored, and the residual read, in whole runs of 16 NT columns.
+template <int MT, int NT, int EPI>
+__device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4_t (&acc)[MT][NT], int m0, int n0, int li, int lg,
+                                           char* lds) {
+  constexpr int RB = NT * 32 + 8;                             // bytes of a row in LDS
+  constexpr int LR = NT * 4;                                  // lanes of a row, four columns each
+  const int lane = lg * 16 + li;
+  const int n = n0 + lane % LR * 4;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    char* buf = lds + (m & 1) * 16 * RB;
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = EPI == MX_EPI_GELU ? mx4_gelu(acc[m][c][i]) : acc[m][c][i];
+      if constexpr (EPI == MX_EPI_RESIDUAL) {                 // added before the one rounding: in place, not through LDS
+        const int row = m0 + m * 16 + li, nn = n0 + c * 16 + lg * 4;
+        if (row < a.M) {
+          const bf16_t* rr = a.R + (int64_t)row * a.ldr + nn;
+          if (a.vec && nn + 4 <= a.N) {
+            float g[4];
+            load_row<bf16_t, 4>(rr, g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] += g[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (nn + i < a.N) f[i] += to_f32(rr[i]);
+          }
+        }
+      }
+      *reinterpret_cast<uint2*>(buf + li * RB + c * 32 + lg * 8) = make_uint2(bf16_pack2(f[0], f[1]), bf16_pack2(f[2], f[3]));
+    }
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {                            // 64 / LR rows at a time
+      const int r = j * (64 / LR) + lane / LR;
+      const int row = m0 + m * 16 + r;
+      const uint2 v = *reinterpret_cast<const uint2*>(buf + r * RB + lane % LR * 8);
+      if (row < a.M) {
+        bf16_t* yr = a.Y + (int64_t)row * a.ldy + n;
+        if (a.vec && n + 4 <= a.N) {
+          *reinterpret_cast<uint2*>(yr) = v;
+        } else {
+          const bf16_t* e = reinterpret_cast<const bf16_t*>(&v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < a.N) yr[i] = e[i];
+        }
+      }
+    }
+    wave_sync();
+  }
+}
+
+// Waits until at most n of this wavefront's copies are on their way (n uniform, up to 15).
+__device__ __forceinline__ void wait_copies(int n) {
+  switch (n) {
+#define TA_WAIT(N) case N: wait_vmcnt_n<N>(); break;
+    TA_WAIT(1) TA_WAIT(2) TA_WAIT(3) TA_WAIT(4) TA_WAIT(5) TA_WAIT(6) TA_WAIT(7) TA_WAIT(8) TA_WAIT(9) TA_WAIT(10)
+    TA_WAIT(11) TA_WAIT(12) TA_WAIT(13) TA_WAIT(14) TA_WAIT(15)
+#undef TA_WAIT
+    default: wait_vmcnt_n<0>();
+  }
 }
 
 // 32 codes as the instruction's operand (which reads its first four registers for 4-bit values).
@@ -71,111 +143,140 @@ __device__ __forceinline__ i32x8_t codes(const uint4& q) {
   return i32x8_t{(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
 }
 
+// The instruction with byte wi of ws and byte xi of xs as scales (the bytes known when unrolled: they are part of it).
+__device__ __forceinline__ f32x4_t multiply4(const i32x8_t& w, const i32x8_t& x, const f32x4_t& c, int ws, int wi, int xs,
+                                             int xi) {
+#define TA_M4(A, B) \
+  if (wi == A && xi == B) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, A, ws, B, xs);
+  TA_M4(0, 0) TA_M4(0, 1) TA_M4(0, 2) TA_M4(0, 3) TA_M4(1, 0) TA_M4(1, 1) TA_M4(1, 2) TA_M4(1, 3)
+  TA_M4(2, 0) TA_M4(2, 1) TA_M4(2, 2) TA_M4(2, 3) TA_M4(3, 0) TA_M4(3, 1) TA_M4(3, 2)
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 3, ws, 3, xs);
+#undef TA_M4
+}
+
 template <bool BOTH, int MT, int NT>
 struct GemmTile {
   static constexpr int BM = 32 * MT, BN = 64 * NT;
-  static constexpr int STEP = BOTH ? 256 : 64;                // of K
-  static constexpr int XB = BM * 128;                         // LDS bytes of X a step
-  static constexpr int WB = BOTH ? BN * 128 : BN * 32;        // of W
-  static constexpr int SB = BOTH ? (BM + BN) * 8 : BN * 4;    // of scales (bf16 X: of two steps)
-  static constexpr int BUFS = BOTH ? 2 : 3;                   // steps in LDS
-  static constexpr int LDS = BUFS * (XB + WB) + 2 * SB;
+  static constexpr int XT = BM / 16, WT = BN / 16;            // 16-row tiles
+  static constexpr int XB = BOTH ? XT * 1024 : BM * 128;      // LDS bytes of a step: X
+  static constexpr int WB = WT * (BOTH ? 1024 : 512);         // W
+  static constexpr int SB = (BOTH ? XT + WT : WT) * 64;       // scales (bf16 X: of two steps), 256 of four tiles
+  static constexpr int BUFS = BOTH ? 4 : 3;
+  static constexpr int LDS = BUFS * (XB + WB) + (BOTH ? BUFS : 2) * SB;
 };
 
-template <bool BOTH, int MT, int NT, int EPI>
+// PAIRED (MT 8, NT 4): the wavefronts stand two to a SIMD, and the second of each pair (w >= 4) runs half a phase behind the
+// first, so that one multiplies (32 instructions, 512 cycles) while the other reads its next operands from LDS, makes bf16
+// of its weights and issues copies.  A barrier ends each phase.
+template <bool BOTH, int MT, int NT, bool PAIRED, int EPI>
 __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
   using G = GemmTile<BOTH, MT, NT>;
-  constexpr int BM = G::BM, BN = G::BN;
+  constexpr int BM = G::BM, BN = G::BN, XT = G::XT, WT = G::WT, BUFS = G::BUFS;
+  constexpr int NX = BOTH ? XT / 8 : BM / 64;                 // copies of X of a wavefront and step
+  constexpr int NSC = (BOTH ? XT + WT : WT) / 4;              // wavefronts that copy scales
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
   const int li = lane & 15, lg = lane >> 4;
-  const int wm = (w & 1) * 16 * MT, wn = (w >> 1) * 16 * NT;
-  // Workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles, in groups of eight rows of tiles,
-  // so that what its workgroups share stays in its L2.
+  const int wm = (w >> 2) * MT, wn = (w & 3) * NT;            // this wavefront's first tiles
   int m0, n0;
-  {
-    const int T = a.tm * a.tn, id = blockIdx.x, x = id & 7, q = T >> 3, r = T & 7;
-    const int t = x * q + (x < r ? x : r) + (id >> 3);
-    const int per = 8 * a.tn, g = t / per, gm = a.tm - g * 8 < 8 ? a.tm - g * 8 : 8;
-    m0 = (g * 8 + (t - g * per) % gm) * BM;
-    n0 = (t - g * per) / gm * BN;
-  }
-  const int kd = a.Kp / 128;                                  // scale dwords of a row
-  const int steps = BOTH ? (a.Kp + 255) / 256 : (a.K + 63) / 64;
+  tile_of(a, m0, n0);
+  m0 *= BM;
+  n0 *= BN;
+  const int steps = BOTH ? a.ks : (a.K + 63) / 64;
+  const int lastx = (a.M - 1) / 16 - m0 / 16, lastw = (a.N - 1) / 16 - n0 / 16;
 
-  // byte offsets, from the tile's first row, of what this lane copies
-  const char* xbase = a.X + (int64_t)m0 * a.xb;
-  const char* wbase = a.W + (int64_t)n0 * (a.Kp / 2);
-  constexpr int NX = BM * 8 / kGemmThreads;                   // copies of X a wavefront and step
-  constexpr int NW = BOTH ? BN * 8 / kGemmThreads : 1;
-  constexpr int NS = BOTH ? (BM + BN) * 2 / kGemmThreads : 1;
-  uint32_t xo[NX], wo[NW];
-  int xc[NX], wc[NW];
-#pragma unroll
-  for (int i = 0; i < NX; ++i) {
-    const int s = (i * 8 + w) * 64 + lane, r = s / 8;
-    xc[i] = (s % 8) ^ turn8(r);
-    xo[i] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (uint32_t)a.xb + xc[i] * 16;
-  }
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    const int s = (i * 8 + w) * 64 + lane;
-    const int r = BOTH ? s / 8 : s / 2;
-    wc[i] = BOTH ? (s % 8) ^ turn8(r) : (s % 2) ^ ((r >> 3) & 1);
-    wo[i] = (uint32_t)(n0 + r < a.N ? r : a.N - 1 - n0) * (uint32_t)(a.Kp / 2) + wc[i] * 16;
-  }
-  const char* xsc = reinterpret_cast<const char*>(a.XS) + (int64_t)m0 * kd * 4;   // scales, from the tile's first row
-  const char* wsc = reinterpret_cast<const char*>(a.S) + (int64_t)n0 * kd * 4;
-  uint32_t so[NS];
-  int sd[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    const int s = (i * 8 + w) * 64 + lane;
-    const int r = BOTH ? (s / 2 < BM ? s / 2 : s / 2 - BM) : s;
-    sd[i] = BOTH ? s & 1 : 0;
-    const int rr = BOTH && s / 2 < BM ? (m0 + r < a.M ? r : a.M - 1 - m0) : (n0 + r < a.N ? r : a.N - 1 - n0);
-    so[i] = (uint32_t)(rr * kd + sd[i]) * 4;
-  }
-  const bool ragged = BOTH ? (a.Kp & 255) != 0 : (a.K & 63) != 0;
-
-  constexpr int BUFS = G::BUFS;
   auto lx = [&](int buf) { return lds + buf * G::XB; };
   auto lw = [&](int buf) { return lds + BUFS * G::XB + buf * G::WB; };
   auto ls = [&](int buf) { return lds + BUFS * (G::XB + G::WB) + buf * G::SB; };
 
+  // what this wavefront copies: uniform bases, and lanes' byte offsets from them
+  const int64_t tstep = (int64_t)a.ks * 1024;                 // from a 16-row tile to the next
+  const char* xb;
+  uint32_t xo[NX];
+  int xc[NX];
+  if constexpr (BOTH) {
+    xb = a.X + (m0 / 16) * tstep;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) xo[i] = lane * 16;
+  } else {
+    xb = a.X + (int64_t)m0 * a.xb;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const int s = (i * 8 + w) * 64 + lane, r = s / 8;
+      xc[i] = (s % 8) ^ turn8(r);
+      xo[i] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (uint32_t)a.xb + xc[i] * 16;
+    }
+  }
+  const char* wb = a.W + (n0 / 16) * tstep;
+  uint32_t wo = lane * 16;
+  if constexpr (!BOTH) {                                      // half tiles 2w and 2w + 1
+    const int t = 2 * w + (lane >> 5);
+    wo = (uint32_t)(t < lastw ? t : lastw) * (uint32_t)(a.ks * 1024) + (lane & 31) * 16;
+  }
+  // scales of four tiles: wavefront w's group of them
+  const char* sb;
+  {
+    const bool x = BOTH && w < XT / 4;
+    const int g = BOTH && !x ? w - XT / 4 : w, l = (x ? lastx + m0 / 16 : lastw + n0 / 16) / 4 - (x ? m0 : n0) / 64;
+    sb = reinterpret_cast<const char*>(x ? a.XS : a.S) + ((int64_t)((x ? m0 : n0) / 64) + (g < l ? g : l)) * a.ks * 256;
+  }
+  const bool ragged = !BOTH && (a.K & 63) != 0;
+
   auto stage = [&](int s, int buf) {
-    const char* xs = xbase + (int64_t)s * 128;
-    const char* ws = wbase + (int64_t)s * (BOTH ? 128 : 32);
-    if (ragged && s == steps - 1) {
+    if constexpr (BOTH) {
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
-        const bool in = BOTH ? s * 8 + xc[i] < kd * 4 : s * 64 + xc[i] * 8 < a.K;
-        copy16(in ? (const void*)(xs + xo[i]) : (const void*)&kZeros, lx(buf) + (i * 8 + w) * 1024);
+        const int t = i * 8 + w;
+        copy16(xb + (t < lastx ? t : lastx) * tstep + (int64_t)s * 1024, xo[i], lx(buf) + t * 1024);
       }
-      if constexpr (BOTH) {
 #pragma unroll
-        for (int i = 0; i < NW; ++i)
-          copy16(s * 8 + wc[i] < kd * 4 ? (const void*)(ws + wo[i]) : (const void*)&kZeros, lw(buf) + (i * 8 + w) * 1024);
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const char* sb = (i * 8 + w) * 32 < BM ? xsc : wsc;
-          copy4(s * 2 + sd[i] < kd ? (const void*)(sb + s * 8 + so[i]) : (const void*)&kZeros, ls(buf) + (i * 8 + w) * 256);
-        }
+      for (int i = 0; i < WT / 8; ++i) {
+        const int t = i * 8 + w;
+        copy16(wb + (t < lastw ? t : lastw) * tstep + (int64_t)s * 1024, wo, lw(buf) + t * 1024);
       }
+      if (w < NSC) copy4(sb + (int64_t)s * 256, lane * 4, ls(buf) + w * 256);
     } else {
+      const char* xs = xb + (int64_t)s * 128;
+      if (ragged && s == steps - 1) {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) copy16(xs, xo[i], lx(buf) + (i * 8 + w) * 1024);
-      if constexpr (BOTH) {
+        for (int i = 0; i < NX; ++i)
+          copy16(s * 64 + xc[i] * 8 < a.K ? (const void*)(xs + xo[i]) : (const void*)&kZeros, lx(buf) + (i * 8 + w) * 1024);
+      } else {
 #pragma unroll
-        for (int i = 0; i < NW; ++i) copy16(ws, wo[i], lw(buf) + (i * 8 + w) * 1024);
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-          copy4(((i * 8 + w) * 32 < BM ? xsc : wsc) + s * 8, so[i], ls(buf) + (i * 8 + w) * 256);
+        for (int i = 0; i < NX; ++i) copy16(xs, xo[i], lx(buf) + (i * 8 + w) * 1024);
       }
+      if (w < WT / 2) copy16(wb + (int64_t)(s >> 1) * 1024 + (s & 1) * 512, wo, lw(buf) + w * 1024);
+      if ((s & 1) == 0 && w < NSC) copy4(sb + (int64_t)(s >> 1) * 256, lane * 4, ls((s >> 1) & 1) + w * 256);
     }
-    if constexpr (!BOTH) {
-      if (w < BN / 32) copy16(ws, wo[0], lw(buf) + w * 1024);
-      if ((s & 1) == 0 && w < BN / 64) copy4(wsc + (s >> 1) * 4, so[0], ls((s >> 1) & 1) + w * 256);
+  };
+  // copies of this wavefront in step s
+  auto copies = [&](int s) {
+    return BOTH ? NX + WT / 8 + (w < NSC) : NX + (w < WT / 2) + ((s & 1) == 0 && w < NSC);
+  };
+  // waits for the copies of every issued step before s; the last issued one is `end` - 1
+  auto wait = [&](int s, int end) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < BUFS - 1; ++i)
+      if (s + i < end) n += copies(s + i);
+    wait_copies(n);
+  };
+  auto phase = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // end of the operands' phase and of the instructions' phase
+  auto begin = [&]() {
+    if constexpr (PAIRED) {
+      phase();
+      __builtin_amdgcn_s_setprio(1);
+    }
+  };
+  auto finish = [&]() {
+    if constexpr (PAIRED) {
+      __builtin_amdgcn_s_setprio(0);
+      phase();
     }
   };
 
@@ -185,143 +286,87 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int c = 0; c < NT; ++c) acc[m][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // The operands of row tile m + 1 are read while the instructions of row tile m run.
-  auto multiply = [&](int s, int buf) {
-    const uint4* x = reinterpret_cast<const uint4*>(lx(buf));
-    if constexpr (BOTH) {
-      const uint4* wl = reinterpret_cast<const uint4*>(lw(buf));
-      const uint16_t* sc = reinterpret_cast<const uint16_t*>(ls(buf));
-      i32x8_t wq[2][NT];
-      int sw[NT];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const int r = wn + c * 16 + li;
-        sw[c] = sc[(BM + r) * 4 + lg];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) wq[k][c] = codes(wl[slot8(r, lg * 2 + k)]);
-      }
-      i32x8_t xq[2][2];
-      int sx[2];
-      auto read = [&](int m, int j) {
-        const int r = wm + m * 16 + li;
-        sx[j] = sc[r * 4 + lg];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) xq[j][k] = codes(x[slot8(r, lg * 2 + k)]);
-      };
-      read(0, 0);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m + 1 < MT) read(m + 1, (m + 1) & 1);
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-          acc[m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wq[0][c], xq[m & 1][0], acc[m][c], 4, 4, 0, sw[c], 0,
-                                                                       sx[m & 1]);
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-          acc[m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wq[1][c], xq[m & 1][1], acc[m][c], 4, 4, 1, sw[c], 1,
-                                                                       sx[m & 1]);
-        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 0);
-      }
-    } else {
-      const uint2* wl = reinterpret_cast<const uint2*>(lw(buf));
-      const uint8_t* sc = reinterpret_cast<const uint8_t*>(ls((s >> 1) & 1)) + 2 * (s & 1) + (lg >> 1);
-      bf16x8_t xv[2][2];
-      auto read = [&](int m, int j) {
-        const int r = wm + m * 16 + li;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) xv[j][k] = __builtin_bit_cast(bf16x8_t, x[slot8(r, lg * 2 + k)]);
-      };
-      uint2 q[NT];
-      uint32_t sb[NT];
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const int r = wn + c * 16 + li;
-        q[c] = wl[slot2(r, lg >> 1) * 2 + (lg & 1)];
-        sb[c] = sc[r * 4];
-      }
-      read(0, 0);
-      bf16x8_t wv[NT][2];
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const float f = mx4_scale(sb[c]);
-        wv[c][0] = mx4_bf16x8(q[c].x, f);
-        wv[c][1] = mx4_bf16x8(q[c].y, f);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m + 1 < MT) read(m + 1, (m + 1) & 1);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int c = 0; c < NT; ++c)
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[c][k], xv[m & 1][k], acc[m][c], 0, 0, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 0);
-      }
-    }
-  };
-
-  // Step s + BUFS - 1 is requested when step s begins, into the buffer of step s - 1, which everyone has left by then.
-  stage(0, 0);
-  if (BUFS == 3 && steps > 1) stage(1, 1);
+  for (int s = 0; s < BUFS - 1; ++s)
+    if (s < steps) stage(s, s);
+  if constexpr (PAIRED) {
+    wait(1, steps < BUFS - 1 ? steps : BUFS - 1);
+    phase();
+    if (w >= 4) phase();
+  }
   int buf = 0;
   for (int s = 0; s < steps; ++s) {
-    // this wavefront's copies of step s have landed; with three buffers those of step s + 1 may be on their way
-    if constexpr (BOTH) {
-      wait_vmcnt_n<0>();
-    } else {
-      const int later = s + 1 < steps ? NX + (w < BN / 32) + ((s & 1) && w < BN / 64) : 0;
-      if (later == NX + 2) wait_vmcnt_n<NX + 2>();
-      else if (later == NX + 1) wait_vmcnt_n<NX + 1>();
-      else if (later == NX) wait_vmcnt_n<NX>();
-      else wait_vmcnt_n<0>();
+    const int next = buf == 0 ? BUFS - 1 : buf - 1;           // the buffer of step s - 1, which everyone has left
+    const int ahead = s + BUFS - 1;
+    if constexpr (!PAIRED) {
+      wait(s + 1, ahead < steps ? ahead : steps);
+      phase();                                                // everyone's copies of step s have landed
+      if (ahead < steps) stage(ahead, next);
     }
-    lds_barrier();       // everyone's have
-    const int next = buf == 0 ? BUFS - 1 : buf - 1;
-    if (s + BUFS - 1 < steps) stage(s + BUFS - 1, next);
-    multiply(s, buf);
+    if constexpr (BOTH) {
+      const uint4* x = reinterpret_cast<const uint4*>(lx(buf)) + wm * 64 + lane;
+      const uint4* wl = reinterpret_cast<const uint4*>(lw(buf)) + wn * 64 + lane;
+      const int* sx = reinterpret_cast<const int*>(ls(buf)) + wm / 4 * 64 + lane;
+      const int sw = reinterpret_cast<const int*>(ls(buf))[(XT + wn) / 4 * 64 + lane] >> (NT < 4 ? wn % 4 * 8 : 0);
+      i32x8_t wq[NT], xq[MT];
+      int fx[MT / 4];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) wq[c] = codes(wl[c * 64]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xq[m] = codes(x[m * 64]);
+#pragma unroll
+      for (int m = 0; m < MT / 4; ++m) fx[m] = sx[m * 64];
+      if constexpr (PAIRED) {
+        if (ahead < steps) stage(ahead, next);
+        if (s + 1 < steps) wait(s + 2, ahead < steps ? ahead + 1 : steps);
+      }
+      begin();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+          acc[m][c] = multiply4(wq[c], xq[m], acc[m][c], sw, c, fx[m / 4], m % 4);
+      finish();
+    } else {
+      const uint4* x = reinterpret_cast<const uint4*>(lx(buf)) + (wm * 16 + li) * 8;
+      const uint2* wl = reinterpret_cast<const uint2*>(lw(buf)) + wn * 64 + ((lg >> 1) * 16 + li) * 2 + (lg & 1);
+      const uint32_t sw = reinterpret_cast<const uint32_t*>(ls((s >> 1) & 1))[wn / 4 * 64 + (2 * (s & 1) + (lg >> 1)) * 16 + li] >>
+                          (NT < 4 ? wn % 4 * 8 : 0);
+      uint2 q[NT];
+      float f[NT];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        q[c] = wl[c * 64];
+        f[c] = mx4_scale_of(sw, c);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        bf16x8_t wv[NT], xv[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xv[m] = __builtin_bit_cast(bf16x8_t, x[m * 128 + ((lg * 2 + k) ^ turn8(li))]);
+#pragma unroll
+        for (int c = 0; c < NT; ++c) wv[c] = mx4_bf16x8(k ? q[c].y : q[c].x, f[c]);
+        if constexpr (PAIRED) {
+          if (k == 0 && ahead < steps) stage(ahead, next);
+          if (k == 1 && s + 1 < steps) wait(s + 2, ahead < steps ? ahead + 1 : steps);
+        }
+        begin();
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[c], xv[m], acc[m][c], 0, 0, 0);
+        finish();
+      }
+    }
     buf = buf == BUFS - 1 ? 0 : buf + 1;
   }
-
-  // element (row n, col m) of an instruction tile is register n % 4 of lane (n / 4) * 16 + m
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int row = m0 + wm + m * 16 + li;
-    if (row >= a.M) continue;
-    bf16_t* yr = a.Y + (int64_t)row * a.ldy;
-    const bf16_t* rr = a.R + (int64_t)row * a.ldr;
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      const int n = n0 + wn + c * 16 + lg * 4;
-      float f[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = acc[m][c][i];
-      if constexpr (EPI == MX_EPI_GELU) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = mx4_gelu(f[i]);
-      }
-      if (a.vec && n + 4 <= a.N) {
-        if constexpr (EPI == MX_EPI_RESIDUAL) {
-          float g[4];
-          load_row<bf16_t, 4>(rr + n, g);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] += g[i];
-        }
-        *reinterpret_cast<uint2*>(yr + n) = make_uint2(bf16_pack2(f[0], f[1]), bf16_pack2(f[2], f[3]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (n + i >= a.N) break;
-          if constexpr (EPI == MX_EPI_RESIDUAL) f[i] += to_f32(rr[n + i]);
-          yr[n + i] = bf16_from(f[i]);
-        }
-      }
-    }
-  }
+  if (PAIRED && w < 4) phase();
+  __syncthreads();                                            // everyone has left the operands' LDS
+  store_tile<MT, NT, EPI>(a, acc, m0 + wm * 16, n0 + wn * 16, li, lg, lds + w * 32 * (NT * 32 + 8));
 }
 
-template <bool BOTH, int MT, int NT>
+template <bool BOTH, int MT, int NT, bool PAIRED>
 int launch_tile(GemmArgs a, int epilogue, hipStream_t st) {
   using G = GemmTile<BOTH, MT, NT>;
   a.tm = (a.M + G::BM - 1) / G::BM;
@@ -329,13 +374,13 @@ int launch_tile(GemmArgs a, int epilogue, hipStream_t st) {
   const dim3 grid((unsigned)(a.tm * a.tn)), blk(kGemmThreads);
   switch (epilogue) {
     case MX_EPI_NONE:
-      hipLaunchKernelGGL((mx4_gemm_kernel<BOTH, MT, NT, MX_EPI_NONE>), grid, blk, G::LDS, st, a);
+      hipLaunchKernelGGL((mx4_gemm_kernel<BOTH, MT, NT, PAIRED, MX_EPI_NONE>), grid, blk, G::LDS, st, a);
       break;
     case MX_EPI_GELU:
-      hipLaunchKernelGGL((mx4_gemm_kernel<BOTH, MT, NT, MX_EPI_GELU>), grid, blk, G::LDS, st, a);
+      hipLaunchKernelGGL((mx4_gemm_kernel<BOTH, MT, NT, PAIRED, MX_EPI_GELU>), grid, blk, G::LDS, st, a);
       break;
     default:
-      hipLaunchKernelGGL((mx4_gemm_kernel<BOTH, MT, NT, MX_EPI_RESIDUAL>), grid, blk, G::LDS, st, a);
+      hipLaunchKernelGGL((mx4_gemm_kernel<BOTH, MT, NT, PAIRED, MX_EPI_RESIDUAL>), grid, blk, G::LDS, st, a);
       break;
   }
   return check_launch("mx4_gemm_kernel");
@@ -344,23 +389,23 @@ int launch_tile(GemmArgs a, int epilogue, hipStream_t st) {
 template <bool BOTH>
 int launch_gemm(GemmArgs a, int epilogue, hipStream_t st) {
   // offsets inside a tile and tile counts are 32-bit
-  if (a.xb * 256 > 0xffffffffLL || (int64_t)a.Kp * 128 > 0xffffffffLL ||
+  if ((!BOTH && a.xb * 256 > 0xffffffffLL) || a.ks > 65536 ||
       (int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128) > 0x7fffffffLL) {
-    set_error("mx4 product: too large (rows of X of at most 16 MiB apart)");
+    set_error("mx4 product: too large (K of at most 8388608, rows of X of at most 16 MiB apart)");
     return TA_ERR_UNSUPPORTED;
   }
   a.vec = a.ldy % 4 == 0 && (uintptr_t)a.Y % 8 == 0 && (a.R == nullptr || (a.ldr % 4 == 0 && (uintptr_t)a.R % 8 == 0));
   const int64_t big = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
-  if (big * 4 >= (int64_t)device_cus() * 3) return launch_tile<BOTH, 8, 4>(a, epilogue, st);
-  return launch_tile<BOTH, 4, 2>(a, epilogue, st);
+  if (big * 4 >= (int64_t)device_cus() * 3) return launch_tile<BOTH, 8, 4, true>(a, epilogue, st);
+  return launch_tile<BOTH, 4, 2, false>(a, epilogue, st);
 }
 
 }  // namespace
 
 int mx4_gemm_bf16(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,
                   int64_t ldr, int M, int N, int K, int epilogue, hipStream_t st) {
-  GemmArgs a{(const char*)X, ldx * 2, nullptr, (const char*)Wp, (const uint32_t*)Ws, (bf16_t*)Y, ldy, (const bf16_t*)R,
-             ldr, M, N, K, mx4_padded(K), 0, 0, 0};
+  GemmArgs a{(const char*)X, ldx * 2, nullptr, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N, K,
+             mx4_padded(K) / 128, 0, 0, 0};
   return launch_gemm<false>(a, epilogue, st);
 }
 
@@ -381,7 +426,7 @@ extern "C" int ta_mx4_both(const void* Xp, const uint8_t* Xs, const void* Wp, co
     set_error("ta_mx4_both: packed rows must be 16-byte aligned, scales 4-byte aligned");
     return TA_ERR_ARG;
   }
-  GemmArgs a{(const char*)Xp, mx4_padded(K) / 2, (const uint32_t*)Xs, (const char*)Wp, (const uint32_t*)Ws, (bf16_t*)Y,
-             ldy, (const bf16_t*)R, ldr, M, N, K, mx4_padded(K), 0, 0, 0};
+  GemmArgs a{(const char*)Xp, 0, Xs, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N, K,
+             mx4_padded(K) / 128, 0, 0, 0};
   return launch_gemm<true>(a, epilogue, (hipStream_t)stream);
 }

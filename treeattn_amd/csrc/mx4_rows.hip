@@ -2,8 +2,8 @@
 //   Y[M, N] = epilogue(LN(X)[M, K] . W[N, K]^T), M <= 64.
 //
 // The step is bound by the weights' bytes (17 of 32 a value), so they go straight from memory to the registers that the
-// conversion reads: a lane of v_mfma_f32_16x16x32_bf16 takes row lane % 16 of W and 32 consecutive values of it (one
-// block, 16 bytes, one scale), and the four instructions over them take eight each.  The order of k inside a block of
+// conversion reads, a tile of 16 columns and 128 of K a load: a lane of v_mfma_f32_16x16x32_bf16 takes one block (16 bytes,
+// one scale) of one column, and the four instructions over the tile take eight values of it each.  The order of k inside a block of
 // 128 is thus (i, lane / 16, 8): X is read from LDS in the same order.  Dequantised weights are exact in bf16, so the
 // product is that of the bf16 rows with the values the 4 bits stand for, summed in float32.
 //
@@ -28,8 +28,8 @@ namespace {
 struct RowsArgs {
   const bf16_t* X;
   int64_t ldx;
-  const uint4* W;        // blocks of 32: row n's at W + n * (Kp / 32)
-  const uint32_t* S;     // four scale bytes each: row n's at S + n * (Kp / 128)
+  const char* W;         // tiles of 1024 bytes
+  const uint8_t* S;      // scales, 256 bytes for four tiles one below the other
   bf16_t* Y;
   int64_t ldy;
   const bf16_t* R;
@@ -74,17 +74,13 @@ __device__ __forceinline__ float squares8(const uint4& x, float mean) {
   return q;
 }
 
-// Scales of a workgroup's columns that fit this many dwords are read once, whole rows at a time, into LDS (a lane's own
-// dword per step and column is a cache line's visit each: 2.3 of 16.5 us at 32 x 4096 x 16384); longer rows' are not.
-constexpr int kScales = 4096;
-
 // The slot of 16-byte vector c (of 16) of row r of a step's slice of X in LDS.  A 16-byte read is served 16 lanes at a time:
 // lanes 0-3 and 12-15 of one group of 16 with lanes 4-11 of the next; the groups read vectors four apart.  With rows 4-7
 // turned like 0-3 and rows 8-11 like 12-15 those 16 lanes touch every bank once.
 __device__ __forceinline__ int x_slot(int r, int c) { return r * 256 + (c ^ ((r & 3) | ((r >> 3) & 1) * 12)) * 16; }
 
-// MT 16-row tiles of X, CT 16-column tiles; LN: normalised on the way, SL: scales through LDS.
-template <int MT, int CT, bool LN, bool SL, int EPI>
+// MT 16-row tiles of X, CT 16-column tiles; LN: normalised on the way.
+template <int MT, int CT, bool LN, int EPI>
 __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) {
   constexpr int R = MT * 16;
   constexpr int COLS = 16 * CT;
@@ -98,29 +94,25 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
   const int st0 = w * per;                       // this wavefront's steps: st0 .. st0 + mine - 1
   const int mine = ks - st0 < per ? (ks > st0 ? ks - st0 : 0) : per;
 
-  // Byte offsets from the workgroup's first column and row (what lies past the last repeats it and is not stored); a
-  // step's are 64 bytes of a weight row, 256 of a row of X.
-  const char* wbase = reinterpret_cast<const char*>(a.W) + (int64_t)n0 * ks * 64;
-  const uint32_t* sbase = a.S + (int64_t)n0 * ks;
-  const char* xbase = reinterpret_cast<const char*>(a.X) + (int64_t)m0 * a.ldx * 2;
-  uint32_t so[CT], wo[CT], xo[MT * 4];
+  // tiles of columns past the last repeat the last tile, rows of X the last row; they are not stored
+  const int last = (a.N - 1) / 16;
+  int64_t wt[CT];                                // each tile's first
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    so[c] = (uint32_t)(n0 + c * 16 + li < a.N ? c * 16 + li : a.N - 1 - n0) * (uint32_t)ks;
-    wo[c] = so[c] * 64 + lg * 16;
-  }
+  for (int c = 0; c < CT; ++c) wt[c] = (int64_t)(n0 / 16 + c < last ? n0 / 16 + c : last) * ks;
+  const uint8_t* sw = a.S + (int64_t)(n0 / 64) * ks * 256 + lane * 4 + n0 / 16 % 4;
+  const char* xbase = reinterpret_cast<const char*>(a.X) + (int64_t)m0 * a.ldx * 2;
+  uint32_t xo[MT * 4];
 #pragma unroll
   for (int t = 0; t < MT * 4; ++t) {
     const int r = t * 4 + lg;
     xo[t] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (uint32_t)(a.ldx * 2) + li * 16;
   }
   const bool ragged = (a.K & 127) != 0;
-  // this wavefront's step i: column li of each tile of the weights, block lg of the step's four; rows lg, lg + 4, ... of
-  // X's slice, vector li of each
+  // this wavefront's step i: its tiles of the weights; rows lg, lg + 4, ... of X's slice, vector li of each
   struct Step {
     uint4 x[LN ? 1 : MT * 4];
     uint4 q[CT];
-    uint32_t s[CT];
+    uint32_t s;                                  // the tiles' scales, a byte each
   };
   auto load = [&](int i, Step& v) {
     const int st = st0 + i;
@@ -138,30 +130,12 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
         for (int t = 0; t < MT * 4; ++t) v.x[t] = ldg16(xs + xo[t]);
       }
     }
-    const char* ws = wbase + (int64_t)st * 64;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      v.q[c] = ldg16(ws + wo[c]);
-      if constexpr (!SL) v.s[c] = sbase[so[c] + st];
-    }
+    for (int c = 0; c < CT; ++c) v.q[c] = ldg16(a.W + (wt[c] + st) * 1024 + lane * 16);
+    const uint8_t* ss = sw + (int64_t)st * 256;
+    v.s = CT == 4 ? *reinterpret_cast<const uint32_t*>(ss) : CT == 2 ? *reinterpret_cast<const uint16_t*>(ss) : *ss;
   };
 
-  uint32_t* s_sc = reinterpret_cast<uint32_t*>(lds + (LN ? kFused * 2 : kWaves8 * XB));
-  constexpr int NS = kScales / kThreads;
-  uint32_t sv[NS];
-  const int ns = (a.N - n0 < COLS ? a.N - n0 : COLS) * ks;
-  if constexpr (SL) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (i * kThreads < ns) sv[i] = sbase[i * kThreads + tid < ns ? i * kThreads + tid : ns - 1];
-  }
-  auto keep_scales = [&]() {
-    if constexpr (SL) {
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        if (i * kThreads < ns) s_sc[i * kThreads + tid] = sv[i];
-    }
-  };
   Step va, vb;
   if constexpr (LN) {
     // row r of the workgroup's by G lanes, eight vectors each at most
@@ -197,8 +171,7 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
     if (mine > 0) load(0, va);
     if (mine > 1) load(1, vb);
   }
-  keep_scales();
-  if constexpr (LN || SL) lds_barrier();
+  if constexpr (LN) lds_barrier();
 
   f32x4_t acc[MT][CT];
 #pragma unroll
@@ -216,10 +189,7 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
     }
     float sc[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      if constexpr (SL) sc[c] = mx4_scale(reinterpret_cast<const uint8_t*>(s_sc + so[c] + st0 + i)[lg]);
-      else sc[c] = mx4_scale((v.s[c] >> (8 * lg)) & 255u);
-    }
+    for (int c = 0; c < CT; ++c) sc[c] = mx4_scale_of(v.s, c);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       bf16x8_t ax[MT];
@@ -321,11 +291,7 @@ int launch_one(const RowsArgs& a, hipStream_t st) {
   constexpr int x = LN ? kFused * 2 : kWaves8 * R * 256, red = kWaves8 * R * (COLS + 1) * 4;
   const int ny = (a.M + R - 1) / R;
   const dim3 grid((unsigned)((a.N + COLS - 1) / COLS * ny)), blk(kThreads);
-  if (COLS * (a.Kp / 128) <= kScales)
-    hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, LN, true, EPI>), grid, blk, x + kScales * 4 > red ? x + kScales * 4 : red,
-                       st, a, ny);
-  else
-    hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, LN, false, EPI>), grid, blk, x > red ? x : red, st, a, ny);
+  hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, LN, EPI>), grid, blk, x > red ? x : red, st, a, ny);
   return check_launch("mx4_rows_kernel");
 }
 
@@ -378,7 +344,7 @@ extern "C" int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uin
     return TA_ERR_ARG;
   }
   hipStream_t st = (hipStream_t)stream;
-  RowsArgs a{(const bf16_t*)X, ldx, (const uint4*)Wp, (const uint32_t*)Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr,
+  RowsArgs a{(const bf16_t*)X, ldx, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr,
              (const bf16_t*)ln_w, ln_eps, M, N, K, mx4_padded(K)};
   if (ln_w != nullptr && !norm_fused(M, K)) {
     const int64_t need = ta_mx4_rows_workspace_size(M, K, 1);

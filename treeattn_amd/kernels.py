@@ -1118,36 +1118,56 @@ def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, 
 # ----------------------------------------------------------------------------------------------- 4-bit rows
 class Mx4:
     """Rows of microscaled 4-bit floats (the OCP MX format with e2m1 values): blocks of 32 along a row share a scale
-    2^(byte - 127), byte 255 meaning NaN.  packed (rows, Kp / 2) uint8, the value of the lower index in the low half;
-    scale (rows, Kp / 32) uint8; Kp is K rounded up to a multiple of 128, the values past K being 0."""
+    2^(byte - 127), byte 255 meaning NaN.  Mx4(packed, scale, K) takes them row by row: packed (rows, Kp / 2) uint8, the
+    value of the lower index in the low half, and scale (rows, Kp / 32) uint8, with Kp = K rounded up to a multiple of 128
+    and zeros past K; the attributes packed and scale give that form back.  They are kept as the products read them, in
+    tiles of 16 rows by 128 values: tiles (row tiles, Kp / 128, 4, 16, 16), the blocks of a tile's 16 rows one after
+    another, and tile_scale (row tiles / 4, Kp / 128, 4, 16, 4), the scales of four tiles one below the other together; rows
+    past the last are zeros."""
 
     def __init__(self, packed, scale, K):
-        Kp = (int(K) + 127) // 128 * 128
+        K = int(K)
+        Kp = (K + 127) // 128 * 128
         if (K < 1 or packed.dtype != torch.uint8 or scale.dtype != torch.uint8 or packed.dim() != 2
-                or packed.shape[1] != Kp // 2 or scale.shape != (packed.shape[0], Kp // 32)
-                or not packed.is_contiguous() or not scale.is_contiguous()):
-            raise ValueError('Mx4: contiguous uint8 packed (rows, Kp / 2) and scale (rows, Kp / 32), Kp = K rounded up to '
-                             'a multiple of 128')
+                or packed.shape[1] != Kp // 2 or scale.shape != (packed.shape[0], Kp // 32)):
+            raise ValueError('Mx4: uint8 packed (rows, Kp / 2) and scale (rows, Kp / 32), Kp = K rounded up to a multiple '
+                             'of 128')
         self.index = L.device_index(packed)
         _on('Mx4', self.index, scale)
-        self.packed, self.scale, self.K = packed, scale, int(K)
-        self.shape, self.device = (packed.shape[0], int(K)), packed.device
+        M = packed.shape[0]
+        # one allocation, the tiles and then their scales
+        self._hold(torch.zeros(self._bytes(M, K), dtype=torch.uint8, device=packed.device), M, K, self.index)
+        rows = torch.arange(M, device=packed.device)
+        self.tiles.transpose(2, 3).transpose(1, 2)[rows // 16, rows % 16] = packed.view(M, Kp // 128, 4, 16)
+        self.tile_scale.permute(0, 4, 3, 1, 2)[rows // 64, rows // 16 % 4, rows % 16] = scale.view(M, Kp // 128, 4)
 
-    @classmethod
-    def _of(cls, packed, scale, rows, K, index):
-        """An Mx4 of tensors made here, without the checks."""
-        w = object.__new__(cls)
-        w.packed, w.scale, w.K, w.shape, w.device, w.index = packed, scale, K, (rows, K), packed.device, index
-        return w
+    @staticmethod
+    def _bytes(M, K):
+        return ((K + 127) // 128) * ((M + 15) // 16 * 1024 + (M + 63) // 64 * 256)
+
+    def _hold(self, buf, M, K, index):
+        S, T = (K + 127) // 128, (M + 15) // 16
+        self.tiles = buf.as_strided((T, S, 4, 16, 16), (S * 1024, 1024, 256, 16, 1))
+        self.tile_scale = buf.as_strided(((M + 63) // 64, S, 4, 16, 4), (S * 256, 256, 64, 4, 1), T * S * 1024)
+        self.at, self.scale_at = buf.data_ptr(), buf.data_ptr() + T * S * 1024
+        self.K, self.shape, self.device, self.index, self._buf = K, (M, K), buf.device, index, buf
+
+    @property
+    def packed(self):
+        return self.tiles.permute(0, 3, 1, 2, 4).flatten(2).flatten(0, 1)[:self.shape[0]]
+
+    @property
+    def scale(self):
+        return self.tile_scale.permute(0, 4, 3, 1, 2).flatten(3).flatten(0, 2)[:self.shape[0]]
 
     def values(self, dtype=torch.float32):
         """What the rows stand for, (rows, K)."""
+        packed, scale = self.packed, self.scale
         grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], device=self.device)
-        code = torch.stack((self.packed & 15, self.packed >> 4), -1).flatten(-2)
+        code = torch.stack((packed & 15, packed >> 4), -1).flatten(-2)
         v = grid[(code & 7).long()]
         v = torch.where(code >= 8, -v, v).view(self.shape[0], -1, 32)
-        e = self.scale.long() - 127
-        s = torch.where(self.scale == 255, float('nan'), ((e + 1023) << 52).view(torch.float64))
+        s = torch.where(scale == 255, float('nan'), ((scale.long() - 127 + 1023) << 52).view(torch.float64))
         return (v * s.unsqueeze(-1)).flatten(-2)[:, :self.K].to(dtype)
 
 
@@ -1167,15 +1187,10 @@ def mx4_quant(x, values=False):
     ld, one = x.stride()
     if K < 1 or (K > 1 and one != 1):
         raise ValueError('mx4_quant: rows (M, K) with contiguous rows, K at least 1')
-    Kp = (K + 127) // 128 * 128
-    # one allocation: the packed rows, then their scales
-    buf = torch.empty(M * (Kp // 2 + Kp // 32), dtype=torch.uint8, device=x.device)
-    packed = buf.as_strided((M, Kp // 2), (Kp // 2, 1))
-    scale = buf.as_strided((M, Kp // 32), (Kp // 32, 1), M * (Kp // 2))
+    w = object.__new__(Mx4)
+    w._hold(torch.empty(Mx4._bytes(M, K), dtype=torch.uint8, device=x.device), M, K, dev)
     v = torch.empty(M, K, dtype=x.dtype, device=x.device) if values else None
-    _mx4_quant(dev, x.data_ptr(), L.dtype_code(x), ld, M, K, packed.data_ptr(), scale.data_ptr(),
-               v.data_ptr() if values else None, K)
-    w = Mx4._of(packed, scale, M, K, dev)
+    _mx4_quant(dev, x.data_ptr(), L.dtype_code(x), ld, M, K, w.at, w.scale_at, v.data_ptr() if values else None, K)
     return (w, v) if values else w
 
 
@@ -1209,9 +1224,9 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     if isinstance(x, Mx4):
         if ln_w is not None:
             raise ValueError('mx4_mm: the LayerNorm prologue takes bf16 rows')
-        _on('mx4_mm', dev, x.packed)
-        _mx4_both(dev, x.packed.data_ptr(), x.scale.data_ptr(), w.packed.data_ptr(), w.scale.data_ptr(), out.data_ptr(),
-                  ldo, rp, ldr, M, N, K, epi)
+        if x.index != dev:
+            raise ValueError('mx4_mm: x and w must be on one device')
+        _mx4_both(dev, x.at, x.scale_at, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, M, N, K, epi)
         return out
     ldx, one = x.stride()
     if x.dtype != torch.bfloat16 or one != 1:
@@ -1226,8 +1241,8 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
         nbytes = L.lib().ta_mx4_rows_workspace_size(M, K, 1)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-    _mx4_rows(dev, x.data_ptr(), ldx, w.packed.data_ptr(), w.scale.data_ptr(), out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K,
-              epi, ws.data_ptr() if nbytes else None, nbytes)
+    _mx4_rows(dev, x.data_ptr(), ldx, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K, epi,
+              ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
