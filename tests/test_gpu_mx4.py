@@ -117,7 +117,8 @@ def close(got, y, tol):
 
 ROWS = [(1, 1, 32), (1, 100, 96), (2, 16, 128), (5, 1024, 1024), (16, 33, 160), (17, 130, 2080), (32, 768, 768), (31, 17, 4096),
         (33, 300, 512), (64, 65, 1056), (32, 16400, 256), (8, 16500, 1152), (50, 16384, 544), (65, 40, 96), (128, 128, 128),
-        (129, 257, 416), (300, 1000, 1024), (511, 129, 2016)]
+        (129, 257, 416), (300, 1000, 1024), (511, 129, 2016),
+        (200, 16500, 96), (1111, 4095, 160), (2100, 2050, 224)]
 
 
 @pytest.mark.parametrize('M,N,Kd', ROWS)
@@ -144,7 +145,8 @@ def test_layernorm_of_rows_far_from_zero(M, Kd):
 
 
 @pytest.mark.parametrize('M,N,Kd', [(1, 1, 1), (1, 130, 33), (3, 16, 128), (64, 64, 100), (65, 200, 160), (128, 128, 256),
-                                    (130, 257, 1000), (500, 1025, 2049), (17, 5000, 384)])
+                                    (130, 257, 1000), (500, 1025, 2049), (17, 5000, 384), (3500, 3600, 130),
+                                    (4096, 3333, 520)])
 @pytest.mark.parametrize('epilogue', [None, 'gelu', 'residual'])
 def test_both(M, N, Kd, epilogue):
     a, av = K.mx4_quant(rnd(M, Kd, seed=1).to(DEV), values=True)

@@ -127,12 +127,13 @@ __device__ __forceinline__ void store_tile(const GemmArgs& a, const f32x4_t (&ac
   }
 }
 
-// Waits until at most n of this wavefront's copies are on their way (n uniform, up to 15).
+// Waits until at most n of this wavefront's copies are on their way (n uniform, up to 24).
 __device__ __forceinline__ void wait_copies(int n) {
   switch (n) {
 #define TA_WAIT(N) case N: wait_vmcnt_n<N>(); break;
     TA_WAIT(1) TA_WAIT(2) TA_WAIT(3) TA_WAIT(4) TA_WAIT(5) TA_WAIT(6) TA_WAIT(7) TA_WAIT(8) TA_WAIT(9) TA_WAIT(10)
-    TA_WAIT(11) TA_WAIT(12) TA_WAIT(13) TA_WAIT(14) TA_WAIT(15)
+    TA_WAIT(11) TA_WAIT(12) TA_WAIT(13) TA_WAIT(14) TA_WAIT(15) TA_WAIT(16) TA_WAIT(17) TA_WAIT(18) TA_WAIT(19)
+    TA_WAIT(20) TA_WAIT(21) TA_WAIT(22) TA_WAIT(23) TA_WAIT(24)
 #undef TA_WAIT
     default: wait_vmcnt_n<0>();
   }
@@ -161,8 +162,9 @@ struct GemmTile {
   static constexpr int XB = BOTH ? XT * 1024 : BM * 128;      // LDS bytes of a step: X
   static constexpr int WB = WT * (BOTH ? 1024 : 512);         // W
   static constexpr int SB = (BOTH ? XT + WT : WT) * 64;       // scales (bf16 X: of two steps), 256 of four tiles
-  static constexpr int BUFS = BOTH ? 4 : 3;
-  static constexpr int LDS = BUFS * (XB + WB) + (BOTH ? BUFS : 2) * SB;
+  static constexpr int BUFS = BOTH ? 4 : 3;   // (six for MT 4: 256 x 4096 x 16384 54 -> 59 us, one workgroup a unit)
+  static constexpr int SBUFS = BOTH ? BUFS : 2;
+  static constexpr int LDS = BUFS * (XB + WB) + SBUFS * SB;
 };
 
 // PAIRED (MT 8, NT 4): the wavefronts stand two to a SIMD, and the second of each pair (w >= 4) runs half a phase behind the
@@ -222,31 +224,40 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
   }
   const bool ragged = !BOTH && (a.K & 63) != 0;
 
-  auto stage = [&](int s, int buf) {
-    if constexpr (BOTH) {
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
+  // copy i of step s by this wavefront (i known when unrolled): those of X, of W, of scales
+  constexpr int NC = NX + (BOTH ? WT / 8 : 1) + 1;
+  auto copy = [&](int s, int buf, int i, bool tail) {
+    if (i < NX) {
+      if constexpr (BOTH) {
         const int t = i * 8 + w;
         copy16(xb + (t < lastx ? t : lastx) * tstep + (int64_t)s * 1024, xo[i], lx(buf) + t * 1024);
-      }
-#pragma unroll
-      for (int i = 0; i < WT / 8; ++i) {
-        const int t = i * 8 + w;
-        copy16(wb + (t < lastw ? t : lastw) * tstep + (int64_t)s * 1024, wo, lw(buf) + t * 1024);
-      }
-      if (w < NSC) copy4(sb + (int64_t)s * 256, lane * 4, ls(buf) + w * 256);
-    } else {
-      const char* xs = xb + (int64_t)s * 128;
-      if (ragged && s == steps - 1) {
-#pragma unroll
-        for (int i = 0; i < NX; ++i)
-          copy16(s * 64 + xc[i] * 8 < a.K ? (const void*)(xs + xo[i]) : (const void*)&kZeros, lx(buf) + (i * 8 + w) * 1024);
       } else {
-#pragma unroll
-        for (int i = 0; i < NX; ++i) copy16(xs, xo[i], lx(buf) + (i * 8 + w) * 1024);
+        const char* xs = xb + (int64_t)s * 128;
+        char* dst = lx(buf) + (i * 8 + w) * 1024;
+        if (tail)                                              // what lies past K is zeros
+          copy16(s * 64 + xc[i] * 8 < a.K ? (const void*)(xs + xo[i]) : (const void*)&kZeros, dst);
+        else
+          copy16(xs, xo[i], dst);
       }
-      if (w < WT / 2) copy16(wb + (int64_t)(s >> 1) * 1024 + (s & 1) * 512, wo, lw(buf) + w * 1024);
-      if ((s & 1) == 0 && w < NSC) copy4(sb + (int64_t)(s >> 1) * 256, lane * 4, ls((s >> 1) & 1) + w * 256);
+    } else if (i < NC - 1) {
+      if constexpr (BOTH) {
+        const int t = (i - NX) * 8 + w;
+        copy16(wb + (t < lastw ? t : lastw) * tstep + (int64_t)s * 1024, wo, lw(buf) + t * 1024);
+      } else if (w < WT / 2) {
+        copy16(wb + (int64_t)(s >> 1) * 1024 + (s & 1) * 512, wo, lw(buf) + w * 1024);
+      }
+    } else if (w < NSC) {
+      if constexpr (BOTH) copy4(sb + (int64_t)s * 256, lane * 4, ls(buf) + w * 256);
+      else if ((s & 1) == 0) copy4(sb + (int64_t)(s >> 1) * 256, lane * 4, ls((s >> 1) % G::SBUFS) + w * 256);
+    }
+  };
+  auto stage = [&](int s, int buf) {
+    if (ragged && s == steps - 1) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) copy(s, buf, i, true);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) copy(s, buf, i, false);
     }
   };
   // copies of this wavefront in step s
@@ -316,21 +327,29 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
       for (int m = 0; m < MT; ++m) xq[m] = codes(x[m * 64]);
 #pragma unroll
       for (int m = 0; m < MT / 4; ++m) fx[m] = sx[m * 64];
-      if constexpr (PAIRED) {
-        if (ahead < steps) stage(ahead, next);
-        if (s + 1 < steps) wait(s + 2, ahead < steps ? ahead + 1 : steps);
-      }
+      if (PAIRED && s + 1 < steps) wait(s + 2, ahead < steps ? ahead : steps);
       begin();
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int c = 0; c < NT; ++c)
           acc[m][c] = multiply4(wq[c], xq[m], acc[m][c], sw, c, fx[m / 4], m % 4);
+        if constexpr (PAIRED) {
+          // a copy of step `ahead` between two row tiles' instructions, where issuing it costs nothing (as a phase of its own
+          // with the LDS reads it cost 12 of 86 us at 4096 x 4096 x 8192; with bf16 X, whose copies are a smaller part, the
+          // same move lost 2 of 57 us at 2001 x 2048 x 8192)
+          if (m < NC && ahead < steps) {
+            __builtin_amdgcn_sched_barrier(0);
+            copy(ahead, next, m, false);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
       finish();
     } else {
       const uint4* x = reinterpret_cast<const uint4*>(lx(buf)) + (wm * 16 + li) * 8;
       const uint2* wl = reinterpret_cast<const uint2*>(lw(buf)) + wn * 64 + ((lg >> 1) * 16 + li) * 2 + (lg & 1);
-      const uint32_t sw = reinterpret_cast<const uint32_t*>(ls((s >> 1) & 1))[wn / 4 * 64 + (2 * (s & 1) + (lg >> 1)) * 16 + li] >>
+      const uint32_t sw = reinterpret_cast<const uint32_t*>(ls((s >> 1) % G::SBUFS))[wn / 4 * 64 + (2 * (s & 1) + (lg >> 1)) * 16 + li] >>
                           (NT < 4 ? wn % 4 * 8 : 0);
       uint2 q[NT];
       float f[NT];

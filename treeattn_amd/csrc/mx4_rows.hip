@@ -1,5 +1,5 @@
 // Few bf16 rows times 4-bit weights (a decode step's products), on the bf16 matrix instructions:
-//   Y[M, N] = epilogue(LN(X)[M, K] . W[N, K]^T), M <= 64.
+//   Y[M, N] = epilogue(LN(X)[M, K] . W[N, K]^T).
 //
 // The step is bound by the weights' bytes (17 of 32 a value), so they go straight from memory to the registers that the
 // conversion reads, a tile of 16 columns and 128 of K a load: a lane of v_mfma_f32_16x16x32_bf16 takes one block (16 bytes,
@@ -282,6 +282,11 @@ __global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, bf16_t* 
         normalised(ldg16(xr + (int64_t)v * 8), ldg16(a.gam + (int64_t)v * 8), mean, rstd);
 }
 
+// Whether the product runs as workgroups of 32 rows or as tiles of many rows (mx4_gemm.hip).  The former cost about 8.5 us
+// at K = 4096 for every compute unit's worth of workgroups (512 x 4096 x 4096: 1024 of them, 36 us; 128 x 16384: 1024, 42 us;
+// 256 x 16384: 2048, 72 us), the latter's 128 x 128 tiles 50 us up to two for a unit.
+bool few_rows(int M, int N) { return M <= 64 || (int64_t)((M + 31) / 32) * ((N + 63) / 64) <= 5 * (int64_t)device_cus(); }
+
 // Whether ta_mx4_rows normalises M rows of K values within the product.
 bool norm_fused(int M, int K) { return M <= 64 && (int64_t)(M <= 16 ? 16 : 32) * mx4_padded(K) <= kFused; }
 
@@ -309,9 +314,9 @@ int launch_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
 // The widest workgroup (of 16, 32 or 64 columns) that still leaves every compute unit one: X is read once per workgroup.
 template <int MT>
 int pick_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
-  const int cus = device_cus();
-  if ((a.N + 63) / 64 >= cus) return launch_rows<MT, 4>(a, epilogue, st);
-  if ((a.N + 31) / 32 >= cus) return launch_rows<MT, 2>(a, epilogue, st);
+  const int cus = device_cus(), ny = (a.M + MT * 16 - 1) / (MT * 16);
+  if ((int64_t)((a.N + 63) / 64) * ny >= cus) return launch_rows<MT, 4>(a, epilogue, st);
+  if ((int64_t)((a.N + 31) / 32) * ny >= cus) return launch_rows<MT, 2>(a, epilogue, st);
   return launch_rows<MT, 1>(a, epilogue, st);
 }
 
@@ -359,6 +364,6 @@ extern "C" int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uin
     a.ldx = K;
     a.gam = nullptr;
   }
-  if (M > 64) return mx4_gemm_bf16(a.X, a.ldx, Wp, Ws, Y, ldy, R, ldr, M, N, K, epilogue, st);
+  if (!few_rows(M, N)) return mx4_gemm_bf16(a.X, a.ldx, Wp, Ws, Y, ldy, R, ldr, M, N, K, epilogue, st);
   return M <= 16 ? pick_rows<1>(a, epilogue, st) : pick_rows<2>(a, epilogue, st);
 }
