@@ -45,6 +45,47 @@ __host__ __device__ constexpr int list8_cap(int wl, int nb_S) { return ((wl + 3)
 // LDS words of a wavefront: per entry its first row, its leaf id and its two scales.
 __host__ __device__ constexpr int list8_ints(int cap) { return 4 * cap; }
 
+// The larger of x over the wavefront, in every lane.
+__device__ __forceinline__ float max64(float x) {
+  x = fmaxf(x, dpp_f<0xB1>(x));
+  x = fmaxf(x, dpp_f<0x4E>(x));
+  x = fmaxf(x, dpp_f<0x141>(x));
+  x = fmaxf(x, dpp_f<0x140>(x));
+  // (with one register in both places the exchange gives its halves, each spread over the lanes)
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum64(float x) {
+  x = group_sum<16>(x);
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// Sums of acc over the lanes that share lane % LPR.  Each exchange of halves leaves a lane half as many sums: lane l ends
+// with elements 8 * (l / 32) + 4 * (l / 16 % 2) + 0 .. 3 of its 16 in out, the same in all lanes of its 16 that share l % LPR.
+template <int LPR>
+__device__ __forceinline__ void sum_rows(float (&acc)[16], float (&out)[4]) {
+  float h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i]), __float_as_uint(acc[i + 8]), false, false);
+    h[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[i]), __float_as_uint(h[i + 4]), false, false);
+    float x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    if constexpr (LPR <= 8) x += dpp_f<0x128>(x);   // rotations within 16 lanes
+    if constexpr (LPR <= 4) x += dpp_f<0x124>(x);
+    if constexpr (LPR <= 2) x += dpp_f<0x122>(x);
+    if constexpr (LPR <= 1) x += dpp_f<0x121>(x);
+    out[i] = x;
+  }
+}
+
 // SPLIT: the four wavefronts of a workgroup, and p.gsplit workgroups, share one query; else a wavefront has a query of
 // its own.
 template <typename T, int D, bool SPLIT>
@@ -78,46 +119,69 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
   const int rg = lane / LPR;
   const int ds = (lane % LPR) * E;
 
-  float qv[E];
-  load_row_g<T, E>(reinterpret_cast<const T*>(p.q) + b * p.qsb + h * p.qsh + n * p.qsn + ds, qv);
-  int t = p.tq[b * p.tq_sb + n];
-  if (t < 0 || t >= c.tcap) t = -1;   // out of range: attend nothing
-  const int held = c.tail_block[b * c.tb_sb + h];
+  // everything whose place is known at once: the query, its position, the block in the tail, the selected leaves
   const int32_t* idr = p.ids + qi * p.wl;
   const uint8_t* vr = p.vld + qi * p.wl;
   const int32_t* trow = c.table + b * c.sb + h * c.sh;
-  int nv = 0;
-  for (int i0 = 0; i0 < p.wl; i0 += kWave) {
-    const int i = i0 + lane;
-    nv += __popcll(__ballot(i < p.wl && vr[i] != 0));
-  }
+  int t = p.tq[b * p.tq_sb + n];
+  const int held = c.tail_block[b * c.tb_sb + h];
   const int nt = p.n_tree ? p.n_tree[qi] : p.wl;
-  int nused = t < 0 ? 0 : (nv < nt ? nv : (nt > 0 ? nt : 0));
+  const int id0 = lane < p.wl ? idr[lane] : -1;
+  const bool v0 = lane < p.wl && vr[lane] != 0;
+  float qv[E];
+  load_row_g<T, E>(reinterpret_cast<const T*>(p.q) + b * p.qsb + h * p.qsh + n * p.qsn + ds, qv);
+
+  if (t < 0 || t >= c.tcap) t = -1;   // out of range: attend nothing
   const int own = t < 0 ? -1 : t >> c.blog2;
   const int lb = t < 0 ? 0 : own << c.blog2;
-
-  // An entry: block id, its page's first row and scales; row -1 where the block has no page, lies outside the table or
-  // is the one in the tail (whose keys are added from there).
-  auto entry = [&](int slot, int id, int row_in) {
+  const int tr = t & mask;
+  // Page reads: the first 64 leaves'; the static keys' [0, t, t-1, ..., t-Lw+1] by lanes 0 .. Lw and the own block's by lane
+  // Lw + 1.  The first row of the block's page, -1 where it has none, lies outside the table or is the one in the tail
+  // (whose keys are added from there).
+  auto first_row = [&](int id) {
     int row = -1;
-    float2 sc = make_float2(1.0f, 1.0f);
     if (id >= 0 && id < nblk && id != held) {
       const int pg = c.page(trow, id);
-      if (pg >= 0) {
-        row = (pg << (c.blog2 + 1)) + row_in;
-        sc = *reinterpret_cast<const float2*>(c.scale + 2 * (int64_t)pg);
-      }
+      if (pg >= 0) row = pg << (c.blog2 + 1);
     }
-    s_row[slot] = row;
-    s_id[slot] = id;
-    s_sc[slot] = sc;
+    return row;
   };
-  bool all = false;   // the tail's block is among the selected ones
-  for (int i0 = 0; i0 < nused; i0 += kWave) {
+  int pe = -1;
+  if (lane <= p.Lw && t >= 0) pe = lane == 0 ? 0 : t - (lane - 1);
+  const int pb = lane == p.Lw + 1 ? own : (pe >= 0 ? pe >> c.blog2 : -1);
+  const int row0 = first_row(id0);
+  const int srow = first_row(pb);
+
+  // The block in the tail: its first rows are requested here, behind the page reads.
+  const bool mine = held == own;
+  const int stride = SPLIT ? p.gsplit * kWaves : 1;
+  const int first = SPLIT ? g * kWaves + w : 0;
+  const int trows = t >= 0 && held >= 0 ? (mine ? tr + 1 : leaf) : 0;
+  const T* tk = reinterpret_cast<const T*>(c.tail) + b * c.tail_sb + h * c.tail_sh + ds;
+  float tkv[E], tvv[E];
+  auto load_tail = [&](int r) {
+    const int64_t rc = r < trows ? r : 0;
+    load_row_g<T, E>(tk + rc * D, tkv);
+    load_row_g<T, E>(tk + (int64_t)leaf * D + rc * D, tvv);
+  };
+  if (first * RPI < trows) load_tail(first * RPI + rg);
+
+  int nv = __popcll(__ballot(v0));
+  for (int i0 = kWave; i0 < p.wl; i0 += kWave) nv += __popcll(__ballot(i0 + lane < p.wl && vr[i0 + lane] != 0));
+  int nused = t < 0 ? 0 : (nv < nt ? nv : (nt > 0 ? nt : 0));
+  bool all = __ballot(lane < nused && id0 == held && held >= 0) != 0;   // the tail's block is among the selected ones
+  if (lane < nused) {
+    s_id[lane] = id0;
+    s_row[lane] = row0;
+  }
+  for (int i0 = kWave; i0 < nused; i0 += kWave) {
     const int i = i0 + lane;
     const int id = i < nused ? idr[i] : -1;
-    if (i < nused) entry(i, id, 0);
-    all |= __ballot(i < nused && id == held && id >= 0) != 0;
+    if (i < nused) {
+      s_id[i] = id;
+      s_row[i] = first_row(id);
+    }
+    all |= __ballot(i < nused && id == held && held >= 0) != 0;
   }
   wave_sync();
   if (p.nb_S > 0 && t >= 0) {
@@ -135,14 +199,16 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
       if (((cm >> s2) & 1) && s2 < lane && o == id) keep = false;
     }
     const uint64_t km = __ballot(keep);
-    if (keep) entry(nused + __popcll(km & ((1ull << lane) - 1)), id, 0);
+    if (keep) {
+      const int slot = nused + __popcll(km & ((1ull << lane) - 1));
+      s_id[slot] = id;
+      s_row[slot] = first_row(id);
+    }
     all |= __ballot(keep && id == held) != 0;
     nused += __popcll(km);
     wave_sync();
   }
-  // static keys [0, t, t-1, ..., t-Lw+1]: those >= 0, outside the own block, whose block is not used, the sink once
-  int pe = -1;
-  if (lane <= p.Lw && t >= 0) pe = lane == 0 ? 0 : t - (lane - 1);
+  // static keys: those >= 0, outside the own block, whose block is not used, the sink once
   bool keep = pe >= 0 && pe < lb && !(lane > 0 && pe == 0);
   if (keep) {
     const int lf = pe >> c.blog2;
@@ -152,8 +218,8 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
   const uint64_t bal = __ballot(keep);
   const int next = __popcll(bal);
   const int nblocks = nused + (t < 0 ? 0 : 1);   // the own block is the last of the blocks
-  if (keep) entry(nblocks + __popcll(bal & ((1ull << lane) - 1)), pe >> c.blog2, pe & mask);
-  if (t >= 0 && lane == 0) entry(nused, own, 0);
+  if (keep) s_row[nblocks + __popcll(bal & ((1ull << lane) - 1))] = srow < 0 ? -1 : srow + (pe & mask);
+  if (t >= 0 && lane == p.Lw + 1) s_row[nused] = srow;
   wave_sync();
   const int nl = nblocks << c.blog2;    // keys of the blocks (the own block's past t masked), then the static ones
   const int N8 = nl + next;
@@ -161,14 +227,10 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
   const char* kb = reinterpret_cast<const char*>(c.pool) + ds;
   const int64_t vofs = (int64_t)leaf * D;
   const int nchunks = (N8 + KPC - 1) / KPC;
-  const int stride = SPLIT ? p.gsplit * kWaves : 1;
-  const int first = SPLIT ? g * kWaves + w : 0;
-  const int tr = t & mask;
 
   struct Chunk {
     uint4 k[NL], v[NL];
-    float ks[NL], vs[NL];
-    bool ok[NL];
+    int e[NL];     // entry of the key, -1: none
   };
   auto fetch = [&](int ci, Chunk& x) {
     int row[NL];
@@ -179,16 +241,10 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
       const int kc = key < N8 ? key : 0;
       const int e = blk ? kc >> c.blog2 : (key < N8 ? nblocks + (kc - nl) : 0);
       const int rr = blk ? kc & mask : 0;
-      int r0 = -1;
-      float2 sc = make_float2(0.0f, 0.0f);
-      if (N8 > 0) {
-        r0 = s_row[e];
-        sc = s_sc[e];
-      }
-      x.ok[i] = key < N8 && r0 >= 0 && !(blk && e == nused && rr > tr);
-      row[i] = x.ok[i] ? r0 + rr : 0;
-      x.ks[i] = sc.x * p.scale;
-      x.vs[i] = sc.y;
+      const int r0 = N8 > 0 ? s_row[e] : -1;
+      const bool ok = key < N8 && r0 >= 0 && !(blk && e == nused && rr > tr);
+      x.e[i] = ok ? e : -1;
+      row[i] = ok ? r0 + rr : 0;
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -221,31 +277,69 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
       for (int d = 0; d < E; ++d) d0 = fmaf(qv[d], kv[d], d0);
       sc[i] = d0;
     }
-    float cm = kLowest;
+    float cm = kLowest, vs[NL];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      sc[i] = group_sum<LPR>(sc[i]) * x.ks[i];
-      if (x.ok[i]) cm = fmaxf(cm, sc[i]);
+      const float2 s = s_sc[x.e[i] < 0 ? 0 : x.e[i]];
+      sc[i] = group_sum<LPR>(sc[i]) * (s.x * p.scale);
+      vs[i] = s.y;
+      if (x.e[i] >= 0) cm = fmaxf(cm, sc[i]);
     }
     rescale(fmaxf(m, cm));
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const float pw = x.ok[i] ? __expf(sc[i] - m) : 0.0f;
+      const float pw = x.e[i] >= 0 ? __expf(sc[i] - m) : 0.0f;
       l += pw;
-      const float pv = x.ok[i] ? pw * x.vs[i] : 0.0f;
+      const float pv = pw * vs[i];
       float vv[E];
       e4m3_x16(x.v[i], vv);
-      if (x.ok[i]) {
+      if (x.e[i] >= 0) {
 #pragma unroll
         for (int d = 0; d < E; ++d) acc[d] = fmaf(pv, vv[d], acc[d]);
       }
     }
   };
 
+  // keys of the tail: all its rows when it is selected, those up to t when it is the own block, else its static keys
+  auto consume_tail = [&](int r) {
+    const int pos = (held << c.blog2) + r;
+    const bool ok = r < trows && (mine || all || (held < own && (pos == 0 || pos > t - p.Lw)));
+    float s = 0.0f;
+#pragma unroll
+    for (int d = 0; d < E; ++d) s = fmaf(qv[d], tkv[d], s);
+    s = group_sum<LPR>(s) * p.scale;
+    rescale(fmaxf(m, ok ? s : kLowest));
+    if (ok) {
+      const float pw = __expf(s - m);
+      l += pw;
+#pragma unroll
+      for (int d = 0; d < E; ++d) acc[d] = fmaf(pw, tvv[d], acc[d]);
+    }
+  };
+  auto tail = [&]() {
+    for (int r0 = first * RPI; r0 < trows; r0 += stride * RPI) {
+      if (r0 > first * RPI) load_tail(r0 + rg);
+      consume_tail(r0 + rg);
+    }
+  };
+
   if (nchunks > 0) {
+    // The entries' scales: requested with the first keys, so that they are no round trip of their own, and before them,
+    // since loads return in order (lists of more than 64 entries take the rest at once).
+    const int entries = nblocks + next;
+    auto scales = [&](int i) {
+      const int row = i < entries ? s_row[i] : -1;
+      return row >= 0 ? *reinterpret_cast<const float2*>(c.scale + 2 * (int64_t)(row >> (c.blog2 + 1)))
+                      : make_float2(0.0f, 0.0f);
+    };
+    for (int i = kWave + lane; i < entries; i += kWave) s_sc[i] = scales(i);
+    const float2 sc0 = scales(lane);
     Chunk x[PF];
 #pragma unroll
     for (int j = 0; j < PF; ++j) fetch(first + j * stride, x[j]);
+    if (lane < entries) s_sc[lane] = sc0;
+    tail();
+    wave_sync();
     for (int c0 = first; c0 < nchunks; c0 += PF * stride) {
 #pragma unroll
       for (int j = 0; j < PF; ++j) {
@@ -256,52 +350,20 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
     }
   }
 
-  // the block in the tail: all its rows when selected, those up to t when it is the own block, else its static keys
-  if (t >= 0 && held >= 0 && (held <= own || all)) {
-    const bool mine = held == own;
-    const T* tk = reinterpret_cast<const T*>(c.tail) + b * c.tail_sb + h * c.tail_sh + ds;
-    const int rows = mine ? tr + 1 : leaf;
-    for (int r0 = first * RPI; r0 < rows; r0 += stride * RPI) {
-      const int r = r0 + rg;
-      const int pos = (held << c.blog2) + r;
-      const bool ok = r < rows && (mine || all || pos == 0 || pos > t - p.Lw);
-      if (__ballot(ok) == 0) continue;
-      const int rc = ok ? r : 0;
-      float kv[E], vv[E];
-      load_row_g<T, E>(tk + (int64_t)rc * D, kv);
-      load_row_g<T, E>(tk + (int64_t)leaf * D + (int64_t)rc * D, vv);
-      float s = 0.0f;
-#pragma unroll
-      for (int d = 0; d < E; ++d) s = fmaf(qv[d], kv[d], s);
-      s = group_sum<LPR>(s) * p.scale;
-      rescale(fmaxf(m, ok ? s : kLowest));
-      if (ok) {
-        const float pw = __expf(s - m);
-        l += pw;
-#pragma unroll
-        for (int d = 0; d < E; ++d) acc[d] = fmaf(pw, vv[d], acc[d]);
-      }
-    }
-  }
-
   // bring the row groups to the wavefront's maximum and add them
-  {
-    const float M = wave_max(m);
-    rescale(M);
-  }
-  float L = wave_sum(lane % LPR == 0 ? l : 0.0f);
-#pragma unroll
-  for (int o = LPR; o < kWave; o <<= 1) {
-#pragma unroll
-    for (int d = 0; d < E; ++d) acc[d] += __shfl_xor(acc[d], o, kWave);
-  }
+  rescale(max64(m));
+  const float L = sum64(lane % LPR == 0 ? l : 0.0f);
+  float sums[4];
+  sum_rows<LPR>(acc, sums);
+  const bool holds = (lane & 15) < LPR;          // this lane's sums are elements de .. de + 3 of the row
+  const int de = ds + 8 * (lane >> 5) + 4 * ((lane >> 4) & 1);
   const float keys = t < 0 ? 0.0f : (float)((nused << c.blog2) + tr + 1 + next);
   T* orow = reinterpret_cast<T*>(p.out) + b * p.osb + h * p.osh + n * p.osn;
   if constexpr (!SPLIT) {
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-    if (rg == 0) {
+    if (holds) {
 #pragma unroll
-      for (int d = 0; d < E; ++d) orow[ds + d] = from_f32<T>(acc[d] * inv);
+      for (int i = 0; i < 4; ++i) orow[de + i] = from_f32<T>(sums[i] * inv);
     }
     if (lane == 0) {
       if (p.lse) p.lse[qi] = L != 0.0f ? m + __logf(L) : kNegBig;
@@ -311,9 +373,9 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
   }
   // the four wavefronts' partials through LDS (past the lists, so no wavefront's list is overwritten)
   float* red = smem_f + kWaves * list8_ints(cap);   // [4][D + 2]
-  if (rg == 0) {
+  if (holds) {
 #pragma unroll
-    for (int d = 0; d < E; ++d) red[w * (D + 2) + 2 + ds + d] = acc[d];
+    for (int i = 0; i < 4; ++i) red[w * (D + 2) + 2 + de + i] = sums[i];
   }
   if (lane == 0) {
     red[w * (D + 2)] = m;
@@ -367,9 +429,9 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
     ms = ldgf_dc(base + lane * (D + 2));
     Ls = ldgf_dc(base + lane * (D + 2) + 1);
   }
-  const float Mq = wave_max(Ls != 0.0f ? ms : kLowest);
+  const float Mq = max64(Ls != 0.0f ? ms : kLowest);
   const float fac = Ls != 0.0f ? __expf(ms - Mq) : 0.0f;
-  const float Lq = wave_sum(Ls * fac);
+  const float Lq = sum64(Ls * fac);
   const float inv = Lq != 0.0f ? 1.0f / Lq : 0.0f;
   float* s_fac = red;   // this wavefront has read its partials
   wave_sync();
