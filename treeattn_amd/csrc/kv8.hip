@@ -6,7 +6,6 @@
 // the same tokens one by one give the same bytes, and the node sums are those of the unrounded keys.  Scales are
 // powers of two: e4m3 has the same relative step over its whole range, so a scale that is up to twice too large
 // costs nothing but the lowest of its subnormals, and multiplying by it is exact.
-#include "append.hpp"
 #include "kv8.hpp"
 
 namespace ta {
@@ -82,7 +81,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8 c, const
                                                                     int64_t vnsb, int64_t vnsh, int H, int D,
                                                                     const int32_t* __restrict__ t_pos, LevelRW8 lv,
                                                                     int n_levels, int arity_log2) {
-  extern __shared__ float stk[];   // the carry stack [16][D]
+  extern __shared__ float stk[];   // carry stacks [16][threads]
   __shared__ float s_max[2][kAppendThreads / kWave];
   constexpr int VE = vec_elems<T>();
   const int tid = threadIdx.x;
@@ -123,51 +122,147 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8 c, const
   if (tid == 0) *tag = blk;
   if (r != leaf - 1) return;
 
-  // the block is whole: its scales, its page, then the nodes that end here
+  // The block is whole.  Its nodes' first level: thread (segment, d) sums an aligned run of rows of dimension d by adjacent
+  // pairs, and the runs are joined the same way -- the tree of sums ta_level_sums forms, so the same bits.  The loads of the
+  // runs and of the whole block are in flight together.
+  const int S = n_levels > 0 ? (kAppendThreads / D < leaf / 2 ? kAppendThreads / D : leaf / 2) : 0;   // runs
+  const int seg = tid / D, d = tid % D, run = S > 0 ? leaf / S : 0;
+  constexpr int U = 8;
+  float rv[U];
+  const bool sums = seg < S;
+  auto load_run = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r1 = seg * run + i0 + u;
+      rv[u] = i0 + u < run ? to_f32(tk[(int64_t)r1 * D + d]) : 0.0f;
+    }
+  };
+  if (sums) load_run(0);
   const int64_t nv = half / VE;
+  constexpr int R = 4;                          // vectors of K and of V a thread holds; larger blocks are read twice
+  float f[R][VE], g[R][VE];
   float m[2] = {0.0f, 0.0f};
-  for (int64_t i = tid; i < nv; i += kAppendThreads) {
-    float f[VE], g[VE];
-    load_vec<T>(tk + i * VE, f);
-    load_vec<T>(tv + i * VE, g);
+  auto amax = [&](const float (&x)[VE], const float (&y)[VE]) {
 #pragma unroll
     for (int u = 0; u < VE; ++u) {
-      m[0] = fmaxf(m[0], finite_abs(f[u]));
-      m[1] = fmaxf(m[1], finite_abs(g[u]));
+      m[0] = fmaxf(m[0], finite_abs(x[u]));
+      m[1] = fmaxf(m[1], finite_abs(y[u]));
     }
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int64_t v = (int64_t)i * kAppendThreads + tid;
+    if (v < nv) {
+      load_vec<T>(tk + v * VE, f[i]);
+      load_vec<T>(tv + v * VE, g[i]);
+    }
+  }
+  // run sums: a carry stack of the widths 1, 2, 4, ... below the run's length
+  float x = 0.0f;
+  if (sums) {
+    for (int i0 = 0; i0 < run; i0 += U) {
+      if (i0 > 0) load_run(i0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u;
+        if (i >= run) break;
+        x = (blk == 0 && seg == 0 && i == 0) ? 0.0f : rv[u];   // position 0 counts as zero
+        int lvl = 0;
+        while ((i >> lvl) & 1) {
+          x = __fadd_rn(stk[lvl * kAppendThreads + tid], x);
+          ++lvl;
+        }
+        stk[lvl * kAppendThreads + tid] = x;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if ((int64_t)i * kAppendThreads + tid < nv) amax(f[i], g[i]);
+  for (int64_t v = (int64_t)R * kAppendThreads + tid; v < nv; v += kAppendThreads) {
+    float y[VE], z[VE];
+    load_vec<T>(tk + v * VE, y);
+    load_vec<T>(tv + v * VE, z);
+    amax(y, z);
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     m[s] = wave_max(m[s]);
     if (lane_id() == 0) s_max[s][wave_id()] = m[s];
   }
-  __syncthreads();
+  __syncthreads();   // the stacks are done with too: a thread's run sum goes to slot tid
+  if (sums) stk[tid] = x;
   int e[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    float x = s_max[s][0];
+    float y = s_max[s][0];
 #pragma unroll
-    for (int w = 1; w < kAppendThreads / kWave; ++w) x = fmaxf(x, s_max[s][w]);
-    e[s] = e4m3_exponent(x);
+    for (int w = 1; w < kAppendThreads / kWave; ++w) y = fmaxf(y, s_max[s][w]);
+    e[s] = e4m3_exponent(y);
   }
-  for (int64_t i = tid; i < nv; i += kAppendThreads) {
-    float f[VE], g[VE];
-    load_vec<T>(tk + i * VE, f);
-    load_vec<T>(tv + i * VE, g);
-    store_e4m3<T>(page + i * VE, f, e[0]);
-    store_e4m3<T>(page + half + i * VE, g, e[1]);
+  __syncthreads();
+  // nodes: levels j >= 1 that end here need their children before the last, which are read together, eight levels at a time
+  if (tid < D && n_levels > 0) {
+    for (int w = 1; w < S; w *= 2)
+      for (int i = 0; i + w < S; i += 2 * w) stk[i * D + d] = __fadd_rn(stk[i * D + d], stk[(i + w) * D + d]);
+    x = stk[d];
+    auto level = [&](int j) { return lv.ptr[j] + b * lv.sb[j] + h * lv.sh[j]; };
+    level(0)[(int64_t)blk * D + d] = x;
+    const int arity = 1 << arity_log2;
+    int ends = 1;   // levels whose node ends at t
+    while (ends < n_levels && c.blog2 + ends * arity_log2 < 31 &&
+           ((t + 1) & ((1 << (c.blog2 + ends * arity_log2)) - 1)) == 0)
+      ++ends;
+    if (arity == 2) {
+      for (int j0 = 1; j0 < ends; j0 += 8) {
+        float sib[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          sib[u] = j0 + u < ends ? level(j0 + u - 1)[((int64_t)(t >> (c.blog2 + (j0 + u - 1))) - 1) * D + d] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (j0 + u >= ends) break;
+          x = __fadd_rn(sib[u], x);
+          level(j0 + u)[(int64_t)(t >> (c.blog2 + (j0 + u))) * D + d] = x;
+        }
+      }
+    } else {
+      for (int j = 1; j < ends; ++j) {
+        const int64_t node = t >> (c.blog2 + j * arity_log2);
+        const float* child = level(j - 1) + node * arity * D + d;
+        float kid[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) kid[k] = k < arity - 1 ? child[(int64_t)k * D] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (k == arity - 1) kid[k] = x;
+#pragma unroll
+        for (int w = 1; w < 16; w *= 2) {
+#pragma unroll
+          for (int k = 0; k + w < 16; k += 2 * w)
+            if (w < arity && k < arity) kid[k] = __fadd_rn(kid[k], kid[k + w]);
+        }
+        x = kid[0];
+        level(j)[node * D + d] = x;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int64_t v = (int64_t)i * kAppendThreads + tid;
+    if (v < nv) {
+      store_e4m3<T>(page + v * VE, f[i], e[0]);
+      store_e4m3<T>(page + half + v * VE, g[i], e[1]);
+    }
+  }
+  for (int64_t v = (int64_t)R * kAppendThreads + tid; v < nv; v += kAppendThreads) {
+    float y[VE], z[VE];
+    load_vec<T>(tk + v * VE, y);
+    load_vec<T>(tv + v * VE, z);
+    store_e4m3<T>(page + v * VE, y, e[0]);
+    store_e4m3<T>(page + half + v * VE, z, e[1]);
   }
   if (tid < 2) c.scale[2 * (int64_t)pg + tid] = ldexpf(1.0f, e[tid]);
-  if (tid < D && n_levels > 0) {
-    KvRows rows{};
-    rows.cst = D;
-    rows.blog2 = c.blog2;
-    const T* nk = kn + b * nsb + h * nsh;
-    // append_dim_with writes row t again (the value it holds) and forms the nodes from the tail's rows
-    append_dim_with<T>(tid, D, t, AppendPre<T>{nk[tid], vn[b * vnsb + h * vnsh + tid], (int64_t)r * D}, tk, tv, rows,
-                       n_levels, c.blog2, arity_log2, stk,
-                       [&](int j) { return lv.ptr[j] + b * lv.sb[j] + h * lv.sh[j]; });
-  }
 }
 
 // Prompts.  A unit is the K or the V rows of one leaf block of one (sequence, head); G lanes (a power of two up to the
@@ -310,7 +405,7 @@ extern "C" int ta_kv8_append(const void* k_new, const void* v_new, int dtype, in
     lv.sb[j] = lv_sb[j];
     lv.sh[j] = lv_sh[j];
   }
-  const size_t lds = (size_t)16 * D * sizeof(float);
+  const size_t lds = (size_t)16 * kAppendThreads * sizeof(float);
 #define TA_APPEND(TT)                                                                                             \
   hipLaunchKernelGGL((kv8_append_kernel<TT>), dim3((unsigned)(B * H)), dim3(kAppendThreads), lds, (hipStream_t)stream, c, \
                      (const TT*)k_new, (const TT*)v_new, nsb, nsh, vnsb, vnsh, H, D, t_pos, lv, n_levels, arity_log2)
