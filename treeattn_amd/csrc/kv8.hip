@@ -279,11 +279,12 @@ __global__ __launch_bounds__(256) void kv8_fill_kernel(Kv8 c, const T* __restric
   const int64_t unit = blockIdx.x * (int64_t)(256 / G) + tid / G;
   const int g = tid & (G - 1);
   const bool live = unit < units;
-  const int side = (int)(unit & 1);
-  const int64_t bj = live ? unit >> 1 : 0;
-  const int j = (int)(bj % nblk);
-  const int64_t bh = bj / nblk;
-  const int b = (int)(bh / H), h = (int)(bh % H);
+  // heads first, then keys and values: neighbours read what lies together in the output of a projection
+  const int64_t hs = live ? unit / H : 0;
+  const int h = live ? (int)(unit - hs * H) : 0;
+  const int side = (int)(hs & 1);
+  const int64_t bj = hs >> 1;
+  const int b = (int)(bj / nblk), j = (int)(bj - (int64_t)b * nblk);
   const int leaf = 1 << c.blog2;
   const int64_t half = (int64_t)leaf * D;
   int n = T_;
@@ -358,7 +359,9 @@ template <typename T>
 int launch_fill(const Kv8& c, const void* k, const void* v, int64_t ksb, int64_t ksh, int64_t kst, int64_t vsb,
                 int64_t vsh, int64_t vst, int B, int H, int T_, int D, const int32_t* lens, hipStream_t st) {
   const int64_t nv = ((int64_t)D << c.blog2) / vec_elems<T>();
-  const int G = nv < 256 ? (int)nv : 256;
+  // a wavefront a unit as long as eight vectors a lane hold it (64 keys of 64 bf16: 75.7 -> 56.6 us for 8 x 12 x 8191 against four
+  // wavefronts with two each), more lanes for larger blocks
+  const int G = nv <= 64 ? (int)nv : nv <= 512 ? 64 : nv < 2048 ? (int)(nv / 8) : 256;
   const int64_t R = nv / G;
   const int leaf = 1 << c.blog2;
   const int nblk = T_ > 0 ? (int)(((int64_t)T_ + leaf - 1) / leaf) : 1;
