@@ -6,6 +6,9 @@ and step(tok, t) -> (logits, keys), weights_from_ours / weights_from_nanogpt -- 
 
 * batch: SegState(..., batch=B) and Decoder(..., batch=B); step(tok: LongTensor(B), t) -> logits (B, V);
 * dtype: the caches take the weights' dtype (bf16 models keep bf16 K/V; node sums are always float32);
+* fewer bits: Decoder(..., cache='e4m3') holds K and V in 8-bit pages with one scale for a page's keys and one for its
+  values, the block being filled unrounded beside them (kernels.Cache8); weights_mx4(W) rounds the layers' weights to
+  microscaled 4-bit floats (kernels.Mx4), for a bf16 decoder;
 * tree shape: cfg.leaf / cfg.arity (the reference is leaf=2, arity=2);
 * paged caches: a Decoder keeps K and V in pages of one leaf block of one (sequence, head) (PagePool), handed
   out as positions are reached (max_tokens bounds the pool, not Tcap); a stand-alone SegState is contiguous;
@@ -41,14 +44,21 @@ class PagePool:
     as positions are reached (ensure, on the host, outside captured steps) and returned per sequence (release);
     the pool holds num_pages pages, so memory follows the tokens provisioned rather than Tcap."""
 
-    def __init__(self, B, H, dh, leaf, Tcap, num_pages, n_layers, dtype, dev):
+    def __init__(self, B, H, dh, leaf, Tcap, num_pages, n_layers, dtype, dev, cache=None):
+        """cache 'e4m3': pages of float8_e4m3fn with a (P, 2) float32 tensor of scales per layer."""
         self.B, self.H, self.leaf, self.Tcap, self.P = B, H, leaf, Tcap, int(num_pages)
         nblk = Tcap // leaf
         self.table = torch.full((B, H, nblk), -1, dtype=torch.int32, device=dev)
         self.host = torch.full((B, H, nblk), -1, dtype=torch.int32)
         self.nblk = [0] * B                        # leaf blocks of each sequence that have pages
         self.free = list(range(self.P - 1, -1, -1))   # pages handed out in increasing order
-        self.pools = [torch.zeros(self.P, 2, leaf, dh, dtype=dtype, device=dev) for _ in range(n_layers)]
+        if cache is None:
+            self.pools = [torch.zeros(self.P, 2, leaf, dh, dtype=dtype, device=dev) for _ in range(n_layers)]
+            self.scales = None
+        else:
+            self.pools = [torch.zeros(self.P, 2, leaf, dh, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+                          for _ in range(n_layers)]
+            self.scales = [torch.ones(self.P, 2, device=dev) for _ in range(n_layers)]
 
     def ensure(self, t_end, seqs=None):
         """Pages for positions < t_end (at most Tcap) of the given sequences (all by default): a sequence's
@@ -91,6 +101,14 @@ class PagePool:
     def cache(self, layer):
         return K.PagedCache(self.pools[layer], self.table, self.Tcap)
 
+    def cache8(self, layer, dtype):
+        """A layer's 8-bit cache, with a tail of its own in the model's dtype."""
+        B, H, dev = self.B, self.H, self.table.device
+        _, two, leaf, dh = self.pools[layer].shape
+        return K.Cache8(self.pools[layer], self.scales[layer], self.table,
+                        torch.zeros(B, H, two, leaf, dh, device=dev, dtype=dtype),
+                        torch.full((B, H), -1, dtype=torch.int32, device=dev), self.Tcap)
+
 
 class SegState:
     """Per-layer cache (engine.py:18-71): K, V in the model dtype -- contiguous (B,H,Tcap,dh), or the pages of a
@@ -105,7 +123,11 @@ class SegState:
         self.shape = SEL.cfg_shape(cfg, Tcap)
         self.Lm = self.shape.blevels[-1] if self.shape.n_levels else 0
         self.pages = pages
-        if pages is None:
+        self.cache8 = None
+        if pages is not None and pages.scales is not None:
+            self.cache8 = pages.cache8(layer, dtype)
+            self.cache = None
+        elif pages is None:
             self.K = torch.zeros(batch, H, Tcap, dh, device=dev, dtype=dtype)
             self.V = torch.zeros(batch, H, Tcap, dh, device=dev, dtype=dtype)
             self.cache = None
@@ -119,6 +141,12 @@ class SegState:
         if self.gated:
             self.lg = [torch.zeros_like(t) for t in self.levels]
             self.gl = [torch.zeros_like(t) if f else None for t, f in zip(self.levels, SEL.gated_flags(cfg, self.shape))]
+            if self.cache8 is not None:
+                # the tail as a cache whose every block is on the sequence's one page: what gate_append reads the block a
+                # position ends from
+                own = torch.arange(batch * H, dtype=torch.int32, device=dev).view(batch, H, 1)
+                self.tail_rows = K.PagedCache(self.cache8.tail.view(batch * H, 2, self.shape.leaf, dh),
+                                              own.expand(-1, -1, pages.table.shape[2]).contiguous(), Tcap)
         else:
             self.lg = self.gl = None
         NS = cfg.nb_store
@@ -136,12 +164,17 @@ class SegState:
     def dense_kv(self, b, t_end=None):
         """Contiguous (1, H, t_end, dh) K and V of sequence b (a copy when paged)."""
         t_end = self.Tcap if t_end is None else t_end
+        if self.cache8 is not None:
+            return self.cache8.dense(b, t_end)
         if self.cache is None:
             return self.K[b:b + 1, :, :t_end], self.V[b:b + 1, :, :t_end]
         return self.cache.dense(b, t_end)
 
     def row(self, t):
         """Row t of K and V for every sequence and head: (B, H, dh) copies."""
+        if self.cache8 is not None:
+            kv = [self.cache8.dense(b, t + 1) for b in range(self.B)]
+            return torch.cat([k[:, :, t] for k, _ in kv]), torch.cat([v[:, :, t] for _, v in kv])
         if self.cache is None:
             return self.K[:, :, t].clone(), self.V[:, :, t].clone()
         c = self.cache
@@ -153,6 +186,9 @@ class SegState:
     def write_rows(self, b0, k, v):
         """Store positions 0..T-1 of sequences b0.. from k, v (n, H, T, dh) (a prompt's keys and values)."""
         n, H, T, dh = k.shape
+        if self.cache8 is not None:
+            K.kv8_fill(k.to(self.dtype), v.to(self.dtype), self.cache8.rows(b0, b0 + n))
+            return
         if self.cache is None:
             self.K[b0:b0 + n, :, :T].copy_(k)
             self.V[b0:b0 + n, :, :T].copy_(v)
@@ -188,7 +224,7 @@ class SegState:
         """The gate's part of appending positions tpos (after kv_append): log sums and gated vectors of the
         nodes ending there (engine.py:47, 53-54)."""
         if self.gated and self.shape.n_levels:
-            Kc, _ = self.kv()
+            Kc = self.tail_rows if self.cache8 is not None else self.kv()[0]
             K.gate_append(Kc, tpos, self.levels, self.lg, self.gl, self.shape.blevels, self.shape.arity,
                           float(self.cfg.gate_q))
 
@@ -199,12 +235,18 @@ class SegState:
 
     def add(self, t, k, v):
         """Store position t (k, v: (B,H,dh)) and form the nodes it completes (engine.py:41-55)."""
-        Kc, Vc = self.kv()
         tpos = self._tpos(t)
-        K.kv_append(k.to(self.dtype), v.to(self.dtype), Kc, Vc, tpos, self.levels, self.shape.leaf,
-                    self.shape.arity)
+        self.append(k.to(self.dtype), v.to(self.dtype), tpos)
         self.gate_append(tpos)
         self.ksum += k.float()
+
+    def append(self, k, v, tpos):
+        """The cache's part of add (k, v in the cache dtype, tpos int32 (B,))."""
+        if self.cache8 is not None:
+            K.kv8_append(k, v, self.cache8, tpos, self.levels, self.shape.arity)
+        else:
+            Kc, Vc = self.kv()
+            K.kv_append(k, v, Kc, Vc, tpos, self.levels, self.shape.leaf, self.shape.arity)
 
     def rows(self, b0, b1):
         """A view of sequences b0..b1-1 of this cache (the tensors are shared, not copied)."""
@@ -216,6 +258,10 @@ class SegState:
                 setattr(v, name, getattr(self, name)[b0:b1])
         if self.cache is not None:
             v.cache = self.cache.rows(b0, b1)
+        if self.cache8 is not None:
+            v.cache8 = self.cache8.rows(b0, b1)
+            if self.gated:
+                v.tail_rows = self.tail_rows.rows(b0, b1)
         v.levels = [t[b0:b1] for t in self.levels]
         if self.gated:
             v.lg = [t[b0:b1] for t in self.lg]
@@ -272,6 +318,8 @@ class _Scratch:
         another on its stream.  In a decoder of at most ROWVEC_MAX_ROWS sequences (self.rowvec), products
         without a tail run ta_rowvec_bf16 instead: rowmm's arithmetic without matrix cores, whose 32-row tiles
         would compute 30 or more idle rows; results within one bf16 unit of rowmm's."""
+        if isinstance(w, K.Mx4):
+            return K.mx4_mm(x, w, **kw)
         M, Kd = x.shape
         if (self.rowvec and M <= ROWVEC_MAX_ROWS and not {'ln_next', 'tok_out', 'cols', 'splits'} & kw.keys()
                 and K.rowvec_bf16_supported(x, w)):
@@ -382,15 +430,25 @@ def seg_attend_(state, pw, q, k, v, t, update=True, scratch=None):
     lhat = None if head is not None else _pw_budget(state, pw, q, tpos, k=k[:, :, 0] if update else None)
     pooled = cfg.beam_mode == 'pred' and cfg.global_pool and update   # the head's launch adds k to ksum
     wl = state.shape.leaf_width(cfg.wmax)
+    c8 = state.cache8
     if scratch is None:
-        scratch = _Scratch(B, H, dh, wl, q.device, decode_nsplit(B, H, wl, leaf))
+        ns = decode_nsplit(B, H, wl, leaf) if c8 is None else decode_nsplit8(B, H, 1, wl, leaf)
+        scratch = _Scratch(B, H, dh, wl, q.device, ns)
     structural = (not cfg.neighbors) and cfg.beam_mode != 'pred'
     # the descent's launch also appends (row t and the nodes ending at t, which the descent does not read); with
     # the gate it scores the gated vectors while the append forms the raw sums, then the gate's log sums and gated
     # vectors of those nodes
-    appendable = update and B * H < 4096 and q.dtype == k.dtype == state.dtype
+    appendable = update and B * H < 4096 and q.dtype == k.dtype == state.dtype and c8 is None
     fused = structural and appendable and not state.gated
-    Kc, Vc = state.kv()
+    Kc, Vc = state.kv() if c8 is None else (None, None)
+
+    def attend(n_tree, out, nb=None):
+        if c8 is None:
+            K.seg_attn(q, Kc, Vc, tpos.view(B, 1), ids, vld, n_tree, leaf, cfg.local, scale, out=out, keys=scratch.keys,
+                       nsplit=scratch.nsplit, ws=scratch.ws, nb=nb)
+        else:
+            K.seg_attn8(q, c8, tpos.view(B, 1), ids, vld, n_tree, cfg.local, scale, out=out, keys=scratch.keys,
+                        nsplit=scratch.nsplit, ws=scratch.ws, nb=nb)
     if fused and scratch.nsplit == 4 and dh in (64, 128) and wl <= 64 and not cfg.global_pool:
         # append, descent and attention in one launch (one workgroup per (sequence, head))
         if scratch.n_tree is None:
@@ -415,7 +473,7 @@ def seg_attend_(state, pw, q, k, v, t, update=True, scratch=None):
     if structural:
         if update:
             if not appendable:
-                K.kv_append(k[:, :, 0], v[:, :, 0], Kc, Vc, tpos, state.levels, leaf, state.shape.arity)
+                state.append(k[:, :, 0], v[:, :, 0], tpos)
                 state.gate_append(tpos)
             if cfg.global_pool:
                 state.ksum += k[:, :, 0].float()
@@ -423,8 +481,7 @@ def seg_attend_(state, pw, q, k, v, t, update=True, scratch=None):
         if scratch.n_tree is None:
             scratch.n_tree = torch.full((B, H, 1), SEL.fixed_n_tree(cfg), dtype=torch.int32, device=q.device)
         n_tree = scratch.n_tree
-        K.seg_attn(q, Kc, Vc, tpos.view(B, 1), ids, vld, n_tree, leaf, cfg.local, scale, out=out,
-                   keys=scratch.keys, nsplit=scratch.nsplit, ws=scratch.ws)
+        attend(n_tree, out)
         return out, scratch.keys
     # reference-default mode: neighbour borrowing and/or the budget head.  The neighbour pass reads the store of
     # positions t-1 .. t-Wn and gives the budget split (engine.py:100-102, seg.py:111-117); the top nb_store
@@ -451,13 +508,12 @@ def seg_attend_(state, pw, q, k, v, t, update=True, scratch=None):
         n_tree = SEL.budget_split(torch.zeros_like(lhat.view(B, H, 1)), lhat.view(B, H, 1), cfg.wmax).to(torch.int32)
     if update:
         if not appendable:
-            K.kv_append(k[:, :, 0], v[:, :, 0], Kc, Vc, tpos, state.levels, leaf, state.shape.arity)
+            state.append(k[:, :, 0], v[:, :, 0], tpos)
             state.gate_append(tpos)
         if cfg.global_pool and not pooled:
             state.ksum += k[:, :, 0].float()
     out = torch.empty(B, H, 1, dh, device=q.device, dtype=state.dtype)
-    K.seg_attn(q, Kc, Vc, tpos.view(B, 1), ids, vld, n_tree, leaf, cfg.local, scale, out=out, keys=scratch.keys,
-               nsplit=scratch.nsplit, ws=scratch.ws, nb=(nid, match))
+    attend(n_tree, out, nb=(nid, match))
     return out, scratch.keys
 
 
@@ -496,14 +552,37 @@ def weights_from_nanogpt(sd, n_layer):
     return W
 
 
+_PRODUCTS = ('c_attn', 'c_proj', 'c_fc', 'c_mlp')
+
+
+def weights_mx4(W):
+    """An engine weight dict with every layer's four weight matrices rounded to microscaled 4-bit floats (kernels.Mx4);
+    embeddings (the output layer among them) and LayerNorm weights stay as they are.  For a bf16 Decoder."""
+    return dict(W, layers=[dict(L, **{n: K.mx4_quant(L[n]) for n in _PRODUCTS}) for L in W['layers']])
+
+
+def _product(x, w, ln_w=None, bits=None):
+    """LN(x) @ w.T of a prompt's rows x (..., K); w a matrix or an Mx4.  bits 4: the rows are rounded to Mx4 as well."""
+    if not isinstance(w, K.Mx4):
+        return F.linear(x if ln_w is None else _ln(x, ln_w), w)
+    rows = x.reshape(-1, x.shape[-1])
+    if bits == 4:
+        y = K.mx4_mm(K.mx4_quant(rows if ln_w is None else _ln(rows, ln_w)), w)
+    else:
+        y = K.mx4_mm(rows, w, ln_w=ln_w)
+    return y.view(*x.shape[:-1], y.shape[-1])
+
+
 class Decoder:
     """Layer loop around seg_attend (engine.py:149-177), batched and graph-capturable."""
 
     def __init__(self, W, n_layer, n_head, n_embd, Tcap, mode, cfg=None, dev='cuda', batch=1, dtype=None,
-                 groups=None, one_launch=None, attn_split=None, paged=None, max_tokens=None, reserve_ahead=256):
+                 groups=None, one_launch=None, attn_split=None, paged=None, max_tokens=None, reserve_ahead=256,
+                 cache=None):
         """paged (default: on, except for the one-launch step, which takes contiguous caches): K and V in pages
         of a PagePool sized for max_tokens positions per sequence (default Tcap); pages are handed out as
-        positions are reached, reserve_ahead positions at a time for captured steps."""
+        positions are reached, reserve_ahead positions at a time for captured steps.  cache: None (K and V in the model's
+        dtype) or 'e4m3' (8-bit pages, kernels.Cache8; paged caches only)."""
         self.W, self.nl, self.H, self.C, self.Tcap = W, n_layer, n_head, n_embd, Tcap
         self.dh, self.mode, self.cfg, self.dev = n_embd // n_head, mode, cfg, torch.device(dev)
         self.B = batch
@@ -511,15 +590,23 @@ class Decoder:
         self.dtype = dtype or W['wte'].dtype
         self.graph = None
         # the fused row-block kernels serve bf16 models whose widths are multiples of 64
+        mx4 = [isinstance(L[n], K.Mx4) for L in W['layers'] for n in _PRODUCTS]
+        self.mx4 = any(mx4)
         self.fused = (mode == 'seg' and self.dtype == torch.bfloat16 and n_embd % 64 == 0
-                      and all(L['c_attn'].dtype == torch.bfloat16 for L in W['layers'])
-                      and all(W['layers'][0][n].is_contiguous() for n in ('c_attn', 'c_proj', 'c_fc', 'c_mlp')))
+                      and (self.mx4 or (all(L['c_attn'].dtype == torch.bfloat16 for L in W['layers'])
+                                        and all(W['layers'][0][n].is_contiguous() for n in _PRODUCTS))))
+        if self.mx4 and not (all(mx4) and self.fused):
+            raise ValueError('Mx4 weights: all four matrices of every layer, in a bf16 seg decoder whose width is a '
+                             'multiple of 64')
+        if cache not in (None, 'e4m3'):
+            raise ValueError("cache: None or 'e4m3'")
+        self.cache = cache
         # the whole step as one launch (ta_decode_step): bf16, head_dim 64, up to 32 sequences, the structural
         # key set (no neighbour borrowing, fixed budget) and one sequence group
         # attn_split: workgroups per query of the per-op decode attention (default: decode_nsplit's choice)
         self.attn_split = attn_split
         can = (self.fused and self.dh == 64 and batch <= 32 and not groups and not cfg.neighbors
-               and cfg.beam_mode != 'pred' and n_layer <= 64 and not SEL.gate_on(cfg))
+               and cfg.beam_mode != 'pred' and n_layer <= 64 and not SEL.gate_on(cfg) and not self.mx4)
         if one_launch and not can:
             raise ValueError('one_launch: needs a bf16 model with head_dim 64, batch <= 32, neighbours off and a '
                              'fixed budget')
@@ -528,6 +615,8 @@ class Decoder:
         self.paged = (mode == 'seg' and not self.one_launch) if paged is None else bool(paged)
         if self.paged and (self.one_launch or mode != 'seg'):
             raise ValueError('paged caches serve the per-op seg decoder (not the one-launch step or dense mode)')
+        if cache is not None and not (self.paged and self.dh in (16, 32, 64, 128)):
+            raise ValueError('cache %r: paged caches of the seg decoder, head size 16, 32, 64 or 128' % cache)
         self.max_tokens = min(int(max_tokens), Tcap) if max_tokens else Tcap
         self.reserve_ahead = int(reserve_ahead)
         self.reset()
@@ -540,7 +629,7 @@ class Decoder:
             if self.paged:
                 leaf = SEL.cfg_shape(self.cfg, self.Tcap).leaf
                 npages = B * H * ((self.max_tokens + leaf - 1) // leaf)
-                self.pool = PagePool(B, H, dh, leaf, self.Tcap, npages, self.nl, self.dtype, self.dev)
+                self.pool = PagePool(B, H, dh, leaf, self.Tcap, npages, self.nl, self.dtype, self.dev, self.cache)
             self.states = [SegState(self.cfg, self.Tcap, H, dh, self.dev, B, self.dtype, pages=self.pool, layer=i)
                            for i in range(self.nl)]
             if self.cfg.beam_mode == 'pred':
@@ -574,7 +663,7 @@ class Decoder:
     def _nsplit(self, B, wl, leaf):
         if self.attn_split:
             return 4 * int(self.attn_split)
-        return decode_nsplit(B, self.H, wl, leaf)
+        return decode_nsplit(B, self.H, wl, leaf) if self.cache is None else decode_nsplit8(B, self.H, 1, wl, leaf)
 
     def step_kernel(self):
         """The one-launch step over this decoder's weights and caches (built on first use)."""
@@ -726,8 +815,9 @@ class Decoder:
 
     # ------------------------------------------------------------------------------------------ prefill
     @torch.no_grad()
-    def prefill(self, idx, chunk=None):
-        """Run the model over prompts idx (B, T0) and fill every layer's cache (positions 0..T0-1).
+    def prefill(self, idx, chunk=None, bits=None):
+        """Run the model over prompts idx (B, T0) and fill every layer's cache (positions 0..T0-1).  bits 4 (with Mx4
+        weights): the products' rows are rounded to 4 bits too.
         Selection and attention are those of the forward pass (fastseg.py:345-405 semantics over the cache's
         tree).  Returns the last position's logits (B, V)."""
         if self.mode != 'seg':
@@ -736,6 +826,8 @@ class Decoder:
         B, T0 = idx.shape
         if B != self.B or T0 > self.Tcap:
             raise ValueError('prompt shape does not fit the decoder')
+        if bits not in (None, 4) or (bits == 4 and not self.mx4):
+            raise ValueError('prefill: bits None, or 4 with Mx4 weights')
         cfg = self.cfg
         chunk = chunk or B
         tq = torch.arange(T0, device=self.dev, dtype=torch.int32)
@@ -750,7 +842,7 @@ class Decoder:
             x = W['wte'][idx[b0:b1].to(self.dev)] + W['wpe'][:T0].unsqueeze(0)
             for i, L in enumerate(W['layers']):
                 st = self.states[i]
-                qkv = F.linear(_ln(x, L['ln1']), L['c_attn'])
+                qkv = _product(x, L['c_attn'], L['ln1'], bits)
                 q, k, v = [a.view(nb, T0, H, dh).transpose(1, 2) for a in qkv.split(C, -1)]
                 st.write_rows(b0, k, v)
                 lv = [t[b0:b1] for t in st.levels]
@@ -796,8 +888,8 @@ class Decoder:
                     K.seg_attn(q, k, v, tq, ids, vld, n_tree, st.shape.leaf, cfg.local, scale,
                                out=out.transpose(1, 2))
                     del ids, vld, sct, n_tree
-                x = x + F.linear(out.view(nb, T0, C), L['c_proj'])
-                x = x + F.linear(F.gelu(F.linear(_ln(x, L['ln2']), L['c_fc'])), L['c_mlp'])
+                x = x + _product(out.view(nb, T0, C), L['c_proj'], None, bits)
+                x = x + _product(F.gelu(_product(x, L['c_fc'], L['ln2'], bits)), L['c_mlp'], None, bits)
                 if cfg.global_pool:
                     st.ksum[b0:b1] = k.float().sum(2)
             last.append(F.linear(_ln(x[:, -1], W['ln_f']), W['wte']))
