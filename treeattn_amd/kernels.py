@@ -1063,8 +1063,13 @@ def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, 
     512), the own block and the static keys; nb = (nid, match) as for seg_attn.  Keys of the block in the tail are read
     unrounded.  Returns (out, lse, keys)."""
     dev = cache.index
-    qt, _ = _cache8_rows('seg_attn8', cache, q, q, 4)
     B, H, Nq, D = shape = q.shape
+    qt = q.stride()
+    if B != cache.B or H != cache.H or D != cache.D or qt[3] != 1:
+        raise ValueError('seg_attn8: q of %d sequences, %d heads and head size %d as (B, H, Nq, D), the last dimension '
+                         'contiguous, got %s' % (cache.B, cache.H, cache.D, tuple(shape)))
+    if q.dtype != cache.dtype:
+        raise TypeError('seg_attn8: q must have the cache dtype %s' % cache.dtype)
     wl = ids.shape[-1]
     per = (B, H, Nq)
     if tq.dtype != torch.int32 or not tq.is_contiguous():
@@ -1146,11 +1151,19 @@ class Mx4:
         return ((K + 127) // 128) * ((M + 15) // 16 * 1024 + (M + 63) // 64 * 256)
 
     def _hold(self, buf, M, K, index):
-        S, T = (K + 127) // 128, (M + 15) // 16
-        self.tiles = buf.as_strided((T, S, 4, 16, 16), (S * 1024, 1024, 256, 16, 1))
-        self.tile_scale = buf.as_strided(((M + 63) // 64, S, 4, 16, 4), (S * 256, 256, 64, 4, 1), T * S * 1024)
-        self.at, self.scale_at = buf.data_ptr(), buf.data_ptr() + T * S * 1024
         self.K, self.shape, self.device, self.index, self._buf = K, (M, K), buf.device, index, buf
+        self.at = buf.data_ptr()
+        self.scale_at = self.at + ((M + 15) // 16) * ((K + 127) // 128) * 1024
+
+    @property
+    def tiles(self):
+        S, T = (self.K + 127) // 128, (self.shape[0] + 15) // 16
+        return self._buf.as_strided((T, S, 4, 16, 16), (S * 1024, 1024, 256, 16, 1))
+
+    @property
+    def tile_scale(self):
+        S, M = (self.K + 127) // 128, self.shape[0]
+        return self._buf.as_strided(((M + 63) // 64, S, 4, 16, 4), (S * 256, 256, 64, 4, 1), self.scale_at - self.at)
 
     @property
     def packed(self):
@@ -1231,6 +1244,11 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     ldx, one = x.stride()
     if x.dtype != torch.bfloat16 or one != 1:
         raise ValueError('mx4_mm: x (M, K) bf16 with contiguous rows, or an Mx4')
+    if M == 1:
+        ldx = K
+    at = x.data_ptr()
+    if at == out.data_ptr() and M:
+        raise ValueError('mx4_mm: out must not be x')
     if ln_w is not None and (ln_w.dtype != torch.bfloat16 or ln_w.shape != (K,) or not ln_w.is_contiguous()):
         raise ValueError('mx4_mm: ln_w (K,) bf16, contiguous')
     _on('mx4_mm', dev, x, ln_w)
@@ -1241,7 +1259,7 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
         nbytes = L.lib().ta_mx4_rows_workspace_size(M, K, 1)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-    _mx4_rows(dev, x.data_ptr(), ldx, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K, epi,
+    _mx4_rows(dev, at, ldx, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K, epi,
               ws.data_ptr() if nbytes else None, nbytes)
     return out
 
