@@ -108,7 +108,7 @@ typedef struct ta_kv8 {
  * is rounded into its page, and the nodes ending there are formed from the unrounded keys as ta_kv_append forms them
  * (tree level j of n_levels, leaf * arity^j positions per node).  A position outside [0, tcap) or in a block without a
  * page is not stored.  Going back to a position inside an earlier block restores that block's rows before it from its
- * page.
+ * page (rounded) and drops what the tail held: the positions after it are to be appended again.
  */
 int ta_kv8_append(const void* k_new, const void* v_new, int dtype, int64_t nsb, int64_t nsh, int64_t vnsb,
                   int64_t vnsh, const ta_kv8* cache, int B, int H, int D, const int32_t* t_pos, int n_levels,
@@ -129,8 +129,8 @@ int ta_kv8_fill(const void* k, const void* v, int dtype, int64_t ksb, int64_t ks
  * min(valid ids, n_tree) selected leaf blocks (distinct, before the own block), the matched neighbour leaves (nb_S
  * slots; 0: none), the own block up to the position and the static keys.  At most 512 leaves; ids outside the table and
  * blocks without a page contribute nothing; a query at a position outside [0, tcap), or with no key, gives zeros and
- * lse -1e30.  nsplit and ws as for ta_seg_attn_fwd (ta_seg_attn_workspace_size; zero-filled once, calls that share it
- * must not overlap in time).  lse (B, H, Nq) and keys (B, H, Nq; the number of keys) may be NULL.
+ * lse -1e30.  nsplit and ws as for ta_seg_attn_fwd (ta_seg_attn_workspace_size; zero-filled once; calls that share it
+ * have the same B * H * Nq and do not overlap in time).  lse (B, H, Nq) and keys (B, H, Nq; the number of keys) may be NULL.
  */
 int ta_seg_attn8_fwd(const void* q, int dtype, int64_t qsb, int64_t qsh, int64_t qsn, const ta_kv8* cache, int B, int H,
                      int Nq, int D, const int32_t* tq, int64_t tq_sb, const int32_t* ids, const uint8_t* vld,

@@ -135,6 +135,17 @@ def test_rows(M, N, Kd, epilogue):
     close(got, *want(x2, wv.cpu(), ln_w=g, epilogue=epilogue, residual=r))
 
 
+@pytest.mark.parametrize('M,N,Kd', [(2049, 4097, 32), (2500, 4500, 96), (3300, 3500, 672), (4353, 4000, 192)])
+@pytest.mark.parametrize('epilogue', [None, 'gelu', 'residual'])
+def test_rows_of_large_tiles(M, N, Kd, epilogue):
+    """Tiles of 256 x 256, with one step of K, ragged ones and many; the last shape would need two rounds of them and takes
+    the small ones."""
+    x = rnd(M, Kd, seed=1, dtype=BF16)
+    w, wv = K.mx4_quant(rnd(N, Kd, seed=2, scale=1 / math.sqrt(Kd)).to(DEV), values=True)
+    r = rnd(M, N, seed=3, dtype=BF16)
+    close(K.mx4_mm(x.to(DEV), w, epilogue=epilogue, residual=r.to(DEV)), *want(x, wv.cpu(), epilogue=epilogue, residual=r))
+
+
 @pytest.mark.parametrize('M,Kd', [(3, 768), (20, 1024), (20, 2048), (5, 20000)])
 def test_layernorm_of_rows_far_from_zero(M, Kd):
     """Rows whose mean is far above their deviation: the variance is taken about the mean."""

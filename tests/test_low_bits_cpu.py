@@ -71,11 +71,15 @@ def test_cache_calls_refuse_bad_descriptions(lib):
     refused(lib, append(kv8(), dtype=7), 1, b'dtype')
     refused(lib, append(kv8(), arity=5), 1, b'arity')
     refused(lib, append(kv8(), levels=33), 1, b'32 levels')
+    refused(lib, append(kv8(), levels=2), 1, b'addresses')
+    one = (ctypes.c_int64 * 1)(0)
+    refused(lib, L.ta_kv8_append(P, P, 2, 64, 64, 64, 64, kv8(), 1, 2, 64, P, 1, one, one, one, 1, None), 1, b'addresses')
 
     def fill(T=64, k=P, kst=64):
         return L.ta_kv8_fill(k, P, 2, 4096, 4096, kst, 4096, 4096, 64, kv8(), 1, 2, T, 64, None, None)
     refused(lib, fill(T=65), 1, b'tcap')
     refused(lib, fill(k=P + 2), 1, b'16-byte')
+    refused(lib, fill(k=P + 1), 1, b'16-byte')
     refused(lib, fill(kst=65), 1, b'16-byte')
 
     def attend(c=None, wl=4, local=3, nsplit=1, ws=None, nb=0, q=P, B=1, Nq=1):
@@ -101,6 +105,8 @@ def test_products_refuse_bad_arguments(lib):
         return L.ta_mx4_rows(X, ldx, W, P, Y, ldy, R, 8, ln, 1e-5, M, N, K, epi, ws, 0, None)
     refused(lib, rows(K=48, ldx=48), 1, b'multiple of 32')
     refused(lib, rows(ldx=32), 1, b'bad sizes')
+    refused(lib, rows(N=0x7fffffff, M=1), 1, b'bad sizes')
+    refused(lib, rows(M=0x7fffffff), 1, b'bad sizes')
     refused(lib, rows(epi=3), 1, b'bad sizes')
     refused(lib, rows(epi=2), 1, b'residual')
     refused(lib, rows(X=P + 2), 1, b'16-byte')
@@ -115,6 +121,7 @@ def test_products_refuse_bad_arguments(lib):
     def both(K=64, M=4, N=8, ldy=8, Xs=P, Xp=P):
         return L.ta_mx4_both(Xp, Xs, P, P, P, ldy, None, 0, M, N, K, 0, None)
     refused(lib, both(K=0), 1, b'bad sizes')
+    refused(lib, both(N=0x7fffffff, M=1), 1, b'bad sizes')
     refused(lib, both(ldy=4), 1, b'bad sizes')
     refused(lib, both(Xp=P + 4), 1, b'aligned')
     refused(lib, both(Xs=P + 2), 1, b'aligned')
@@ -144,3 +151,12 @@ def test_wrappers_refuse_host_tensors():
                          (3, torch.zeros(1, 1, 2, 8, 8), 'tail'), (4, torch.zeros(1, 1), 'tail_block'), (5, 0, 'table')):
         with pytest.raises(ValueError, match=text):
             K.Cache8(*[bad if j == i else a for j, a in enumerate(args)])
+
+
+def test_wavefronts_per_query():
+    from treeattn_amd.engine import decode_nsplit, decode_nsplit8
+    assert decode_nsplit8(32, 12, 1, 32, 64) == decode_nsplit(32, 12, 32, 64) == 4
+    assert decode_nsplit8(1, 12, 1, 64, 128) == decode_nsplit(1, 12, 64, 128) == 64
+    assert decode_nsplit8(4, 12, 32, 16, 64) == 4 and decode_nsplit8(4, 12, 128, 16, 64) == 1
+    assert all(n == 1 or n % 4 == 0 and n <= 256 for B in (1, 7, 400) for H in (1, 12) for Nq in (1, 5, 900) for wl in (0, 4, 512)
+               for leaf in (2, 64) for n in [decode_nsplit8(B, H, Nq, wl, leaf)])

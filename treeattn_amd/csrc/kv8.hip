@@ -402,8 +402,16 @@ extern "C" int ta_kv8_append(const void* k_new, const void* v_new, int dtype, in
     set_error("ta_kv8_append: bad sizes (at most 32 levels, arity 2 to 16) or a missing pointer");
     return TA_ERR_ARG;
   }
+  if (n_levels > 0 && (lv_ptr == nullptr || lv_sb == nullptr || lv_sh == nullptr)) {
+    set_error("ta_kv8_append: levels without their addresses or strides");
+    return TA_ERR_ARG;
+  }
   LevelRW8 lv;
   for (int j = 0; j < n_levels; ++j) {
+    if (lv_ptr[j] == nullptr) {
+      set_error("ta_kv8_append: levels without their addresses or strides");
+      return TA_ERR_ARG;
+    }
     lv.ptr[j] = lv_ptr[j];
     lv.sb[j] = lv_sb[j];
     lv.sh[j] = lv_sh[j];
@@ -432,8 +440,8 @@ extern "C" int ta_kv8_fill(const void* k, const void* v, int dtype, int64_t ksb,
     set_error("ta_kv8_fill: the prompt must have between 0 and tcap positions");
     return TA_ERR_ARG;
   }
-  for (int64_t s : {ksb, ksh, kst, vsb, vsh, vst, (int64_t)((uintptr_t)k / sz), (int64_t)((uintptr_t)v / sz)})
-    if ((s * sz) % 16) {
+  for (int64_t s : {ksb * sz, ksh * sz, kst * sz, vsb * sz, vsh * sz, vst * sz, (int64_t)(uintptr_t)k, (int64_t)(uintptr_t)v})
+    if (s % 16) {
       set_error("ta_kv8_fill: k and v rows not 16-byte aligned");
       return TA_ERR_ARG;
     }

@@ -414,9 +414,13 @@ int launch_gemm(GemmArgs a, int epilogue, hipStream_t st) {
     return TA_ERR_UNSUPPORTED;
   }
   a.vec = a.ldy % 4 == 0 && (uintptr_t)a.Y % 8 == 0 && (a.R == nullptr || (a.ldr % 4 == 0 && (uintptr_t)a.R % 8 == 0));
-  const int64_t big = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
-  if (big * 4 >= (int64_t)device_cus() * 3) return launch_tile<BOTH, 8, 4, true>(a, epilogue, st);
-  return launch_tile<BOTH, 4, 2, false>(a, epilogue, st);
+  // Rounds of tiles over the compute units: one of 256 x 256 tiles takes about three of 128 x 128 (bf16 X, N 8192, K 4096;
+  // M 1024: 97 against 70 us, 1536: 101 against 108, 2048: 108 against 140, 2304, whose 288 large tiles are two rounds: 193
+  // against 167.  Both in 4 bits: 35 and 27, 36.9 and 37.4, 38.6 and 46.8, 65 and 56 us).
+  const int64_t cus = device_cus(), rounds = ((int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) + cus - 1) / cus,
+                small = ((int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128) + cus - 1) / cus;
+  if (small < 3 * rounds) return launch_tile<BOTH, 4, 2, false>(a, epilogue, st);
+  return launch_tile<BOTH, 8, 4, true>(a, epilogue, st);
 }
 
 }  // namespace
@@ -434,7 +438,7 @@ using namespace ta;
 
 extern "C" int ta_mx4_both(const void* Xp, const uint8_t* Xs, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy,
                            const void* R, int64_t ldr, int M, int N, int K, int epilogue, void* stream) {
-  if (M < 0 || N < 1 || K < 1 || K > 0x7fffff00 || (M > 1 && ldy < N) || epilogue < 0 || epilogue > 2 ||
+  if (M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x7fffff00 || (M > 1 && ldy < N) || epilogue < 0 || epilogue > 2 ||
       (epilogue == MX_EPI_RESIDUAL && (R == nullptr || (M > 1 && ldr < N)))) {
     set_error("ta_mx4_both: bad sizes (a residual needs its rows)");
     return TA_ERR_ARG;

@@ -935,8 +935,11 @@ class Cache8:
     scale[p, 0] and scale[p, 1] ((P, 2) float32, powers of two); table (B, H, n_blocks) int32 maps leaf block j of
     (b, h) to its page (-1: none) and may be shared by several layers.  The block being filled stands unrounded in
     tail (B, H, 2, leaf, D), in the model's type, and tail_block (B, H) int32 says which it is (-1: none); it is
-    rounded into its page when its last row arrives.  tcap: positions per sequence.  The tensors are the caller's;
-    a new cache is pool of zeros, scale of ones, tail_block of -1."""
+    rounded into its page when its last row arrives.  tcap: positions per sequence.  The tensors are the caller's and
+    change in place (another table or pool is another Cache8); a page belongs to one block of one sequence and head.  A
+    new cache is pool of zeros, scale of ones, tail_block of -1."""
+
+    pool, scale, table, tail, tail_block = (property(lambda self, i=i: self._tensors[i]) for i in range(5))
 
     def __init__(self, pool, scale, table, tail, tail_block, tcap):
         P, two, leaf, D = pool.shape
@@ -953,7 +956,7 @@ class Cache8:
             raise ValueError('Cache8: tail_block (B, H) int32')
         self.index = L.device_index(pool)
         _on('Cache8', self.index, scale, table, tail, tail_block)
-        self.pool, self.scale, self.table, self.tail, self.tail_block = pool, scale, table, tail, tail_block
+        self._tensors = pool, scale, table, tail, tail_block   # (their addresses are in desc)
         self.B, self.H, self.leaf, self.D, self.tcap = B, H, leaf, D, int(tcap)
         self.dtype, self.device, self.code, self.block_log2 = tail.dtype, pool.device, L._DT[tail.dtype], _ilog2(leaf)
         self.desc = L.Kv8(pool.data_ptr(), scale.data_ptr(), table.data_ptr(), table.stride(0), table.stride(1), P,
@@ -1013,7 +1016,8 @@ def kv8_append(k_new, v_new, cache, t_pos, levels, arity):
     """Append one position of every (sequence, head) to a Cache8: k_new, v_new (B,H,D) at t_pos (B,) int32, forming the
     tree nodes that end there in `levels` (tree levels 0.. of (B,H,nodes,D) float32, arity children per node) from the
     unrounded keys.  The block a token ends is rounded into its page.  A position outside [0, tcap), or in a block
-    without a page, is not stored.  Going back to an earlier block restores its rows from its page."""
+    without a page, is not stored.  Going back to an earlier block restores its rows from its page and drops what the tail
+    held: the positions after it are to be appended again."""
     dev = cache.index
     kt, vt = _cache8_rows('kv8_append', cache, k_new, v_new, 3)
     if t_pos.dtype != torch.int32 or t_pos.dim() != 1 or t_pos.shape[0] != cache.B or not t_pos.is_contiguous():
@@ -1053,7 +1057,8 @@ def kv8_fill(k, v, cache, lengths=None):
 
 
 def seg_attn8_workspace(B, H, Nq, D, nsplit, device):
-    """Zero-filled workspace for seg_attn8 with `nsplit` (None when none is needed); as seg_attn_workspace."""
+    """Zero-filled workspace for seg_attn8 with `nsplit` (None when none is needed); as seg_attn_workspace.  Calls that share
+    it have the same B * H * Nq and do not overlap in time."""
     return seg_attn_workspace(B, H, Nq, D, nsplit, device)
 
 
