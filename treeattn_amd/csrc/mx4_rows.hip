@@ -15,7 +15,13 @@
 //
 // A LayerNorm of short rows (kFused values in all) happens on the way: the workgroup reads X once, 16 or 32 lanes a row,
 // and leaves it normalised in LDS for its wavefronts.  Every workgroup does that for itself, so longer rows are normalised
-// once by a kernel of their own, into the workspace.
+// once by a kernel of their own, into the workspace.  Either way the normalised rows are rounded to bf16, which the
+// matrix instructions take.
+//
+// 32 x 4096 x 16384 (35.7 MB of weights) takes 12.6 us, 2.9 TB/s, and 3.7 for the LayerNorm in front; a floor of 6.5 us at a
+// large copy's rate.  What is left is the start (the first weights' round trip), X (every workgroup reads all of it from L2 and
+// turns it round in LDS, twice the weights' bytes) and the sums of eight wavefronts at the end.  1 x 1024 x 1024 takes 3.1
+// us, a launch with one round trip.
 #include "mx4.hpp"
 
 namespace ta {
