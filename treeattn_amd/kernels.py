@@ -1095,7 +1095,7 @@ def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, 
         if n_tree.dtype != torch.int32 or not n_tree.is_contiguous():
             n_tree = n_tree.to(torch.int32).contiguous()
     if out is None:
-        out = torch.empty(shape, device=q.device, dtype=q.dtype)
+        out = q.new_empty(shape)
         ot = (H * Nq * D, Nq * D, D)
     else:
         ot = out.stride()
@@ -1206,8 +1206,8 @@ def mx4_quant(x, values=False):
     if K < 1 or (K > 1 and one != 1):
         raise ValueError('mx4_quant: rows (M, K) with contiguous rows, K at least 1')
     w = object.__new__(Mx4)
-    w._hold(torch.empty(Mx4._bytes(M, K), dtype=torch.uint8, device=x.device), M, K, dev)
-    v = torch.empty(M, K, dtype=x.dtype, device=x.device) if values else None
+    w._hold(x.new_empty((Mx4._bytes(M, K),), dtype=torch.uint8), M, K, dev)
+    v = x.new_empty((M, K)) if values else None
     _mx4_quant(dev, x.data_ptr(), L.dtype_code(x), ld, M, K, w.at, w.scale_at, v.data_ptr() if values else None, K)
     return (w, v) if values else w
 
@@ -1228,7 +1228,7 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     if epi is None:
         raise ValueError('mx4_mm: epilogue None, gelu or residual')
     if out is None:
-        out = torch.empty((M, N), device=w.device, dtype=torch.bfloat16)
+        out = w._buf.new_empty((M, N), dtype=torch.bfloat16)
         ldo = N
     else:
         _mx4_out(dev, out, M, N)
@@ -1263,7 +1263,7 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
         gp = ln_w.data_ptr()
         nbytes = L.lib().ta_mx4_rows_workspace_size(M, K, 1)
         if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+            ws = w._buf.new_empty((nbytes,))
     _mx4_rows(dev, at, ldx, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K, epi,
               ws.data_ptr() if nbytes else None, nbytes)
     return out
