@@ -51,7 +51,7 @@ MODES = [dict(neighbors=False), dict(neighbors=True), dict(neighbors=False, gate
 
 
 @pytest.mark.parametrize('mode', MODES, ids=lambda m: '-'.join('%s' % k for k, x in m.items() if x) or 'plain')
-@pytest.mark.parametrize('dtype,dh,leaf', [(torch.bfloat16, 64, 8), (torch.float32, 32, 2)])
+@pytest.mark.parametrize('dtype,dh,leaf', [(torch.bfloat16, 64, 8), (torch.float32, 32, 2), (torch.float16, 16, 16)])
 def test_steps_of_every_selection_mode(mode, dtype, dh, leaf):
     """Selections, stores, nodes and key counts are those of the cache in the model's type; the outputs are those of that
     cache holding the rounded values (two float32 evaluations, each rounded once: eps / 2 of the larger each, and 2^-18 of

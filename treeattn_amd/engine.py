@@ -564,15 +564,17 @@ def weights_mx4(W):
     return dict(W, layers=[dict(L, **{n: K.mx4_quant(L[n]) for n in _PRODUCTS}) for L in W['layers']])
 
 
-def _product(x, w, ln_w=None, bits=None):
-    """LN(x) @ w.T of a prompt's rows x (..., K); w a matrix or an Mx4.  bits 4: the rows are rounded to Mx4 as well."""
+def _product(x, w, ln_w=None, bits=None, gelu=False, residual=None):
+    """LN(x) @ w.T of a prompt's rows x (..., K), then GELU or the sum with residual (..., N); w a matrix or an Mx4, whose
+    product does both before its one rounding.  bits 4: the rows are rounded to Mx4 as well."""
     if not isinstance(w, K.Mx4):
-        return F.linear(x if ln_w is None else _ln(x, ln_w), w)
+        y = F.linear(x if ln_w is None else _ln(x, ln_w), w)
+        return F.gelu(y) if gelu else y if residual is None else residual + y
     rows = x.reshape(-1, x.shape[-1])
     if bits == 4:
-        y = K.mx4_mm(K.mx4_quant(rows if ln_w is None else _ln(rows, ln_w)), w)
-    else:
-        y = K.mx4_mm(rows, w, ln_w=ln_w)
+        rows, ln_w = K.mx4_quant(rows if ln_w is None else _ln(rows, ln_w)), None
+    y = K.mx4_mm(rows, w, ln_w=ln_w, epilogue='gelu' if gelu else None if residual is None else 'residual',
+                 residual=None if residual is None else residual.reshape(-1, residual.shape[-1]))
     return y.view(*x.shape[:-1], y.shape[-1])
 
 
@@ -891,8 +893,8 @@ class Decoder:
                     K.seg_attn(q, k, v, tq, ids, vld, n_tree, st.shape.leaf, cfg.local, scale,
                                out=out.transpose(1, 2))
                     del ids, vld, sct, n_tree
-                x = x + _product(out.view(nb, T0, C), L['c_proj'], None, bits)
-                x = x + _product(F.gelu(_product(x, L['c_fc'], L['ln2'], bits)), L['c_mlp'], None, bits)
+                x = _product(out.view(nb, T0, C), L['c_proj'], bits=bits, residual=x)
+                x = _product(_product(x, L['c_fc'], L['ln2'], bits, gelu=True), L['c_mlp'], bits=bits, residual=x)
                 if cfg.global_pool:
                     st.ksum[b0:b1] = k.float().sum(2)
             last.append(F.linear(_ln(x[:, -1], W['ln_f']), W['wte']))
