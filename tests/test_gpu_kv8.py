@@ -1,5 +1,6 @@
 """The decode cache in 8 bits (kernels.Cache8: kv8_append, kv8_fill, seg_attn8) against its float64 restatement
 (oracle/low_bits.py) and against the cache in the model's type.  GPU only."""
+import copy
 import math
 
 import pytest
@@ -449,3 +450,16 @@ def test_refusals():
         K.seg_attn8(q, c, t.view(B, 1), ids.long(), vld, None, 3, 1.0)
     with pytest.raises(RuntimeError, match='workspace'):
         K.seg_attn8(q, c, t.view(B, 1), ids, vld, None, 3, 1.0, nsplit=16, ws=torch.zeros(256, dtype=torch.uint8, device=DEV))
+
+
+def test_copies_hold_their_own_tensors():
+    pool = torch.zeros(3, 2, 8, 16, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    c = K.Cache8(pool, torch.ones(3, 2, device=DEV), torch.tensor([[[2, 0]]], dtype=torch.int32, device=DEV),
+                 torch.zeros(1, 1, 2, 8, 16, device=DEV), torch.full((1, 1), -1, dtype=torch.int32, device=DEV), 16)
+    d = copy.deepcopy(c)
+    row = torch.randn(1, 1, 16, generator=torch.Generator().manual_seed(1)).to(DEV)
+    K.kv8_append(row, row, d, torch.zeros(1, dtype=torch.int32, device=DEV), [], 2)
+    assert torch.equal(d.tail[0, 0, 1, 0], row[0, 0]) and int(d.tail_block) == 0
+    assert not c.tail.any() and int(c.tail_block) == -1 and c.desc.tail != d.desc.tail
+    with pytest.raises(AttributeError):
+        c.table = d.table

@@ -1,5 +1,7 @@
 """Microscaled 4-bit rows (kernels.Mx4: mx4_quant, mx4_mm) against their float64 restatement.  GPU only."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -253,3 +255,15 @@ def test_empty_and_refusals():
         K.mx4_quant(torch.zeros(2, 32, device=DEV, dtype=torch.float64))
     with pytest.raises(RuntimeError, match='GPU'):
         K.mx4_quant(torch.zeros(2, 32))
+
+
+def test_copies_hold_their_own_rows():
+    w = K.mx4_quant(rnd(50, 200, seed=1).to(DEV))
+    x = rnd(3, 200, seed=2).to(DEV)
+    want = K.mx4_mm(K.mx4_quant(x), w)
+    for c in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert c.at == c._buf.data_ptr() != w.at and c.shape == w.shape
+        assert c.scale_at - c.at == w.scale_at - w.at and torch.equal(c.packed, w.packed)
+        assert torch.equal(K.mx4_mm(K.mx4_quant(x), c), want)
+    c = copy.copy(w)
+    assert c.at == w.at and torch.equal(K.mx4_mm(K.mx4_quant(x), c), want)

@@ -964,6 +964,9 @@ class Cache8:
                           self.block_log2, self.tcap)
         self.ref = ctypes.byref(self.desc)
 
+    def __reduce__(self):   # copies and files hold the tensors, not their addresses
+        return Cache8, (*self._tensors, self.tcap)
+
     def rows(self, b0, b1):
         """The same cache seen from sequences b0..b1-1."""
         return Cache8(self.pool, self.scale, self.table[b0:b1], self.tail[b0:b1], self.tail_block[b0:b1], self.tcap)
@@ -1159,6 +1162,13 @@ class Mx4:
         self.K, self.shape, self.device, self.index, self._buf = K, (M, K), buf.device, index, buf
         self.at = buf.data_ptr()
         self.scale_at = self.at + ((M + 15) // 16) * ((K + 127) // 128) * 1024
+
+    def __getstate__(self):   # copies and files hold the rows, not their address
+        return self._buf, self.shape
+
+    def __setstate__(self, state):
+        buf, (M, K) = state
+        self._hold(buf, M, K, L.device_index(buf))
 
     @property
     def tiles(self):
