@@ -158,9 +158,11 @@ int ta_mx4_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int K, voi
  * Y[M, N] = epilogue(LN(X) . W^T), bf16, for weights W (N, K) in 4 bits (packed and scale as above, packed 16-byte
  * and scale 4-byte aligned): the weights are exact in bf16, products are summed in float32, and the result is
  * rounded once, after the epilogue (0 none, 1 GELU in the erf form, 2 R + product).  ln_w (K bf16): the rows of X are
- * normalised first (as ta_rowmm does, rounded to bf16); where that is not part of the product's launch it needs ws, 16-byte
- * aligned, of ta_mx4_rows_workspace_size bytes (0: none).  K a multiple of 32, X 16-byte aligned with rows of a multiple of
- * 8 elements.  Y may be R, not X.
+ * normalised first, in float32, and each normalised value is held to 2^-16 of it as the sum of two bf16, both multiplied:
+ * over many rows twice the matrix instructions of a product without.  Where that is not part of the product's launch it
+ * needs ws, 16-byte aligned, of at least ta_mx4_rows_workspace_size bytes (0: none); with 4 * M * (K rounded up to a
+ * multiple of 128) bytes it takes all rows at once, with fewer as many at a time as fit, to the same result.  K a multiple
+ * of 32, X 16-byte aligned with rows of a multiple of 8 elements.  Y may be R, not X.
  */
 int64_t ta_mx4_rows_workspace_size(int M, int K, int layernorm);
 int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,

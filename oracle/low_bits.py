@@ -129,3 +129,25 @@ def quant4(x):
     code = code + 8 * neg.long()
     byte = torch.where(bad, 255, e.long() + 127)
     return code.view(rows, Kp), byte, val.view(rows, Kp)[:, :K]
+
+
+def layernorm_product(x, w, g, eps):
+    """LN(x) @ w.T of x (M, K), w (N, K), g (K,) in float64, and how far an evaluation may be from it that takes mean and
+    deviation in float32 and holds every normalised value n to 2^-16 of it:
+    - the mean is off by d * 2^-24 of the mean magnitude and the deviation by d * 2^-24 of itself (d roundings one after
+      another: eight values a vector, a vector for every 4096 of a row, and the joins); both are common to a row, so the first
+      moves a result by that times |sum of g w| / deviation, the second by that times the result;
+    - the values' own errors, 2^-16 and three float32 roundings, are independent: six times their root sum of squares;
+    - so are the 2 K roundings of the float32 sums (2^-23 each of a partial sum, which stays within six times the root sum
+      of squares of the products)."""
+    x, w, g = x.double(), w.double(), g.double()
+    K = x.shape[1]
+    var, mean = torch.var_mean(x, -1, unbiased=False, keepdim=True)
+    dev = torch.sqrt(var + eps)
+    n = (x - mean) / dev * g
+    y = n @ w.T
+    d = (30 + K / 4096) * 2.0 ** -24
+    rss = torch.sqrt((n * n) @ (w * w).T)
+    tol = (d * y.abs() + d * x.abs().mean(-1, keepdim=True) / dev * (w @ g).abs()
+           + 6 * (2.0 ** -16 + 3 * 2.0 ** -24) * rss + 6 * 2.0 ** -23 * math.sqrt(2 * K) * 6 * rss)
+    return y, tol

@@ -35,7 +35,8 @@ struct GemmArgs {
   int64_t ldy;
   const bf16_t* R;
   int64_t ldr;
-  int M, N, K, ks;       // ks: steps of 128 in a row
+  int M, N, K, ks;       // ks: steps of 128 in a row of W
+  int wsteps;            // bf16 X: steps of 64 after which W starts again (X holds its upper and then its lower halves)
   int tm, tn;            // tiles along M and N
   int vec;               // Y and R take 8-byte accesses
 };
@@ -236,6 +237,7 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
   // copy i of step s by this wavefront (i known when unrolled): those of X, of W, of scales
   constexpr int NC = NX + (BOTH ? WT / 8 : 1) + 1;
   auto copy = [&](int s, int buf, int i, bool tail) {
+    const int u = !BOTH && s >= a.wsteps ? s - a.wsteps : s;   // step of W
     if (i < NX) {
       if constexpr (BOTH) {
         const int t = i * 8 + w;
@@ -253,11 +255,11 @@ __global__ __launch_bounds__(kGemmThreads) void mx4_gemm_kernel(GemmArgs a) {
         const int t = (i - NX) * 8 + w;
         copy16(wb + (t < lastw ? t : lastw) * tstep + (int64_t)s * 1024, wo, lw(buf) + t * 1024);
       } else if (w < WT / 2) {
-        copy16(wb + (int64_t)(s >> 1) * 1024 + (s & 1) * 512, wo, lw(buf) + w * 1024);
+        copy16(wb + (int64_t)(u >> 1) * 1024 + (u & 1) * 512, wo, lw(buf) + w * 1024);
       }
     } else if (w < NSC) {
       if constexpr (BOTH) copy4(sb + (int64_t)s * 256, lane * 4, ls(buf) + w * 256);
-      else if ((s & 1) == 0) copy4(sb + (int64_t)(s >> 1) * 256, lane * 4, ls((s >> 1) % G::SBUFS) + w * 256);
+      else if ((s & 1) == 0) copy4(sb + (int64_t)(u >> 1) * 256, lane * 4, ls((s >> 1) % G::SBUFS) + w * 256);
     }
   };
   auto stage = [&](int s, int buf) {
@@ -419,7 +421,8 @@ int launch_gemm(GemmArgs a, int epilogue, hipStream_t st) {
   // offsets inside a tile and tile counts are 32-bit
   if ((!BOTH && a.xb * 256 > 0xffffffffLL) || a.ks > 65536 ||
       (int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128) > 0x7fffffffLL) {
-    set_error("mx4 product: too large (K of at most 8388608, rows of X of at most 16 MiB apart)");
+    set_error("mx4 product: too large (K of at most 8388608, rows of X of at most 16 MiB apart; with a LayerNorm K of at "
+              "most 4194304)");
     return TA_ERR_UNSUPPORTED;
   }
   a.vec = a.ldy % 4 == 0 && (uintptr_t)a.Y % 8 == 0 && (a.R == nullptr || (a.ldr % 4 == 0 && (uintptr_t)a.R % 8 == 0));
@@ -434,10 +437,12 @@ int launch_gemm(GemmArgs a, int epilogue, hipStream_t st) {
 
 }  // namespace
 
-int mx4_gemm_bf16(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,
-                  int64_t ldr, int M, int N, int K, int epilogue, hipStream_t st) {
-  GemmArgs a{(const char*)X, ldx * 2, nullptr, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N, K,
-             mx4_padded(K) / 128, 0, 0, 0};
+// parts 2: a row of X is its values' upper halves and then their lower halves, and K a multiple of 128 (so that W starts again
+// at a whole tile).
+int mx4_gemm_bf16(const void* X, int64_t ldx, int parts, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy,
+                  const void* R, int64_t ldr, int M, int N, int K, int epilogue, hipStream_t st) {
+  GemmArgs a{(const char*)X, ldx * 2, nullptr, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N, K * parts,
+             mx4_padded(K) / 128, (K + 63) / 64, 0, 0, 0};
   return launch_gemm<false>(a, epilogue, st);
 }
 
@@ -459,6 +464,6 @@ extern "C" int ta_mx4_both(const void* Xp, const uint8_t* Xs, const void* Wp, co
     return TA_ERR_ARG;
   }
   GemmArgs a{(const char*)Xp, 0, Xs, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N, K,
-             mx4_padded(K) / 128, 0, 0, 0};
+             mx4_padded(K) / 128, 0, 0, 0, 0};
   return launch_gemm<true>(a, epilogue, (hipStream_t)stream);
 }

@@ -15,24 +15,26 @@
 //
 // A LayerNorm of short rows (kFused values in all) happens on the way: the workgroup reads X once, 16 or 32 lanes a row,
 // and leaves it normalised in LDS for its wavefronts.  Every workgroup does that for itself, so longer rows are normalised
-// once by a kernel of their own, into the workspace.  Either way the normalised rows are rounded to bf16, which the
-// matrix instructions take.
+// once by a kernel of their own, into the workspace.  The matrix instructions take bf16, and a normalised value rounded to
+// it would be as far off as the result's own rounding: it is held as two of them, its upper half and what that leaves
+// (2^-16 of the value is lost), and both are multiplied.
 //
-// 32 x 4096 x 16384 (35.7 MB of weights) takes 12.6 us, 2.9 TB/s, and 3.7 for the LayerNorm in front; a floor of 6.5 us at a
-// large copy's rate.  What is left is the start (the first weights' round trip), X (every workgroup reads all of it from L2 and
-// turns it round in LDS, twice the weights' bytes) and the sums of eight wavefronts at the end.  1 x 1024 x 1024 takes 3.1
-// us, a launch with one round trip.
+// 32 x 4096 x 16384 (35.7 MB of weights) takes 12.4 us, 2.9 TB/s; a floor of 6.5 us at a large copy's rate.  What is left is
+// the start (the first weights' round trip), X (every workgroup reads all of it from L2 and turns it round in LDS, twice the
+// weights' bytes) and the sums of eight wavefronts at the end.  With a LayerNorm in front it takes 15.2 us and the LayerNorm
+// 4.2 (12.4 and 3.6 with its rows rounded to bf16, which made the results' error 1.4 times as large): X is twice the bytes and
+// instructions.  1 x 1024 x 1024 takes 3.1 us, a launch with one round trip.
 #include "mx4.hpp"
 
 namespace ta {
 
-int mx4_gemm_bf16(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy, const void* R,
-                  int64_t ldr, int M, int N, int K, int epilogue, hipStream_t st);
+int mx4_gemm_bf16(const void* X, int64_t ldx, int parts, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy,
+                  const void* R, int64_t ldr, int M, int N, int K, int epilogue, hipStream_t st);
 
 namespace {
 
 struct RowsArgs {
-  const bf16_t* X;
+  const bf16_t* X;       // PARTS: vector c (of 8 values) of row r, in 16-byte units, at c * M + r, the lower halves Kp / 8 * M on
   int64_t ldx;
   const char* W;         // tiles of 1024 bytes
   const uint8_t* S;      // scales, 256 bytes for four tiles one below the other
@@ -53,14 +55,27 @@ constexpr int kFused = 32768;   // values of X, rows and K rounded up to whole t
 template <int G>
 __device__ __forceinline__ float row_sum(float x) { return group_sum<G>(x); }
 
-// (x - mean) * rstd * g of eight values, as bf16.
-__device__ __forceinline__ uint4 normalised(const uint4& x, const uint4& g, float mean, float rstd) {
+// (x - mean) * rstd * g of eight values, each as the upper half of its float32 (a bf16; the sign, exponent and first bits cut
+// off, so nothing overflows) and the rest, rounded to bf16 (0 beside an infinity or NaN).
+__device__ __forceinline__ void normalised(const uint4& x, const uint4& g, float mean, float rstd, uint4& hi, uint4& lo) {
   const bf16_t* e = reinterpret_cast<const bf16_t*>(&x);
   const bf16_t* ge = reinterpret_cast<const bf16_t*>(&g);
-  float f[8];
+  uint32_t h[4], l[4];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) f[u] = (to_f32(e[u]) - mean) * rstd * to_f32(ge[u]);
-  return make_uint4(bf16_pack2(f[0], f[1]), bf16_pack2(f[2], f[3]), bf16_pack2(f[4], f[5]), bf16_pack2(f[6], f[7]));
+  for (int u = 0; u < 4; ++u) {
+    uint32_t b[2];
+    float r[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float f = (to_f32(e[2 * u + i]) - mean) * rstd * to_f32(ge[2 * u + i]);
+      b[i] = __float_as_uint(f) & 0xffff0000u;
+      r[i] = fabsf(f) < INFINITY ? f - __uint_as_float(b[i]) : 0.0f;
+    }
+    h[u] = b[1] | b[0] >> 16;
+    l[u] = bf16_pack2(r[0], r[1]);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 __device__ __forceinline__ float sum8(const uint4& x) {
   const bf16_t* e = reinterpret_cast<const bf16_t*>(&x);
@@ -85,9 +100,14 @@ __device__ __forceinline__ float squares8(const uint4& x, float mean) {
 // turned like 0-3 and rows 8-11 like 12-15 those 16 lanes touch every bank once.
 __device__ __forceinline__ int x_slot(int r, int c) { return r * 256 + (c ^ ((r & 3) | ((r >> 3) & 1) * 12)) * 16; }
 
-// MT 16-row tiles of X, CT 16-column tiles; LN: normalised on the way.
-template <int MT, int CT, bool LN, int EPI>
+// Where the products take X from: bf16 rows; bf16 rows normalised on the way; the two halves of normalised rows in memory, in
+// the order the lanes take them.
+enum { X_ROWS = 0, X_NORM = 1, X_PARTS = 2 };
+
+// MT 16-row tiles of X, CT 16-column tiles.
+template <int MT, int CT, int SRC, int EPI>
 __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) {
+  constexpr bool LN = SRC == X_NORM, PARTS = SRC == X_PARTS;
   constexpr int R = MT * 16;
   constexpr int COLS = 16 * CT;
   constexpr int XB = R * 256;                    // bytes of a step's slice of X
@@ -106,23 +126,33 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
 #pragma unroll
   for (int c = 0; c < CT; ++c) wt[c] = (int64_t)(n0 / 16 + c < last ? n0 / 16 + c : last) * ks;
   const uint8_t* sw = a.S + (int64_t)(n0 / 64) * ks * 256 + lane * 4 + n0 / 16 % 4;
-  const char* xbase = reinterpret_cast<const char*>(a.X) + (int64_t)m0 * a.ldx * 2;
+  const char* xbase = reinterpret_cast<const char*>(a.X) + (PARTS ? (int64_t)m0 * 16 : (int64_t)m0 * a.ldx * 2);
+  const int64_t vec = (int64_t)a.M * 16;         // PARTS: bytes from a vector of the rows to the next
   uint32_t xo[MT * 4];
 #pragma unroll
   for (int t = 0; t < MT * 4; ++t) {
-    const int r = t * 4 + lg;
-    xo[t] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (uint32_t)(a.ldx * 2) + li * 16;
+    const int r = PARTS ? t * 16 + li : t * 4 + lg;
+    xo[t] = (uint32_t)(m0 + r < a.M ? r : a.M - 1 - m0) * (PARTS ? 16u : (uint32_t)(a.ldx * 2)) + (PARTS ? 0 : li * 16);
   }
   const bool ragged = (a.K & 127) != 0;
   // this wavefront's step i: its tiles of the weights; rows lg, lg + 4, ... of X's slice, vector li of each
   struct Step {
-    uint4 x[LN ? 1 : MT * 4];
+    uint4 x[LN ? 1 : PARTS ? MT * 8 : MT * 4];
     uint4 q[CT];
     uint32_t s;                                  // the tiles' scales, a byte each
   };
   auto load = [&](int i, Step& v) {
     const int st = st0 + i;
-    if constexpr (!LN) {
+    if constexpr (PARTS) {
+      const char* xs = xbase + (st * 16 + lg * 4) * vec;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          v.x[(u * MT + m) * 2] = ldg16(xs + u * vec + xo[m]);
+          v.x[(u * MT + m) * 2 + 1] = ldg16(xs + (a.Kp / 8 + u) * vec + xo[m]);
+        }
+    } else if constexpr (!LN) {
       const char* xs = xbase + (int64_t)st * 256;
       if (ragged && st == ks - 1) {              // what lies past K is zero
         const bool in = st * 128 + li * 8 < a.K;
@@ -171,7 +201,10 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = i * G + j;                   // vector of the row (past K: weight 0, value 0)
-      if (v * 8 < a.Kp) *reinterpret_cast<uint4*>(lds + (v / 16) * XB + x_slot(r, v % 16)) = normalised(x[i], g[i], mean, rstd);
+      if (v * 8 < a.Kp) {
+        char* slot = lds + (v / 16) * XB + x_slot(r, v % 16);
+        normalised(x[i], g[i], mean, rstd, *reinterpret_cast<uint4*>(slot), *reinterpret_cast<uint4*>(slot + ks * XB));
+      }
     }
   } else {
     if (mine > 0) load(0, va);
@@ -187,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
 
   auto multiply = [&](int i, Step& v) {
     const char* xs = lds + (LN ? st0 + i : w) * XB;
-    if constexpr (!LN) {
+    if constexpr (SRC == X_ROWS) {
       wave_sync();                               // the previous step's slice has been read
 #pragma unroll
       for (int t = 0; t < MT * 4; ++t) *reinterpret_cast<uint4*>(lds + w * XB + x_slot(t * 4 + lg, li)) = v.x[t];
@@ -198,14 +231,21 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
     for (int c = 0; c < CT; ++c) sc[c] = mx4_scale_of(v.s, c);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      bf16x8_t ax[MT];
+      constexpr int P = SRC == X_ROWS ? 1 : 2;
+      bf16x8_t ax[MT][P];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) ax[m] = *reinterpret_cast<const bf16x8_t*>(xs + x_slot(m * 16 + li, lg * 4 + u));
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < P; ++h)
+          if constexpr (PARTS) ax[m][h] = __builtin_bit_cast(bf16x8_t, v.x[(u * MT + m) * 2 + h]);
+          else ax[m][h] = *reinterpret_cast<const bf16x8_t*>(xs + h * ks * XB + x_slot(m * 16 + li, lg * 4 + u));
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const bf16x8_t bw = mx4_bf16x8(u == 0 ? v.q[c].x : u == 1 ? v.q[c].y : u == 2 ? v.q[c].z : v.q[c].w, sc[c]);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ax[m], bw, acc[m][c], 0, 0, 0);
+        for (int h = 0; h < P; ++h)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ax[m][h], bw, acc[m][c], 0, 0, 0);
       }
     }
     if (i + 2 < mine) load(i + 2, v);
@@ -240,13 +280,14 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
   }
 }
 
-// LayerNorm of one row per workgroup, from X to Y (rows of K, contiguous); up to 16384 values are held in registers, longer
-// rows read again.  The mean, then the squares about it.  32 x 4096: 3.7 us, a launch with one read and two joined sums.
-__global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, bf16_t* __restrict__ Y) {
+// LayerNorm of one row per workgroup, from X to Y, as upper and lower halves, zeros from K to Kp: vector c (of 8 values) of
+// row r at byte c * vs + r * rs, the lower half's Kp / 8 vectors on.  Up to 16384 values are held in registers, longer rows
+// read again.  The mean, then the squares about it.  32 x 4096: 4.2 us, a launch with one read and two joined sums.
+__global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, char* __restrict__ Y, int64_t rs, int64_t vs) {
   __shared__ float s_red[2][kWaves8];
   const int tid = threadIdx.x;
   const bf16_t* xr = a.X + (int64_t)blockIdx.x * a.ldx;
-  bf16_t* yr = Y + (int64_t)blockIdx.x * a.K;
+  char* yr = Y + blockIdx.x * rs;
   const int nv = a.K / 8;
   auto total = [&](float x, int which) {
     x = group_sum<64>(x);
@@ -278,14 +319,22 @@ __global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, bf16_t* 
     if (i * kThreads + tid < nv) q += squares8(x[i], mean);
   for (int v = NV * kThreads + tid; v < nv; v += kThreads) q += squares8(ldg16(xr + (int64_t)v * 8), mean);
   const float rstd = rsqrtf(total(q, 1) / (float)a.K + a.eps);
+  const int np = a.Kp / 8;
+  auto store = [&](int v, const uint4& xv, const uint4& gv) {   // (past K both are 0, and so is the result)
+    char* o = yr + v * vs;
+    normalised(xv, gv, mean, rstd, *reinterpret_cast<uint4*>(o), *reinterpret_cast<uint4*>(o + np * vs));
+  };
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * kThreads + tid;
-    if (v < nv) *reinterpret_cast<uint4*>(yr + v * 8) = normalised(x[i], g[i], mean, rstd);
+  for (int i = 0; i < NV; ++i)
+    if (i * kThreads + tid < np) store(i * kThreads + tid, x[i], g[i]);
+  for (int v = NV * kThreads + tid; v < np; v += kThreads) {
+    uint4 xv = make_uint4(0, 0, 0, 0), gv = xv;
+    if (v < nv) {
+      xv = ldg16(xr + (int64_t)v * 8);
+      gv = ldg16(a.gam + (int64_t)v * 8);
+    }
+    store(v, xv, gv);
   }
-  for (int v = NV * kThreads + tid; v < nv; v += kThreads)
-    *reinterpret_cast<uint4*>(yr + (int64_t)v * 8) =
-        normalised(ldg16(xr + (int64_t)v * 8), ldg16(a.gam + (int64_t)v * 8), mean, rstd);
 }
 
 // Whether the product runs as workgroups of 32 rows or as tiles of many rows (mx4_gemm.hip).  The former cost about 8.5 us
@@ -294,38 +343,46 @@ __global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, bf16_t* 
 bool few_rows(int M, int N) { return M <= 64 || (int64_t)((M + 31) / 32) * ((N + 63) / 64) <= 5 * (int64_t)device_cus(); }
 
 // Whether ta_mx4_rows normalises M rows of K values within the product: wherever a workgroup's LDS holds them (32 x 768 x
-// 2304: 5.6 us against 3.3 + 3.6 with the kernel of its own, 4 x 1024 x 4096: 5.4 against 2.8 + 3.2).
+// 2304: 6.6 us against 3.1 + 3.8 with the kernel of its own, 4 x 1024 x 4096: 6.0 against 3.1 + 3.4; at the most values 4 x
+// 1984 x 8192: 8.4 against 3.1 + 4.4, 32 x 1024 x 4096: 7.6 against 3.3 + 4.3, kernels alone: the second launch is not in it).
 bool norm_fused(int M, int K) { return M <= 64 && (int64_t)(M <= 16 ? 16 : 32) * mx4_padded(K) <= kFused; }
 
-template <int MT, int CT, bool LN, int EPI>
+template <int MT, int CT, int SRC, int EPI>
 int launch_one(const RowsArgs& a, hipStream_t st) {
   constexpr int R = MT * 16, COLS = 16 * CT;
-  constexpr int x = LN ? kFused * 2 : kWaves8 * R * 256, red = kWaves8 * R * (COLS + 1) * 4;
+  const int x = SRC == X_NORM ? a.Kp / 128 * R * 512 : SRC == X_ROWS ? kWaves8 * R * 256 : 0, red = kWaves8 * R * (COLS + 1) * 4;
   const int ny = (a.M + R - 1) / R;
   const dim3 grid((unsigned)((a.N + COLS - 1) / COLS * ny)), blk(kThreads);
-  hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, LN, EPI>), grid, blk, x > red ? x : red, st, a, ny);
+  hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, SRC, EPI>), grid, blk, x > red ? x : red, st, a, ny);
   return check_launch("mx4_rows_kernel");
 }
 
+template <int MT, int CT, int EPI>
+int launch_src(const RowsArgs& a, int src, hipStream_t st) {
+  switch (src) {
+    case X_ROWS: return launch_one<MT, CT, X_ROWS, EPI>(a, st);
+    case X_NORM: return launch_one<MT, CT, X_NORM, EPI>(a, st);
+    default: return launch_one<MT, CT, X_PARTS, EPI>(a, st);
+  }
+}
+
 template <int MT, int CT>
-int launch_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
-  const bool ln = a.gam != nullptr;
+int launch_rows(const RowsArgs& a, int src, int epilogue, hipStream_t st) {
   switch (epilogue) {
-    case MX_EPI_NONE: return ln ? launch_one<MT, CT, true, MX_EPI_NONE>(a, st) : launch_one<MT, CT, false, MX_EPI_NONE>(a, st);
-    case MX_EPI_GELU: return ln ? launch_one<MT, CT, true, MX_EPI_GELU>(a, st) : launch_one<MT, CT, false, MX_EPI_GELU>(a, st);
-    default:
-      return ln ? launch_one<MT, CT, true, MX_EPI_RESIDUAL>(a, st) : launch_one<MT, CT, false, MX_EPI_RESIDUAL>(a, st);
+    case MX_EPI_NONE: return launch_src<MT, CT, MX_EPI_NONE>(a, src, st);
+    case MX_EPI_GELU: return launch_src<MT, CT, MX_EPI_GELU>(a, src, st);
+    default: return launch_src<MT, CT, MX_EPI_RESIDUAL>(a, src, st);
   }
 }
 
 // The widest workgroup (of 16, 32 or 64 columns) that still leaves every compute unit one: X is read once per workgroup.  32
 // rows, K = 4096, in the order 16, 32, 64 columns: N = 4096 7.0, 8.0, 9.7 us; 8192 12.8, 9.8, 11.2; 16384 22.8, 16.6, 12.2.
 template <int MT>
-int pick_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
+int pick_rows(const RowsArgs& a, int src, int epilogue, hipStream_t st) {
   const int cus = device_cus(), ny = (a.M + MT * 16 - 1) / (MT * 16);
-  if ((int64_t)((a.N + 63) / 64) * ny >= cus) return launch_rows<MT, 4>(a, epilogue, st);
-  if ((int64_t)((a.N + 31) / 32) * ny >= cus) return launch_rows<MT, 2>(a, epilogue, st);
-  return launch_rows<MT, 1>(a, epilogue, st);
+  if ((int64_t)((a.N + 63) / 64) * ny >= cus) return launch_rows<MT, 4>(a, src, epilogue, st);
+  if ((int64_t)((a.N + 31) / 32) * ny >= cus) return launch_rows<MT, 2>(a, src, epilogue, st);
+  return launch_rows<MT, 1>(a, src, epilogue, st);
 }
 
 }  // namespace
@@ -334,7 +391,9 @@ int pick_rows(const RowsArgs& a, int epilogue, hipStream_t st) {
 using namespace ta;
 
 extern "C" int64_t ta_mx4_rows_workspace_size(int M, int K, int layernorm) {
-  return !layernorm || M <= 0 || K <= 0 || norm_fused(M, K) ? 0 : (int64_t)M * K * 2;
+  if (!layernorm || M <= 0 || K <= 0 || norm_fused(M, K)) return 0;
+  const int64_t half = (int64_t)M * K * 2, few = (int64_t)(M < 8 ? M : 8) * mx4_padded(K) * 4;
+  return half > few ? half : few;
 }
 
 extern "C" int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy,
@@ -359,19 +418,33 @@ extern "C" int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uin
   hipStream_t st = (hipStream_t)stream;
   RowsArgs a{(const bf16_t*)X, ldx, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr,
              (const bf16_t*)ln_w, ln_eps, M, N, K, mx4_padded(K)};
+  const bool few = few_rows(M, N);
   if (ln_w != nullptr && !norm_fused(M, K)) {
-    const int64_t need = ta_mx4_rows_workspace_size(M, K, 1);
+    const int64_t need = ta_mx4_rows_workspace_size(M, K, 1), row = (int64_t)a.Kp * 4;
     if (ws == nullptr || ws_bytes < need || (uintptr_t)ws % 16) {
       set_error("ta_mx4_rows: workspace missing, too small or not 16-byte aligned");
       return TA_ERR_WORKSPACE;
     }
-    hipLaunchKernelGGL(mx4_norm_kernel, dim3((unsigned)M), dim3(kThreads), 0, st, a, (bf16_t*)ws);
-    const int rc = check_launch("mx4_norm_kernel");
-    if (rc != TA_OK) return rc;
-    a.X = (const bf16_t*)ws;
-    a.ldx = K;
-    a.gam = nullptr;
+    // as many rows at a time as the workspace holds (the results do not depend on how many)
+    const int fit = ws_bytes / row < M ? (int)(ws_bytes / row) : M;
+    for (int m = 0; m < M; m += fit) {
+      RowsArgs c = a;
+      c.X += m * ldx;
+      c.Y += m * ldy;
+      if (R != nullptr) c.R += m * ldr;
+      c.M = M - m < fit ? M - m : fit;
+      hipLaunchKernelGGL(mx4_norm_kernel, dim3((unsigned)c.M), dim3(kThreads), 0, st, c, (char*)ws, few ? 16 : row,
+                         few ? (int64_t)c.M * 16 : 16);
+      int rc = check_launch("mx4_norm_kernel");
+      if (rc != TA_OK) return rc;
+      c.X = (const bf16_t*)ws;
+      if (!few) rc = mx4_gemm_bf16(ws, row / 2, 2, Wp, Ws, c.Y, ldy, c.R, ldr, c.M, N, a.Kp, epilogue, st);
+      else rc = M <= 16 ? pick_rows<1>(c, X_PARTS, epilogue, st) : pick_rows<2>(c, X_PARTS, epilogue, st);
+      if (rc != TA_OK) return rc;
+    }
+    return TA_OK;
   }
-  if (!few_rows(M, N)) return mx4_gemm_bf16(a.X, a.ldx, Wp, Ws, Y, ldy, R, ldr, M, N, K, epilogue, st);
-  return M <= 16 ? pick_rows<1>(a, epilogue, st) : pick_rows<2>(a, epilogue, st);
+  if (!few) return mx4_gemm_bf16(X, ldx, 1, Wp, Ws, Y, ldy, R, ldr, M, N, K, epilogue, st);
+  const int src = ln_w != nullptr ? X_NORM : X_ROWS;
+  return M <= 16 ? pick_rows<1>(a, src, epilogue, st) : pick_rows<2>(a, src, epilogue, st);
 }

@@ -566,14 +566,18 @@ def weights_mx4(W):
 
 def _product(x, w, ln_w=None, bits=None, gelu=False, residual=None):
     """LN(x) @ w.T of a prompt's rows x (..., K), then GELU or the sum with residual (..., N); w a matrix or an Mx4, whose
-    product does both before its one rounding.  bits 4: the rows are rounded to Mx4 as well."""
+    product does both before its one rounding.  The normalised rows are x's dtype, as the model's LayerNorm gives them
+    (mx4_mm's own LayerNorm keeps twice the bits for twice the matrix instructions).  bits 4: the rows are rounded to Mx4
+    as well."""
+    if ln_w is not None:
+        x = _ln(x, ln_w)
     if not isinstance(w, K.Mx4):
-        y = F.linear(x if ln_w is None else _ln(x, ln_w), w)
+        y = F.linear(x, w)
         return F.gelu(y) if gelu else y if residual is None else residual + y
     rows = x.reshape(-1, x.shape[-1])
     if bits == 4:
-        rows, ln_w = K.mx4_quant(rows if ln_w is None else _ln(rows, ln_w)), None
-    y = K.mx4_mm(rows, w, ln_w=ln_w, epilogue='gelu' if gelu else None if residual is None else 'residual',
+        rows = K.mx4_quant(rows)
+    y = K.mx4_mm(rows, w, epilogue='gelu' if gelu else None if residual is None else 'residual',
                  residual=None if residual is None else residual.reshape(-1, residual.shape[-1]))
     return y.view(*x.shape[:-1], y.shape[-1])
 

@@ -1225,7 +1225,7 @@ def mx4_quant(x, values=False):
 def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     """epilogue(LN(x) @ w.T) in bf16 for weights w (Mx4, (N,K)): x (M,K) bf16, K a multiple of 32 -- the weights are exact in
     bf16 -- or x an Mx4 (M,K), whose product runs on the 4-bit matrix instructions.  ln_w (K,) bf16: a LayerNorm of x's
-    rows first (bf16 x).  epilogue None | 'gelu' | 'residual' (adds `residual`, (M,N) bf16); sums are
+    rows first (bf16 x), its values held to 2^-16 (as two bf16 each).  epilogue None | 'gelu' | 'residual' (adds `residual`, (M,N) bf16); sums are
     float32, rounded once at the end.  `out` may be `residual` (not x)."""
     if not isinstance(w, Mx4):
         raise TypeError('mx4_mm: w must be an Mx4')
@@ -1273,6 +1273,7 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
         gp = ln_w.data_ptr()
         nbytes = L.lib().ta_mx4_rows_workspace_size(M, K, 1)
         if nbytes:
+            nbytes = 4 * M * ((K + 127) // 128 * 128)   # all rows in one pass
             ws = w._buf.new_empty((nbytes,))
     _mx4_rows(dev, at, ldx, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K, epi,
               ws.data_ptr() if nbytes else None, nbytes)
