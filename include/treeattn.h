@@ -85,7 +85,8 @@ typedef struct ta_leaf_store_out {
  * unrounded, in the model's type, in tail: K rows at tail + b*tail_sb + h*tail_sh, V rows leaf * D elements after them;
  * tail_block[b*tb_sb + h] is its index (-1: the tail holds nothing).  A block is rounded into its page when its last
  * row arrives, with the smallest power-of-two scale that brings its largest finite magnitude to 448 or less (1 for
- * all zeros); what is not finite is stored as NaN.  The block the tail holds is read from the tail.
+ * all zeros); what is not finite is stored as NaN.  Rows read back in float16, and attention's results, are at most 65504 in
+ * magnitude where a value rounded up in its page would pass that.  The block the tail holds is read from the tail.
  * D 16, 32, 64 or 128; the dtype of a call is that of q, the new rows and the tail.
  */
 typedef struct ta_kv8 {

@@ -373,7 +373,7 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
     if (holds) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) orow[de + i] = from_f32<T>(sums[i] * inv);
+      for (int i = 0; i < 4; ++i) orow[de + i] = page_value<T>(sums[i] * inv);
     }
     if (lane == 0) {
       if (p.lse) p.lse[qi] = L != 0.0f ? m + __logf(L) : kNegBig;
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
   };
   if (p.gsplit == 1) {
     const float inv = Lt != 0.0f ? 1.0f / Lt : 0.0f;
-    for (int d = lane; d < D; d += kWave) orow[d] = from_f32<T>(merged(d) * inv);
+    for (int d = lane; d < D; d += kWave) orow[d] = page_value<T>(merged(d) * inv);
     if (lane == 0) {
       if (p.lse) p.lse[qi] = Lt != 0.0f ? M + __logf(Lt) : kNegBig;
       if (p.keys) p.keys[qi] = keys;
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(kWaves * kWave) void attn8_kernel(Attn8 p) {
       for (int i = 0; i < 8; ++i)
         if (s0 + i < p.gsplit) a += pv[i] * s_fac[s0 + i];
     }
-    orow[d] = from_f32<T>(a * inv);
+    orow[d] = page_value<T>(a * inv);
   }
   if (lane == 0) {
     if (p.lse) p.lse[qi] = Lq != 0.0f ? Mq + __logf(Lq) : kNegBig;

@@ -66,14 +66,6 @@ __device__ __forceinline__ void store_e4m3(uint8_t* dst, const float (&f)[vec_el
   }
 }
 
-// An e4m3 number times its scale in the tail's type; a rounded-up half that passes float16's range becomes its
-// largest number.
-template <typename T>
-__device__ __forceinline__ T tail_value(float x) {
-  if constexpr (sizeof(T) == 2 && __is_same(T, f16_t)) x = fabsf(x) > 65504.0f && fabsf(x) < INFINITY ? copysignf(65504.0f, x) : x;
-  return from_f32<T>(x);
-}
-
 // One workgroup per (sequence, head).  A row is 2 D values, so what a call costs is a launch and its round trips (position,
 // page, tag, then the rows): 32 x 12 rows of 64 bf16 3.4 us.  The call that ends a block reads it once more from L2: its
 // sums by runs of rows beside the rounding, 6 blocks of 32 x 64 float32 6.6 us (8.8 with the sums by one thread a
@@ -109,10 +101,10 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8 c, const
       float f[16];
       e4m3_x16(ldg16(page + i), f);
 #pragma unroll
-      for (int u = 0; u < 16; ++u) tk[i + u] = tail_value<T>(f[u] * ks);
+      for (int u = 0; u < 16; ++u) tk[i + u] = page_value<T>(f[u] * ks);
       e4m3_x16(ldg16(page + half + i), f);
 #pragma unroll
-      for (int u = 0; u < 16; ++u) tv[i + u] = tail_value<T>(f[u] * vs);
+      for (int u = 0; u < 16; ++u) tv[i + u] = page_value<T>(f[u] * vs);
     }
   }
   if (tid < 2 * D) {

@@ -48,6 +48,14 @@ __device__ __forceinline__ void e4m3_x16(const uint4& u, float (&f)[16]) {
   }
 }
 
+// A page's value (an e4m3 number times its scale), or a mean of such values, in the model's type.  A magnitude near float16's
+// largest, 65504, is rounded up to 65536 in a page; what passes the range that way is the largest number, not infinity.
+template <typename T>
+__device__ __forceinline__ T page_value(float x) {
+  if constexpr (__is_same(T, f16_t)) x = fabsf(x) > 65504.0f && fabsf(x) < INFINITY ? copysignf(65504.0f, x) : x;
+  return from_f32<T>(x);
+}
+
 // A finite magnitude, 0 for what is not finite: what a scale is chosen from.
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);

@@ -980,6 +980,8 @@ class Cache8:
         ok = ((pg >= 0) & (pg < self.pool.shape[0])).view(self.H, nb, 1, 1, 1)
         pg = torch.where(ok.view(self.H, nb), pg, 0)
         kv = self.pool.view(torch.uint8)[pg].view(torch.float8_e4m3fn).float() * self.scale[pg].view(self.H, nb, 2, 1, 1)
+        if self.dtype == torch.float16:   # what was rounded up past its range is its largest number
+            kv = torch.where(kv.isfinite(), kv.clamp(-65504.0, 65504.0), kv)
         kv = torch.where(ok, kv, 0.0).to(self.dtype)
         mine = torch.arange(nb, device=self.device) == self.tail_block[b].view(self.H, 1)
         kv = torch.where(mine.view(self.H, nb, 1, 1, 1), self.tail[b].unsqueeze(1), kv)
