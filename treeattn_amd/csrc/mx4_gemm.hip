@@ -54,20 +54,23 @@ __device__ __forceinline__ int turn8(int r) { return ((r >> 1) & 1) | ((r >> 3) 
 // places in LDS.  Written as instructions because the compiler waits for every such copy before the next read of LDS, also
 // of another buffer: here copies are in flight while LDS is read, and are waited for by count.  They have no result
 // registers, and their operands are read when they issue.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // (m0 is one of the compiler's own registers, as meant)
 __device__ __forceinline__ void copy16(const void* base, uint32_t off, const void* dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(off),
                "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void copy16(const void* src, const void* dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(src)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(const void* base, uint32_t off, const void* dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"((uint32_t)(uintptr_t)(lds_void*)dst), "v"(off),
                "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles, in groups of eight rows of tiles, so
 // that what its workgroups share stays in its L2.
