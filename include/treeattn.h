@@ -116,6 +116,15 @@ int ta_kv8_append(const void* k_new, const void* v_new, int dtype, int64_t nsb, 
                   float* const* lv_ptr, const int64_t* lv_sb, const int64_t* lv_sh, int arity_log2, void* stream);
 
 /*
+ * ta_gate_append after a ta_kv8_append of the same positions: the log sums and gated vectors of the nodes ending there, a leaf
+ * block's from its unrounded rows in the tail.  A position outside [0, tcap), in a block without a page or in one that the
+ * tail does not hold forms nothing.
+ */
+int ta_kv8_gate_append(const ta_kv8* cache, int dtype, int B, int H, int D, const int32_t* t_pos, int n_levels,
+                       const float* const* raw, float* const* lg, float* const* out, const int64_t* sb, const int64_t* sh,
+                       const int32_t* blevel, int arity_log2, float gate_q, void* stream);
+
+/*
  * Positions 0 .. lengths[b]-1 of k, v (B, H, T, D; 16-byte aligned rows) into an 8-bit cache (engine.py:57-71,
  * SegState.fill): whole leaf blocks into their pages, the rows of the last partial block into the tail (tail_block -1
  * when there is none).  lengths (B,) int32, clamped to [0, T]; NULL: T for every sequence.  Rows, pages and tails past a

@@ -129,6 +129,8 @@ SIGNATURES = {
                              c_i32, _P(KvPages), c_vp]),
     'ta_kv8_append': (c_i32, [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, _P(Kv8), c_i32, c_i32, c_i32, c_vp, c_i32,
                               c_vp, c_vp, c_vp, c_i32, c_vp]),
+    'ta_kv8_gate_append': (c_i32, [_P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, _P(c_vp), _P(c_vp), _P(c_vp), _P(c_i64),
+                                   _P(c_i64), _P(c_i32), c_i32, c_f32, c_vp]),
     'ta_kv8_fill': (c_i32, [c_vp, c_vp, c_i32] + [c_i64] * 6 + [_P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]),
     'ta_seg_attn8_fwd': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, _P(Kv8), c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp,
                                  c_vp, c_vp, c_i32, c_i32, c_f32, c_vp, c_vp, c_i32, c_vp, c_i64, c_i64, c_i64, c_vp,

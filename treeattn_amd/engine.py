@@ -141,12 +141,6 @@ class SegState:
         if self.gated:
             self.lg = [torch.zeros_like(t) for t in self.levels]
             self.gl = [torch.zeros_like(t) if f else None for t, f in zip(self.levels, SEL.gated_flags(cfg, self.shape))]
-            if self.cache8 is not None:
-                # the tail as a cache whose every block is on the sequence's one page: what gate_append reads the block a
-                # position ends from
-                own = torch.arange(batch * H, dtype=torch.int32, device=dev).view(batch, H, 1)
-                self.tail_rows = K.PagedCache(self.cache8.tail.view(batch * H, 2, self.shape.leaf, dh),
-                                              own.expand(-1, -1, pages.table.shape[2]).contiguous(), Tcap)
         else:
             self.lg = self.gl = None
         NS = cfg.nb_store
@@ -224,7 +218,7 @@ class SegState:
         """The gate's part of appending positions tpos (after kv_append): log sums and gated vectors of the
         nodes ending there (engine.py:47, 53-54)."""
         if self.gated and self.shape.n_levels:
-            Kc = self.tail_rows if self.cache8 is not None else self.kv()[0]
+            Kc = self.cache8 if self.cache8 is not None else self.kv()[0]
             K.gate_append(Kc, tpos, self.levels, self.lg, self.gl, self.shape.blevels, self.shape.arity,
                           float(self.cfg.gate_q))
 
@@ -260,8 +254,6 @@ class SegState:
             v.cache = self.cache.rows(b0, b1)
         if self.cache8 is not None:
             v.cache8 = self.cache8.rows(b0, b1)
-            if self.gated:
-                v.tail_rows = self.tail_rows.rows(b0, b1)
         v.levels = [t[b0:b1] for t in self.levels]
         if self.gated:
             v.lg = [t[b0:b1] for t in self.lg]

@@ -183,8 +183,11 @@ def gate_apply(raw, lgsum, size, gate_q):
 
 def gate_append(Kc, t_pos, raw, lg, out, blevels, arity, gate_q):
     """The gate's share of a decode append (engine.py:47, 53-54), after kv_append: log sums and gated vectors
-    of the nodes ending at t_pos[b].  Kc: contiguous (B,H,Tcap,D) K cache or a PagedCache; raw / lg / out the
-    tree levels (out[j] None: not gated)."""
+    of the nodes ending at t_pos[b].  Kc: contiguous (B,H,Tcap,D) K cache, a PagedCache or a Cache8 (after kv8_append: the
+    block's keys are those in its tail; a block without a page forms nothing); raw / lg / out the tree levels (out[j]
+    None: not gated)."""
+    if isinstance(Kc, Cache8):
+        return _kv8_gate_append(Kc, t_pos, raw, lg, out, blevels, arity, gate_q)
     L.require_gpu(t_pos, *raw, *lg, *_cache_tensors(Kc, Kc))
     B, H, _, D = raw[0].shape
     sb, sh = _level_strides(raw, D)
@@ -991,6 +994,7 @@ class Cache8:
 
 _kv8_append = L.entry('ta_kv8_append')
 _kv8_fill = L.entry('ta_kv8_fill')
+_gate_append8 = L.entry('ta_kv8_gate_append')
 _seg_attn8_fwd = L.entry('ta_seg_attn8_fwd')
 
 
@@ -1044,6 +1048,26 @@ def kv8_append(k_new, v_new, cache, t_pos, levels, arity):
     pack = struct.Struct('%dq' % n).pack if n else bytes
     _kv8_append(dev, k_new.data_ptr(), v_new.data_ptr(), cache.code, kt[0], kt[1], vt[0], vt[1], cache.ref, B, H, D,
                 t_pos.data_ptr(), n, pack(*at[::3]), pack(*at[1::3]), pack(*at[2::3]), s)
+
+
+def _kv8_gate_append(cache, t_pos, raw, lg, out, blevels, arity, gate_q):
+    """gate_append over a Cache8."""
+    if t_pos.dtype != torch.int32 or t_pos.shape != (cache.B,) or not t_pos.is_contiguous():
+        raise ValueError('gate_append: contiguous int32 positions (B,)')
+    _on('gate_append', cache.index, t_pos, *raw, *lg, *out)
+    want = (cache.B, cache.H, cache.D)
+    for j, t in enumerate(raw):
+        n = cache.tcap >> blevels[j]
+        for x in (t, lg[j], out[j]):
+            if x is not None and (x.dtype != torch.float32 or (*x.shape[:2], x.shape[3]) != want or x.shape[2] < n
+                                  or any(s > 1 and a != b for s, a, b in zip(t.shape[:2], x.stride(), t.stride()))
+                                  or x.stride(3) != 1 or x.stride(2) != cache.D):
+                raise ValueError('gate_append: levels (B, H, nodes, D) float32 with contiguous node rows for every whole node '
+                                 'of tcap positions, a level\'s raw, log sums and gated vectors with the same strides')
+    sb, sh = _level_strides(raw, cache.D)
+    optr = (ctypes.c_void_p * len(out))(*[o.data_ptr() if o is not None else None for o in out])
+    _gate_append8(cache.index, cache.ref, cache.code, cache.B, cache.H, cache.D, t_pos.data_ptr(), len(raw), L.ptr_array(raw),
+                  L.ptr_array(lg), optr, sb, sh, L.i32_array(list(blevels)), _ilog2(arity), float(gate_q))
 
 
 def kv8_fill(k, v, cache, lengths=None):
