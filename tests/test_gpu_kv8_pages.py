@@ -82,3 +82,44 @@ def test_gate_refusals():
         K.gate_append(st.cache8, t, [x[:, :, :1] for x in st.levels], *args[1:])
     with pytest.raises(RuntimeError, match='leaf blocks'):
         K.gate_append(st.cache8, t, *args[:3], [b + 1 for b in st.shape.blevels], *args[4:])
+
+
+@pytest.mark.parametrize('T', [5, 16, 21])
+def test_released_sequence_is_forgotten(T):
+    """After PagePool.release a sequence has no row, in no layer, in the middle of a block as at its end; the others keep theirs,
+    and the slot's next sequence is that of a new cache."""
+    cfg = Config(leaf=8, wmax=4, beam=4, neighbors=False)
+    B, H, dh, Tcap = 3, 2, 32, 64
+    pool = PagePool(B, H, dh, 8, Tcap, B * H * 8, 2, torch.bfloat16, DEV, cache='e4m3')
+    pool.ensure(Tcap)
+    sts = [SegState(cfg, Tcap, H, dh, DEV, B, torch.bfloat16, pages=pool, layer=i) for i in range(2)]
+    part = sts[1].rows(1, 3)
+    for t in range(T):
+        for i, st in enumerate(sts):
+            st.add(t, rnd(B, H, dh, seed=t + 50 * i), rnd(B, H, dh, seed=200 + t + 50 * i))
+    kept = [[x.clone() for b in (0, 2) for x in st.dense_kv(b, T)] for st in sts]
+    pool.release(1)
+    for st in sts:
+        assert not any(x.any() for x in st.dense_kv(1, T))
+        assert not any(x[1].any() for x in st.row(T - 1))
+    assert not any(x.any() for x in part.dense_kv(0, T))
+    for st, old in zip(sts, kept):
+        assert all(torch.equal(x, y) for x, y in zip([x for b in (0, 2) for x in st.dense_kv(b, T)], old))
+    q = rnd(B, H, 1, dh, seed=9)
+    ids = torch.zeros(B, H, 1, 1, dtype=torch.int32, device=DEV)
+    tq = torch.full((B, 1), T - 1, dtype=torch.int32, device=DEV)
+    lse = torch.empty(B, H, 1, device=DEV)
+    for st in sts:
+        for nsplit in (1, 4, 8):
+            out, _, _ = K.seg_attn8(q, st.cache8, tq, ids, torch.full_like(ids, T > 8, dtype=torch.bool), None, 3, 0.2, lse=lse,
+                                    nsplit=nsplit)
+            assert not out[1].any() and (lse[1] == -1e30).all() and out[0].any() and (lse[0] > -1e30).all()
+    pool.ensure(Tcap, [1])
+    new = state(cfg, 1, H, dh, Tcap, Tcap)
+    for t in range(11):
+        k, v = rnd(B, H, dh, seed=400 + t), rnd(B, H, dh, seed=500 + t)
+        at = torch.tensor([-1, t, -1], dtype=torch.int32, device=DEV)
+        sts[0].append(k, v, at)
+        new.append(k[1:2], v[1:2], at[1:2].contiguous())
+    for x, y in zip(sts[0].dense_kv(1, 11), new.dense_kv(0, 11)):
+        assert torch.equal(x, y)

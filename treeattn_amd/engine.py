@@ -59,6 +59,7 @@ class PagePool:
             self.pools = [torch.zeros(self.P, 2, leaf, dh, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
                           for _ in range(n_layers)]
             self.scales = [torch.ones(self.P, 2, device=dev) for _ in range(n_layers)]
+        self.held = []                             # tail_block of every 8-bit cache over these pages
 
     def ensure(self, t_end, seqs=None):
         """Pages for positions < t_end (at most Tcap) of the given sequences (all by default): a sequence's
@@ -90,13 +91,15 @@ class PagePool:
             self.table[rows, :, lo:need].copy_(src)
 
     def release(self, b):
-        """Return sequence b's pages (its cache rows are forgotten)."""
+        """Return sequence b's pages (its cache rows are forgotten, those of the block an 8-bit cache's tail holds too)."""
         n = self.nblk[b]
         for h in range(self.H - 1, -1, -1):
             self.free.extend(int(p) for p in self.host[b, h, :n].flip(0).tolist())
         self.host[b, :, :n] = -1
         self.table[b, :, :n].fill_(-1)
         self.nblk[b] = 0
+        for held in self.held:
+            held[b].fill_(-1)
 
     def cache(self, layer):
         return K.PagedCache(self.pools[layer], self.table, self.Tcap)
@@ -105,9 +108,10 @@ class PagePool:
         """A layer's 8-bit cache, with a tail of its own in the model's dtype."""
         B, H, dev = self.B, self.H, self.table.device
         _, two, leaf, dh = self.pools[layer].shape
+        held = torch.full((B, H), -1, dtype=torch.int32, device=dev)
+        self.held.append(held)
         return K.Cache8(self.pools[layer], self.scales[layer], self.table,
-                        torch.zeros(B, H, two, leaf, dh, device=dev, dtype=dtype),
-                        torch.full((B, H), -1, dtype=torch.int32, device=dev), self.Tcap)
+                        torch.zeros(B, H, two, leaf, dh, device=dev, dtype=dtype), held, self.Tcap)
 
 
 class SegState:
