@@ -123,3 +123,21 @@ def test_released_sequence_is_forgotten(T):
         new.append(k[1:2], v[1:2], at[1:2].contiguous())
     for x, y in zip(sts[0].dense_kv(1, 11), new.dense_kv(0, 11)):
         assert torch.equal(x, y)
+
+
+def test_fill_takes_any_layout():
+    """A prompt's rows off a 16-byte boundary, values with the head size not innermost (keys have it there for their node sums, in
+    every cache), rows shared by the heads: the cache that a contiguous copy gives."""
+    cfg = Config(leaf=8, wmax=4, beam=4, neighbors=False, gate=True)
+    B, H, dh, T = 2, 3, 16, 21
+    wide = rnd(B, H, T, dh + 1, seed=1)
+    turned = rnd(B, H, dh, T, seed=2).transpose(2, 3)
+    shared = rnd(B, 1, T, dh, seed=3).expand(B, H, T, dh)
+    odd = rnd(B * H * T * dh + 1, seed=4)[1:].view(B, H, T, dh)
+    for k, v in ((wide[..., 1:], wide[..., :dh]), (shared, turned), (odd, odd), (odd.float(), wide[..., 1:])):
+        a, b = state(cfg, B, H, dh, 64, 0), state(cfg, B, H, dh, 64, 0)
+        a.fill(k, v)
+        b.fill(k.contiguous().clone(), v.contiguous().clone())
+        assert torch.equal(a.cache8.pool.view(torch.uint8), b.cache8.pool.view(torch.uint8))
+        for x, y in zip(a.dense_kv(1, T) + tuple(node_arrays(a)), b.dense_kv(1, T) + tuple(node_arrays(b))):
+            assert torch.equal(x, y)

@@ -23,7 +23,9 @@ the selected leaf blocks + own leaf block + static keys with its merge.  With ne
 reference's default) the candidate list of engine.py:107-114 is built on the device and attended by the
 candidate-list kernel.
 """
+import functools
 import math
+import operator
 
 import torch
 import torch.nn.functional as F
@@ -35,6 +37,15 @@ from .forest import gather_nodes
 
 def _ln(x, w):
     return F.layer_norm(x, (x.shape[-1],), w, None, 1e-5)
+
+
+def _rows16(x):
+    """x (.., T, dh), or a contiguous copy of it where its rows are not whole 16-byte pieces of memory (as kernels that read a
+    prompt's rows need them; the rows of a projection are)."""
+    z = x.element_size()
+    if x.stride(-1) == 1 and (x.data_ptr() | functools.reduce(operator.or_, x.stride()[:-1]) * z) % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 class PagePool:
@@ -185,7 +196,8 @@ class SegState:
         """Store positions 0..T-1 of sequences b0.. from k, v (n, H, T, dh) (a prompt's keys and values)."""
         n, H, T, dh = k.shape
         if self.cache8 is not None:
-            K.kv8_fill(k.to(self.dtype), v.to(self.dtype), self.cache8.rows(b0, b0 + n))
+            k, v = (_rows16(x.to(self.dtype)) for x in (k, v))
+            K.kv8_fill(k, v, self.cache8.rows(b0, b0 + n))
             return
         if self.cache is None:
             self.K[b0:b0 + n, :, :T].copy_(k)
