@@ -8,13 +8,16 @@
 //
 // One pass over the keys with a running maximum and sum.  A key row is D bytes, so D / 16 lanes hold a row, a load brings 64 *
 // 16 / D keys' K or V, and a chunk is two of each; four chunks are in flight.  No matrix instruction: one query a page
-// leaves 15 of a tile's 16 rows idle, and the vector units are far from the limit.
+// leaves 15 of a tile's 16 rows idle, and the vector units are busy 30 % of a launch of many queries.
 //
-// Many queries are bound by the bytes, 2 D a key: 32 x 12 queries over 2048 + 32 keys of 64 (102 MB) take 25 us, 4.1 TB/s of
-// about 4.8 that reads alone reach here (the unquantised cache's 204 MB take 40.5 us).  Few queries are bound by a chain of
-// round trips -- position and leaf ids, page table, scales with the keys, the workgroups' partials and their join: 12
-// queries over 8192 keys of 64 by 64 wavefronts each 12.8 us (12.7 MB; 14.1 with the tail's rows requested behind the keys,
-// the page reads behind the count of the valid leaves and sums across lanes by shuffles).
+// Many queries are bound by the bytes, 2 D a key: 32 x 12 queries over 2048 + 32 keys of 64 (102 MB) take 25 us, 4.1 TB/s; as
+// many workgroups that do nothing but read such pages take 21 (the unquantised cache's 204 MB take 40.5 us).  Few queries
+// have one wavefront to a SIMD, so that nothing runs beside its waits and its instructions: 12 queries over 8192 keys of 64
+// by 64 wavefronts each take 12.8 us (12.7 MB), of which a wavefront waits 52 % -- a chain of round trips: position and leaf
+// ids, page table, scales with the keys, the workgroups' partials and their join -- and issues instructions 42 %: its key
+// list, which every wavefront makes for itself, four or five chunks of keys and as many requests past the last key, the sums
+// across lanes (14.1 us with the tail's rows requested behind the keys, the page reads behind the count of the valid leaves
+// and sums across lanes by shuffles).
 //
 // Reference functions replaced: engine.py:107-119 (decode attention).
 #include "attn.hpp"

@@ -67,8 +67,8 @@ __device__ __forceinline__ void store_e4m3(uint8_t* dst, const float (&f)[vec_el
 }
 
 // One workgroup per (sequence, head).  A row is 2 D values, so what a call costs is a launch and its round trips (position,
-// page, tag, then the rows): 32 x 12 rows of 64 bf16 3.4 us.  The call that ends a block reads it once more from L2: its
-// sums by runs of rows beside the rounding, 6 blocks of 32 x 64 float32 6.6 us (8.8 with the sums by one thread a
+// page, tag, then the rows): 32 x 12 rows of 64 bf16 3.6 us.  The call that ends a block reads it once more from L2: its
+// sums by runs of rows beside the rounding, 6 blocks of 32 x 64 float32 6.5 us (8.8 with the sums by one thread a
 // dimension and a second read for the rounding).
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8 c, const T* __restrict__ kn,

@@ -4,7 +4,7 @@
 // largest number, 6, being 2), so the scaled values lie in (-8, 8); each is rounded to the nearest of 0, .5, 1, 1.5, 2,
 // 3, 4, 6 (ties to the even code) and saturates at 6.  Scaling by a power of two is exact.
 //
-// Bound by the bytes: 16384 x 4096 float32 with its rounded values written beside the codes (573 MB) in 116 us, 4.9 TB/s
+// Bound by the bytes: 16384 x 4096 float32 with its rounded values written beside the codes (573 MB) in 118 us, 4.9 TB/s
 // (a large copy reaches 5.1 to 5.7 here); 37 x 1000 bf16 3.3 us, a launch and a round trip.  Eight values a thread are one
 // or two 16-byte loads and one dword of codes, a block's largest magnitude two exchanges between neighbouring lanes.
 #include "mx4.hpp"

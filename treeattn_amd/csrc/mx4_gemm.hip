@@ -12,12 +12,14 @@
 // bytes of codes and one scale serve its two instructions.  Rows and tiles past the last repeat it and are not stored; what
 // a step has past K is read as zeros.
 //
-// Bound by the matrix instructions and what feeds them.  bf16 X, 2001 x 2048 x 8192: 53 to 59 us, 1140 to 1260 TFLOP/s (a
-// large library product of bf16 matrices reaches 1390 here); the instructions are busy 46 % of the time, the rest is the
-// phases' barriers, the conversions and a fixed part (start, first copies, 32 MB of results).  Both in 4 bits, 4096 x 4096 x
-// 8192: 74 us, 3.7 PFLOP/s of the 8.9 that the instructions alone reach from registers: about 31 us of instructions, 8 of
-// barriers, 15 of the fixed part (67 MB of results) and 20 in which LDS reads, copies and instructions hold each other up.  The
-// clock is part of it: fifty calls in a row take 88 us each on random values and 67 on zeros.  Four wavefronts of 128 x
+// Bound by the matrix instructions and what feeds them.  Times are medians of kernel traces, calls of several inputs in turn
+// (many calls of one input in a row differ by the clock and by what stays in the caches).  bf16 X, 2001 x 2048 x 8192: 58 us,
+// 1157 TFLOP/s (a large library product of bf16 matrices 1377 on that card, twenty in a row); the instructions are busy 46 %
+// of the time, the rest is the phases' barriers, the conversions and a fixed part (start, first copies, 32 MB of results).  Both
+// in 4 bits, 4096 x 4096 x 8192: 74 us, 3.7 PFLOP/s of the 8.5 to 9.6 that the instructions alone reach from registers: about
+// 31 us of instructions, 8 of barriers, 15 of the fixed part (67 MB of results) and 20 in which LDS reads, copies and
+// instructions hold each other up.  The clock is part of it: fifty such products of one input in a row take 87 us each on
+// random values and 66 on zeros.  Four wavefronts of 128 x
 // 128, one to a SIMD with the next operands read during a step's instructions (two thirds of the LDS reads, one barrier a
 // step), took 82 us.
 #include "mx4.hpp"
@@ -431,7 +433,8 @@ int launch_gemm(GemmArgs a, int epilogue, hipStream_t st) {
   a.vec = a.ldy % 4 == 0 && (uintptr_t)a.Y % 8 == 0 && (a.R == nullptr || (a.ldr % 4 == 0 && (uintptr_t)a.R % 8 == 0));
   // Rounds of tiles over the compute units: one of 256 x 256 tiles takes about three of 128 x 128 (bf16 X, N 8192, K 4096;
   // M 1024: 97 against 70 us, 1536: 101 against 108, 2048: 108 against 140, 2304, whose 288 large tiles are two rounds: 193
-  // against 167.  Both in 4 bits: 35 and 27, 36.9 and 37.4, 38.6 and 46.8, 65 and 56 us).
+  // against 167.  Both in 4 bits: 35 and 27, 36.9 and 37.4, 38.6 and 46.8, 65 and 56 us).  Few rows of 4 bits have no form of
+  // their own: 1 to 128 rows x 4096 x 4096 or 16384 take 15 to 16 us, a workgroup's whole walk along K.
   const int64_t cus = device_cus(), rounds = ((int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) + cus - 1) / cus,
                 small = ((int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128) + cus - 1) / cus;
   if (small < 3 * rounds) return launch_tile<BOTH, 4, 2, false>(a, epilogue, st);
@@ -444,8 +447,8 @@ int launch_gemm(GemmArgs a, int epilogue, hipStream_t st) {
 // at a whole tile).
 int mx4_gemm_bf16(const void* X, int64_t ldx, int parts, const void* Wp, const uint8_t* Ws, void* Y, int64_t ldy,
                   const void* R, int64_t ldr, int M, int N, int K, int epilogue, hipStream_t st) {
-  GemmArgs a{(const char*)X, ldx * 2, nullptr, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N, K * parts,
-             mx4_padded(K) / 128, (K + 63) / 64, 0, 0, 0};
+  GemmArgs a{(const char*)X, ldx * 2, nullptr, (const char*)Wp, Ws, (bf16_t*)Y, ldy, (const bf16_t*)R, ldr, M, N,
+             (int)((int64_t)K * parts), mx4_padded(K) / 128, (K + 63) / 64, 0, 0, 0};
   return launch_gemm<false>(a, epilogue, st);
 }
 

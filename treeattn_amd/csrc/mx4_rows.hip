@@ -15,15 +15,15 @@
 //
 // A LayerNorm of short rows (kFused values in all) happens on the way: the workgroup reads X once, 16 or 32 lanes a row,
 // and leaves it normalised in LDS for its wavefronts.  Every workgroup does that for itself, so longer rows are normalised
-// once by a kernel of their own, into the workspace.  The matrix instructions take bf16, and a normalised value rounded to
-// it would be as far off as the result's own rounding: it is held as two of them, its upper half and what that leaves
-// (2^-16 of the value is lost), and both are multiplied.
+// once by a kernel of their own, into the workspace, from where they go straight to the lanes' registers.  The matrix
+// instructions take bf16, and a normalised value rounded to it would be as far off as the result's own rounding: it is held
+// as two of them, its upper half and what that leaves (2^-16 of the value is lost), and both are multiplied.
 //
 // 32 x 4096 x 16384 (35.7 MB of weights) takes 12.4 us, 2.9 TB/s; a floor of 6.5 us at a large copy's rate.  What is left is
 // the start (the first weights' round trip), X (every workgroup reads all of it from L2 and turns it round in LDS, twice the
-// weights' bytes) and the sums of eight wavefronts at the end.  With a LayerNorm in front it takes 15.2 us and the LayerNorm
-// 4.2 (12.4 and 3.6 with its rows rounded to bf16, which made the results' error 1.4 times as large): X is twice the bytes and
-// instructions.  1 x 1024 x 1024 takes 3.1 us, a launch with one round trip.
+// weights' bytes) and the sums of eight wavefronts at the end.  With a LayerNorm in front it takes 15.0 us and the LayerNorm
+// 4.3 (12.4 and 3.5 with its rows rounded to bf16, which made the results' error 1.4 times as large): X has twice the bytes and
+// instructions.  1 x 1024 x 1024 takes 3.3 us, a launch with one round trip.
 #include "mx4.hpp"
 
 namespace ta {
@@ -34,7 +34,7 @@ int mx4_gemm_bf16(const void* X, int64_t ldx, int parts, const void* Wp, const u
 namespace {
 
 struct RowsArgs {
-  const bf16_t* X;       // PARTS: vector c (of 8 values) of row r, in 16-byte units, at c * M + r, the lower halves Kp / 8 * M on
+  const bf16_t* X;       // X_PARTS: 16-byte unit c * M + r is vector c (of 8 values) of row r, the lower halves Kp / 8 * M on
   int64_t ldx;
   const char* W;         // tiles of 1024 bytes
   const uint8_t* S;      // scales, 256 bytes for four tiles one below the other
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a, int ny) 
 
 // LayerNorm of one row per workgroup, from X to Y, as upper and lower halves, zeros from K to Kp: vector c (of 8 values) of
 // row r at byte c * vs + r * rs, the lower half's Kp / 8 vectors on.  Up to 16384 values are held in registers, longer rows
-// read again.  The mean, then the squares about it.  32 x 4096: 4.2 us, a launch with one read and two joined sums.
+// read again.  The mean, then the squares about it.  32 x 4096: 4.3 us, a launch with one read and two joined sums.
 __global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, char* __restrict__ Y, int64_t rs, int64_t vs) {
   __shared__ float s_red[2][kWaves8];
   const int tid = threadIdx.x;
@@ -338,8 +338,10 @@ __global__ __launch_bounds__(kThreads) void mx4_norm_kernel(RowsArgs a, char* __
 }
 
 // Whether the product runs as workgroups of 32 rows or as tiles of many rows (mx4_gemm.hip).  The former cost about 8.5 us
-// at K = 4096 for every compute unit's worth of workgroups (512 x 4096 x 4096: 1024 of them, 36 us; 128 x 16384: 1024, 42 us;
-// 256 x 16384: 2048, 72 us), the latter's 128 x 128 tiles 50 us up to two for a unit.
+// at K = 4096 for every compute unit's worth of workgroups (512 x 4096 x 4096: 1024 of them, 36 us; 128 x 16384: 1024, 40 us;
+// 256 x 16384: 2048, 72 us), the latter's 128 x 128 tiles 50 us up to two for a unit.  (Measured at that K alone.  Every
+// 32 rows read and convert the weights anew, and 128 x 128 tiles leave half the rate: between 65 and about 512 rows both are
+// two to three and a half times their floors.)
 bool few_rows(int M, int N) { return M <= 64 || (int64_t)((M + 31) / 32) * ((N + 63) / 64) <= 5 * (int64_t)device_cus(); }
 
 // Whether ta_mx4_rows normalises M rows of K values within the product: wherever a workgroup's LDS holds them (32 x 768 x
@@ -350,7 +352,8 @@ bool norm_fused(int M, int K) { return M <= 64 && (int64_t)(M <= 16 ? 16 : 32) *
 template <int MT, int CT, int SRC, int EPI>
 int launch_one(const RowsArgs& a, hipStream_t st) {
   constexpr int R = MT * 16, COLS = 16 * CT;
-  const int x = SRC == X_NORM ? a.Kp / 128 * R * 512 : SRC == X_ROWS ? kWaves8 * R * 256 : 0, red = kWaves8 * R * (COLS + 1) * 4;
+  const int x = SRC == X_NORM ? a.Kp / 128 * R * 512 : SRC == X_ROWS ? kWaves8 * R * 256 : 0;
+  const int red = kWaves8 * R * (COLS + 1) * 4;
   const int ny = (a.M + R - 1) / R;
   const dim3 grid((unsigned)((a.N + COLS - 1) / COLS * ny)), blk(kThreads);
   hipLaunchKernelGGL((mx4_rows_kernel<MT, CT, SRC, EPI>), grid, blk, x > red ? x : red, st, a, ny);

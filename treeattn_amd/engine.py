@@ -375,7 +375,7 @@ def decode_nsplit(B, H, wl, leaf):
 
 def decode_nsplit8(B, H, Nq, wl, leaf):
     """decode_nsplit for a cache of 8-bit pages (kernels.seg_attn8) and Nq queries per (sequence, head): the same workgroups
-    (384 queries over 2k keys 25 us at one each, 12 queries over 8k keys 13.0 us at 16 each), and one wavefront a query
+    (384 queries over 2k keys 25 us at one each, 12 queries over 8k keys 12.8 us at 16 each), and one wavefront a query
     where those fill the GPU several times over: 48 heads x 32 queries over 1k keys 36.1 us with a workgroup each and
     38.9 with a wavefront, x 128 queries 112.8 and 98.6, x 512 399 and 313."""
     return 1 if B * H * Nq >= 4096 else decode_nsplit(B, H * Nq, wl, leaf)
