@@ -76,6 +76,20 @@ def test_least_workspace(M, N, Kd):
     assert torch.equal(r, want) and (ws[nbytes:] == 0x5a).all()
 
 
+def test_many_rows_in_several_passes():
+    """A prompt whose normalised rows do not fit the wrapper's workspace: the rows on both sides of a pass's border, the first and
+    the last."""
+    M, N, Kd = 70000, 24, 2048
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(M, Kd, generator=gen, device=DEV, dtype=BF16)
+    w, wv = K.mx4_quant(rnd(N, Kd, seed=2, scale=1 / math.sqrt(Kd)).to(DEV), values=True)
+    g = (1 + 0.2 * rnd(Kd, seed=4)).to(BF16)
+    fit = L.lib().ta_mx4_rows_workspace_size(M, Kd, 1) // (4 * Kd)
+    assert fit < M
+    at = torch.tensor([0, 1, fit - 1, fit, fit + 1, M - 2, M - 1], device=DEV)
+    close(K.mx4_mm(x, w, ln_w=g.to(DEV))[at], *O.layernorm_product(x[at].cpu(), wv.cpu(), g, EPS))
+
+
 @pytest.mark.parametrize('M,Kd', [(2, 256), (20, 2048), (70, 128)])
 def test_infinities_and_constant_rows(M, Kd):
     """A weight that takes a value past bf16's range gives an infinity of its sign, not NaN, in that row's products; a row of

@@ -1298,8 +1298,8 @@ def mx4_mm(x, w, ln_w=None, eps=1e-5, epilogue=None, residual=None, out=None):
     if ln_w is not None:
         gp = ln_w.data_ptr()
         nbytes = L.lib().ta_mx4_rows_workspace_size(M, K, 1)
-        if nbytes:
-            nbytes = 4 * M * ((K + 127) // 128 * 128)   # all rows in one pass
+        if nbytes:   # all rows in one pass, as long as that is 256 MiB (16384 rows of 4096 values) or what has to be there
+            nbytes = max(nbytes, min(4 * M * ((K + 127) // 128 * 128), 1 << 28))
             ws = w._buf.new_empty((nbytes,))
     _mx4_rows(dev, at, ldx, w.at, w.scale_at, out.data_ptr(), ldo, rp, ldr, gp, eps, M, N, K, epi,
               ws.data_ptr() if nbytes else None, nbytes)
