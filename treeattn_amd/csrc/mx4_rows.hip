@@ -430,12 +430,12 @@ extern "C" int ta_mx4_rows(const void* X, int64_t ldx, const void* Wp, const uin
     }
     // as many rows at a time as the workspace holds (the results do not depend on how many)
     const int fit = ws_bytes / row < M ? (int)(ws_bytes / row) : M;
-    for (int m = 0; m < M; m += fit) {
+    for (int64_t m = 0; m < M; m += fit) {
       RowsArgs c = a;
       c.X += m * ldx;
       c.Y += m * ldy;
       if (R != nullptr) c.R += m * ldr;
-      c.M = M - m < fit ? M - m : fit;
+      c.M = M - m < fit ? (int)(M - m) : fit;
       hipLaunchKernelGGL(mx4_norm_kernel, dim3((unsigned)c.M), dim3(kThreads), 0, st, c, (char*)ws, few ? 16 : row,
                          few ? (int64_t)c.M * 16 : 16);
       int rc = check_launch("mx4_norm_kernel");
