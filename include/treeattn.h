@@ -149,6 +149,55 @@ int ta_seg_attn8_fwd(const void* q, int dtype, int64_t qsb, int64_t qsh, int64_t
                      float* ws, int64_t ws_bytes, void* stream);
 
 /*
+ * Attention of new tokens over a whole decode cache (engine.py:74-81, DenseState.attend): q (B, Hq, Nq, D) at positions
+ * tq[b*tq_sb + n] over the keys 0 .. tq of k, v (B, H, Tk, D), or of the pages (which hold Tk positions a sequence; the
+ * K/V sequence and head strides are then not used).  Query head h reads key head h / (Hq / H).  Keys of a block without a
+ * page do not count; a query at a position outside [0, Tk), or without a key, gives zeros and lse -1e30.  What stands in
+ * rows past a query's position has no effect on it, whatever it is.  D 16, 32, 64 or 128; q, K and V rows 16-byte aligned.
+ * nsplit: wavefronts that share the keys of one set of 16 query rows (the Hq / H heads of a key head times Nq): 1, or a
+ * multiple of 4 up to 1024; past 4 it needs ws, 256-byte aligned, of ta_dense_attn_workspace_size bytes, zero-filled once
+ * (each call leaves its counters at zero; calls that share it are of one size and do not overlap in time, two captured
+ * graphs included).  lse (B, Hq, Nq) may be NULL.
+ */
+int64_t ta_dense_attn_workspace_size(int B, int Hq, int H, int Nq, int D, int nsplit);
+int ta_dense_attn_fwd(const void* q, const void* k, const void* v, int dtype, int64_t qsb, int64_t qsh, int64_t qsn,
+                      int64_t ksb, int64_t ksh, int64_t kst, int64_t vsb, int64_t vsh, int64_t vst, int B, int Hq, int H,
+                      int Nq, int D, int Tk, const int32_t* tq, int64_t tq_sb, float scale, void* out, int64_t osb,
+                      int64_t osh, int64_t osn, float* lse, int nsplit, float* ws, int64_t ws_bytes,
+                      const ta_kv_pages* pages, void* stream);
+
+/*
+ * Rotary positions: y (B, H, T, D) = x with the first rot (even) elements of every row turned in pairs by its position's
+ * angles, the others as they are.  Pair i of a row at position t = pos[b*pos_sb + n] is elements (i, i + rot/2), or with
+ * interleaved (2i, 2i + 1): (a, c) becomes amp * (a cos - c sin, a sin + c cos) of the angle 2 pi t turns[i] (float64, on the
+ * device; the product is taken modulo 1 in float64).  inverse: by the negative angle, with the same amp (the gradient).  y may
+ * be x with the same strides; else the two do not overlap.
+ */
+int ta_rope(const void* x, int dtype, int64_t xsb, int64_t xsh, int64_t xst, void* y, int64_t ysb, int64_t ysh, int64_t yst,
+            int B, int H, int T, int D, int rot, const double* turns, int interleaved, float amp, int inverse,
+            const int32_t* pos, int64_t pos_sb, void* stream);
+
+/*
+ * N new tokens of every sequence into a decode cache (engine.py:41-55 without the tree): row pos[b*pos_sb + n] of K and V
+ * takes k (turned as ta_rope does; rot 0: as it is) and v (B, H, N, D), and q_out (B, Hq, N, D) takes q turned (Hq 0: no
+ * queries; q_out may be q with the same strides).  A position outside [0, Tcap) or in a block without a page is not stored
+ * (its query is turned all the same).  The positions of a sequence in one call are distinct.  K and V share their strides.
+ */
+int ta_kv_store(const void* k, const void* v, int dtype, int64_t ksb, int64_t ksh, int64_t kst, int64_t vsb, int64_t vsh,
+                int64_t vst, const void* q, int64_t qsb, int64_t qsh, int64_t qst, void* q_out, int64_t osb, int64_t osh,
+                int64_t ost, int Hq, void* Kc, void* Vc, int64_t csb, int64_t csh, int64_t cst, int B, int H, int N, int D,
+                int Tcap, const int32_t* pos, int64_t pos_sb, int rot, const double* turns, int interleaved, float amp,
+                const ta_kv_pages* pages, void* stream);
+
+/*
+ * Rows of n tensors copied by one list: row dst[i] of to[k] takes row src[i] of from[k], i < pairs (src, dst on the device),
+ * for tensors of from_rows[k] and to_rows[k] rows of row_bytes[k] bytes, one after another.  to[k] may be from[k].  A pair
+ * with an id outside its tensor copies nothing.  No two pairs have the same dst, and where to[k] is from[k] no dst is a src.
+ */
+int ta_copy_rows(int n, const void* const* from, void* const* to, const int64_t* row_bytes, const int64_t* from_rows,
+                 const int64_t* to_rows, const int32_t* src, const int32_t* dst, int pairs, void* stream);
+
+/*
  * Rows of microscaled 4-bit floats (the OCP MX format, e2m1 values): blocks of 32 along a row share a scale
  * 2^(byte - 127), two values a byte, the lower index in the low half.  Rows are kept as tiles of 16 rows by 128 values:
  * with steps = ceil(K / 128), tile t * steps + s holds rows 16t .. 16t + 15 and values 128s .. 128s + 127 as 64 blocks of 16

@@ -140,6 +140,15 @@ SIGNATURES = {
     'ta_mx4_rows': (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_f32, c_i32, c_i32, c_i32, c_i32,
                             c_vp, c_i64, c_vp]),
     'ta_mx4_both': (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp]),
+    'ta_dense_attn_workspace_size': (c_i64, [c_i32] * 6),
+    'ta_dense_attn_fwd': (c_i32, [c_vp, c_vp, c_vp, c_i32] + [c_i64] * 9 + [c_i32] * 6 + [c_vp, c_i64, c_f32, c_vp, c_i64,
+                                  c_i64, c_i64, c_vp, c_i32, c_vp, c_i64, _P(KvPages), c_vp]),
+    'ta_rope': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64] + [c_i32] * 5
+                + [c_vp, c_i32, c_f32, c_i32, c_vp, c_i64, c_vp]),
+    'ta_kv_store': (c_i32, [c_vp, c_vp, c_i32] + [c_i64] * 6 + [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_i32,
+                            c_vp, c_vp, c_i64, c_i64, c_i64] + [c_i32] * 5
+                    + [c_vp, c_i64, c_i32, c_vp, c_i32, c_f32, _P(KvPages), c_vp]),
+    'ta_copy_rows': (c_i32, [c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp]),
     'ta_argmax_rows': (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp]),
     'ta_embed': (c_i32, [c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i64, c_i64, c_vp,
                          c_i64, c_vp, c_vp, c_f32, c_vp, c_i64, c_vp]),

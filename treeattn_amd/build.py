@@ -42,6 +42,9 @@ SOURCES = {
     'mx4.hip': [],
     'mx4_rows.hip': [],
     'mx4_gemm.hip': [],
+    'dense_attn.hip': [],
+    'rope.hip': [],
+    'copy_rows.hip': [],
 }
 
 COMMON = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function',

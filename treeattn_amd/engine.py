@@ -381,6 +381,12 @@ def decode_nsplit8(B, H, Nq, wl, leaf):
     return 1 if B * H * Nq >= 4096 else decode_nsplit(B, H * Nq, wl, leaf)
 
 
+def decode_nsplit_dense(B, H, rows, keys, D=64):
+    """dense_attn's nsplit for B * H (sequence, key head) pairs of `rows` query rows (query heads of a key head times tokens)
+    over up to `keys` keys."""
+    return 1
+
+
 def _budget_weights(state, pw):
     """The budget head's weights as ta_budget_head takes them (float32, W1 transposed, classes int32), prepared
     once per layer state and kept while the same weight dict is passed."""

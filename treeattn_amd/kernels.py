@@ -1154,6 +1154,215 @@ def seg_attn8(q, cache, tq, ids, vld, n_tree, local, scale, out=None, lse=None, 
     return out, lse, keys
 
 
+# ----------------------------------------------------------------------------------------------- the whole cache
+_dense_attn_fwd = L.entry('ta_dense_attn_fwd')
+_rope = L.entry('ta_rope')
+_kv_store = L.entry('ta_kv_store')
+_copy_rows = L.entry('ta_copy_rows')
+
+
+def _positions(name, pos, B, N):
+    """pos as int32 (N,) or (B, N) contiguous, and its sequence stride."""
+    if pos.dtype != torch.int32 or not pos.is_contiguous():
+        if pos.dtype not in (torch.int32, torch.int64):
+            raise TypeError('%s: positions int32 (or int64)' % name)
+        pos = pos.to(torch.int32).contiguous()
+    if pos.shape == (B, N):
+        return pos, N
+    if pos.shape == (N,):
+        return pos, 0
+    raise ValueError('%s: positions (N,) or (B, N) for N = %d tokens of %d sequences, got %s' % (name, N, B, tuple(pos.shape)))
+
+
+def dense_attn_workspace(B, Hq, Nq, D, nsplit, device, kv_heads=None):
+    """Zero-filled workspace for dense_attn with `nsplit` over a cache of kv_heads heads (default Hq; any gives enough for
+    fewer), None when none is needed.  Calls that share it are of one size and do not overlap in time."""
+    nbytes = L.lib().ta_dense_attn_workspace_size(B, Hq, kv_heads or Hq, Nq, D, nsplit)
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def dense_attn(q, k, v, tq, scale=None, out=None, lse=None, nsplit=1, ws=None):
+    """Attention over the whole cache: q (B,Hq,Nq,D) at positions tq ((Nq,) or (B,Nq)) over every key 0 .. tq of k, v
+    (B,H,Tk,D) or of a PagedCache (as k; v None), Hq a multiple of H (query head h reads key head h // (Hq // H)).  Keys of a
+    block without a page do not count; a query without any key, or at a position outside [0, Tk), gives zeros and lse -1e30.
+    lse: None, or (B,Hq,Nq) float32 to receive the log-sum-exp.  nsplit: wavefronts that share the keys of 16 query rows, 1 or
+    a multiple of 4 up to 1024 (engine.decode_nsplit_dense chooses); past 4 with a workspace (dense_attn_workspace).  Returns
+    (out in q's dtype, lse)."""
+    dev = L.device_index(q)
+    B, Hq, Nq, D = shape = q.shape
+    qt = q.stride()
+    paged = isinstance(k, PagedCache)
+    if paged:
+        if v is not None:
+            raise ValueError('dense_attn: v is None with a PagedCache')
+        Bk, H, Dk, Tk, dt = k.B, k.H, k.D, k.tcap, k.dtype
+        kt = vt = (0, 0, D)
+        ka, va, pages = k.k, k.v, ctypes.byref(k.desc)
+    else:
+        Bk, H, Tk, Dk = k.shape
+        if v.shape != k.shape or v.dtype != k.dtype or k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError('dense_attn: k and v (B, H, Tk, D) of one dtype, the last dimension contiguous')
+        dt, kt, vt, ka, va, pages = k.dtype, k.stride(), v.stride(), k, v, None
+    if Bk != B or Dk != D or H < 1 or Hq % H or qt[3] != 1:
+        raise ValueError('dense_attn: q (B, Hq, Nq, D) with the cache\'s %d sequences and head size %d, Hq a multiple of its %d '
+                         'heads, the last dimension contiguous, got %s' % (Bk, Dk, H, tuple(shape)))
+    if q.dtype != dt:
+        raise TypeError('dense_attn: q must have the cache dtype %s' % dt)
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dt or out.stride(3) != 1:
+        raise ValueError('dense_attn: out must have the shape and dtype of q, the last dimension contiguous')
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq, Nq) or not lse.is_contiguous()):
+        raise ValueError('dense_attn: lse (B, Hq, Nq) float32, contiguous')
+    tq, tq_sb = _positions('dense_attn', tq, B, Nq)
+    if ws is None and nsplit > 4:
+        ws = dense_attn_workspace(B, Hq, Nq, D, nsplit, q.device, H)
+    _on('dense_attn', dev, ka, va, tq, out, lse, ws)
+    if not Tk:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(-1e30)
+        return out, lse
+    ot = out.stride()
+    _dense_attn_fwd(dev, q.data_ptr(), ka.data_ptr(), va.data_ptr(), L.dtype_code(q), qt[0], qt[1], qt[2], kt[0], kt[1], kt[2],
+                    vt[0], vt[1], vt[2], B, Hq, H, Nq, D, Tk, tq.data_ptr(), tq_sb, D ** -0.5 if scale is None else scale,
+                    out.data_ptr(), ot[0], ot[1], ot[2], lse.data_ptr() if lse is not None else None, nsplit,
+                    ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, pages)
+    return out, lse
+
+
+class Rope:
+    """Rotary positions: inv_freq, the angle in radians of each pair of a head for one position (float64: a sequence or a
+    tensor; 2 * len(inv_freq) elements of a head are turned, the rest left), the layout of the pairs ('half': elements i and
+    i + len(inv_freq); 'interleaved': 2i and 2i + 1) and the amplitude, a factor on what is turned.  positions.rope_frequencies
+    gives the usual frequencies."""
+
+    def __init__(self, inv_freq, device, layout='half', amplitude=1.0):
+        if layout not in ('half', 'interleaved'):
+            raise ValueError("Rope: layout 'half' or 'interleaved'")
+        w = torch.as_tensor(inv_freq, dtype=torch.float64)
+        if w.dim() != 1 or not len(w) or not bool(torch.isfinite(w).all()) or not math.isfinite(amplitude):
+            raise ValueError('Rope: one finite frequency a pair, and a finite amplitude')
+        self.turns = (w / (2 * math.pi)).to(device).contiguous()
+        self.rot, self.layout, self.amplitude = 2 * len(w), layout, float(amplitude)
+        self.interleaved = int(layout == 'interleaved')
+
+
+def rope(x, pos, rope, out=None, inverse=False):
+    """x (B,H,T,D) with every row turned by its position's angles (pos (T,) or (B,T)); inverse: turned back (the gradient: the
+    amplitude is applied again, not taken back).  out: None, x itself (in place) or a tensor that does not overlap it."""
+    dev = L.device_index(x)
+    B, H, T, D = shape = x.shape
+    xt = x.stride()
+    if rope.rot > D or xt[3] != 1:
+        raise ValueError('rope: x (B, H, T, D) with a contiguous last dimension of at least %d' % rope.rot)
+    if out is None:
+        out = _grad_rows(x, torch.empty, x.dtype)
+    elif out.shape != shape or out.dtype != x.dtype or out.stride(3) != 1:
+        raise ValueError('rope: out must have the shape and dtype of x, the last dimension contiguous')
+    _own_rows('rope', x, out)
+    pos, pos_sb = _positions('rope', pos, B, T)
+    _on('rope', dev, pos, out, rope.turns)
+    if not x.numel():
+        return out
+    ot = out.stride()
+    _rope(dev, x.data_ptr(), L.dtype_code(x), xt[0], xt[1], xt[2], out.data_ptr(), ot[0], ot[1], ot[2], B, H, T, D, rope.rot,
+          rope.turns.data_ptr(), rope.interleaved, rope.amplitude, int(inverse), pos.data_ptr(), pos_sb)
+    return out
+
+
+def _own_rows(name, x, out):
+    """out is written row by row while x is read: it repeats no row of its own, and where it starts at x it is x."""
+    if any(s > 1 and t == 0 for s, t in zip(out.shape, out.stride())):
+        raise ValueError('%s: out repeats its rows (an expanded tensor)' % name)
+    if out.data_ptr() == x.data_ptr() and out.numel() and out.stride() != x.stride():
+        raise ValueError('%s: out must be x itself or not overlap it' % name)
+
+
+def kv_store(k, v, Kc, Vc, pos, q=None, rope=None, q_out=None):
+    """New tokens of every sequence into a decode cache without a tree: rows pos ((N,) or (B,N), distinct within a sequence)
+    of the cache (Kc, Vc (B,H,Tcap,D), or a PagedCache as Kc) take k, v (B,H,N,D), the keys turned by `rope` (a Rope; None: as
+    they are).  With q (B,Hq,N,D): returns the queries turned, in q_out (q itself: in place) or a new tensor.  A position
+    outside [0, Tcap) or in a block without a page is not stored."""
+    dev = L.device_index(k)
+    B, H, N, D = k.shape
+    if isinstance(Kc, PagedCache):
+        if Vc is not None:
+            raise ValueError('kv_store: Vc is None with a PagedCache')
+        want, dt, Ka, Va = (Kc.B, Kc.H, Kc.D), Kc.dtype, Kc.k, Kc.v
+        ct, tcap, pages = (0, 0, D), Kc.tcap, ctypes.byref(Kc.desc)
+    elif isinstance(Kc, torch.Tensor):
+        if Kc.shape != Vc.shape or Kc.stride() != Vc.stride() or Kc.dtype != Vc.dtype or Kc.stride(3) != 1:
+            raise ValueError('kv_store: K and V caches (B, H, Tcap, D) need one dtype, the same strides and contiguous rows')
+        want, dt, Ka, Va = (Kc.shape[0], Kc.shape[1], Kc.shape[3]), Kc.dtype, Kc, Vc
+        ct, tcap, pages = Kc.stride(), Kc.shape[2], None
+        _own_rows('kv_store', k, Kc)
+    else:
+        raise TypeError('kv_store: contiguous caches or a PagedCache')
+    kt, vt = k.stride(), v.stride()
+    if (B, H, D) != want or v.shape != k.shape or kt[3] != 1 or vt[3] != 1:
+        raise ValueError('kv_store: k and v (B, H, N, D) of %d sequences, %d heads and head size %d, the last dimension contiguous'
+                         % want)
+    if k.dtype != dt or v.dtype != dt or (q is not None and q.dtype != dt):
+        raise TypeError('kv_store: new rows must have the cache dtype %s' % dt)
+    rot, turns, inter, amp = 0, None, 0, 1.0
+    if rope is not None:
+        if rope.rot > D:
+            raise ValueError('kv_store: the head size must be at least %d' % rope.rot)
+        rot, turns, inter, amp = rope.rot, rope.turns.data_ptr(), rope.interleaved, rope.amplitude
+        _on('kv_store', dev, rope.turns)
+    Hq, qp, op, qt, ot = 0, None, None, (0, 0, 0), (0, 0, 0)
+    if q is not None:
+        Hq = q.shape[1]
+        qt = q.stride()
+        if q.shape != (B, Hq, N, D) or qt[3] != 1:
+            raise ValueError('kv_store: q (B, Hq, N, D) beside k, the last dimension contiguous')
+        if q_out is None:
+            q_out = q.new_empty(q.shape)
+        elif q_out.shape != q.shape or q_out.dtype != dt or q_out.stride(3) != 1:
+            raise ValueError('kv_store: q_out must have the shape and dtype of q, the last dimension contiguous')
+        _own_rows('kv_store', q, q_out)
+        qp, op, ot = q.data_ptr(), q_out.data_ptr(), q_out.stride()
+    elif q_out is not None:
+        raise ValueError('kv_store: q_out without q')
+    pos, pos_sb = _positions('kv_store', pos, B, N)
+    _on('kv_store', dev, v, Ka, Va, pos, q, q_out)
+    if tcap and k.numel():
+        _kv_store(dev, k.data_ptr(), v.data_ptr(), L.dtype_code(k), kt[0], kt[1], kt[2], vt[0], vt[1], vt[2], qp, qt[0], qt[1],
+                  qt[2], op, ot[0], ot[1], ot[2], Hq, Ka.data_ptr(), Va.data_ptr(), ct[0], ct[1], ct[2], B, H, N, D, tcap,
+                  pos.data_ptr(), pos_sb, rot, turns, inter, amp, pages)
+    return q_out
+
+
+def copy_rows(tensors, src, dst, out=None):
+    """Row dst[i] of every tensor of `out` (default: of `tensors` themselves) takes row src[i] of its tensor, in as few launches
+    as there are 32 tensors: pages of all layers, their scales, a sequence's rows of the tree's state.  tensors: contiguous, any
+    dtypes and row shapes; src, dst (n,) int32 on the device.  A pair with an id outside a tensor copies nothing.  No two pairs
+    have the same dst, and within one tensor no dst is a src."""
+    if not tensors:
+        return
+    out = tensors if out is None else out
+    if len(out) != len(tensors):
+        raise ValueError('copy_rows: as many tensors out as in')
+    dev = L.device_index(src)
+    if (src.dtype != torch.int32 or dst.dtype != torch.int32 or src.dim() != 1 or dst.shape != src.shape
+            or not src.is_contiguous() or not dst.is_contiguous()):
+        raise ValueError('copy_rows: src and dst (n,) int32, contiguous')
+    size, fr, tr = [], [], []
+    for x, y in zip(tensors, out):
+        if (x.dtype != y.dtype or x.dim() < 1 or x.shape[1:] != y.shape[1:] or not x.is_contiguous()
+                or not y.is_contiguous()):
+            raise ValueError('copy_rows: contiguous tensors, each with the dtype and row shape of its target')
+        size.append(x.element_size() * math.prod(x.shape[1:]))
+        fr.append(x.shape[0])
+        tr.append(y.shape[0])
+    _on('copy_rows', dev, dst, *tensors, *out)
+    n = len(size)
+    pack = struct.Struct('%dq' % n).pack
+    _copy_rows(dev, n, pack(*[x.data_ptr() for x in tensors]), pack(*[y.data_ptr() for y in out]), pack(*size), pack(*fr),
+               pack(*tr), src.data_ptr(), dst.data_ptr(), src.shape[0])
+
+
 # ----------------------------------------------------------------------------------------------- 4-bit rows
 class Mx4:
     """Rows of microscaled 4-bit floats (the OCP MX format with e2m1 values): blocks of 32 along a row share a scale
