@@ -5,6 +5,21 @@
 // over the keys j = 0 .. t that have a page.  Query head h reads key head h / (Hq / H).  Scores, sums and the accumulators
 // are float32, the output is rounded once.
 //
+// One pass over the keys with a running maximum and sum, on the matrix cores even for a single query: the 16 rows of a tile
+// are the query heads of a key head times the new tokens, and what a lone row wastes of the instructions is less than the
+// vector units would take (32 keys of 64: 12 instructions of 16 cycles, against some 150 of 4).  Nothing passes through
+// LDS: with S^T = K Q^T a lane holds four scores of one query row, which are what the next product, O^T = V^T P^T, takes as
+// its B operand when that product counts the keys in the order the first leaves them in; V^T's operand is a lane's eight
+// keys at its own columns, turned round in registers; the running maximum, the sum and their corrections are then one
+// number a lane.
+//
+// Weights of 16-bit rows go into the second product as the sum of two 16-bit numbers (2^-17 of a weight is lost, where
+// one would lose 2^-9, as much as the rounding of the result).  The maximum is renewed only when a score passes it by more
+// than kSlack: until then weights are at most 2^kSlack.
+//
+// Bound by bytes, 2 D a key and key head, where rows are few; the keys of a sequence are split over wavefronts and
+// workgroups, whose partial results the last workgroup to arrive joins.
+//
 // Reference functions replaced: engine.py:74-81 (DenseState.attend).
 #include "attn.hpp"
 
@@ -31,60 +46,655 @@ struct Dense {
   const int32_t* ptab;
   int64_t pt_sb, pt_sh, pstride, npages;
   int blog2;
+  int BH, R;            // (sequence, key head) pairs; query rows of one: G * Nq
+  int gsplit;           // workgroups a set of 16 rows
+  float* ws;            // their parts (set, workgroup, row, D + 2) and
+  uint32_t* cnt;        // arrival counters (zero between calls)
 };
 
-// A wavefront a query: a lane scores a key, then holds elements lane and lane + 64 of the output.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kRows = 16;            // query rows of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T, int D> struct Tile {
+  static constexpr int EB = (int)sizeof(T);
+  static constexpr int KT = EB == 2 ? 2 : (D == 128 ? 1 : 2);   // tiles of 16 keys a step
+  static constexpr int KEYS = 16 * KT;
+  static constexpr int KS = EB == 2 ? (D + 31) / 32 : D / 16;   // 16-byte pieces of a key row a lane
+  static constexpr int DJ = D / 16;                             // columns of V a lane holds
+  static constexpr int VB = DJ * EB;                            // their bytes, of one key
+  static constexpr int VW = (VB + 3) / 4;
+  // weights are exp2(x - max + kShift): float16 keeps 2^-24 absolutely, which is far below the largest weight then
+  static constexpr float kShift = __is_same(T, f16_t) ? 10.0f : 0.0f;
+  static constexpr float kSlack = __is_same(T, f16_t) ? 4.0f : 8.0f;
+};
+
+// The keys and values of one step, in a lane: K rows 16 i + lane % 16 at pieces lane / 16; V rows 16 i + 4 (lane / 16) + u at
+// columns DJ (lane % 16) ...
+template <typename T, int D> struct Step {
+  uint4 k[Tile<T, D>::KT][Tile<T, D>::KS];
+  uint32_t v[Tile<T, D>::KT * 4][Tile<T, D>::VW];
+  uint32_t have;     // bit 4 i + u: key 16 i + 4 (lane / 16) + u has a page
+  int key0;
+};
+
 template <typename T>
-__global__ __launch_bounds__(kWave) void dense_attn_kernel(Dense p) {
-  const int lane = lane_id();
-  const int n = blockIdx.x, hq = blockIdx.y % p.Hq, b = blockIdx.y / p.Hq;
-  const int h = hq / p.G;
-  int t = p.tq[b * p.tq_sb + n];
-  if (t < 0 || t >= p.Tk) t = -1;
-  const T* q = reinterpret_cast<const T*>(p.q) + b * p.qsb + hq * p.qsh + n * p.qsn;
-  const T* kb = reinterpret_cast<const T*>(p.k) + (p.ptab ? 0 : b * p.ksb + h * p.ksh);
-  const T* vb = reinterpret_cast<const T*>(p.v) + (p.ptab ? 0 : b * p.vsb + h * p.vsh);
-  float m = kLowest, l = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int j0 = 0; j0 <= t; j0 += kWave) {
-    const int j = j0 + lane;
-    int64_t ko = -1, vo = -1;
-    if (j <= t) {
-      if (p.ptab) {
-        const int pg = p.ptab[b * p.pt_sb + h * p.pt_sh + (j >> p.blog2)];
-        const int r = j & ((1 << p.blog2) - 1);
-        if (pg >= 0 && pg < p.npages) {
-          ko = pg * p.pstride + r * p.kst;
-          vo = pg * p.pstride + r * p.vst;
-        }
-      } else {
-        ko = j * p.kst;
-        vo = j * p.vst;
+__device__ __forceinline__ f32x4 mfma32(const uint4& a, const uint4& b, f32x4 c) {
+  if constexpr (__is_same(T, f16_t))
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// two floats rounded to two elements of T, the first in the low half
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, f16_t)) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (f16x2){(_Float16)a, (_Float16)b});
+  } else {
+    return bf16_pack2(a, b);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float unpack_lo(uint32_t x) {
+  if constexpr (__is_same(T, f16_t)) return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
+  else return __uint_as_float(x << 16);
+}
+template <typename T>
+__device__ __forceinline__ float unpack_hi(uint32_t x) {
+  if constexpr (__is_same(T, f16_t)) return (float)__builtin_bit_cast(_Float16, (uint16_t)(x >> 16));
+  else return __uint_as_float(x & 0xffff0000u);
+}
+
+// The larger / the sum of x over the four lanes that share lane % 16.
+__device__ __forceinline__ float max_rows(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_rows(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// One wavefront's share: keys [k0, k1) for NT tiles of 16 query rows of one (sequence, key head).
+template <typename T, int D, bool WIDE, int NT>
+struct Share {
+  using C = Tile<T, D>;
+  const Dense& p;
+  const int lane, c, g;
+  const T* kb;
+  const T* vb;
+  const int32_t* tab;
+  int t[NT];            // the lane's row's position (pad rows: as far as any)
+  int tmin, tmax;       // of the wavefront's rows
+  int seen;             // values past this position count as zeros
+  uint4 q[NT][C::KS];
+  f32x4 acc[NT][C::DJ];
+  float m[NT], l[NT];   // the reference of the weights (max - kShift), and the lane's part of their sum
+  int pg;               // page (WIDE), or the page of key lane % 32, of the step that is fetched next
+
+  __device__ __forceinline__ Share(const Dense& p_, int b, int h, int row0)
+      : p(p_), lane(lane_id()), c(lane & 15), g(lane >> 4) {
+    kb = reinterpret_cast<const T*>(p.k) + (p.ptab ? 0 : b * p.ksb + h * p.ksh);
+    vb = reinterpret_cast<const T*>(p.v) + (p.ptab ? 0 : b * p.vsb + h * p.vsh);
+    tab = p.ptab ? p.ptab + b * p.pt_sb + h * p.pt_sh : nullptr;
+    int lo = 0x7fffffff, hi = -1;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int r = row0 + kRows * i + c;
+      const bool in = r < p.R;
+      const int j = in ? r / p.Nq : 0, n = in ? r % p.Nq : 0;
+      int tt = in ? p.tq[b * p.tq_sb + n] : 0x7fffffff;
+      if (in && (tt < 0 || tt >= p.Tk)) tt = -1;
+      t[i] = tt;
+      lo = tt < lo ? tt : lo;
+      hi = in && tt > hi ? tt : hi;
+      const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + j) * p.qsh + n * p.qsn;
+#pragma unroll
+      for (int s = 0; s < C::KS; ++s) {
+        const int d = C::EB == 2 ? 32 * s + 8 * g : 16 * s + 4 * g;
+        q[i][s] = in && d < D ? ldg16(qr + d) : make_uint4(0, 0, 0, 0);
       }
     }
-    float s = 0.0f;
-    if (ko >= 0)
-      for (int d = 0; d < p.D; ++d) s = fmaf(to_f32(q[d]), to_f32(kb[ko + d]), s);
-    s *= p.scale;
-    const float mn = fmaxf(m, wave_max(ko >= 0 ? s : kLowest));
-    const float alpha = __expf(m - mn);
-    m = mn;
-    const float w = ko >= 0 ? __expf(s - m) : 0.0f;
-    l = l * alpha + wave_sum(w);
-    acc[0] *= alpha;
-    acc[1] *= alpha;
-    for (int i = 0; i < kWave; ++i) {
-      const int64_t o = __shfl(vo, i, kWave);
-      const float wi = __shfl(w, i, kWave);
-      if (o < 0) continue;
-      if (lane < p.D) acc[0] = fmaf(wi, to_f32(vb[o + lane]), acc[0]);
-      if (lane + kWave < p.D) acc[1] = fmaf(wi, to_f32(vb[o + lane + kWave]), acc[1]);
+    reset();
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      const int a = __shfl_xor(lo, o, kWave), e = __shfl_xor(hi, o, kWave);
+      lo = a < lo ? a : lo;
+      hi = e > hi ? e : hi;
+    }
+    tmin = __builtin_amdgcn_readfirstlane(lo);
+    tmax = __builtin_amdgcn_readfirstlane(hi);
+    seen = tmax;
+  }
+
+  __device__ __forceinline__ int page_of(int key0) const {
+    if (WIDE) return tab ? tab[key0 >> p.blog2] : 0;
+    const int key = key0 + (lane & 31);
+    return tab[(key < tmax ? key : tmax) >> p.blog2];
+  }
+
+  // Requests step x's rows (keys key0 ...) from the pages in pg, and before them the pages of the step at next0.
+  __device__ __forceinline__ void fetch(Step<T, D>& x, int key0, int next0) {
+    x.key0 = key0;
+    const int mine = pg;
+    pg = page_of(next0);
+    __builtin_amdgcn_sched_barrier(0);
+    const char* kr[C::KT];
+    const char* vr[C::KT * 4];
+    if constexpr (WIDE) {
+      int64_t ko, vo;
+      bool ok = true;
+      // offsets of a step's rows in 32 bits, from one base; a contiguous cache may end inside a step: the last row that any
+      // query sees in place of those behind it
+      uint32_t klast = 0xffffffffu, vlast = 0xffffffffu;
+      const uint32_t ks = (uint32_t)p.kst * C::EB, vs = (uint32_t)p.vst * C::EB;
+      if (tab) {
+        const int page = __builtin_amdgcn_readfirstlane(mine);
+        ok = page >= 0 && page < p.npages;
+        const int64_t to = (ok ? page : 0) * p.pstride;
+        const int r = key0 & ((1 << p.blog2) - 1);
+        ko = to + r * p.kst;
+        vo = to + r * p.vst;
+      } else {
+        ko = key0 * p.kst;
+        vo = key0 * p.vst;
+        klast = (uint32_t)(tmax - key0) * ks;
+        vlast = (uint32_t)(tmax - key0) * vs;
+        if (tmax - key0 >= C::KEYS) klast = vlast = 0xffffffffu;
+      }
+      x.have = ok ? 0xffffffffu : 0u;
+      const char* k0p = reinterpret_cast<const char*>(kb + ko);
+      const char* v0p = reinterpret_cast<const char*>(vb + vo);
+#pragma unroll
+      for (int i = 0; i < C::KT; ++i) {
+        const uint32_t o = c * ks + 16 * i * ks;
+        kr[i] = k0p + (o < klast ? o : klast);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t e = 4 * g * vs + (16 * i + u) * vs;
+          vr[4 * i + u] = v0p + (e < vlast ? e : vlast);
+        }
+      }
+    } else {
+      const int mask = (1 << p.blog2) - 1;
+      x.have = 0;
+#pragma unroll
+      for (int i = 0; i < C::KT; ++i) {
+        int page = __shfl(mine, 16 * i + c, kWave);
+        page = page >= 0 && page < p.npages ? page : 0;
+        kr[i] = reinterpret_cast<const char*>(kb + page * p.pstride + (int64_t)((key0 + 16 * i + c) & mask) * p.kst);
+#pragma unroll
+        for (int u = 0; u < 4; u += 2) {
+          const int e = 16 * i + 4 * g + u;
+          int pv = __shfl(mine, e, kWave);
+          const bool ok = pv >= 0 && pv < p.npages;
+          x.have |= ok ? 3u << (4 * i + u) : 0u;
+          const T* row = vb + (ok ? pv : 0) * p.pstride;
+          vr[4 * i + u] = reinterpret_cast<const char*>(row + (int64_t)((key0 + e) & mask) * p.vst);
+          vr[4 * i + u + 1] = reinterpret_cast<const char*>(row + (int64_t)((key0 + e + 1) & mask) * p.vst);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < C::KT; ++i)
+#pragma unroll
+      for (int s = 0; s < C::KS; ++s) {
+        const int d = C::EB == 2 ? 32 * s + 8 * g : 16 * s + 4 * g;
+        x.k[i][s] = ldg16(kr[i] + (d < D ? d : 0) * C::EB);
+      }
+#pragma unroll
+    for (int e = 0; e < C::KT * 4; ++e) {
+      const char* a = vr[e] + C::VB * c;
+      if constexpr (C::VB >= 16) {
+#pragma unroll
+        for (int w = 0; w < C::VW; w += 4) *reinterpret_cast<uint4*>(&x.v[e][w]) = ldg16(a + 4 * w);
+      } else if constexpr (C::VB == 8) {
+        const u32x2 r = *(const TA_GLOBAL u32x2*)a;
+        x.v[e][0] = r.x;
+        x.v[e][1] = r.y;
+      } else if constexpr (C::VB == 4) {
+        x.v[e][0] = *(const TA_GLOBAL uint32_t*)a;
+      } else {
+        x.v[e][0] = *(const TA_GLOBAL uint16_t*)a;
+      }
     }
   }
-  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-  T* o = reinterpret_cast<T*>(p.out) + b * p.osb + hq * p.osh + n * p.osn;
-  if (lane < p.D) o[lane] = from_f32<T>(acc[0] * inv);
-  if (lane + kWave < p.D) o[lane + kWave] = from_f32<T>(acc[1] * inv);
-  if (lane == 0 && p.lse) p.lse[((int64_t)b * p.Hq + hq) * p.Nq + n] = l != 0.0f ? m + __logf(l) : kNegBig;
+
+  // Scores of tile row set i: in lane (c, g) those of row c and keys 16 a + 4 g + u.
+  __device__ __forceinline__ void scores(const Step<T, D>& x, int i, f32x4 (&s)[C::KT]) const {
+#pragma unroll
+    for (int a = 0; a < C::KT; ++a) {
+      s[a] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < C::KS; ++e) {
+        if constexpr (C::EB == 2) {
+          uint4 k = x.k[a][e];
+          if (D < 32 && g >= D / 8) k = make_uint4(0, 0, 0, 0);
+          s[a] = mfma32<T>(k, q[i][e], s[a]);
+        } else {
+          const float* kf = reinterpret_cast<const float*>(&x.k[a][e]);
+          const float* qf = reinterpret_cast<const float*>(&q[i][e]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[u], qf[u], s[a], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ bool sees(const Step<T, D>& x, int i, int a, int u) const {
+    return x.key0 + 16 * a + 4 * g + u <= t[i] && (x.have >> (4 * a + u)) & 1;
+  }
+
+  // The weights of row set i in place of its scores (0 where masked), the running maximum renewed when one passes it by more
+  // than kSlack.
+  template <bool MASKED>
+  __device__ __forceinline__ void weights(const Step<T, D>& x, int i, f32x4 (&s)[C::KT]) {
+    const float f = p.scale * kLog2e;
+    float top = kLowest;
+#pragma unroll
+    for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (!MASKED || sees(x, i, a, u)) top = fmaxf(top, s[a][u] * f);
+    if (__ballot(top > m[i] + (C::kShift + C::kSlack)) != 0) {
+      // only the rows that need it: what a row gives does not depend on the others
+      const float mx = max_rows(top);
+      const float mn = mx > m[i] + (C::kShift + C::kSlack) ? mx - C::kShift : m[i];
+      const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
+      m[i] = mn;
+      l[i] *= alpha;
+#pragma unroll
+      for (int d = 0; d < C::DJ; ++d) acc[i][d] *= alpha;
+    }
+#pragma unroll
+    for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[a][u], f, -m[i]));
+        s[a][u] = MASKED && !sees(x, i, a, u) ? 0.0f : w;
+        l[i] += s[a][u];
+      }
+  }
+
+  template <bool MASKED>
+  __device__ __forceinline__ void consume(Step<T, D>& x) {
+    if constexpr (MASKED) {
+      // values that no query sees count as zeros (0 times what stands there need not be 0)
+#pragma unroll
+      for (int e = 0; e < C::KT * 4; ++e) {
+        const bool ok = x.key0 + 16 * (e / 4) + 4 * g + e % 4 <= seen && (x.have >> e) & 1;
+#pragma unroll
+        for (int w = 0; w < C::VW; ++w) x.v[e][w] = ok ? x.v[e][w] : 0u;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      f32x4 s[C::KT];
+      scores(x, i, s);
+      weights<MASKED>(x, i, s);
+      if constexpr (C::EB == 2) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float w0 = s[e / 2][2 * (e % 2)], w1 = s[e / 2][2 * (e % 2) + 1];
+          hi[e] = pack2<T>(w0, w1);
+          lo[e] = pack2<T>(w0 - unpack_lo<T>(hi[e]), w1 - unpack_hi<T>(hi[e]));
+        }
+        const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]), pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int d = 0; d < C::DJ; ++d) {
+          uint32_t vt[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            vt[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][d / 2], x.v[2 * e][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+          const uint4 va = make_uint4(vt[0], vt[1], vt[2], vt[3]);
+          acc[i][d] = mfma32<T>(va, ph, acc[i][d]);
+          acc[i][d] = mfma32<T>(va, pl, acc[i][d]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < C::KT * 4; ++e)
+#pragma unroll
+          for (int d = 0; d < C::DJ; ++d)
+            acc[i][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[e][d]), s[e / 4][e % 4], acc[i][d], 0, 0, 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void step(Step<T, D>& x) {
+    const bool full = x.key0 + C::KEYS - 1 <= (tmin < seen ? tmin : seen) &&
+                      __ballot((x.have & ((1u << (4 * C::KT)) - 1)) != (1u << (4 * C::KT)) - 1) == 0;
+    if (full) consume<false>(x);
+    else consume<true>(x);
+  }
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      m[i] = kLowest;
+      l[i] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+
+  // Keys [k0, k1) of row set i, key by key without matrix instructions: each weight times each value of the keys the row sees,
+  // nothing else.  Lane (c, g) takes a quarter of row c.
+  __device__ __forceinline__ void careful(int i, int row0, int b, int h, int k0, int k1) {
+    m[i] = kLowest;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const int r = row0 + kRows * i + c;
+    const int j = r < p.R ? r / p.Nq : 0, n = r < p.R ? r % p.Nq : 0;
+    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + j) * p.qsh + n * p.qsn + g * (D / 4);
+    for (int key = k0; key < k1; ++key) {
+      int64_t ko = key * p.kst, vo = key * p.vst;
+      if (tab) {
+        const int page = tab[key >> p.blog2];
+        if (page < 0 || page >= p.npages) continue;
+        ko = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.kst;
+        vo = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.vst;
+      }
+      const T* kr = kb + ko + g * (D / 4);
+      const T* vr = vb + vo + g * (D / 4);
+      float s = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < D / 4; ++d) s = fmaf(to_f32(qr[d]), to_f32(kr[d]), s);
+      s = sum_rows(s) * (p.scale * kLog2e);
+      if (key > t[i] || r >= p.R) continue;
+      const float mn = fmaxf(m[i], s - C::kShift);
+      const float alpha = __builtin_amdgcn_exp2f(m[i] - mn), w = __builtin_amdgcn_exp2f(s - mn);
+      m[i] = mn;
+      l[i] = l[i] * alpha + (g == 0 ? w : 0.0f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int d = 0; d < C::DJ; ++d) acc[i][d][u] = fmaf(w, to_f32(vr[u * C::DJ + d]), acc[i][d][u] * alpha);
+    }
+  }
+
+  __device__ __forceinline__ void pass(int k0, int k1) {
+    const int last = k0 + (k1 - 1 - k0) / C::KEYS * C::KEYS;   // the last step's first key
+    auto at = [&](int n) {
+      const int key = k0 + n * C::KEYS;
+      return key < last ? key : last;
+    };
+    pg = page_of(k0);
+    // two steps in registers: one arrives while the other is used (past the last one, the last again)
+    Step<T, D> x[2];
+    fetch(x[0], at(0), at(1));
+    for (int n = 0; k0 + n * C::KEYS < k1; n += 2) {
+      fetch(x[1], at(n + 1), at(n + 2));
+      step(x[0]);
+      fetch(x[0], at(n + 2), at(n + 3));
+      if (k0 + (n + 1) * C::KEYS < k1) step(x[1]);
+    }
+  }
+
+  // The rows (bit 16 i + c) whose accumulators are not finite.
+  __device__ __forceinline__ uint32_t unsound() const {
+    uint32_t rows = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      bool bad = false;
+#pragma unroll
+      for (int d = 0; d < C::DJ; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) bad |= !(fabsf(acc[i][d][u]) < INFINITY);
+      const uint64_t w = __ballot(bad);
+      rows |= (uint32_t)((w | w >> 16 | w >> 32 | w >> 48) & 0xffff) << (16 * i);
+    }
+    return rows;
+  }
+
+  // Keys [k0, k1) for the rows of `want`; emit(mask) takes the results of some rows at a time.
+  //
+  // A value that is infinite or NaN reaches, in the matrix instructions, rows that do not see its key (as 0 times it), and comes
+  // as a sum of two products (which may be inf - inf).  So a row whose result is not finite goes through its keys again by
+  // itself, values that it does not see taken as zeros (the same sums as if they had been finite); one that is still not finite
+  // goes through them without matrix instructions.
+  template <typename Emit>
+  __device__ __forceinline__ void run(int row0, int b, int h, int k0, int k1, uint32_t want, Emit emit) {
+    int only = -1;
+    while (true) {
+      if (k0 < k1) pass(k0, k1);
+      uint32_t bad = unsound() & want, done = want & ~bad;
+      if (only >= 0) {
+        if (bad >> only & 1) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (only / kRows == i) careful(i, row0, b, h, k0, k1);
+        }
+        done = 1u << only;
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) l[i] = sum_rows(l[i]);
+      emit(done);
+      want &= ~done;
+      if (want == 0) return;
+      only = __ffs(want) - 1;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (only / kRows == i) seen = __builtin_amdgcn_readlane(t[i], only % kRows);
+      reset();
+    }
+  }
+
+  // The column of acc[.][d][u] in a row.
+  __device__ __forceinline__ int col(int d, int u) const { return C::DJ * (4 * g + u) + d; }
+};
+
+__device__ __forceinline__ void row_place(const Dense& p, int b, int h, int r, int64_t& out, int64_t& lse) {
+  const int j = r / p.Nq, n = r % p.Nq;
+  out = b * p.osb + (int64_t)(h * p.G + j) * p.osh + n * p.osn;
+  lse = ((int64_t)b * p.Hq + h * p.G + j) * p.Nq + n;
+}
+__device__ __forceinline__ float lse_of(float m, float l) { return l != 0.0f ? (m + __log2f(l)) * kLn2 : kNegBig; }
+
+// A wavefront a set of 16 NT rows, no split.
+template <typename T, int D, bool WIDE, int NT>
+__global__ __launch_bounds__(kWaves * kWave, 2) void dense_rows_kernel(Dense p) {
+  const int64_t per = (p.R + kRows * NT - 1) / (kRows * NT);
+  // consecutive sets share their keys: those of one XCD (workgroups go round robin over the 8) are consecutive
+  const unsigned n8 = gridDim.x / 8;
+  const int64_t wg = (int64_t)(blockIdx.x % 8) * n8 + blockIdx.x / 8;
+  const int64_t id = wg * kWaves + __builtin_amdgcn_readfirstlane(wave_id());
+  if (id >= per * p.BH) return;
+  const int bh = (int)(id / per), row0 = (int)(id % per) * kRows * NT;
+  const int b = bh / p.H, h = bh % p.H;
+  Share<T, D, WIDE, NT> s(p, b, h, row0);
+  const int left = p.R - row0;
+  s.run(row0, b, h, 0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1,
+        [&](uint32_t done) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int r = row0 + kRows * i + s.c;
+      if (!(done >> (kRows * i + s.c) & 1)) continue;
+      int64_t at, le;
+      row_place(p, b, h, r, at, le);
+      T* o = reinterpret_cast<T*>(p.out) + at;
+      const float inv = s.l[i] != 0.0f ? 1.0f / s.l[i] : 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[s.col(d, u)] = from_f32<T>(s.acc[i][d][u] * inv);
+      if (s.g == 0 && p.lse) p.lse[le] = lse_of(s.m[i], s.l[i]);
+    }
+  });
+}
+
+constexpr int kMinKeys = 64;         // of a wavefront
+
+// gsplit workgroups of four wavefronts a set of 16 rows.
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int KEYS = Tile<T, D>::KEYS;
+  const int tiles = (p.R + kRows - 1) / kRows;
+  const int gs = blockIdx.x % p.gsplit;
+  const int tile = blockIdx.x / p.gsplit % tiles;
+  const int bh = blockIdx.x / p.gsplit / tiles;
+  const int b = bh / p.H, h = bh % p.H;
+  const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
+  const int row0 = tile * kRows;
+  const int rows = p.R - row0 < kRows ? p.R - row0 : kRows;
+  Share<T, D, WIDE, 1> s(p, b, h, row0);
+  // equal runs of whole steps a wavefront; workgroups without one are not needed
+  const int nkeys = s.tmax + 1;
+  int run = (nkeys + p.gsplit * kWaves - 1) / (p.gsplit * kWaves);
+  run = (run < kMinKeys ? kMinKeys : run) + KEYS - 1;
+  run -= run % KEYS;
+  const int64_t wgrun = (int64_t)run * kWaves;
+  const int active = nkeys > 0 ? (int)((nkeys + wgrun - 1) / wgrun) : 1;
+  if (gs >= active) return;
+  const int64_t k0 = gs * wgrun + (int64_t)w * run;
+  const int from = k0 < nkeys ? (int)k0 : nkeys, to = k0 + run < nkeys ? (int)(k0 + run) : nkeys;
+  // the four wavefronts' parts: [4][rows][D + 2], first the reference and the sum
+  s.run(row0, b, h, from, to, (1u << rows) - 1, [&](uint32_t done) {
+    if (!(done >> s.c & 1)) return;
+    float* part = smem + (w * rows + s.c) * (D + 2);
+    if (s.g == 0) {
+      part[0] = s.m[0];
+      part[1] = s.l[0];
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) part[2 + s.col(d, u)] = s.acc[0][d][u];
+  });
+  __syncthreads();
+  float* ws = p.ws + ((int64_t)(bh * tiles + tile) * p.gsplit + gs) * kRows * (D + 2);
+  for (int i = tid; i < rows * D; i += kWaves * kWave) {
+    const int r = i / D, d = i % D;
+    float M = kLowest, L = 0.0f, a = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      const float* q = smem + (k * rows + r) * (D + 2);
+      if (q[1] != 0.0f) M = fmaxf(M, q[0]);
+    }
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      const float* q = smem + (k * rows + r) * (D + 2);
+      const float f = q[1] != 0.0f ? __builtin_amdgcn_exp2f(q[0] - M) : 0.0f;
+      if (q[1] != 0.0f) {
+        L = fmaf(q[1], f, L);
+        a = fmaf(q[2 + d], f, a);
+      }
+    }
+    if (active == 1) {
+      int64_t at, le;
+      row_place(p, b, h, row0 + r, at, le);
+      reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
+      if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
+    } else {
+      stgf_dc(ws + r * (D + 2) + 2 + d, a);
+      if (d == 0) {
+        stgf_dc(ws + r * (D + 2), M);
+        stgf_dc(ws + r * (D + 2) + 1, L);
+      }
+    }
+  }
+  if (active == 1) return;
+  // each workgroup has written its part through to memory and counts itself in; the last to arrive joins them and resets the
+  // counter (no workgroup waits for another)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint32_t* cnt = p.cnt + (int64_t)bh * tiles + tile;
+  int* flag = reinterpret_cast<int*>(smem);
+  if (tid == 0)
+    *flag = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(active - 1);
+  __syncthreads();
+  const int last = *flag;
+  __syncthreads();
+  if (!last) return;
+  const float* all = p.ws + (int64_t)(bh * tiles + tile) * p.gsplit * kRows * (D + 2);
+  float* fac = smem;                       // [rows][gsplit]
+  float* sums = smem + rows * p.gsplit;    // [rows][2]: reference, sum
+  for (int r = w; r < rows; r += kWaves) {
+    float M = kLowest;
+    for (int k = lane_id(); k < active; k += kWave) {
+      const float* q = all + ((int64_t)k * kRows + r) * (D + 2);
+      const float mk = ldgf_dc(q), lk = ldgf_dc(q + 1);
+      fac[r * p.gsplit + k] = mk;
+      M = lk != 0.0f ? fmaxf(M, mk) : M;
+    }
+    M = wave_max(M);
+    float L = 0.0f;
+    for (int k = lane_id(); k < active; k += kWave) {
+      const float lk = ldgf_dc(all + ((int64_t)k * kRows + r) * (D + 2) + 1);
+      const float f = lk != 0.0f ? __builtin_amdgcn_exp2f(fac[r * p.gsplit + k] - M) : 0.0f;
+      fac[r * p.gsplit + k] = f;
+      if (lk != 0.0f) L = fmaf(lk, f, L);
+    }
+    L = wave_sum(L);
+    if (lane_id() == 0) {
+      sums[2 * r] = M;
+      sums[2 * r + 1] = L;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * D; i += kWaves * kWave) {
+    const int r = i / D, d = i % D;
+    float a = 0.0f;
+    for (int k0 = 0; k0 < active; k0 += 16) {
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        v[k] = k0 + k < active ? ldgf_dc(all + ((int64_t)(k0 + k) * kRows + r) * (D + 2) + 2 + d) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (k0 + k < active && fac[r * p.gsplit + k0 + k] != 0.0f) a = fmaf(v[k], fac[r * p.gsplit + k0 + k], a);
+    }
+    int64_t at, le;
+    row_place(p, b, h, row0 + r, at, le);
+    const float L = sums[2 * r + 1];
+    reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
+    if (d == 0 && p.lse) p.lse[le] = lse_of(sums[2 * r], L);
+  }
+  if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // ready for the next call
+}
+
+template <typename T, int D, bool WIDE>
+int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
+  const dim3 blk(kWaves * kWave);
+  if (nsplit == 1) {
+    const int64_t sets = (int64_t)p.BH * ((p.R + kRows - 1) / kRows);
+    int64_t wgs = (sets + kWaves - 1) / kWaves;
+    wgs = (wgs + 7) / 8 * 8;
+    hipLaunchKernelGGL((dense_rows_kernel<T, D, WIDE, 1>), dim3((unsigned)wgs), blk, 0, st, p);
+    return check_launch("dense_rows_kernel");
+  }
+  const int rows = p.R < kRows ? p.R : kRows;
+  const int64_t wgs = (int64_t)p.BH * ((p.R + kRows - 1) / kRows) * p.gsplit;
+  const size_t parts = (size_t)kWaves * rows * (D + 2), join = (size_t)rows * (p.gsplit + 2);
+  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE>), dim3((unsigned)wgs), blk, (parts > join ? parts : join) * sizeof(float),
+                     st, p);
+  return check_launch("dense_split_kernel");
+}
+
+template <typename T>
+int dispatch_dense(const Dense& p, int nsplit, hipStream_t st) {
+  const bool wide = p.ptab == nullptr || p.blog2 >= 5;   // a step's 32 keys in one run of rows
+#define TA_DENSE(DD) return wide ? launch_dense<T, DD, true>(p, nsplit, st) : launch_dense<T, DD, false>(p, nsplit, st)
+  switch (p.D) {
+    case 16: TA_DENSE(16);
+    case 32: TA_DENSE(32);
+    case 64: TA_DENSE(64);
+    default: TA_DENSE(128);
+  }
+#undef TA_DENSE
 }
 
 }  // namespace
@@ -111,15 +721,15 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
     set_error("ta_dense_attn_fwd: head dim must be 16, 32, 64 or 128");
     return TA_ERR_UNSUPPORTED;
   }
-  if (B < 0 || H < 1 || Hq < 1 || Hq % H || Nq < 0 || Tk < 1 || (int64_t)B * Hq > 65535) {
-    set_error("ta_dense_attn_fwd: bad sizes (query heads a multiple of the key heads, at most 65535 (sequence, head) pairs)");
+  if (B < 0 || H < 1 || Hq < 1 || Hq % H || Nq < 0 || Tk < 1) {
+    set_error("ta_dense_attn_fwd: bad sizes (query heads a multiple of the key heads)");
     return TA_ERR_ARG;
   }
   if (nsplit < 1 || (nsplit > 1 && nsplit % 4) || nsplit > 1024) {
     set_error("ta_dense_attn_fwd: nsplit must be 1 or a multiple of 4, at most 1024");
     return TA_ERR_ARG;
   }
-  if (pages && (pages->table == nullptr || pages->num_pages <= 0 || pages->block_log2 < 0 || pages->block_log2 > 14)) {
+  if (pages && (pages->table == nullptr || pages->num_pages <= 0 || pages->block_log2 < 1 || pages->block_log2 > 14)) {
     set_error("ta_dense_attn_fwd: bad page description");
     return TA_ERR_ARG;
   }
@@ -134,6 +744,17 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
   if (bits % 16) {
     set_error("ta_dense_attn_fwd: q, K and V rows must be 16-byte aligned");
     return TA_ERR_ARG;
+  }
+  const int64_t R = (int64_t)(Hq / H) * Nq;
+  const int64_t sets = (int64_t)B * H * ((R + kRows - 1) / kRows);
+  if (R > (1 << 30) || (int64_t)B * H > (1 << 30) || sets * (nsplit > 4 ? nsplit / 4 : 1) > 0x7ffffff0LL ||
+      Tk > 0x7fffffff - 4096) {
+    set_error("ta_dense_attn_fwd: too large");
+    return TA_ERR_UNSUPPORTED;
+  }
+  if (kst < 0 || vst < 0 || kst * sz * 32 > 0x7fffffffLL || vst * sz * 32 > 0x7fffffffLL) {
+    set_error("ta_dense_attn_fwd: row strides from 0 to 64 MiB");
+    return TA_ERR_UNSUPPORTED;
   }
   const int64_t need = ta_dense_attn_workspace_size(B, Hq, H, Nq, D, nsplit);
   if (need > 0 && (ws == nullptr || ws_bytes < need || (uintptr_t)ws % 256)) {
@@ -150,10 +771,15 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
     p.npages = pages->num_pages;
     p.blog2 = pages->block_log2;
   }
-  const dim3 grid(Nq, B * Hq), blk(kWave);
+  p.BH = B * H;
+  p.R = (int)R;
+  p.gsplit = nsplit > 4 ? nsplit / 4 : 1;
+  if (need > 0) {
+    p.cnt = reinterpret_cast<uint32_t*>(ws);
+    p.ws = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + (sets * 4 + 255) / 256 * 256);
+  }
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == TA_F32) hipLaunchKernelGGL((dense_attn_kernel<float>), grid, blk, 0, st, p);
-  else if (dtype == TA_F16) hipLaunchKernelGGL((dense_attn_kernel<f16_t>), grid, blk, 0, st, p);
-  else hipLaunchKernelGGL((dense_attn_kernel<bf16_t>), grid, blk, 0, st, p);
-  return check_launch("dense_attn_kernel");
+  if (dtype == TA_F32) return dispatch_dense<float>(p, nsplit, st);
+  if (dtype == TA_F16) return dispatch_dense<f16_t>(p, nsplit, st);
+  return dispatch_dense<bf16_t>(p, nsplit, st);
 }

@@ -384,7 +384,11 @@ def decode_nsplit8(B, H, Nq, wl, leaf):
 def decode_nsplit_dense(B, H, rows, keys, D=64):
     """dense_attn's nsplit for B * H (sequence, key head) pairs of `rows` query rows (query heads of a key head times tokens)
     over up to `keys` keys."""
-    return 1
+    sets = max(1, B * H * ((rows + 15) // 16))
+    if sets >= 4096:
+        return 1
+    g = min(max(1, 2048 // sets // 4 * 2), max(1, keys // 256), 256)
+    return 4 * g
 
 
 def _budget_weights(state, pw):
