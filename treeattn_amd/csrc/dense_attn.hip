@@ -22,6 +22,7 @@
 //
 // Reference functions replaced: engine.py:74-81 (DenseState.attend).
 #include "attn.hpp"
+#include "trace.hpp"
 
 namespace ta {
 namespace {
@@ -47,7 +48,7 @@ struct Dense {
   int64_t pt_sb, pt_sh, pstride, npages;
   int blog2;
   int BH, R;            // (sequence, key head) pairs; query rows of one: G * Nq
-  int gsplit;           // workgroups a set of 16 rows
+  int gsplit;           // workgroups a set of rows
   float* ws;            // their parts (set, workgroup, row, D + 2) and
   uint32_t* cnt;        // arrival counters (zero between calls)
 };
@@ -56,6 +57,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kRows = 16;            // query rows of a tile
@@ -64,19 +67,24 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 template <typename T, int D> struct Tile {
   static constexpr int EB = (int)sizeof(T);
-  static constexpr int KT = EB == 2 ? 2 : (D == 128 ? 1 : 2);   // tiles of 16 keys a step
+  // Tiles of 16 keys a step.  Heads of 128 take one: two steps of 32 keys in registers leave no room for two wavefronts on a
+  // SIMD (256 registers and spills).
+  static constexpr int KT = D == 128 ? 1 : 2;
   static constexpr int KEYS = 16 * KT;
   static constexpr int KS = EB == 2 ? (D + 31) / 32 : D / 16;   // 16-byte pieces of a key row a lane
   static constexpr int DJ = D / 16;                             // columns of V a lane holds
   static constexpr int VB = DJ * EB;                            // their bytes, of one key
   static constexpr int VW = (VB + 3) / 4;
+  // LDS bytes of a key row (16 more than the row, so that 8 rows' pieces lie in different banks) and of a wavefront's step
+  static constexpr int LROW = (D * EB < 64 ? 64 : D * EB) + 16;
+  static constexpr int LSTEP = KEYS * LROW;
   // weights are exp2(x - max + kShift): float16 keeps 2^-24 absolutely, which is far below the largest weight then
   static constexpr float kShift = __is_same(T, f16_t) ? 10.0f : 0.0f;
   static constexpr float kSlack = __is_same(T, f16_t) ? 4.0f : 8.0f;
 };
 
-// The keys and values of one step, in a lane: K rows 16 i + lane % 16 at pieces lane / 16; V rows 16 i + 4 (lane / 16) + u at
-// columns DJ (lane % 16) ...
+// The keys and values of one step, in a lane: K rows 16 i + lane / 4 at pieces lane % 4 (four lanes next to each other read 64
+// bytes of a row); V rows 16 i + 4 (lane / 16) + u at columns DJ (lane % 16) ...
 template <typename T, int D> struct Step {
   uint4 k[Tile<T, D>::KT][Tile<T, D>::KS];
   uint32_t v[Tile<T, D>::KT * 4][Tile<T, D>::VW];
@@ -90,6 +98,14 @@ __device__ __forceinline__ f32x4 mfma32(const uint4& a, const uint4& b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f32x4 c) {
+  if constexpr (__is_same(T, f16_t))
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
 }
 
 // two floats rounded to two elements of T, the first in the low half
@@ -127,6 +143,20 @@ __device__ __forceinline__ float sum_rows(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Row r of a key head's query rows: query head j of its group, token n.
+__device__ __forceinline__ void head_token(const Dense& p, int r, int& j, int& n) {
+  j = p.Nq == 1 ? r : r / p.Nq;
+  n = p.Nq == 1 ? 0 : r - j * p.Nq;
+}
+
+// The smaller of x over 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ int min_dpp(int x) {
+  const int y = __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false);
+  return y < x ? y : x;
+}
+__device__ __forceinline__ int min16(int x) { return min_dpp<0x140>(min_dpp<0x141>(min_dpp<0x4E>(min_dpp<0xB1>(x)))); }
+
 // One wavefront's share: keys [k0, k1) for NT tiles of 16 query rows of one (sequence, key head).
 template <typename T, int D, bool WIDE, int NT>
 struct Share {
@@ -142,10 +172,11 @@ struct Share {
   uint4 q[NT][C::KS];
   f32x4 acc[NT][C::DJ];
   float m[NT], l[NT];   // the reference of the weights (max - kShift), and the lane's part of their sum
+  char* lds;            // this wavefront's LSTEP bytes
   int pg;               // page (WIDE), or the page of key lane % 32, of the step that is fetched next
 
-  __device__ __forceinline__ Share(const Dense& p_, int b, int h, int row0)
-      : p(p_), lane(lane_id()), c(lane & 15), g(lane >> 4) {
+  __device__ __forceinline__ Share(const Dense& p_, int b, int h, int row0, char* lds_)
+      : p(p_), lane(lane_id()), c(lane & 15), g(lane >> 4), lds(lds_) {
     kb = reinterpret_cast<const T*>(p.k) + (p.ptab ? 0 : b * p.ksb + h * p.ksh);
     vb = reinterpret_cast<const T*>(p.v) + (p.ptab ? 0 : b * p.vsb + h * p.vsh);
     tab = p.ptab ? p.ptab + b * p.pt_sb + h * p.pt_sh : nullptr;
@@ -154,7 +185,8 @@ struct Share {
     for (int i = 0; i < NT; ++i) {
       const int r = row0 + kRows * i + c;
       const bool in = r < p.R;
-      const int j = in ? r / p.Nq : 0, n = in ? r % p.Nq : 0;
+      int j = 0, n = 0;
+      if (in) head_token(p, r, j, n);
       int tt = in ? p.tq[b * p.tq_sb + n] : 0x7fffffff;
       if (in && (tt < 0 || tt >= p.Tk)) tt = -1;
       t[i] = tt;
@@ -168,12 +200,8 @@ struct Share {
       }
     }
     reset();
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      const int a = __shfl_xor(lo, o, kWave), e = __shfl_xor(hi, o, kWave);
-      lo = a < lo ? a : lo;
-      hi = e > hi ? e : hi;
-    }
+    lo = min16(lo);
+    hi = -min16(-hi);
     tmin = __builtin_amdgcn_readfirstlane(lo);
     tmax = __builtin_amdgcn_readfirstlane(hi);
     seen = tmax;
@@ -185,8 +213,10 @@ struct Share {
     return tab[(key < tmax ? key : tmax) >> p.blog2];
   }
 
-  // Requests step x's rows (keys key0 ...) from the pages in pg, and before them the pages of the step at next0.
-  __device__ __forceinline__ void fetch(Step<T, D>& x, int key0, int next0) {
+  // Requests step x's rows (keys key0 ...) from the pages in pg, and before them the pages of the step at next0.  A step that
+  // is not needed (past the last one; loads are not left out, so that what is waited for is a fixed number of loads) reads one
+  // row of its first key.
+  __device__ __forceinline__ void fetch(Step<T, D>& x, int key0, int next0, bool live) {
     x.key0 = key0;
     const int mine = pg;
     pg = page_of(next0);
@@ -214,12 +244,13 @@ struct Share {
         vlast = (uint32_t)(tmax - key0) * vs;
         if (tmax - key0 >= C::KEYS) klast = vlast = 0xffffffffu;
       }
+      if (!live) klast = vlast = 0;
       x.have = ok ? 0xffffffffu : 0u;
       const char* k0p = reinterpret_cast<const char*>(kb + ko);
       const char* v0p = reinterpret_cast<const char*>(vb + vo);
 #pragma unroll
       for (int i = 0; i < C::KT; ++i) {
-        const uint32_t o = c * ks + 16 * i * ks;
+        const uint32_t o = (lane >> 2) * ks + 16 * i * ks;
         kr[i] = k0p + (o < klast ? o : klast);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -228,20 +259,20 @@ struct Share {
         }
       }
     } else {
-      const int mask = (1 << p.blog2) - 1;
+      const int mask = live ? (1 << p.blog2) - 1 : 0;
       x.have = 0;
 #pragma unroll
       for (int i = 0; i < C::KT; ++i) {
-        int page = __shfl(mine, 16 * i + c, kWave);
-        page = page >= 0 && page < p.npages ? page : 0;
-        kr[i] = reinterpret_cast<const char*>(kb + page * p.pstride + (int64_t)((key0 + 16 * i + c) & mask) * p.kst);
+        int page = __shfl(mine, 16 * i + (lane >> 2), kWave);
+        page = page >= 0 && page < p.npages && live ? page : 0;
+        kr[i] = reinterpret_cast<const char*>(kb + page * p.pstride + (int64_t)((key0 + 16 * i + (lane >> 2)) & mask) * p.kst);
 #pragma unroll
         for (int u = 0; u < 4; u += 2) {
           const int e = 16 * i + 4 * g + u;
           int pv = __shfl(mine, e, kWave);
           const bool ok = pv >= 0 && pv < p.npages;
           x.have |= ok ? 3u << (4 * i + u) : 0u;
-          const T* row = vb + (ok ? pv : 0) * p.pstride;
+          const T* row = vb + (ok && live ? pv : 0) * p.pstride;
           vr[4 * i + u] = reinterpret_cast<const char*>(row + (int64_t)((key0 + e) & mask) * p.vst);
           vr[4 * i + u + 1] = reinterpret_cast<const char*>(row + (int64_t)((key0 + e + 1) & mask) * p.vst);
         }
@@ -251,8 +282,8 @@ struct Share {
     for (int i = 0; i < C::KT; ++i)
 #pragma unroll
       for (int s = 0; s < C::KS; ++s) {
-        const int d = C::EB == 2 ? 32 * s + 8 * g : 16 * s + 4 * g;
-        x.k[i][s] = ldg16(kr[i] + (d < D ? d : 0) * C::EB);
+        const int o = 64 * s + 16 * (lane & 3);
+        x.k[i][s] = ldg16(kr[i] + (o < D * C::EB ? o : 0));
       }
 #pragma unroll
     for (int e = 0; e < C::KT * 4; ++e) {
@@ -270,6 +301,24 @@ struct Share {
         x.v[e][0] = *(const TA_GLOBAL uint16_t*)a;
       }
     }
+  }
+
+  // The step's keys from the lanes that loaded them to the lanes whose operand they are: lane (c, g) takes piece g of row c.
+  // (Loaded in that order, each 16 bytes would be an access of their own to the first cache: 371 accesses a step of 32 keys of
+  // 64, now 180, which a piece of a prompt is bound by.)
+  __device__ __forceinline__ void turn(Step<T, D>& x) const {
+    wave_sync();
+#pragma unroll
+    for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+      for (int e = 0; e < C::KS; ++e)
+        *reinterpret_cast<uint4*>(lds + (16 * a + (lane >> 2)) * C::LROW + 64 * e + 16 * (lane & 3)) = x.k[a][e];
+    wave_sync();
+#pragma unroll
+    for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+      for (int e = 0; e < C::KS; ++e)
+        x.k[a][e] = *reinterpret_cast<const uint4*>(lds + (16 * a + c) * C::LROW + 64 * e + 16 * g);
   }
 
   // Scores of tile row set i: in lane (c, g) those of row c and keys 16 a + 4 g + u.
@@ -345,23 +394,28 @@ struct Share {
       scores(x, i, s);
       weights<MASKED>(x, i, s);
       if constexpr (C::EB == 2) {
-        uint32_t hi[4], lo[4];
+        uint32_t hi[2 * C::KT], lo[2 * C::KT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2 * C::KT; ++e) {
           const float w0 = s[e / 2][2 * (e % 2)], w1 = s[e / 2][2 * (e % 2) + 1];
           hi[e] = pack2<T>(w0, w1);
           lo[e] = pack2<T>(w0 - unpack_lo<T>(hi[e]), w1 - unpack_hi<T>(hi[e]));
         }
-        const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]), pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
         for (int d = 0; d < C::DJ; ++d) {
-          uint32_t vt[4];
+          uint32_t vt[2 * C::KT];   // the eight (four) keys' values of one column
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 2 * C::KT; ++e)
             vt[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][d / 2], x.v[2 * e][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-          const uint4 va = make_uint4(vt[0], vt[1], vt[2], vt[3]);
-          acc[i][d] = mfma32<T>(va, ph, acc[i][d]);
-          acc[i][d] = mfma32<T>(va, pl, acc[i][d]);
+          if constexpr (C::KT == 2) {
+            const uint4 va = make_uint4(vt[0], vt[1], vt[2], vt[3]);
+            acc[i][d] = mfma32<T>(va, make_uint4(hi[0], hi[1], hi[2], hi[3]), acc[i][d]);
+            acc[i][d] = mfma32<T>(va, make_uint4(lo[0], lo[1], lo[2], lo[3]), acc[i][d]);
+          } else {
+            const u32x2 va = {vt[0], vt[1]};
+            acc[i][d] = mfma16<T>(va, (u32x2){hi[0], hi[1]}, acc[i][d]);
+            acc[i][d] = mfma16<T>(va, (u32x2){lo[0], lo[1]}, acc[i][d]);
+          }
         }
       } else {
 #pragma unroll
@@ -373,6 +427,7 @@ struct Share {
     }
   }
   __device__ __forceinline__ void step(Step<T, D>& x) {
+    turn(x);
     const bool full = x.key0 + C::KEYS - 1 <= (tmin < seen ? tmin : seen) &&
                       __ballot((x.have & ((1u << (4 * C::KT)) - 1)) != (1u << (4 * C::KT)) - 1) == 0;
     if (full) consume<false>(x);
@@ -397,7 +452,8 @@ struct Share {
 #pragma unroll
     for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     const int r = row0 + kRows * i + c;
-    const int j = r < p.R ? r / p.Nq : 0, n = r < p.R ? r % p.Nq : 0;
+    int j = 0, n = 0;
+    if (r < p.R) head_token(p, r, j, n);
     const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + j) * p.qsh + n * p.qsn + g * (D / 4);
     for (int key = k0; key < k1; ++key) {
       int64_t ko = key * p.kst, vo = key * p.vst;
@@ -432,13 +488,13 @@ struct Share {
       return key < last ? key : last;
     };
     pg = page_of(k0);
-    // two steps in registers: one arrives while the other is used (past the last one, the last again)
+    // two steps in registers: one arrives while the other is used
     Step<T, D> x[2];
-    fetch(x[0], at(0), at(1));
+    fetch(x[0], at(0), at(1), true);
     for (int n = 0; k0 + n * C::KEYS < k1; n += 2) {
-      fetch(x[1], at(n + 1), at(n + 2));
+      fetch(x[1], at(n + 1), at(n + 2), k0 + (n + 1) * C::KEYS < k1);
       step(x[0]);
-      fetch(x[0], at(n + 2), at(n + 3));
+      fetch(x[0], at(n + 2), at(n + 3), k0 + (n + 2) * C::KEYS < k1);
       if (k0 + (n + 1) * C::KEYS < k1) step(x[1]);
     }
   }
@@ -497,7 +553,8 @@ struct Share {
 };
 
 __device__ __forceinline__ void row_place(const Dense& p, int b, int h, int r, int64_t& out, int64_t& lse) {
-  const int j = r / p.Nq, n = r % p.Nq;
+  int j, n;
+  head_token(p, r, j, n);
   out = b * p.osb + (int64_t)(h * p.G + j) * p.osh + n * p.osn;
   lse = ((int64_t)b * p.Hq + h * p.G + j) * p.Nq + n;
 }
@@ -514,7 +571,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_rows_kernel(Dense p) 
   if (id >= per * p.BH) return;
   const int bh = (int)(id / per), row0 = (int)(id % per) * kRows * NT;
   const int b = bh / p.H, h = bh % p.H;
-  Share<T, D, WIDE, NT> s(p, b, h, row0);
+  __shared__ __align__(16) char stage[kWaves * Tile<T, D>::LSTEP];
+  Share<T, D, WIDE, NT> s(p, b, h, row0, stage + wave_id() * Tile<T, D>::LSTEP);
   const int left = p.R - row0;
   s.run(row0, b, h, 0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1,
         [&](uint32_t done) {
@@ -535,22 +593,33 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_rows_kernel(Dense p) 
   });
 }
 
-constexpr int kMinKeys = 64;         // of a wavefront
+constexpr int kMinKeys = 32;         // of a wavefront
 
-// gsplit workgroups of four wavefronts a set of 16 rows.
-template <typename T, int D, bool WIDE>
+// gsplit workgroups of four wavefronts a set of 16 NT rows.
+template <typename T, int D, bool WIDE, int NT>
 __global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p) {
   extern __shared__ __align__(16) float smem[];
   constexpr int KEYS = Tile<T, D>::KEYS;
-  const int tiles = (p.R + kRows - 1) / kRows;
-  const int gs = blockIdx.x % p.gsplit;
-  const int tile = blockIdx.x / p.gsplit % tiles;
-  const int bh = blockIdx.x / p.gsplit / tiles;
-  const int b = bh / p.H, h = bh % p.H;
+  constexpr int kSet = kRows * NT;
+  TA_DMARK(0);
+  // x: workgroup of the set, y: set; sets of one key head, which share its keys, come on one XCD (workgroups go round robin
+  // over the 8)
+  const int sets = (p.R + kSet - 1) / kSet;
+  unsigned gs = blockIdx.x, at = blockIdx.y;
+  if (sets > 1) {
+    const unsigned id = blockIdx.y * gridDim.x + blockIdx.x, n8 = gridDim.x * gridDim.y / 8;
+    const unsigned to = (id & 7) * n8 + id / 8;   // (the grid is a multiple of 8)
+    gs = to % gridDim.x;
+    at = to / gridDim.x;
+    if (at >= (unsigned)(p.BH * sets)) return;
+  }
+  const int set = sets > 1 ? at % sets : 0;
+  const int bh = sets > 1 ? at / sets : at;
+  const int b = bh / p.H, h = bh - b * p.H;
   const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
-  const int row0 = tile * kRows;
-  const int rows = p.R - row0 < kRows ? p.R - row0 : kRows;
-  Share<T, D, WIDE, 1> s(p, b, h, row0);
+  const int row0 = set * kSet;
+  const int rows = p.R - row0 < kSet ? p.R - row0 : kSet;
+  Share<T, D, WIDE, NT> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP);
   // equal runs of whole steps a wavefront; workgroups without one are not needed
   const int nkeys = s.tmax + 1;
   int run = (nkeys + p.gsplit * kWaves - 1) / (p.gsplit * kWaves);
@@ -558,35 +627,41 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p)
   run -= run % KEYS;
   const int64_t wgrun = (int64_t)run * kWaves;
   const int active = nkeys > 0 ? (int)((nkeys + wgrun - 1) / wgrun) : 1;
-  if (gs >= active) return;
+  if ((int)gs >= active) return;
   const int64_t k0 = gs * wgrun + (int64_t)w * run;
+  TA_DMARK(1);
   const int from = k0 < nkeys ? (int)k0 : nkeys, to = k0 + run < nkeys ? (int)(k0 + run) : nkeys;
-  // the four wavefronts' parts: [4][rows][D + 2], first the reference and the sum
-  s.run(row0, b, h, from, to, (1u << rows) - 1, [&](uint32_t done) {
-    if (!(done >> s.c & 1)) return;
-    float* part = smem + (w * rows + s.c) * (D + 2);
-    if (s.g == 0) {
-      part[0] = s.m[0];
-      part[1] = s.l[0];
+  // the four wavefronts' parts, behind their keys: [4][rows][D + 2], first the reference and the sum
+  float* const parts = smem + kWaves * Tile<T, D>::LSTEP / 4;
+  s.run(row0, b, h, from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, [&](uint32_t done) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (!(done >> (kRows * i + s.c) & 1)) continue;
+      float* part = parts + (w * rows + kRows * i + s.c) * (D + 2);
+      if (s.g == 0) {
+        part[0] = s.m[i];
+        part[1] = s.l[i];
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) part[2 + s.col(d, u)] = s.acc[i][d][u];
     }
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) part[2 + s.col(d, u)] = s.acc[0][d][u];
   });
+  TA_DMARK(2);
   __syncthreads();
-  float* ws = p.ws + ((int64_t)(bh * tiles + tile) * p.gsplit + gs) * kRows * (D + 2);
+  float* ws = p.ws + ((int64_t)at * p.gsplit + gs) * kSet * (D + 2);
   for (int i = tid; i < rows * D; i += kWaves * kWave) {
     const int r = i / D, d = i % D;
     float M = kLowest, L = 0.0f, a = 0.0f;
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
-      const float* q = smem + (k * rows + r) * (D + 2);
+      const float* q = parts + (k * rows + r) * (D + 2);
       if (q[1] != 0.0f) M = fmaxf(M, q[0]);
     }
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
-      const float* q = smem + (k * rows + r) * (D + 2);
+      const float* q = parts + (k * rows + r) * (D + 2);
       const float f = q[1] != 0.0f ? __builtin_amdgcn_exp2f(q[0] - M) : 0.0f;
       if (q[1] != 0.0f) {
         L = fmaf(q[1], f, L);
@@ -611,83 +686,117 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p)
   // counter (no workgroup waits for another)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  uint32_t* cnt = p.cnt + (int64_t)bh * tiles + tile;
+  TA_DMARK(3);
+  uint32_t* cnt = p.cnt + at;
   int* flag = reinterpret_cast<int*>(smem);
   if (tid == 0)
     *flag = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(active - 1);
   __syncthreads();
   const int last = *flag;
   __syncthreads();
+  TA_DMARK(4);
   if (!last) return;
-  const float* all = p.ws + (int64_t)(bh * tiles + tile) * p.gsplit * kRows * (D + 2);
-  float* fac = smem;                       // [rows][gsplit]
-  float* sums = smem + rows * p.gsplit;    // [rows][2]: reference, sum
-  for (int r = w; r < rows; r += kWaves) {
-    float M = kLowest;
-    for (int k = lane_id(); k < active; k += kWave) {
-      const float* q = all + ((int64_t)k * kRows + r) * (D + 2);
-      const float mk = ldgf_dc(q), lk = ldgf_dc(q + 1);
-      fac[r * p.gsplit + k] = mk;
-      M = lk != 0.0f ? fmaxf(M, mk) : M;
-    }
-    M = wave_max(M);
-    float L = 0.0f;
-    for (int k = lane_id(); k < active; k += kWave) {
-      const float lk = ldgf_dc(all + ((int64_t)k * kRows + r) * (D + 2) + 1);
-      const float f = lk != 0.0f ? __builtin_amdgcn_exp2f(fac[r * p.gsplit + k] - M) : 0.0f;
-      fac[r * p.gsplit + k] = f;
-      if (lk != 0.0f) L = fmaf(lk, f, L);
-    }
-    L = wave_sum(L);
-    if (lane_id() == 0) {
-      sums[2 * r] = M;
-      sums[2 * r + 1] = L;
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < rows * D; i += kWaves * kWave) {
+  // a thread an element, or several with a share of the parts each where there are few elements: all loads of eight parts at
+  // once, so that the parts cost one round trip to memory and not one each
+  const float* all = p.ws + (int64_t)at * p.gsplit * kSet * (D + 2);
+  const int E = rows * D;
+  const int groups = E < kWaves * kWave ? kWaves * kWave / E : 1;
+  for (int base = 0; base < E; base += kWaves * kWave) {
+    const int i = groups > 1 ? tid % E : base + tid, first = groups > 1 ? tid / E : 0;
     const int r = i / D, d = i % D;
-    float a = 0.0f;
-    for (int k0 = 0; k0 < active; k0 += 16) {
-      float v[16];
+    const bool in = i < E && first < groups;
+    float M = kLowest, L = 0.0f, a = 0.0f;
+    if (in) {
+      for (int k0 = first; k0 < active; k0 += 8 * groups) {
+        float mk[8], lk[8], vk[8];
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        v[k] = k0 + k < active ? ldgf_dc(all + ((int64_t)(k0 + k) * kRows + r) * (D + 2) + 2 + d) : 0.0f;
+        for (int k = 0; k < 8; ++k) {
+          const int part = k0 + k * groups;
+          const float* q = all + ((int64_t)(part < active ? part : first) * kSet + r) * (D + 2);
+          mk[k] = ldgf_dc(q);
+          lk[k] = part < active ? ldgf_dc(q + 1) : 0.0f;
+          vk[k] = ldgf_dc(q + 2 + d);
+        }
+        float mn = M;
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (k0 + k < active && fac[r * p.gsplit + k0 + k] != 0.0f) a = fmaf(v[k], fac[r * p.gsplit + k0 + k], a);
+        for (int k = 0; k < 8; ++k) mn = lk[k] != 0.0f ? fmaxf(mn, mk[k]) : mn;
+        const float alpha = __builtin_amdgcn_exp2f(M - mn);
+        M = mn;
+        L *= alpha;
+        a *= alpha;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (lk[k] != 0.0f) {
+            const float f = __builtin_amdgcn_exp2f(mk[k] - M);
+            L = fmaf(lk[k], f, L);
+            a = fmaf(vk[k], f, a);
+          }
+        }
+      }
     }
-    int64_t at, le;
-    row_place(p, b, h, row0 + r, at, le);
-    const float L = sums[2 * r + 1];
-    reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
-    if (d == 0 && p.lse) p.lse[le] = lse_of(sums[2 * r], L);
+    if (groups > 1) {
+      float* mine = smem + 3 * tid;
+      mine[0] = M;
+      mine[1] = L;
+      mine[2] = a;
+      __syncthreads();
+      if (in && first == 0) {
+        for (int k = 1; k < groups; ++k) {
+          const float* q = smem + 3 * (tid + k * E);
+          if (q[1] != 0.0f) {
+            const float mn = fmaxf(M, q[0]);
+            const float f0 = __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(q[0] - mn);
+            M = mn;
+            L = fmaf(q[1], f1, L * f0);
+            a = fmaf(q[2], f1, a * f0);
+          }
+        }
+      }
+    }
+    if (in && first == 0) {
+      int64_t at, le;
+      row_place(p, b, h, row0 + r, at, le);
+      reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
+      if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
+    }
   }
+  TA_DMARK(5);
   if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // ready for the next call
 }
 
-template <typename T, int D, bool WIDE>
+template <typename T, int D, bool WIDE, int NT>
 int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const dim3 blk(kWaves * kWave);
+  const int64_t per = (p.R + kRows * NT - 1) / (kRows * NT), sets = p.BH * per;
   if (nsplit == 1) {
-    const int64_t sets = (int64_t)p.BH * ((p.R + kRows - 1) / kRows);
-    int64_t wgs = (sets + kWaves - 1) / kWaves;
-    wgs = (wgs + 7) / 8 * 8;
-    hipLaunchKernelGGL((dense_rows_kernel<T, D, WIDE, 1>), dim3((unsigned)wgs), blk, 0, st, p);
+    const int64_t wgs = ((sets + kWaves - 1) / kWaves + 7) / 8 * 8;
+    hipLaunchKernelGGL((dense_rows_kernel<T, D, WIDE, NT>), dim3((unsigned)wgs), blk, 0, st, p);
     return check_launch("dense_rows_kernel");
   }
-  const int rows = p.R < kRows ? p.R : kRows;
-  const int64_t wgs = (int64_t)p.BH * ((p.R + kRows - 1) / kRows) * p.gsplit;
-  const size_t parts = (size_t)kWaves * rows * (D + 2), join = (size_t)rows * (p.gsplit + 2);
-  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE>), dim3((unsigned)wgs), blk, (parts > join ? parts : join) * sizeof(float),
+  const int rows = p.R < kRows * NT ? p.R : kRows * NT;
+  const size_t stage = kWaves * Tile<T, D>::LSTEP, parts = (size_t)kWaves * rows * (D + 2), join = 3 * kWaves * kWave;
+  const dim3 grid((unsigned)p.gsplit, (unsigned)(per > 1 ? (sets + 7) / 8 * 8 : sets));
+  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT>), grid, blk, stage + (parts > join ? parts : join) * sizeof(float),
                      st, p);
   return check_launch("dense_split_kernel");
+}
+
+// Two tiles of rows a wavefront where there are more rows than one takes: they share the keys' way into the registers.  Not
+// with float32 rows (their matrix instructions take longer than that way) nor heads of 128 (registers).
+template <typename T, int D>
+constexpr int two_tiles() { return sizeof(T) == 2 && D < 128 ? 2 : 1; }
+
+template <typename T, int D, bool WIDE>
+int rows_dense(const Dense& p, int nsplit, hipStream_t st) {
+  if constexpr (two_tiles<T, D>() == 2)
+    if (p.R > kRows) return launch_dense<T, D, WIDE, 2>(p, nsplit, st);
+  return launch_dense<T, D, WIDE, 1>(p, nsplit, st);
 }
 
 template <typename T>
 int dispatch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const bool wide = p.ptab == nullptr || p.blog2 >= 5;   // a step's 32 keys in one run of rows
-#define TA_DENSE(DD) return wide ? launch_dense<T, DD, true>(p, nsplit, st) : launch_dense<T, DD, false>(p, nsplit, st)
+#define TA_DENSE(DD) return wide ? rows_dense<T, DD, true>(p, nsplit, st) : rows_dense<T, DD, false>(p, nsplit, st)
   switch (p.D) {
     case 16: TA_DENSE(16);
     case 32: TA_DENSE(32);
@@ -704,8 +813,10 @@ using namespace ta;
 
 extern "C" int64_t ta_dense_attn_workspace_size(int B, int Hq, int H, int Nq, int D, int nsplit) {
   if (B <= 0 || H <= 0 || Hq <= 0 || Nq <= 0 || nsplit <= 4) return 0;
-  const int64_t tiles = (int64_t)B * H * (((int64_t)(Hq / H) * Nq + 15) / 16);
-  return (tiles * 4 + 255) / 256 * 256 + tiles * (nsplit / 4) * 16 * (D + 2) * 4;
+  // counters and parts of whole tiles of 32 rows (16 where there are no more), whichever the kernels take
+  const int64_t R = (int64_t)(Hq / H) * Nq;
+  const int64_t rows = R <= 16 ? 16 : (R + 31) / 32 * 32;
+  return ((int64_t)B * H * (rows / 16) * 4 + 255) / 256 * 256 + (int64_t)B * H * rows * (nsplit / 4) * (D + 2) * 4;
 }
 
 extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, int dtype, int64_t qsb, int64_t qsh,
@@ -746,10 +857,11 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
     return TA_ERR_ARG;
   }
   const int64_t R = (int64_t)(Hq / H) * Nq;
-  const int64_t sets = (int64_t)B * H * ((R + kRows - 1) / kRows);
+  const int64_t sets = (int64_t)B * H * (R <= 16 ? 1 : (R + 31) / 32 * 2);   // counters of the workspace
   if (R > (1 << 30) || (int64_t)B * H > (1 << 30) || sets * (nsplit > 4 ? nsplit / 4 : 1) > 0x7ffffff0LL ||
+      (nsplit > 1 && sets > 65528) ||
       Tk > 0x7fffffff - 4096) {
-    set_error("ta_dense_attn_fwd: too large");
+    set_error("ta_dense_attn_fwd: too large (nsplit above 1: at most 65528 (sequence, key head) pairs times sets of 16 rows)");
     return TA_ERR_UNSUPPORTED;
   }
   if (kst < 0 || vst < 0 || kst * sz * 32 > 0x7fffffffLL || vst * sz * 32 > 0x7fffffffLL) {
@@ -783,3 +895,5 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
   if (dtype == TA_F16) return dispatch_dense<f16_t>(p, nsplit, st);
   return dispatch_dense<bf16_t>(p, nsplit, st);
 }
+
+TA_TRACE_EXPORTS

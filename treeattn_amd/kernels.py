@@ -1175,9 +1175,11 @@ def _positions(name, pos, B, N):
 
 
 def dense_attn_workspace(B, Hq, Nq, D, nsplit, device, kv_heads=None):
-    """Zero-filled workspace for dense_attn with `nsplit` over a cache of kv_heads heads (default Hq; any gives enough for
-    fewer), None when none is needed.  Calls that share it are of one size and do not overlap in time."""
-    nbytes = L.lib().ta_dense_attn_workspace_size(B, Hq, kv_heads or Hq, Nq, D, nsplit)
+    """Zero-filled workspace for dense_attn with `nsplit` over a cache of kv_heads heads (default: enough for any number that
+    Hq is a multiple of), None when none is needed.  Calls that share it are of one size and do not overlap in time."""
+    size = L.lib().ta_dense_attn_workspace_size
+    heads = [kv_heads] if kv_heads else [h for h in range(1, Hq + 1) if Hq % h == 0]
+    nbytes = max((size(B, Hq, h, Nq, D, nsplit) for h in heads), default=0)
     return torch.zeros(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
