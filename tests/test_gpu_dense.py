@@ -281,7 +281,7 @@ def test_the_split_rule_and_its_results():
     for B, H, rows_, keys, D in [(1, 1, 1, 1, 64), (1, 1, 1, 131072, 128), (1, 12, 1, 131072, 64), (32, 12, 1, 32768, 64),
                                  (1, 2, 256, 4096, 64), (4, 8, 4, 6000, 128), (512, 12, 1, 100, 16)]:
         n = decode_nsplit_dense(B, H, rows_, keys, D)
-        assert n == 1 or (n % 4 == 0 and 4 <= n <= 1024), n
+        assert n == 1 or (n % 4 == 0 and 4 <= n <= 8192), n
     k, v = rnd(1, 1, 5000, 64, seed=81), rnd(1, 1, 5000, 64, seed=82)
     q = rnd(1, 1, 1, 64, seed=83)
     tq = torch.tensor([[4999]], dtype=torch.int32)
@@ -316,7 +316,7 @@ def test_refusals():
     for bad in (lambda: K.dense_attn(q.float(), k, k, tq), lambda: K.dense_attn(q, k, k, tq.float())):
         with pytest.raises(TypeError):
             bad()
-    for nsplit in (0, 2, 6, 1028, -4):
+    for nsplit in (0, 2, 6, 8196, -4):
         with pytest.raises(RuntimeError, match='nsplit'):
             K.dense_attn(q, k, k, tq, nsplit=nsplit)
     with pytest.raises(RuntimeError, match='workspace'):

@@ -48,9 +48,9 @@ struct Dense {
   int64_t pt_sb, pt_sh, pstride, npages;
   int blog2;
   int BH, R;            // (sequence, key head) pairs; query rows of one: G * Nq
-  int gsplit;           // workgroups a set of rows
-  float* ws;            // their parts (set, workgroup, row, D + 2) and
-  uint32_t* cnt;        // arrival counters (zero between calls)
+  int B;
+  float* ws;            // parts (workgroup, row, D + 2) and
+  uint32_t* cnt;        // arrival counters of the sets (zero between calls)
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -143,6 +143,13 @@ __device__ __forceinline__ float sum_rows(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// One element in device memory.
+__device__ __forceinline__ float number(const TA_GLOBAL float* p) { return *p; }
+__device__ __forceinline__ float number(const TA_GLOBAL f16_t* p) { return (float)*p; }
+__device__ __forceinline__ float number(const TA_GLOBAL bf16_t* p) {
+  return __uint_as_float((uint32_t) * (const TA_GLOBAL uint16_t*)p << 16);
+}
+
 // Row r of a key head's query rows: query head j of its group, token n.
 __device__ __forceinline__ void head_token(const Dense& p, int r, int& j, int& n) {
   j = p.Nq == 1 ? r : r / p.Nq;
@@ -163,8 +170,8 @@ struct Share {
   using C = Tile<T, D>;
   const Dense& p;
   const int lane, c, g;
-  const T* kb;
-  const T* vb;
+  const TA_GLOBAL T* kb;
+  const TA_GLOBAL T* vb;
   const int32_t* tab;
   int t[NT];            // the lane's row's position (pad rows: as far as any)
   int tmin, tmax;       // of the wavefront's rows
@@ -175,10 +182,10 @@ struct Share {
   char* lds;            // this wavefront's LSTEP bytes
   int pg;               // page (WIDE), or the page of key lane % 32, of the step that is fetched next
 
-  __device__ __forceinline__ Share(const Dense& p_, int b, int h, int row0, char* lds_)
+  __device__ __forceinline__ Share(const Dense& p_, int b, int h, int row0, char* lds_, bool one = false, int last = -1)
       : p(p_), lane(lane_id()), c(lane & 15), g(lane >> 4), lds(lds_) {
-    kb = reinterpret_cast<const T*>(p.k) + (p.ptab ? 0 : b * p.ksb + h * p.ksh);
-    vb = reinterpret_cast<const T*>(p.v) + (p.ptab ? 0 : b * p.vsb + h * p.vsh);
+    kb = (const TA_GLOBAL T*)p.k + (p.ptab ? 0 : b * p.ksb + h * p.ksh);
+    vb = (const TA_GLOBAL T*)p.v + (p.ptab ? 0 : b * p.vsb + h * p.vsh);
     tab = p.ptab ? p.ptab + b * p.pt_sb + h * p.pt_sh : nullptr;
     int lo = 0x7fffffff, hi = -1;
 #pragma unroll
@@ -187,8 +194,11 @@ struct Share {
       const bool in = r < p.R;
       int j = 0, n = 0;
       if (in) head_token(p, r, j, n);
-      int tt = in ? p.tq[b * p.tq_sb + n] : 0x7fffffff;
-      if (in && (tt < 0 || tt >= p.Tk)) tt = -1;
+      int tt = 0x7fffffff;
+      if (in) {
+        tt = one ? last : p.tq[b * p.tq_sb + n];   // (one token: its position, checked, is known)
+        if (tt < 0 || tt >= p.Tk) tt = -1;
+      }
       t[i] = tt;
       lo = tt < lo ? tt : lo;
       hi = in && tt > hi ? tt : hi;
@@ -197,6 +207,13 @@ struct Share {
       for (int s = 0; s < C::KS; ++s) {
         const int d = C::EB == 2 ? 32 * s + 8 * g : 16 * s + 4 * g;
         q[i][s] = in && d < D ? ldg16(qr + d) : make_uint4(0, 0, 0, 0);
+        if (p.scale < 0.0f) {
+          const uint32_t sign = C::EB == 2 ? 0x80008000u : 0x80000000u;
+          q[i][s].x ^= sign;
+          q[i][s].y ^= sign;
+          q[i][s].z ^= sign;
+          q[i][s].w ^= sign;
+        }
       }
     }
     reset();
@@ -221,8 +238,31 @@ struct Share {
     const int mine = pg;
     pg = page_of(next0);
     __builtin_amdgcn_sched_barrier(0);
-    const char* kr[C::KT];
-    const char* vr[C::KT * 4];
+    auto load_k = [&](int i, int s2, const TA_GLOBAL char* row) {
+      const int o = 64 * s2 + 16 * (lane & 3);
+      const u32x4_t r = *(const TA_GLOBAL u32x4_t*)(row + (uint32_t)(o < D * C::EB ? o : 0));
+      x.k[i][s2] = make_uint4(r.x, r.y, r.z, r.w);
+    };
+    auto load_v = [&](int e, const TA_GLOBAL char* at) {
+      if constexpr (C::VB >= 16) {
+#pragma unroll
+        for (int w = 0; w < C::VW; w += 4) {
+          const u32x4_t r = *(const TA_GLOBAL u32x4_t*)(at + 4 * w);
+          x.v[e][w] = r.x;
+          x.v[e][w + 1] = r.y;
+          x.v[e][w + 2] = r.z;
+          x.v[e][w + 3] = r.w;
+        }
+      } else if constexpr (C::VB == 8) {
+        const u32x2 r = *(const TA_GLOBAL u32x2*)at;
+        x.v[e][0] = r.x;
+        x.v[e][1] = r.y;
+      } else if constexpr (C::VB == 4) {
+        x.v[e][0] = *(const TA_GLOBAL uint32_t*)at;
+      } else {
+        x.v[e][0] = *(const TA_GLOBAL uint16_t*)at;
+      }
+    };
     if constexpr (WIDE) {
       int64_t ko, vo;
       bool ok = true;
@@ -246,17 +286,18 @@ struct Share {
       }
       if (!live) klast = vlast = 0;
       x.have = ok ? 0xffffffffu : 0u;
-      const char* k0p = reinterpret_cast<const char*>(kb + ko);
-      const char* v0p = reinterpret_cast<const char*>(vb + vo);
+      const TA_GLOBAL char* k0p = (const TA_GLOBAL char*)(kb + ko);
+      const TA_GLOBAL char* v0p = (const TA_GLOBAL char*)(vb + vo);
 #pragma unroll
       for (int i = 0; i < C::KT; ++i) {
         const uint32_t o = (lane >> 2) * ks + 16 * i * ks;
-        kr[i] = k0p + (o < klast ? o : klast);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t e = 4 * g * vs + (16 * i + u) * vs;
-          vr[4 * i + u] = v0p + (e < vlast ? e : vlast);
-        }
+        for (int s2 = 0; s2 < C::KS; ++s2) load_k(i, s2, k0p + (o < klast ? o : klast));
+      }
+#pragma unroll
+      for (int e = 0; e < C::KT * 4; ++e) {
+        const uint32_t o = 4 * g * vs + (16 * (e / 4) + e % 4) * vs;
+        load_v(e, v0p + ((o < vlast ? o : vlast) + C::VB * c));
       }
     } else {
       const int mask = live ? (1 << p.blog2) - 1 : 0;
@@ -265,40 +306,19 @@ struct Share {
       for (int i = 0; i < C::KT; ++i) {
         int page = __shfl(mine, 16 * i + (lane >> 2), kWave);
         page = page >= 0 && page < p.npages && live ? page : 0;
-        kr[i] = reinterpret_cast<const char*>(kb + page * p.pstride + (int64_t)((key0 + 16 * i + (lane >> 2)) & mask) * p.kst);
+        const TA_GLOBAL T* row = kb + page * p.pstride + (int64_t)((key0 + 16 * i + (lane >> 2)) & mask) * p.kst;
 #pragma unroll
-        for (int u = 0; u < 4; u += 2) {
-          const int e = 16 * i + 4 * g + u;
-          int pv = __shfl(mine, e, kWave);
-          const bool ok = pv >= 0 && pv < p.npages;
-          x.have |= ok ? 3u << (4 * i + u) : 0u;
-          const T* row = vb + (ok && live ? pv : 0) * p.pstride;
-          vr[4 * i + u] = reinterpret_cast<const char*>(row + (int64_t)((key0 + e) & mask) * p.vst);
-          vr[4 * i + u + 1] = reinterpret_cast<const char*>(row + (int64_t)((key0 + e + 1) & mask) * p.vst);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < C::KT; ++i)
-#pragma unroll
-      for (int s = 0; s < C::KS; ++s) {
-        const int o = 64 * s + 16 * (lane & 3);
-        x.k[i][s] = ldg16(kr[i] + (o < D * C::EB ? o : 0));
+        for (int s2 = 0; s2 < C::KS; ++s2) load_k(i, s2, (const TA_GLOBAL char*)row);
       }
 #pragma unroll
-    for (int e = 0; e < C::KT * 4; ++e) {
-      const char* a = vr[e] + C::VB * c;
-      if constexpr (C::VB >= 16) {
-#pragma unroll
-        for (int w = 0; w < C::VW; w += 4) *reinterpret_cast<uint4*>(&x.v[e][w]) = ldg16(a + 4 * w);
-      } else if constexpr (C::VB == 8) {
-        const u32x2 r = *(const TA_GLOBAL u32x2*)a;
-        x.v[e][0] = r.x;
-        x.v[e][1] = r.y;
-      } else if constexpr (C::VB == 4) {
-        x.v[e][0] = *(const TA_GLOBAL uint32_t*)a;
-      } else {
-        x.v[e][0] = *(const TA_GLOBAL uint16_t*)a;
+      for (int e = 0; e < C::KT * 4; e += 2) {
+        const int key = 16 * (e / 4) + 4 * g + e % 4;
+        const int page = __shfl(mine, key, kWave);
+        const bool ok = page >= 0 && page < p.npages;
+        x.have |= ok ? 3u << e : 0u;
+        const TA_GLOBAL T* at = vb + (ok && live ? page : 0) * p.pstride;
+        load_v(e, (const TA_GLOBAL char*)(at + (int64_t)((key0 + key) & mask) * p.vst) + C::VB * c);
+        load_v(e + 1, (const TA_GLOBAL char*)(at + (int64_t)((key0 + key + 1) & mask) * p.vst) + C::VB * c);
       }
     }
   }
@@ -350,13 +370,14 @@ struct Share {
   // than kSlack.
   template <bool MASKED>
   __device__ __forceinline__ void weights(const Step<T, D>& x, int i, f32x4 (&s)[C::KT]) {
-    const float f = p.scale * kLog2e;
+    const float f = fabsf(p.scale) * kLog2e;   // (a negative scale turns q round: the largest score is the largest product)
     float top = kLowest;
 #pragma unroll
     for (int a = 0; a < C::KT; ++a)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (!MASKED || sees(x, i, a, u)) top = fmaxf(top, s[a][u] * f);
+        if (!MASKED || sees(x, i, a, u)) top = fmaxf(top, s[a][u]);
+    top = top > kLowest ? top * f : kLowest;   // (a scale of zero, and products below the range, as others)
     if (__ballot(top > m[i] + (C::kShift + C::kSlack)) != 0) {
       // only the rows that need it: what a row gives does not depend on the others
       const float mx = max_rows(top);
@@ -463,11 +484,11 @@ struct Share {
         ko = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.kst;
         vo = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.vst;
       }
-      const T* kr = kb + ko + g * (D / 4);
-      const T* vr = vb + vo + g * (D / 4);
+      const TA_GLOBAL T* kr = kb + ko + g * (D / 4);
+      const TA_GLOBAL T* vr = vb + vo + g * (D / 4);
       float s = 0.0f;
 #pragma unroll 1
-      for (int d = 0; d < D / 4; ++d) s = fmaf(to_f32(qr[d]), to_f32(kr[d]), s);
+      for (int d = 0; d < D / 4; ++d) s = fmaf(to_f32(qr[d]), number(kr + d), s);
       s = sum_rows(s) * (p.scale * kLog2e);
       if (key > t[i] || r >= p.R) continue;
       const float mn = fmaxf(m[i], s - C::kShift);
@@ -477,7 +498,7 @@ struct Share {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int d = 0; d < C::DJ; ++d) acc[i][d][u] = fmaf(w, to_f32(vr[u * C::DJ + d]), acc[i][d][u] * alpha);
+        for (int d = 0; d < C::DJ; ++d) acc[i][d][u] = fmaf(w, number(vr + u * C::DJ + d), acc[i][d][u] * alpha);
     }
   }
 
@@ -562,7 +583,7 @@ __device__ __forceinline__ float lse_of(float m, float l) { return l != 0.0f ? (
 
 // A wavefront a set of 16 NT rows, no split.
 template <typename T, int D, bool WIDE, int NT>
-__global__ __launch_bounds__(kWaves * kWave, 2) void dense_rows_kernel(Dense p) {
+__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_rows_kernel(Dense p) {
   const int64_t per = (p.R + kRows * NT - 1) / (kRows * NT);
   // consecutive sets share their keys: those of one XCD (workgroups go round robin over the 8) are consecutive
   const unsigned n8 = gridDim.x / 8;
@@ -593,104 +614,19 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_rows_kernel(Dense p) 
   });
 }
 
-constexpr int kMinKeys = 32;         // of a wavefront
-
-// gsplit workgroups of four wavefronts a set of 16 NT rows.
-template <typename T, int D, bool WIDE, int NT>
-__global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p) {
-  extern __shared__ __align__(16) float smem[];
-  constexpr int KEYS = Tile<T, D>::KEYS;
-  constexpr int kSet = kRows * NT;
-  TA_DMARK(0);
-  // x: workgroup of the set, y: set; sets of one key head, which share its keys, come on one XCD (workgroups go round robin
-  // over the 8)
-  const int sets = (p.R + kSet - 1) / kSet;
-  unsigned gs = blockIdx.x, at = blockIdx.y;
-  if (sets > 1) {
-    const unsigned id = blockIdx.y * gridDim.x + blockIdx.x, n8 = gridDim.x * gridDim.y / 8;
-    const unsigned to = (id & 7) * n8 + id / 8;   // (the grid is a multiple of 8)
-    gs = to % gridDim.x;
-    at = to / gridDim.x;
-    if (at >= (unsigned)(p.BH * sets)) return;
-  }
-  const int set = sets > 1 ? at % sets : 0;
-  const int bh = sets > 1 ? at / sets : at;
-  const int b = bh / p.H, h = bh - b * p.H;
-  const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
-  const int row0 = set * kSet;
-  const int rows = p.R - row0 < kSet ? p.R - row0 : kSet;
-  Share<T, D, WIDE, NT> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP);
-  // equal runs of whole steps a wavefront; workgroups without one are not needed
-  const int nkeys = s.tmax + 1;
-  int run = (nkeys + p.gsplit * kWaves - 1) / (p.gsplit * kWaves);
-  run = (run < kMinKeys ? kMinKeys : run) + KEYS - 1;
-  run -= run % KEYS;
-  const int64_t wgrun = (int64_t)run * kWaves;
-  const int active = nkeys > 0 ? (int)((nkeys + wgrun - 1) / wgrun) : 1;
-  if ((int)gs >= active) return;
-  const int64_t k0 = gs * wgrun + (int64_t)w * run;
-  TA_DMARK(1);
-  const int from = k0 < nkeys ? (int)k0 : nkeys, to = k0 + run < nkeys ? (int)(k0 + run) : nkeys;
-  // the four wavefronts' parts, behind their keys: [4][rows][D + 2], first the reference and the sum
-  float* const parts = smem + kWaves * Tile<T, D>::LSTEP / 4;
-  s.run(row0, b, h, from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, [&](uint32_t done) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      if (!(done >> (kRows * i + s.c) & 1)) continue;
-      float* part = parts + (w * rows + kRows * i + s.c) * (D + 2);
-      if (s.g == 0) {
-        part[0] = s.m[i];
-        part[1] = s.l[i];
-      }
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) part[2 + s.col(d, u)] = s.acc[i][d][u];
-    }
-  });
-  TA_DMARK(2);
-  __syncthreads();
-  float* ws = p.ws + ((int64_t)at * p.gsplit + gs) * kSet * (D + 2);
-  for (int i = tid; i < rows * D; i += kWaves * kWave) {
-    const int r = i / D, d = i % D;
-    float M = kLowest, L = 0.0f, a = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      const float* q = parts + (k * rows + r) * (D + 2);
-      if (q[1] != 0.0f) M = fmaxf(M, q[0]);
-    }
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      const float* q = parts + (k * rows + r) * (D + 2);
-      const float f = q[1] != 0.0f ? __builtin_amdgcn_exp2f(q[0] - M) : 0.0f;
-      if (q[1] != 0.0f) {
-        L = fmaf(q[1], f, L);
-        a = fmaf(q[2 + d], f, a);
-      }
-    }
-    if (active == 1) {
-      int64_t at, le;
-      row_place(p, b, h, row0 + r, at, le);
-      reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
-      if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
-    } else {
-      stgf_dc(ws + r * (D + 2) + 2 + d, a);
-      if (d == 0) {
-        stgf_dc(ws + r * (D + 2), M);
-        stgf_dc(ws + r * (D + 2) + 1, L);
-      }
-    }
-  }
-  if (active == 1) return;
-  // each workgroup has written its part through to memory and counts itself in; the last to arrive joins them and resets the
-  // counter (no workgroup waits for another)
+// One set's parts joined: each workgroup has written its part through to memory and counts itself in; the last to arrive joins
+// them and resets the counter (no workgroup waits for another).
+template <typename T, int D, int kSet>
+__device__ __forceinline__ void join_parts(const Dense& p, int b, int h, int row0, int rows, int set, int wg0, int count,
+                                           float* smem) {
+  const int tid = threadIdx.x;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   TA_DMARK(3);
-  uint32_t* cnt = p.cnt + at;
+  uint32_t* cnt = p.cnt + set;
   int* flag = reinterpret_cast<int*>(smem);
   if (tid == 0)
-    *flag = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(active - 1);
+    *flag = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(count - 1);
   __syncthreads();
   const int last = *flag;
   __syncthreads();
@@ -698,7 +634,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p)
   if (!last) return;
   // a thread an element, or several with a share of the parts each where there are few elements: all loads of eight parts at
   // once, so that the parts cost one round trip to memory and not one each
-  const float* all = p.ws + (int64_t)at * p.gsplit * kSet * (D + 2);
+  const float* all = p.ws + (int64_t)wg0 * kSet * (D + 2);
   const int E = rows * D;
   const int groups = E < kWaves * kWave ? kWaves * kWave / E : 1;
   for (int base = 0; base < E; base += kWaves * kWave) {
@@ -707,14 +643,14 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p)
     const bool in = i < E && first < groups;
     float M = kLowest, L = 0.0f, a = 0.0f;
     if (in) {
-      for (int k0 = first; k0 < active; k0 += 8 * groups) {
+      for (int k0 = first; k0 < count; k0 += 8 * groups) {
         float mk[8], lk[8], vk[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int part = k0 + k * groups;
-          const float* q = all + ((int64_t)(part < active ? part : first) * kSet + r) * (D + 2);
+          const float* q = all + ((int64_t)(part < count ? part : first) * kSet + r) * (D + 2);
           mk[k] = ldgf_dc(q);
-          lk[k] = part < active ? ldgf_dc(q + 1) : 0.0f;
+          lk[k] = part < count ? ldgf_dc(q + 1) : 0.0f;
           vk[k] = ldgf_dc(q + 2 + d);
         }
         float mn = M;
@@ -764,6 +700,173 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void dense_split_kernel(Dense p)
   if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // ready for the next call
 }
 
+constexpr int kQuantum = 128;        // keys of one unit of work
+
+// Units of work of sequence b: kQuantum keys each, at least one (its rows are written even where they see nothing).  Lane i of
+// a wavefront takes sequence b0 + i; n is the last position that any of its rows sees, -1 for none.
+__device__ __forceinline__ int units_of(const Dense& p, int b0, int& n) {
+  const int lane = lane_id();
+  n = -1;
+  if (p.Nq <= 4) {
+    if (b0 + lane < p.B)
+      for (int i = 0; i < p.Nq; ++i) {
+        const int t = p.tq[(b0 + lane) * p.tq_sb + i];
+        n = t < p.Tk && t > n ? t : n;
+      }
+  } else {
+    for (int k = 0; k < kWave && b0 + k < p.B; ++k) {
+      int m = -1;
+      for (int i = lane; i < p.Nq; i += kWave) {
+        const int t = p.tq[(b0 + k) * p.tq_sb + i];
+        m = t < p.Tk && t > m ? t : m;
+      }
+      m = -min16(-m);
+      m = max(max(__builtin_amdgcn_readlane(m, 0), __builtin_amdgcn_readlane(m, 16)),
+              max(__builtin_amdgcn_readlane(m, 32), __builtin_amdgcn_readlane(m, 48)));
+      n = lane == k ? m : n;
+    }
+  }
+  return b0 + lane < p.B ? (n < kQuantum ? 1 : n / kQuantum + 1) : 0;
+}
+template <int N>
+__device__ __forceinline__ int add_shr(int x) {   // x + that of lane - N of its 16 lanes (0 before the first)
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x110 + N, 0xF, 0xF, false);
+}
+__device__ __forceinline__ int prefix64(int x) {   // sum of lanes 0 .. lane
+  x = add_shr<8>(add_shr<4>(add_shr<2>(add_shr<1>(x))));
+  const int a = __builtin_amdgcn_readlane(x, 15), b = __builtin_amdgcn_readlane(x, 31), c = __builtin_amdgcn_readlane(x, 47);
+  const int row = lane_id() >> 4;
+  return x + (row == 0 ? 0 : row == 1 ? a : row == 2 ? a + b : a + b + c);
+}
+
+// Workgroups of four wavefronts, each with a share of one set of 16 NT rows.  A set gets as many as its sequence is long (each
+// takes at most 1 / nwg of all units of all sets): sequences of any lengths end together, and few long ones fill the GPU.  The
+// grid has a workgroup for each of the nwg and each set, which is as many as there can be; those left over leave at once.
+template <typename T, int D, bool WIDE, int NT>
+__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int KEYS = Tile<T, D>::KEYS;
+  constexpr int kSet = kRows * NT;
+  TA_DMARK(0);
+  const int sets = (p.R + kSet - 1) / kSet;      // of a (sequence, key head)
+  const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
+  const int per = p.H * sets;                    // sets of a sequence (all units: fewer than 2^31)
+  int all = 0;
+  int u0 = 0, n0 = -1;                           // lane i: units of a set of sequence i of the first 64, its last position
+  for (int b0 = 0; b0 < p.B; b0 += kWave) {
+    int n;
+    const int u = units_of(p, b0, n);
+    if (b0 == 0) {
+      u0 = u;
+      n0 = n;
+    }
+    all += __builtin_amdgcn_readlane(prefix64(u), kWave - 1);
+  }
+  all *= per;
+  const int most = (int)(((unsigned)all + nwg - 1) / nwg);       // units of a workgroup
+  int wg = blockIdx.x;
+  if (sets > 1) {
+    // sets of one key head share its keys: the workgroups in use next to each other are those of one XCD (they go round robin
+    // over the 8; the grid is a multiple of 8)
+    int used = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kWave) {
+      int n;
+      const int u = b0 == 0 ? u0 : units_of(p, b0, n);
+      used += __builtin_amdgcn_readlane(prefix64((int)((unsigned)(u + most - 1) / (unsigned)most)), kWave - 1);
+    }
+    const int share = (used * per + 7) / 8;
+    if (wg / 8 >= share) return;
+    wg = wg % 8 * share + wg / 8;
+  }
+  // its sequence, and the workgroups of that one's sets
+  int b = -1, ub = 0, count = 0, start = 0, last = -1;
+  for (int b0 = 0; b0 < p.B; b0 += kWave) {
+    int t = n0;
+    const int u = b0 == 0 ? u0 : units_of(p, b0, t);
+    const int n = (int)((unsigned)(u + most - 1) / (unsigned)most);
+    const int sum = prefix64(n);
+    const uint64_t past = __ballot(start + sum * per > wg);
+    if (past != 0) {
+      const int i = __ffsll((unsigned long long)past) - 1;
+      b = b0 + i;
+      ub = __builtin_amdgcn_readlane(u, i);
+      count = __builtin_amdgcn_readlane(n, i);
+      last = __builtin_amdgcn_readlane(t, i);
+      start += (__builtin_amdgcn_readlane(sum, i) - count) * per;
+      break;
+    }
+    start += __builtin_amdgcn_readlane(sum, kWave - 1) * per;
+  }
+  if (b < 0) return;
+  const int in = (wg - start) / count;           // set of the sequence
+  const int part = wg - start - in * count;
+  const int h = sets > 1 ? in / sets : in, row0 = sets > 1 ? (in - h * sets) * kSet : 0;
+  const int rows = p.R - row0 < kSet ? p.R - row0 : kSet;
+  Share<T, D, WIDE, NT> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, last);
+  // its keys, and the equal runs of whole steps of its wavefronts
+  const int nkeys = s.tmax + 1;
+  const int mine = (int)((unsigned)ub / (unsigned)count), more = ub - mine * count;
+  const int first = part * mine + (part < more ? part : more);
+  int k0 = first * kQuantum, k1 = (first + mine + (part < more ? 1 : 0)) * kQuantum;
+  k0 = k0 < nkeys ? k0 : nkeys;
+  k1 = k1 < nkeys ? k1 : nkeys;
+  int run = (k1 - k0 + kWaves - 1) / kWaves + KEYS - 1;
+  run -= run % KEYS;
+  const int from = k0 + w * run < k1 ? k0 + w * run : k1, to = from + run < k1 ? from + run : k1;
+  TA_DMARK(1);
+  // the four wavefronts' parts, behind their keys: [4][rows][D + 2], first the reference and the sum
+  float* const parts = smem + kWaves * Tile<T, D>::LSTEP / 4;
+  s.run(row0, b, h, from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, [&](uint32_t done) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (!(done >> (kRows * i + s.c) & 1)) continue;
+      float* part = parts + (w * rows + kRows * i + s.c) * (D + 2);
+      if (s.g == 0) {
+        part[0] = s.m[i];
+        part[1] = s.l[i];
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) part[2 + s.col(d, u)] = s.acc[i][d][u];
+    }
+  });
+  TA_DMARK(2);
+  __syncthreads();
+  float* ws = p.ws + (int64_t)wg * kSet * (D + 2);
+  for (int i = tid; i < rows * D; i += kWaves * kWave) {
+    const int r = i / D, d = i % D;
+    float M = kLowest, L = 0.0f, a = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      const float* q = parts + (k * rows + r) * (D + 2);
+      if (q[1] != 0.0f) M = fmaxf(M, q[0]);
+    }
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      const float* q = parts + (k * rows + r) * (D + 2);
+      const float f = q[1] != 0.0f ? __builtin_amdgcn_exp2f(q[0] - M) : 0.0f;
+      if (q[1] != 0.0f) {
+        L = fmaf(q[1], f, L);
+        a = fmaf(q[2 + d], f, a);
+      }
+    }
+    if (count == 1) {
+      int64_t at, le;
+      row_place(p, b, h, row0 + r, at, le);
+      reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
+      if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
+    } else {
+      stgf_dc(ws + r * (D + 2) + 2 + d, a);
+      if (d == 0) {
+        stgf_dc(ws + r * (D + 2), M);
+        stgf_dc(ws + r * (D + 2) + 1, L);
+      }
+    }
+  }
+  if (count > 1) join_parts<T, D, kSet>(p, b, h, row0, rows, b * per + in, wg - part, count, smem);
+}
+
 template <typename T, int D, bool WIDE, int NT>
 int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const dim3 blk(kWaves * kWave);
@@ -775,9 +878,11 @@ int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   }
   const int rows = p.R < kRows * NT ? p.R : kRows * NT;
   const size_t stage = kWaves * Tile<T, D>::LSTEP, parts = (size_t)kWaves * rows * (D + 2), join = 3 * kWaves * kWave;
-  const dim3 grid((unsigned)p.gsplit, (unsigned)(per > 1 ? (sets + 7) / 8 * 8 : sets));
+  const int nwg = nsplit / kWaves;
+  const int64_t wgs = nwg == 1 ? sets : nwg + sets;
+  const dim3 grid((unsigned)(per > 1 ? (wgs + 7) / 8 * 8 : wgs));
   hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT>), grid, blk, stage + (parts > join ? parts : join) * sizeof(float),
-                     st, p);
+                     st, p, nwg);
   return check_launch("dense_split_kernel");
 }
 
@@ -811,12 +916,21 @@ int dispatch_dense(const Dense& p, int nsplit, hipStream_t st) {
 
 using namespace ta;
 
+namespace ta {
+namespace {
+// Counters and sets of whole tiles of 32 rows (16 where there are no more), whichever the kernels take.
+int64_t dense_sets(int B, int Hq, int H, int Nq) {
+  const int64_t R = (int64_t)(Hq / H) * Nq;
+  return (int64_t)B * H * (R <= 16 ? 1 : (R + 31) / 32 * 2);
+}
+}  // namespace
+}  // namespace ta
+
 extern "C" int64_t ta_dense_attn_workspace_size(int B, int Hq, int H, int Nq, int D, int nsplit) {
   if (B <= 0 || H <= 0 || Hq <= 0 || Nq <= 0 || nsplit <= 4) return 0;
-  // counters and parts of whole tiles of 32 rows (16 where there are no more), whichever the kernels take
-  const int64_t R = (int64_t)(Hq / H) * Nq;
-  const int64_t rows = R <= 16 ? 16 : (R + 31) / 32 * 32;
-  return ((int64_t)B * H * (rows / 16) * 4 + 255) / 256 * 256 + (int64_t)B * H * rows * (nsplit / 4) * (D + 2) * 4;
+  const int64_t sets = dense_sets(B, Hq, H, Nq);
+  // a part for each workgroup and each set, of 16 rows, or of 32 for half as many sets
+  return (sets * 4 + 255) / 256 * 256 + (sets + nsplit / 2) * 16 * (D + 2) * 4;
 }
 
 extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, int dtype, int64_t qsb, int64_t qsh,
@@ -836,8 +950,8 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
     set_error("ta_dense_attn_fwd: bad sizes (query heads a multiple of the key heads)");
     return TA_ERR_ARG;
   }
-  if (nsplit < 1 || (nsplit > 1 && nsplit % 4) || nsplit > 1024) {
-    set_error("ta_dense_attn_fwd: nsplit must be 1 or a multiple of 4, at most 1024");
+  if (nsplit < 1 || (nsplit > 1 && nsplit % 4) || nsplit > 8192) {
+    set_error("ta_dense_attn_fwd: nsplit must be 1 or a multiple of 4, at most 8192");
     return TA_ERR_ARG;
   }
   if (pages && (pages->table == nullptr || pages->num_pages <= 0 || pages->block_log2 < 1 || pages->block_log2 > 14)) {
@@ -857,11 +971,10 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
     return TA_ERR_ARG;
   }
   const int64_t R = (int64_t)(Hq / H) * Nq;
-  const int64_t sets = (int64_t)B * H * (R <= 16 ? 1 : (R + 31) / 32 * 2);   // counters of the workspace
-  if (R > (1 << 30) || (int64_t)B * H > (1 << 30) || sets * (nsplit > 4 ? nsplit / 4 : 1) > 0x7ffffff0LL ||
-      (nsplit > 1 && sets > 65528) ||
-      Tk > 0x7fffffff - 4096) {
-    set_error("ta_dense_attn_fwd: too large (nsplit above 1: at most 65528 (sequence, key head) pairs times sets of 16 rows)");
+  const int64_t sets = dense_sets(B, Hq, H, Nq);
+  if (R > (1 << 30) || sets > (1 << 30) || Tk > 0x7fffffff - 4096 ||
+      (nsplit > 1 && sets * ((Tk + 127) / 128) > 0x7fffffffLL)) {
+    set_error("ta_dense_attn_fwd: too large");
     return TA_ERR_UNSUPPORTED;
   }
   if (kst < 0 || vst < 0 || kst * sz * 32 > 0x7fffffffLL || vst * sz * 32 > 0x7fffffffLL) {
@@ -885,7 +998,7 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
   }
   p.BH = B * H;
   p.R = (int)R;
-  p.gsplit = nsplit > 4 ? nsplit / 4 : 1;
+  p.B = B;
   if (need > 0) {
     p.cnt = reinterpret_cast<uint32_t*>(ws);
     p.ws = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + (sets * 4 + 255) / 256 * 256);

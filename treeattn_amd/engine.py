@@ -383,12 +383,19 @@ def decode_nsplit8(B, H, Nq, wl, leaf):
 
 def decode_nsplit_dense(B, H, rows, keys, D=64):
     """dense_attn's nsplit for B * H (sequence, key head) pairs of `rows` query rows (query heads of a key head times tokens)
-    over up to `keys` keys."""
-    sets = max(1, B * H * ((rows + 15) // 16))
+    over up to `keys` keys: four wavefronts for each of the workgroups that the units of 128 keys are dealt to.
+
+    A set of rows gets a whole number of workgroups, so those in use are up to one a set more than that; all at once on the 256
+    compute units they should be: 12 queries over 131000 keys of 64 take 66 us with 244 and 74 with 256 (264 in use), 32 sets of
+    4 x 128 over 6001 keys 23.2 and 25.4.  From 192 sets on, two workgroups a compute unit (384 sets over 32768 keys 491 us with
+    512, 516 with 256), and from 4096 a wavefront a set."""
+    sets = max(1, B * H * ((rows + 31) // 32 if rows > 16 else 1))
+    units = (max(1, keys) + 127) // 128
     if sets >= 4096:
         return 1
-    g = min(max(1, 2048 // sets // 4 * 2), max(1, keys // 256), 256)
-    return 4 * g
+    if units == 1:
+        return 4
+    return 4 * min(256 - sets if sets <= 192 else 512, sets * units)
 
 
 def _budget_weights(state, pw):
