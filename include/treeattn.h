@@ -620,7 +620,8 @@ int ta_argmax_rows(const void* x, int dtype, int64_t rows, int64_t n, int64_t st
 /*
  * First op of a decode step (engine.py:168, x = wte[tok] + wpe[t]): x[b, :] = wte[tok[b], :] + wpe[t[b], :]
  * in dtype (the sum rounded once), pos32[b] = t[b]; with `advance`, t[b] += 1 afterwards (the next step's
- * position, so a captured step can be replayed).  tok, t: int64 (B,); tables with row strides ldw, ldp.
+ * position, so a captured step can be replayed).  tok, t: int64 (B,); tables with row strides ldw, ldp (0: one row
+ * for every position).
  * ln_w != NULL (bf16, C a multiple of 64, at most 4096): also x_ln[b, :] = LN(x[b, :]) with weight ln_w and
  * eps ln_eps, the first layer's LN1 (model.py:43), bit for bit as ta_rowmm computes it.
  */

@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import kernels as K
+from . import positions
 from .fastseg import sparse_attn
 from .forest import gather_nodes
 
@@ -48,8 +49,7 @@ class TreeAttention(nn.Module):
 
     def forward(self, x):
         b, T, C = x.shape
-        q, k, v = self.c_attn(x).split(C, dim=2)
-        q, k, v = [t.view(b, T, self.H, self.dh).transpose(1, 2) for t in (q, k, v)]
+        q, k, v = positions.heads(self, self.c_attn(x))
         out = self.sparse_attend(q, k, v)
         return self.c_proj(out.transpose(1, 2).reshape(b, T, C))
 

@@ -172,7 +172,7 @@ extern "C" int ta_bf16_from_f32(const float* in, uint16_t* out, int64_t n, void*
 extern "C" int ta_embed(const int64_t* tok, int64_t* tpos, int advance, const void* wte, int64_t ldw, const void* wpe,
                         int64_t ldp, int dtype, int B, int C, int64_t V, int64_t P, void* x, int64_t ldx,
                         int32_t* pos32, const void* ln_w, float ln_eps, void* x_ln, int64_t ld_xln, void* stream) {
-  if (B <= 0 || C <= 0 || V <= 0 || P <= 0 || ldw < C || ldp < C || ldx < C) {
+  if (B <= 0 || C <= 0 || V <= 0 || P <= 0 || ldw < C || (ldp < C && ldp != 0) || ldx < C) {
     set_error("ta_embed: bad sizes");
     return TA_ERR_ARG;
   }

@@ -12,6 +12,11 @@ and step(tok, t) -> (logits, keys), weights_from_ours / weights_from_nanogpt -- 
 * tree shape: cfg.leaf / cfg.arity (the reference is leaf=2, arity=2);
 * paged caches: a Decoder keeps K and V in pages of one leaf block of one (sequence, head) (PagePool), handed
   out as positions are reached (max_tokens bounds the pool, not Tcap); a stand-alone SegState is contiguous;
+* whole caches: Decoder(mode='dense', paged=True) attends to every earlier position of paged caches (kernels.dense_attn), any
+  batch, captured or not;
+* rotary positions: cfg.rope, for models without learned positions (weights without 'wpe');
+* Decoder.fork(src, dst, t) lets sequence dst go on from the first t positions of src: whole pages are shared until one of
+  the two writes into them, the one being filled is copied; Decoder.resize(num_pages) makes the page pool larger or smaller;
 * Decoder.prefill(idx) fills every layer's cache from a prompt in one pass (the forward of the model over
   the prompt, sparse attention included) and returns the last position's logits;
 * Decoder.capture(tok, t) captures one greedy step (logits, argmax token, position advance) in a HIP graph
@@ -31,6 +36,7 @@ import torch
 import torch.nn.functional as F
 
 from . import kernels as K
+from . import positions
 from . import selection as SEL
 from .forest import gather_nodes
 
@@ -53,16 +59,24 @@ class PagePool:
     head); every layer has its own pool tensor (P, 2, leaf, dh), and one page table (B, H, Tcap / leaf) int32
     serves all layers (leaf block j of (b, h) has the same page id in every layer's pool).  Pages are handed out
     as positions are reached (ensure, on the host, outside captured steps) and returned per sequence (release);
-    the pool holds num_pages pages, so memory follows the tokens provisioned rather than Tcap."""
+    the pool holds num_pages pages, so memory follows the tokens provisioned rather than Tcap.
+
+    Sequences may share pages: fork(src, dst, t) gives dst the first t positions of src, its whole blocks by sharing their
+    pages and the rest of a block as a copy.  A shared page is only read: before a position in it is written again, own() puts a
+    copy in its place (ensure does so for the positions that it is told to start from).  refs counts the sequences of a page;
+    it is free again when the last of them is released.  resize(num_pages) moves the pages in use, in their sequences' order, to
+    pools of another size."""
 
     def __init__(self, B, H, dh, leaf, Tcap, num_pages, n_layers, dtype, dev, cache=None):
         """cache 'e4m3': pages of float8_e4m3fn with a (P, 2) float32 tensor of scales per layer."""
         self.B, self.H, self.leaf, self.Tcap, self.P = B, H, leaf, Tcap, int(num_pages)
-        nblk = Tcap // leaf
+        nblk = (Tcap + leaf - 1) // leaf
         self.table = torch.full((B, H, nblk), -1, dtype=torch.int32, device=dev)
         self.host = torch.full((B, H, nblk), -1, dtype=torch.int32)
         self.nblk = [0] * B                        # leaf blocks of each sequence that have pages
         self.free = list(range(self.P - 1, -1, -1))   # pages handed out in increasing order
+        self.refs = [0] * self.P                   # sequences that use a page
+        self.n_shared = 0                          # pages that more than one uses
         if cache is None:
             self.pools = [torch.zeros(self.P, 2, leaf, dh, dtype=dtype, device=dev) for _ in range(n_layers)]
             self.scales = None
@@ -72,11 +86,65 @@ class PagePool:
             self.scales = [torch.ones(self.P, 2, device=dev) for _ in range(n_layers)]
         self.held = []                             # tail_block of every 8-bit cache over these pages
 
-    def ensure(self, t_end, seqs=None):
+    def _tensors(self):
+        return self.pools + (self.scales or [])
+
+    def _copy(self, src, dst, out=None):
+        """Pages src of every layer to pages dst (lists of ids), in one launch for the pools of 32 layers."""
+        if not src:
+            return
+        x = self._tensors()
+        ids = torch.tensor([src, dst], dtype=torch.int32)
+        if self.table.is_cuda:
+            ids = ids.pin_memory().to(self.table.device, non_blocking=True)
+            K.copy_rows(x, ids[0], ids[1], out=out)
+        else:
+            ids = ids.long()
+            for a, b in zip(x, x if out is None else out):
+                a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
+                b[ids[1]] = a[ids[0]]
+
+    def _show(self, b0, b1, j0, j1):
+        """Blocks j0 .. j1-1 of sequences b0 .. b1-1 from the host's table to the device's: one copy, ordered on the current
+        stream after the steps already queued, staged in pinned memory so the host does not wait for those steps."""
+        src = self.host[b0:b1, :, j0:j1].contiguous()
+        if self.table.is_cuda:
+            self.table[b0:b1, :, j0:j1].copy_(src.pin_memory(), non_blocking=True)
+        else:
+            self.table[b0:b1, :, j0:j1].copy_(src)
+
+    def _take(self, n):
+        """n free pages, the last of the free list first."""
+        if n > len(self.free):
+            raise RuntimeError('PagePool: out of pages (%d needed, %d free of %d): raise max_tokens'
+                               % (n, len(self.free), self.P))
+        ids = self.free[len(self.free) - n:]
+        del self.free[len(self.free) - n:]
+        ids.reverse()
+        for p in ids:
+            self.refs[p] = 1
+        return ids
+
+    def _use(self, p):
+        self.refs[p] += 1
+        self.n_shared += self.refs[p] == 2
+
+    def _drop(self, p):
+        self.refs[p] -= 1
+        self.n_shared -= self.refs[p] == 1
+        if self.refs[p] == 0:
+            self.free.append(p)
+
+    def ensure(self, t_end, seqs=None, start=None):
         """Pages for positions < t_end (at most Tcap) of the given sequences (all by default): a sequence's
-        blocks get consecutive pages, head by head."""
+        blocks get consecutive pages, head by head.  start: the first position of each of these sequences that will be written
+        (blocks from there on that are shared get pages of their own); None: only positions that no page holds yet."""
         need = (min(int(t_end), self.Tcap) + self.leaf - 1) // self.leaf
-        todo = [b for b in (range(self.B) if seqs is None else seqs) if self.nblk[b] < need]
+        seqs = range(self.B) if seqs is None else seqs
+        if start is not None and self.n_shared:
+            for b, t in zip(seqs, start):
+                self.own(b, t, t_end)
+        todo = [b for b in seqs if self.nblk[b] < need]
         if not todo:
             return
         n_all = sum((need - self.nblk[b]) * self.H for b in todo)
@@ -86,39 +154,119 @@ class PagePool:
         lo = min(self.nblk[b] for b in todo)
         for b in todo:
             have = self.nblk[b]
-            n = (need - have) * self.H
-            ids = self.free[len(self.free) - n:]       # taken from the end of the free list, last entry first
-            del self.free[len(self.free) - n:]
-            ids.reverse()
+            ids = self._take((need - have) * self.H)
             self.host[b, :, have:need] = torch.tensor(ids, dtype=torch.int32).view(self.H, need - have)
             self.nblk[b] = need
-        # one copy of the changed columns, ordered on the current stream after the steps already queued (they
-        # read no entry that changes); staged in pinned memory so the host does not wait for those steps
-        rows = slice(min(todo), max(todo) + 1)
-        src = self.host[rows, :, lo:need].contiguous()
-        if self.table.is_cuda:
-            self.table[rows, :, lo:need].copy_(src.pin_memory(), non_blocking=True)
-        else:
-            self.table[rows, :, lo:need].copy_(src)
+        # the changed columns (the steps already queued read no entry that changes)
+        self._show(min(todo), max(todo) + 1, lo, need)
 
-    def release(self, b):
-        """Return sequence b's pages (its cache rows are forgotten, those of the block an 8-bit cache's tail holds too)."""
+    def own(self, b, t, t_end=None):
+        """Pages of its own for the blocks of sequence b that hold positions t .. t_end-1 (default: to the last) and that it
+        shares: copies of what they hold."""
+        j0 = int(t) // self.leaf
+        j1 = self.nblk[b] if t_end is None else min(self.nblk[b], (int(t_end) + self.leaf - 1) // self.leaf)
+        todo = [(h, j) for j in range(max(0, j0), j1) for h in range(self.H) if self.refs[int(self.host[b, h, j])] > 1]
+        if not todo:
+            return
+        ids = self._take(len(todo))
+        old = [int(self.host[b, h, j]) for h, j in todo]
+        for (h, j), p, q in zip(todo, ids, old):
+            self.host[b, h, j] = p
+            self._drop(q)
+        self._copy(old, ids)
+        self._show(b, b + 1, j0, j1)
+
+    def fork(self, src, dst, t):
+        """Sequence dst takes the first t positions of src (at most those that src holds; what dst had is released): whole blocks
+        share src's pages, the rows of a block that t ends inside are copied into pages of dst's own."""
+        t = int(t)
+        if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
+            raise ValueError('PagePool.fork: two different sequences of %d' % self.B)
+        if not 0 <= t <= min(self.nblk[src] * self.leaf, self.Tcap):
+            raise ValueError('PagePool.fork: sequence %d holds no %d positions' % (src, t))
+        whole, part = divmod(t, self.leaf)
+        back = sum(self.refs[int(p)] == 1 for p in self.host[dst, :, :self.nblk[dst]].reshape(-1).tolist())
+        if part and self.H > len(self.free) + back:
+            raise RuntimeError('PagePool: out of pages (%d needed, %d free of %d): raise max_tokens'
+                               % (self.H, len(self.free) + back, self.P))
+        had = self.nblk[dst]
+        self._forget(dst)
+        for p in self.host[src, :, :whole].reshape(-1).tolist():
+            self._use(p)
+        self.host[dst, :, :whole] = self.host[src, :, :whole]
+        self.nblk[dst] = whole
+        if part:
+            ids = self._take(self.H)
+            self.host[dst, :, whole] = torch.tensor(ids, dtype=torch.int32)
+            self.nblk[dst] = whole + 1
+            self._copy(self.host[src, :, whole].tolist(), ids)
+        if max(had, self.nblk[dst]):
+            self._show(dst, dst + 1, 0, max(had, self.nblk[dst]))
+
+    def _forget(self, b):
+        """Sequence b's pages back, in the host's table."""
         n = self.nblk[b]
         for h in range(self.H - 1, -1, -1):
-            self.free.extend(int(p) for p in self.host[b, h, :n].flip(0).tolist())
+            for p in self.host[b, h, :n].flip(0).tolist():
+                self._drop(int(p))
         self.host[b, :, :n] = -1
-        self.table[b, :, :n].fill_(-1)
         self.nblk[b] = 0
+
+    def release(self, b):
+        """Return sequence b's pages (its cache rows are forgotten, those of the block an 8-bit cache's tail holds too); a page
+        that other sequences use stays theirs."""
+        n = self.nblk[b]
+        self._forget(b)
+        self.table[b, :, :n].fill_(-1)
         for held in self.held:
             held[b].fill_(-1)
+
+    def resize(self, num_pages):
+        """Pools of num_pages pages (at least those in use), the pages in use moved to their front in their sequences' order.
+        The page table keeps its tensor; the pool tensors are new ones: caches over them are made again (cache, cache8), and
+        steps captured with the old ones are captured again."""
+        order = {}
+        for b in range(self.B):
+            for j in range(self.nblk[b]):
+                for p in self.host[b, :, j].tolist():
+                    order.setdefault(p, len(order))
+        P = int(num_pages)
+        if P < max(1, len(order)):
+            raise RuntimeError('PagePool.resize: %d pages are in use' % len(order))
+        old = self._tensors()
+        new = [torch.zeros(P, *x.shape[1:], dtype=torch.uint8, device=x.device).view(x.dtype)
+               if x.dtype == torch.float8_e4m3fn else torch.zeros(P, *x.shape[1:], dtype=x.dtype, device=x.device)
+               for x in old]
+        if self.scales is not None:
+            for x in new[len(self.pools):]:
+                x.fill_(1.0)
+        self._copy(list(order), list(order.values()), out=new)
+        n = len(self.pools)
+        self.pools = new[:n]
+        self.scales = new[n:] if self.scales is not None else None
+        refs = [0] * P
+        for p, q in order.items():
+            refs[q] = self.refs[p]
+        for b in range(self.B):
+            k = self.nblk[b]
+            if k:
+                ids = [order[p] for p in self.host[b, :, :k].reshape(-1).tolist()]
+                self.host[b, :, :k] = torch.tensor(ids, dtype=torch.int32).view(self.H, k)
+        self.refs, self.P = refs, P
+        self.free = list(range(P - 1, len(order) - 1, -1))
+        if max(self.nblk, default=0):
+            self._show(0, self.B, 0, max(self.nblk))
 
     def cache(self, layer):
         return K.PagedCache(self.pools[layer], self.table, self.Tcap)
 
-    def cache8(self, layer, dtype):
-        """A layer's 8-bit cache, with a tail of its own in the model's dtype."""
+    def cache8(self, layer, dtype, of=None):
+        """A layer's 8-bit cache, with a tail of its own in the model's dtype, or with that of `of` (a cache over the pool that
+        resize replaced)."""
         B, H, dev = self.B, self.H, self.table.device
         _, two, leaf, dh = self.pools[layer].shape
+        if of is not None:
+            return K.Cache8(self.pools[layer], self.scales[layer], self.table, of.tail, of.tail_block, self.Tcap)
         held = torch.full((B, H), -1, dtype=torch.int32, device=dev)
         self.held.append(held)
         return K.Cache8(self.pools[layer], self.scales[layer], self.table,
@@ -137,7 +285,7 @@ class SegState:
         self.dev = torch.device(dev)
         self.shape = SEL.cfg_shape(cfg, Tcap)
         self.Lm = self.shape.blevels[-1] if self.shape.n_levels else 0
-        self.pages = pages
+        self.pages, self.layer = pages, layer
         self.cache8 = None
         if pages is not None and pages.scales is not None:
             self.cache8 = pages.cache8(layer, dtype)
@@ -238,6 +386,26 @@ class SegState:
             K.gate_append(Kc, tpos, self.levels, self.lg, self.gl, self.shape.blevels, self.shape.arity,
                           float(self.cfg.gate_q))
 
+    def sequence_tensors(self):
+        """The tensors that hold a row for each sequence (not its pages): what a fork copies."""
+        out = [*self.levels, self.ksum]
+        if self.st_leaf.numel():
+            out += [self.st_leaf, self.st_score, self.st_ok]
+        if self.gated:
+            out += self.lg + [t for t in self.gl if t is not None]
+        if self.cache8 is not None:
+            out += [self.cache8.tail, self.cache8.tail_block]
+        elif self.cache is None:
+            out += [self.K, self.V]
+        return out
+
+    def repage(self):
+        """The cache over the pool's tensors of now (PagePool.resize)."""
+        if self.cache8 is not None:
+            self.cache8 = self.pages.cache8(self.layer, self.dtype, self.cache8)
+        elif self.cache is not None:
+            self.cache = self.pages.cache(self.layer)
+
     def _tpos(self, t):
         if torch.is_tensor(t):
             return t.to(device=self.dev, dtype=torch.int32).reshape(self.B)
@@ -280,7 +448,7 @@ class SegState:
         """Load a whole context (engine.py:57-71).  K_, V_: (B,H,T,dh) with T <= Tcap."""
         T = K_.shape[2]
         if self.pages is not None:
-            self.pages.ensure(T)
+            self.pages.ensure(T, start=[0] * self.B)
         self.write_rows(0, K_, V_)
         t_end = T if t_end is None else t_end
         kd = K_.to(self.dtype)
@@ -302,6 +470,40 @@ class DenseState:
         return F.scaled_dot_product_attention(q, self.K[:, :, :t + 1], self.V[:, :, :t + 1]), float(t + 1)
 
 
+DENSE_PAGE = 64     # rows of a page of a dense decoder's caches
+
+
+class PagedState:
+    """A layer of a dense decoder over pages: every earlier position attended to (engine.py:74-81), any batch."""
+
+    def __init__(self, pages, layer, rope):
+        self.pages, self.layer, self.rope = pages, layer, rope
+        self.cache = pages.cache(layer)
+
+    def sequence_tensors(self):
+        return []
+
+    def repage(self):
+        self.cache = self.pages.cache(self.layer)
+
+    def dense_kv(self, b, t_end=None):
+        return self.cache.dense(b, t_end)
+
+    def rows(self, b0, b1):
+        v = object.__new__(PagedState)
+        v.__dict__.update(self.__dict__, cache=self.cache.rows(b0, b1))
+        return v
+
+    def attend(self, q, k, v, tpos, nsplit, ws):
+        """New tokens q, k, v (B,H,N,dh) at positions tpos (B,N) int32, or (N,): stored, then attended with.  With rotary
+        positions q and k are turned (q in place, k in the cache)."""
+        K.kv_store(k, v, self.cache, None, tpos, q=q if self.rope is not None else None, rope=self.rope,
+                   q_out=q if self.rope is not None else None)
+        B, H, N, dh = q.shape
+        out = torch.empty(B, N, H, dh, device=q.device, dtype=q.dtype).transpose(1, 2)
+        return K.dense_attn(q, self.cache, None, tpos, 1.0 / math.sqrt(dh), out=out, nsplit=nsplit, ws=ws)[0]
+
+
 class _Scratch:
     """Per-decoder buffers reused by every layer of a step (fixed addresses, so a step can be captured)."""
 
@@ -317,6 +519,7 @@ class _Scratch:
         self.ws = K.seg_attn_workspace(B, H, 1, dh, nsplit, dev)
         self.mm_ws = None
         self.lg_ws = None
+        self.dense = (1, None)  # a dense decoder's nsplit and workspace (dense_attn)
         self.rowvec = False     # the decoder's choice of ta_rowvec_bf16 for its products (a batch of at most
                                 # ROWVEC_MAX_ROWS sequences, whatever its grouping)
 
@@ -554,7 +757,7 @@ def seg_attend(state, pw, q, k, v, t, update=True):
 
 def weights_from_ours(sd, cfg):
     """Engine weight dict from a model state_dict (engine.py:123-134)."""
-    W = dict(wte=sd['wte.weight'], wpe=sd['wpe.weight'], ln_f=sd['ln_f.weight'], layers=[])
+    W = dict(wte=sd['wte.weight'], wpe=sd.get('wpe.weight'), ln_f=sd['ln_f.weight'], layers=[])
     for i in range(cfg.n_layer):
         p = 'blocks.%d.' % i
         L = dict(ln1=sd[p + 'ln1.weight'], c_attn=sd[p + 'attn.c_attn.weight'], c_proj=sd[p + 'attn.c_proj.weight'],
@@ -616,7 +819,16 @@ class Decoder:
         """paged (default: on, except for the one-launch step, which takes contiguous caches): K and V in pages
         of a PagePool sized for max_tokens positions per sequence (default Tcap); pages are handed out as
         positions are reached, reserve_ahead positions at a time for captured steps.  cache: None (K and V in the model's
-        dtype) or 'e4m3' (8-bit pages, kernels.Cache8; paged caches only)."""
+        dtype) or 'e4m3' (8-bit pages, kernels.Cache8; paged caches only).
+
+        mode 'seg': the segment tree's selection.  mode 'dense': every earlier position -- with paged=True over pages, any batch,
+        captured or not (kernels.dense_attn); without (the default) the reference's comparison baseline, batch 1, contiguous,
+        torch's attention.  cfg.rope (paged, or mode 'seg'): rotary positions, for weights without 'wpe'."""
+        if W.get('wpe') is None:
+            if not getattr(cfg, 'rope', ''):
+                raise ValueError("weights without 'wpe' need rotary positions (cfg.rope)")
+            # no learned positions: a row of zeros for each
+            W = dict(W, wpe=torch.zeros(1, n_embd, device=W['wte'].device, dtype=W['wte'].dtype).expand(Tcap, n_embd))
         self.W, self.nl, self.H, self.C, self.Tcap = W, n_layer, n_head, n_embd, Tcap
         self.dh, self.mode, self.cfg, self.dev = n_embd // n_head, mode, cfg, torch.device(dev)
         self.B = batch
@@ -626,12 +838,13 @@ class Decoder:
         # the fused row-block kernels serve bf16 models whose widths are multiples of 64
         mx4 = [isinstance(L[n], K.Mx4) for L in W['layers'] for n in _PRODUCTS]
         self.mx4 = any(mx4)
-        self.fused = (mode == 'seg' and self.dtype == torch.bfloat16 and n_embd % 64 == 0
+        self.rope = positions.rope_of(cfg, self.dev) if cfg is not None else None
+        self.fused = ((mode == 'seg' or bool(paged)) and self.dtype == torch.bfloat16 and n_embd % 64 == 0
                       and (self.mx4 or (all(L['c_attn'].dtype == torch.bfloat16 for L in W['layers'])
                                         and all(W['layers'][0][n].is_contiguous() for n in _PRODUCTS))))
         if self.mx4 and not (all(mx4) and self.fused):
-            raise ValueError('Mx4 weights: all four matrices of every layer, in a bf16 seg decoder whose width is a '
-                             'multiple of 64')
+            raise ValueError('Mx4 weights: all four matrices of every layer, in a bf16 seg decoder (or a paged dense one) whose '
+                             'width is a multiple of 64')
         if cache not in (None, 'e4m3'):
             raise ValueError("cache: None or 'e4m3'")
         self.cache = cache
@@ -639,17 +852,21 @@ class Decoder:
         # key set (no neighbour borrowing, fixed budget) and one sequence group
         # attn_split: workgroups per query of the per-op decode attention (default: decode_nsplit's choice)
         self.attn_split = attn_split
-        can = (self.fused and self.dh == 64 and batch <= 32 and not groups and not cfg.neighbors
-               and cfg.beam_mode != 'pred' and n_layer <= 64 and not SEL.gate_on(cfg) and not self.mx4)
+        can = (self.fused and mode == 'seg' and self.rope is None and self.dh == 64 and batch <= 32 and not groups
+               and not cfg.neighbors and cfg.beam_mode != 'pred' and n_layer <= 64 and not SEL.gate_on(cfg) and not self.mx4)
         if one_launch and not can:
-            raise ValueError('one_launch: needs a bf16 model with head_dim 64, batch <= 32, neighbours off and a '
-                             'fixed budget')
+            raise ValueError('one_launch: needs a bf16 model with head_dim 64, batch <= 32, neighbours off, a '
+                             'fixed budget and learned positions')
         # off unless asked for: on MI355X the per-op graph is faster at config 4 (1.40 vs 2.32 ms per step)
         self.one_launch = bool(one_launch)
         self.paged = (mode == 'seg' and not self.one_launch) if paged is None else bool(paged)
-        if self.paged and (self.one_launch or mode != 'seg'):
-            raise ValueError('paged caches serve the per-op seg decoder (not the one-launch step or dense mode)')
-        if cache is not None and not (self.paged and self.dh in (16, 32, 64, 128)):
+        if self.paged and (self.one_launch or mode not in ('seg', 'dense')):
+            raise ValueError('paged caches serve the per-op seg decoder and the dense one (not the one-launch step)')
+        if self.paged and mode == 'dense' and self.dh not in (16, 32, 64, 128):
+            raise ValueError('paged dense decoder: head size 16, 32, 64 or 128')
+        if mode == 'dense' and not self.paged and self.rope is not None:
+            raise ValueError('dense mode with rotary positions: paged=True')
+        if cache is not None and not (self.paged and mode == 'seg' and self.dh in (16, 32, 64, 128)):
             raise ValueError('cache %r: paged caches of the seg decoder, head size 16, 32, 64 or 128' % cache)
         self.max_tokens = min(int(max_tokens), Tcap) if max_tokens else Tcap
         self.reserve_ahead = int(reserve_ahead)
@@ -689,6 +906,17 @@ class Decoder:
                     x=torch.empty(n, self.C, device=self.dev, dtype=self.dtype),
                     pos32=torch.empty(n, device=self.dev, dtype=torch.int32)))
                 self.groups[-1]['scratch'].rowvec = B <= ROWVEC_MAX_ROWS
+        elif self.paged:
+            npages = B * H * ((self.max_tokens + DENSE_PAGE - 1) // DENSE_PAGE)
+            self.pool = PagePool(B, H, dh, DENSE_PAGE, self.Tcap, npages, self.nl, self.dtype, self.dev)
+            self.states = [PagedState(self.pool, i, self.rope) for i in range(self.nl)]
+            self.scratch = sc = _Scratch(B, H, dh, 0, self.dev, 1, self.nl)
+            ns = decode_nsplit_dense(B, H, 1, self.max_tokens, dh) if not self.attn_split else 4 * int(self.attn_split)
+            sc.dense = ns, K.dense_attn_workspace(B, H, 1, dh, ns, self.dev, H)
+            sc.rowvec = B <= ROWVEC_MAX_ROWS
+            self.groups = [dict(b0=0, b1=B, states=self.states, scratch=sc, stream=None,
+                                x=torch.empty(B, self.C, device=self.dev, dtype=self.dtype),
+                                pos32=torch.empty(B, device=self.dev, dtype=torch.int32))]
         else:
             self.states = [DenseState(self.Tcap, H, dh, self.dev, B, self.dtype) for _ in range(self.nl)]
         self.graph = None
@@ -708,27 +936,43 @@ class Decoder:
         return self._step
 
     # ------------------------------------------------------------------------------------------ one step
+    def _attend(self, state, L, qkv, tpos32, sc, i):
+        """Layer i's attention of one step: qkv (B, 3C) of the new tokens (its queries, with the seg cache also its keys, are
+        turned in place where positions are rotary) -> (B, H, 1, dh)."""
+        B, H, C, dh = qkv.shape[0], self.H, self.C, self.dh
+        q, k, v = [a.view(B, 1, H, dh).transpose(1, 2) for a in qkv.view(B, 3 * C).split(C, -1)]
+        sc.keys = sc.keys_all[i]
+        if self.mode == 'dense':
+            out = state.attend(q, k, v, tpos32.view(B, 1), *sc.dense)
+            if i == 0:   # the same for every layer
+                sc.keys_all.copy_((tpos32 + 1).view(1, B, 1, 1).expand_as(sc.keys_all))
+            return out
+        if self.rope is not None:
+            qk = qkv.view(B, 3 * C)[:, :2 * C].view(B, 1, 2 * H, dh).transpose(1, 2)
+            K.rope(qk, tpos32.view(B, 1), self.rope, out=qk)
+        out, kr = seg_attend_(state, L.get('pw'), q, k, v, tpos32, scratch=sc)
+        if kr.data_ptr() != sc.keys_all[i].data_ptr():
+            sc.keys_all[i].copy_(kr.view(B, H, 1))
+        return out
+
     def _forward_step(self, tok, tpos):
         """tok (B,) long, tpos (B,) long on the device -> logits (B, V).  Keys attended per (layer, sequence,
         head) are left in self.scratch.keys_all."""
         W, H, C, dh, B = self.W, self.H, self.C, self.dh, self.B
         if self.fused:
             return self._forward_step_fused(tok, tpos)
-        if self.mode == 'seg' and self._rowvec_ok():
+        if (self.mode == 'seg' or self.paged) and self._rowvec_ok():
             return self._forward_step_rowvec(tok, tpos)
         x = (W['wte'][tok] + W['wpe'][tpos]).view(B, 1, C)
         tpos32 = tpos.to(torch.int32)
         for i, L in enumerate(W['layers']):
-            q, k, v = F.linear(_ln(x, L['ln1']), L['c_attn']).split(C, -1)
-            q, k, v = [a.view(B, 1, H, dh).transpose(1, 2) for a in (q, k, v)]
-            if self.mode == 'seg':
-                self.scratch.keys = self.scratch.keys_all[i]
-                out, kr = seg_attend_(self.states[i], L.get('pw'), q, k, v, tpos32, scratch=self.scratch)
-                if kr.data_ptr() != self.scratch.keys_all[i].data_ptr():
-                    self.scratch.keys_all[i].copy_(kr.view(B, H, 1))
+            qkv = F.linear(_ln(x, L['ln1']), L['c_attn'])
+            if self.mode == 'seg' or self.paged:
+                out = self._attend(self.states[i], L, qkv, tpos32, self.scratch, i)
             else:
                 if B != 1:
                     raise NotImplementedError('dense comparison mode is batch 1')
+                q, k, v = [a.view(B, 1, H, dh).transpose(1, 2) for a in qkv.split(C, -1)]
                 out, kr = self.states[i].attend(q, k, v, int(tpos[0]))
                 self.dense_keys = kr
             x = x + F.linear(out.transpose(1, 2).reshape(B, 1, C), L['c_proj'])
@@ -754,11 +998,7 @@ class Decoder:
         K.embed(tok.contiguous(), tpos.contiguous(), W['wte'], W['wpe'], out=x, pos32=tpos32)
         for i, L in enumerate(W['layers']):
             qkv = K.rowvec_f32(x, L['c_attn'], ln_w=L['ln1'])
-            q, k, v = [a.view(B, 1, H, dh).transpose(1, 2) for a in qkv.view(B, 1, 3 * C).split(C, -1)]
-            self.scratch.keys = self.scratch.keys_all[i]
-            out, kr = seg_attend_(self.states[i], L.get('pw'), q, k, v, tpos32, scratch=self.scratch)
-            if kr.data_ptr() != self.scratch.keys_all[i].data_ptr():
-                self.scratch.keys_all[i].copy_(kr.view(B, H, 1))
+            out = self._attend(self.states[i], L, qkv, tpos32, self.scratch, i)
             K.rowvec_f32(out.transpose(1, 2).reshape(B, C), L['c_proj'], epilogue='residual', residual=x, out=x)
             h = K.rowvec_f32(x, L['c_fc'], ln_w=L['ln2'], epilogue='gelu')
             K.rowvec_f32(h, L['c_mlp'], epilogue='residual', residual=x, out=x)
@@ -781,12 +1021,8 @@ class Decoder:
         tpos32 = grp['pos32']
         for i, L in enumerate(W['layers']):
             qkv = sc.mm(x, L['c_attn'], ln_w=L['ln1'])
-            q, k, v = [a.view(B, 1, H, dh).transpose(1, 2) for a in qkv.split(C, -1)]
-            sc.keys = sc.keys_all[i]
-            out, kr = seg_attend_(grp['states'][i], L.get('pw'), q, k, v, tpos32, scratch=sc)
-            if kr.data_ptr() != sc.keys_all[i].data_ptr():
-                sc.keys_all[i].copy_(kr.view(B, H, 1))
-            sc.mm(out.view(B, C), L['c_proj'], epilogue='residual', residual=x, out=x)
+            out = self._attend(grp['states'][i], L, qkv, tpos32, sc, i)
+            sc.mm(out.transpose(1, 2).reshape(B, C), L['c_proj'], epilogue='residual', residual=x, out=x)
             hmid = sc.mm(x, L['c_fc'], ln_w=L['ln2'], epilogue='gelu')
             sc.mm(hmid, L['c_mlp'], epilogue='residual', residual=x, out=x)
         sc.logits(x, W['wte'], W['ln_f'], logits, tok_out)
@@ -817,7 +1053,7 @@ class Decoder:
 
     def keys_read(self):
         """Mean keys attended per head and layer of the last step, per sequence (B,) float32."""
-        if self.mode != 'seg':
+        if self.mode != 'seg' and not self.paged:
             return torch.full((self.B,), float(self.dense_keys), device=self.dev)
         if self.fused:
             return torch.cat([g['scratch'].keys_all.mean(dim=(0, 2, 3)) for g in self.groups])
@@ -833,19 +1069,61 @@ class Decoder:
         tp = (t.to(self.dev).long().contiguous() if torch.is_tensor(t) else
               torch.full((self.B,), int(t), device=self.dev, dtype=torch.long))
         if self.pool is not None:
-            self.reserve(int(t.max()) + 1 if torch.is_tensor(t) else int(t) + 1)
+            at = t.reshape(-1).tolist() if torch.is_tensor(t) else [int(t)] * self.B
+            self.reserve(max(at) + 1, at)
         logits = self._forward_step(tk, tp)
         keys = self.keys_read()
         if scalar and self.B == 1:
             return logits[0], float(keys[0])
         return logits, keys
 
-    def reserve(self, t_end):
-        """Pages for positions < t_end of every sequence (paged caches; host side, not inside a captured step)."""
+    def reserve(self, t_end, start=None):
+        """Pages for positions < t_end of every sequence (paged caches; host side, not inside a captured step).  start: the
+        position that each sequence goes on from (its pages from there on are its own then); None: behind all it holds."""
         if self.pool is not None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('Decoder.reserve: pages are handed out outside graph capture')
-            self.pool.ensure(t_end)
+            self.pool.ensure(t_end, start=start)
+
+    # ------------------------------------------------------------------------------------------ sequences
+    @torch.no_grad()
+    def fork(self, src, dst, t):
+        """Sequence dst goes on from the first t positions of src (at most those that src holds), as after the same tokens: whole
+        pages of the caches are shared (read only; a step that goes back into one gets a copy), the rows behind them and the
+        tree's state copied.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] and g_t[dst] too.
+        With the budget head's global pool the running sum of keys is that of the cache's rows."""
+        t = int(t)
+        if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
+            raise ValueError('Decoder.fork: two different sequences of %d' % self.B)
+        if not 0 <= t <= self.Tcap:
+            raise ValueError('Decoder.fork: at most %d positions' % self.Tcap)
+        if self.mode != 'seg' and not self.paged:
+            raise NotImplementedError('dense comparison mode is batch 1')
+        if self.pool is not None:
+            self.pool.fork(src, dst, t)
+            if self.graph is not None and self._t_host is not None:
+                self.pool.ensure(self._reserved)
+        ids = torch.tensor([[src], [dst]], dtype=torch.int32).to(self.dev)
+        K.copy_rows([x for st in self.states for x in st.sequence_tensors()], ids[0], ids[1])
+        for st in self.states:
+            c8 = getattr(st, 'cache8', None)
+            if c8 is not None:   # the tail goes along where it holds the block that t lies in
+                blk, part = divmod(t, c8.leaf)
+                held = c8.tail_block[dst]
+                held.copy_(torch.where(held == blk, held, -1) if part else torch.full_like(held, -1))
+            if self.mode == 'seg' and self.cfg.beam_mode == 'pred' and self.cfg.global_pool:
+                st.ksum[dst] = st.dense_kv(dst, t)[0][0].float().sum(1) if t else 0.0
+
+    def resize(self, num_pages):
+        """Page pools of num_pages pages for the caches (PagePool.resize).  A captured step is captured again after it."""
+        if self.pool is None:
+            raise ValueError('Decoder.resize: paged caches')
+        self.pool.resize(num_pages)
+        for st in self.states:
+            st.repage()
+        for grp in self.groups:
+            grp['states'] = [st.rows(grp['b0'], grp['b1']) for st in self.states]
+        self.graph = None
 
     # ------------------------------------------------------------------------------------------ prefill
     @torch.no_grad()
@@ -854,8 +1132,8 @@ class Decoder:
         weights): the products' rows are rounded to 4 bits too.
         Selection and attention are those of the forward pass (fastseg.py:345-405 semantics over the cache's
         tree).  Returns the last position's logits (B, V)."""
-        if self.mode != 'seg':
-            raise NotImplementedError('prefill is for the seg cache')
+        if self.mode != 'seg' and not self.paged:
+            raise NotImplementedError('prefill is for the seg cache and the paged dense one')
         W, H, C, dh = self.W, self.H, self.C, self.dh
         B, T0 = idx.shape
         if B != self.B or T0 > self.Tcap:
@@ -866,9 +1144,9 @@ class Decoder:
         chunk = chunk or B
         tq = torch.arange(T0, device=self.dev, dtype=torch.int32)
         if self.pool is not None:
-            self.reserve(T0)
+            self.reserve(T0, [0] * B)
         scale = 1.0 / math.sqrt(dh)
-        n_tree_val = SEL.fixed_n_tree(cfg)
+        n_tree_val = SEL.fixed_n_tree(cfg) if self.mode == 'seg' else None
         last = []
         for b0 in range(0, B, chunk):
             b1 = min(B, b0 + chunk)
@@ -878,6 +1156,15 @@ class Decoder:
                 st = self.states[i]
                 qkv = _product(x, L['c_attn'], L['ln1'], bits)
                 q, k, v = [a.view(nb, T0, H, dh).transpose(1, 2) for a in qkv.split(C, -1)]
+                if self.mode == 'dense':
+                    ns = decode_nsplit_dense(nb, H, T0, T0, dh)
+                    out = st.rows(b0, b1).attend(q, k, v, tq, ns, None).transpose(1, 2)
+                    x = _product(out.reshape(nb, T0, C), L['c_proj'], bits=bits, residual=x)
+                    x = _product(_product(x, L['c_fc'], L['ln2'], bits, gelu=True), L['c_mlp'], bits=bits, residual=x)
+                    continue
+                if self.rope is not None:
+                    qk = qkv[..., :2 * C].view(nb, T0, 2 * H, dh).transpose(1, 2)
+                    K.rope(qk, tq, self.rope, out=qk)
                 st.write_rows(b0, k, v)
                 lv = [t[b0:b1] for t in st.levels]
                 K.level_sums(k, st.shape.blevels, out=lv, t_end=T0, zero_sink=True)
@@ -944,7 +1231,7 @@ class Decoder:
         # the replays' positions, followed on the host so pages can be handed out ahead of them without a sync
         self._t_host = int(self.g_t.max()) if torch.is_tensor(t) else int(t)
         self._reserved = self._t_host + 1 + self.reserve_ahead
-        self.reserve(self._reserved)
+        self.reserve(self._reserved, self.g_t.tolist() if self.pool is not None and self.pool.n_shared else None)
         self.g_logits = torch.empty(B, V, device=self.dev, dtype=torch.bfloat16 if self.fused else torch.float32)
         main = torch.cuda.current_stream()
         groups = self.groups if (self.fused and len(self.groups) > 1) else [None]
@@ -998,6 +1285,8 @@ class Decoder:
         are ordered by its stream; torch.cuda.synchronize() waits for all of them.  With paged caches the pages
         of the next reserve_ahead positions are handed out (outside the graph) whenever the replays reach the
         end of the reserved range."""
+        if self.graph is None:
+            raise RuntimeError('Decoder.replay: no captured step (capture; again after reset and resize)')
         if self.pool is not None and self._t_host is not None:
             if self._t_host + 1 >= self._reserved:
                 self._reserved = self._t_host + 1 + self.reserve_ahead

@@ -14,6 +14,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import kernels as K
+from . import positions
 from . import selection as SEL
 
 FAST = [True]  # the reference's switch to its PyTorch fallbacks; there are none here, so False raises
@@ -168,8 +169,7 @@ class SegAttention(nn.Module):
 
     def forward(self, x):
         b, T, C = x.shape
-        q, k, v = self.c_attn(x).split(C, dim=2)
-        q, k, v = [t.view(b, T, self.H, self.dh).transpose(1, 2) for t in (q, k, v)]
+        q, k, v = positions.heads(self, self.c_attn(x))
         out = self.sparse_attend(q, k, v)
         return self.c_proj(out.transpose(1, 2).reshape(b, T, C))
 

@@ -63,13 +63,15 @@ def _f(x):
 
 
 class GPT(nn.Module):
-    """Learned positions, tied output layer, pre-LN blocks (model.py:51-93)."""
+    """Learned positions, tied output layer, pre-LN blocks (model.py:51-93).  With cfg.rope the positions are rotary: there is
+    no wpe, and any length that the attention takes."""
 
     def __init__(self, cfg):
         super().__init__()
         self.cfg = cfg
         self.wte = nn.Embedding(cfg.vocab_size, cfg.n_embd)
-        self.wpe = nn.Embedding(cfg.seq_len, cfg.n_embd)
+        if not getattr(cfg, 'rope', ''):
+            self.wpe = nn.Embedding(cfg.seq_len, cfg.n_embd)
         self.blocks = nn.ModuleList([Block(cfg) for _ in range(cfg.n_layer)])
         self.ln_f = LayerNorm(cfg.n_embd)
         self.lm_head = nn.Linear(cfg.n_embd, cfg.vocab_size, bias=False)
@@ -88,7 +90,9 @@ class GPT(nn.Module):
 
     def forward(self, idx, targets=None):
         b, T = idx.shape
-        x = self.wte(idx) + self.wpe(torch.arange(T, device=idx.device))
+        x = self.wte(idx)
+        if not getattr(self.cfg, 'rope', ''):
+            x = x + self.wpe(torch.arange(T, device=idx.device))
         acc = {}
         for blk in self.blocks:
             x = blk(x)

@@ -2,7 +2,8 @@
 
 A Rope (kernels.Rope) holds the angle of each pair of a head's elements for one position; rotate() turns queries and keys by
 their positions' angles, differentiably.  rope_frequencies() gives the angles, also those of a model stretched past the
-length it was trained at.
+length it was trained at.  Models with Config.rope have them in place of learned positions: the attention modules turn what
+their projection gives (heads), the decoder what it stores and asks with.
 """
 import math
 
@@ -52,7 +53,10 @@ class _Rotate(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _Rotate.apply(dy, ctx.saved_tensors[0], ctx.rope, not ctx.inverse), None, None, None
+        pos, = ctx.saved_tensors
+        if torch.is_grad_enabled():     # a gradient that is to be differentiated itself
+            return _Rotate.apply(dy, pos, ctx.rope, not ctx.inverse), None, None, None
+        return K.rope(dy if dy.stride(-1) == 1 else dy.contiguous(), pos, ctx.rope, inverse=not ctx.inverse), None, None, None
 
 
 def rotate(x, pos, rope):
@@ -60,3 +64,31 @@ def rotate(x, pos, rope):
     if torch.is_grad_enabled() and x.requires_grad:
         return _Rotate.apply(x, pos, rope, False)
     return K.rope(x if x.stride(-1) == 1 else x.contiguous(), pos, rope)
+
+
+def rope_of(cfg, device):
+    """The Rope of a model configuration on `device`, None when its positions are learned."""
+    if not getattr(cfg, 'rope', ''):
+        return None
+    dh = cfg.n_embd // cfg.n_head
+    rot = cfg.rope_dim or dh
+    if rot > dh:
+        raise ValueError('rope_dim %d: heads have %d elements' % (rot, dh))
+    freq, amplitude = rope_frequencies(rot, cfg.rope_base, cfg.rope_scaling, cfg.rope_factor, cfg.rope_trained or cfg.seq_len)
+    return K.Rope(freq, device, layout=cfg.rope, amplitude=amplitude)
+
+
+def heads(module, qkv):
+    """The projection qkv (b,T,3C) of an attention module as its queries, keys and values (b,H,T,dh), queries and keys turned
+    by their positions where the module's configuration has rotary positions (one call for both; differentiable)."""
+    b, T, C3 = qkv.shape
+    C, H = C3 // 3, module.H
+    if not getattr(module.cfg, 'rope', ''):
+        return [t.view(b, T, H, C // H).transpose(1, 2) for t in qkv.split(C, dim=2)]
+    r = module.__dict__.get('_rope')
+    if r is None or r.turns.device != qkv.device:
+        r = module.__dict__['_rope'] = rope_of(module.cfg, qkv.device)
+    qk, v = qkv.split((2 * C, C), dim=2)
+    pos = torch.arange(T, device=qkv.device, dtype=torch.int32)
+    qk = rotate(qk.view(b, T, 2 * H, C // H).transpose(1, 2), pos, r)
+    return [qk[:, :H], qk[:, H:], v.view(b, T, H, C // H).transpose(1, 2)]
