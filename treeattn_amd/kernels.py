@@ -1350,19 +1350,31 @@ def copy_rows(tensors, src, dst, out=None):
     if (src.dtype != torch.int32 or dst.dtype != torch.int32 or src.dim() != 1 or dst.shape != src.shape
             or not src.is_contiguous() or not dst.is_contiguous()):
         raise ValueError('copy_rows: src and dst (n,) int32, contiguous')
-    size, fr, tr = [], [], []
+    size, at, fr, to, tr = [], [], [], [], []
     for x, y in zip(tensors, out):
-        if (x.dtype != y.dtype or x.dim() < 1 or x.shape[1:] != y.shape[1:] or not x.is_contiguous()
-                or not y.is_contiguous()):
-            raise ValueError('copy_rows: contiguous tensors, each with the dtype and row shape of its target')
-        size.append(x.element_size() * math.prod(x.shape[1:]))
-        fr.append(x.shape[0])
+        sh = x.shape
+        if not sh or not x.is_contiguous():
+            raise ValueError('copy_rows: contiguous tensors with a row dimension')
+        n = sh[0]
+        size.append(x.nbytes // n if n else x.element_size() * math.prod(sh[1:]))
+        at.append(x.data_ptr())
+        fr.append(n)
+        if x.get_device() != dev:
+            _on('copy_rows', dev, x)
+        if y is x:
+            to.append(at[-1])
+            tr.append(n)
+            continue
+        if x.dtype != y.dtype or not y.dim() or sh[1:] != y.shape[1:] or not y.is_contiguous():
+            raise ValueError('copy_rows: a contiguous target of the dtype and row shape of each tensor')
+        if y.get_device() != dev:
+            _on('copy_rows', dev, y)
+        to.append(y.data_ptr())
         tr.append(y.shape[0])
-    _on('copy_rows', dev, dst, *tensors, *out)
+    _on('copy_rows', dev, dst)
     n = len(size)
     pack = struct.Struct('%dq' % n).pack
-    _copy_rows(dev, n, pack(*[x.data_ptr() for x in tensors]), pack(*[y.data_ptr() for y in out]), pack(*size), pack(*fr),
-               pack(*tr), src.data_ptr(), dst.data_ptr(), src.shape[0])
+    _copy_rows(dev, n, pack(*at), pack(*to), pack(*size), pack(*fr), pack(*tr), src.data_ptr(), dst.data_ptr(), src.shape[0])
 
 
 # ----------------------------------------------------------------------------------------------- 4-bit rows
