@@ -164,8 +164,15 @@ __device__ __forceinline__ int min_dpp(int x) {
 }
 __device__ __forceinline__ int min16(int x) { return min_dpp<0x140>(min_dpp<0x141>(min_dpp<0x4E>(min_dpp<0xB1>(x)))); }
 
+// A load that the caches need not keep (STREAM), or an ordinary one.
+template <bool STREAM, typename V>
+__device__ __forceinline__ V once(const TA_GLOBAL V* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // One wavefront's share: keys [k0, k1) for NT tiles of 16 query rows of one (sequence, key head).
-template <typename T, int D, bool WIDE, int NT>
+template <typename T, int D, bool WIDE, int NT, bool STREAM>
 struct Share {
   using C = Tile<T, D>;
   const Dense& p;
@@ -240,27 +247,27 @@ struct Share {
     __builtin_amdgcn_sched_barrier(0);
     auto load_k = [&](int i, int s2, const TA_GLOBAL char* row) {
       const int o = 64 * s2 + 16 * (lane & 3);
-      const u32x4_t r = *(const TA_GLOBAL u32x4_t*)(row + (uint32_t)(o < D * C::EB ? o : 0));
+      const u32x4_t r = once<STREAM>((const TA_GLOBAL u32x4_t*)(row + (uint32_t)(o < D * C::EB ? o : 0)));
       x.k[i][s2] = make_uint4(r.x, r.y, r.z, r.w);
     };
     auto load_v = [&](int e, const TA_GLOBAL char* at) {
       if constexpr (C::VB >= 16) {
 #pragma unroll
         for (int w = 0; w < C::VW; w += 4) {
-          const u32x4_t r = *(const TA_GLOBAL u32x4_t*)(at + 4 * w);
+          const u32x4_t r = once<STREAM>((const TA_GLOBAL u32x4_t*)(at + 4 * w));
           x.v[e][w] = r.x;
           x.v[e][w + 1] = r.y;
           x.v[e][w + 2] = r.z;
           x.v[e][w + 3] = r.w;
         }
       } else if constexpr (C::VB == 8) {
-        const u32x2 r = *(const TA_GLOBAL u32x2*)at;
+        const u32x2 r = once<STREAM>((const TA_GLOBAL u32x2*)at);
         x.v[e][0] = r.x;
         x.v[e][1] = r.y;
       } else if constexpr (C::VB == 4) {
-        x.v[e][0] = *(const TA_GLOBAL uint32_t*)at;
+        x.v[e][0] = once<STREAM>((const TA_GLOBAL uint32_t*)at);
       } else {
-        x.v[e][0] = *(const TA_GLOBAL uint16_t*)at;
+        x.v[e][0] = once<STREAM>((const TA_GLOBAL uint16_t*)at);
       }
     };
     if constexpr (WIDE) {
@@ -593,7 +600,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   const int bh = (int)(id / per), row0 = (int)(id % per) * kRows * NT;
   const int b = bh / p.H, h = bh % p.H;
   __shared__ __align__(16) char stage[kWaves * Tile<T, D>::LSTEP];
-  Share<T, D, WIDE, NT> s(p, b, h, row0, stage + wave_id() * Tile<T, D>::LSTEP);
+  Share<T, D, WIDE, NT, false> s(p, b, h, row0, stage + wave_id() * Tile<T, D>::LSTEP);
   const int left = p.R - row0;
   s.run(row0, b, h, 0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1,
         [&](uint32_t done) {
@@ -742,7 +749,7 @@ __device__ __forceinline__ int prefix64(int x) {   // sum of lanes 0 .. lane
 // Workgroups of four wavefronts, each with a share of one set of 16 NT rows.  A set gets as many as its sequence is long (each
 // takes at most 1 / nwg of all units of all sets): sequences of any lengths end together, and few long ones fill the GPU.  The
 // grid has a workgroup for each of the nwg and each set, which is as many as there can be; those left over leave at once.
-template <typename T, int D, bool WIDE, int NT>
+template <typename T, int D, bool WIDE, int NT, bool STREAM>
 __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg) {
   extern __shared__ __align__(16) float smem[];
   constexpr int KEYS = Tile<T, D>::KEYS;
@@ -802,7 +809,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   const int part = wg - start - in * count;
   const int h = sets > 1 ? in / sets : in, row0 = sets > 1 ? (in - h * sets) * kSet : 0;
   const int rows = p.R - row0 < kSet ? p.R - row0 : kSet;
-  Share<T, D, WIDE, NT> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, last);
+  Share<T, D, WIDE, NT, STREAM> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, last);
   // its keys, and the equal runs of whole steps of its wavefronts
   const int nkeys = s.tmax + 1;
   const int mine = (int)((unsigned)ub / (unsigned)count), more = ub - mine * count;
@@ -867,6 +874,12 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   if (count > 1) join_parts<T, D, kSet>(p, b, h, row0, rows, b * per + in, wg - part, count, smem);
 }
 
+// Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level cache
+// (256 MiB) is not there any more at the next call, and its reads get in each other's way.  Of 32 x 12 queries over 32768 keys of
+// 64 (2.8 GB) 489 us with ordinary loads and 439 with these, one stream of 131000 (352 MB) 71.7 and 64.9; three caches of 86 MB
+// in turns 23.8 and 25.3.  Only where one set reads a key: several share them in the second cache.
+constexpr int64_t kOnce = (int64_t)256 << 20;
+
 template <typename T, int D, bool WIDE, int NT>
 int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const dim3 blk(kWaves * kWave);
@@ -881,8 +894,14 @@ int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const int nwg = nsplit / kWaves;
   const int64_t wgs = nwg == 1 ? sets : nwg + sets;
   const dim3 grid((unsigned)(per > 1 ? (wgs + 7) / 8 * 8 : wgs));
-  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT>), grid, blk, stage + (parts > join ? parts : join) * sizeof(float),
-                     st, p, nwg);
+  const size_t lds = stage + (parts > join ? parts : join) * sizeof(float);
+  if constexpr (NT == 1) {
+    if (per == 1 && (int64_t)p.BH * p.Tk * 2 * D * (int64_t)sizeof(T) >= kOnce) {
+      hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, 1, true>), grid, blk, lds, st, p, nwg);
+      return check_launch("dense_split_kernel");
+    }
+  }
+  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT, false>), grid, blk, lds, st, p, nwg);
   return check_launch("dense_split_kernel");
 }
 

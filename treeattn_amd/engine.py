@@ -591,10 +591,11 @@ def decode_nsplit_dense(B, H, rows, keys, D=64):
     A set of rows gets a whole number of workgroups, so those in use are up to one a set more than that; all at once on the 256
     compute units they should be: 12 queries over 131000 keys of 64 take 66 us with 244 and 74 with 256 (264 in use), 32 sets of
     4 x 128 over 6001 keys 23.2 and 25.4.  From 192 sets on, two workgroups a compute unit (384 sets over 32768 keys 491 us with
-    512, 516 with 256), and from 4096 a wavefront a set."""
+    512, 516 with 256), and from 4096 a wavefront a set; of 32 rows, as prompts have, from 1024 (16 heads of 128 x 4096 tokens
+    275 us so, 379 with a workgroup a set; 12 heads of 64 x 1024 tokens, 384 sets, 31 and 23)."""
     sets = max(1, B * H * ((rows + 31) // 32 if rows > 16 else 1))
     units = (max(1, keys) + 127) // 128
-    if sets >= 4096:
+    if sets >= (1024 if rows > 16 else 4096):
         return 1
     if units == 1:
         return 4
