@@ -164,6 +164,31 @@ def test_what_is_masked_has_no_effect(dtype, nsplit):
                 (~torch.isfinite(seen[:, 5])).all())
 
 
+@pytest.mark.parametrize('N', [1, 3, 70])
+@pytest.mark.parametrize('nsplit', [4, 64, 1024])
+def test_many_ragged_sequences(N, nsplit):
+    """More sequences than a wavefront has lanes, from no token to many, tokens at positions outside the cache among the others
+    (the padding of a batch): zeros there, and no effect on their neighbours."""
+    B, H, D, T = 131, 2, 32, 700
+    g = torch.Generator().manual_seed(N)
+    lens = torch.randint(1, T + 1, (B,), generator=g) // torch.randint(1, 9, (B,), generator=g)
+    k, v = rnd(B, H, T, D, seed=111, dtype=BF16), rnd(B, H, T, D, seed=112, dtype=BF16)
+    q = rnd(B, 2 * H, N, D, seed=113, dtype=BF16)
+    tq = rows(lens.tolist(), N)
+    if N > 1:
+        tq[3, 1], tq[70, 0], tq[130, N - 1], tq[64] = -1, T, 1 << 30, -7
+    c = paged(k, v, 16, fill=float('nan'))
+    out = K.dense_attn(q.to(DEV), c, None, tq.to(DEV), 0.2, nsplit=nsplit)[0]
+    some = sorted({0, 3, 63, 64, 65, 70, 127, 128, 130} | set(range(0, B, 40)))[::1 if N < 70 else 4]
+    want, _, tol = want64(q[some], k[some], v[some], tq[some], 0.2)
+    close(out[some], want, tol, BF16)
+    one = K.dense_attn(q[64:66].to(DEV), c.rows(64, 66), None, tq[64:66].to(DEV), 0.2, nsplit=1)[0]
+    want, _, tol = want64(q[64:66], k[64:66], v[64:66], tq[64:66], 0.2)
+    close(one, want, tol, BF16)
+    wide = torch.full((B, N), 2 ** 32 + 3, dtype=torch.int64)              # past 32 bits: outside, not position 3
+    assert not K.dense_attn(q.to(DEV), c, None, wide.to(DEV), 0.2, nsplit=nsplit)[0].any()
+
+
 def test_no_keys_at_all():
     """A sequence without pages, and a cache whose blocks have none: zeros and lse -1e30."""
     q = rnd(2, 2, 3, 64, seed=31, dtype=BF16).to(DEV)
@@ -313,7 +338,10 @@ def test_refusals():
                 lambda: K.dense_attn(q, k, k, tq.cpu()), lambda: K.dense_attn(q.cpu(), k, k, tq)):
         with pytest.raises((ValueError, RuntimeError)):
             bad()
-    for bad in (lambda: K.dense_attn(q.float(), k, k, tq), lambda: K.dense_attn(q, k, k, tq.float())):
+    with pytest.raises(ValueError, match='repeats'):
+        K.dense_attn(q, k, k, tq, out=torch.empty(1, 4, 1, 64, device=DEV, dtype=BF16).expand(2, 4, 1, 64))
+    for bad in (lambda: K.dense_attn(q.float(), k, k, tq), lambda: K.dense_attn(q, k, k, tq.float()),
+                lambda: K.dense_attn(q, object(), None, tq)):
         with pytest.raises(TypeError):
             bad()
     for nsplit in (0, 2, 6, 8196, -4):

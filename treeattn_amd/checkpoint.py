@@ -46,11 +46,11 @@ def load_model(path, device='cuda', dtype=None):
     return model.eval(), cfg
 
 
-def load_decoder(path, Tcap=None, device='cuda', dtype=None, **kw):
-    """A seg Decoder over the checkpoint's weights (phase2.py:30: weights_from_ours(ck['model'], cfg)); Tcap
+def load_decoder(path, Tcap=None, device='cuda', dtype=None, mode='seg', **kw):
+    """A Decoder (mode 'seg' or 'dense') over the checkpoint's weights (phase2.py:30: weights_from_ours(ck['model'], cfg)); Tcap
     defaults to the model's seq_len.  Extra keywords go to Decoder (batch, max_tokens, ...)."""
     sd, cfg = read_checkpoint(path)
     sd = {k: (v.to(device=device, dtype=dtype) if dtype is not None and v.is_floating_point() else v.to(device))
           for k, v in sd.items()}
     W = weights_from_ours(sd, cfg)
-    return Decoder(W, cfg.n_layer, cfg.n_head, cfg.n_embd, Tcap or cfg.seq_len, 'seg', cfg, device, **kw), cfg
+    return Decoder(W, cfg.n_layer, cfg.n_head, cfg.n_embd, Tcap or cfg.seq_len, mode, cfg, device, **kw), cfg

@@ -180,7 +180,8 @@ struct Share {
   const TA_GLOBAL T* kb;
   const TA_GLOBAL T* vb;
   const int32_t* tab;
-  int t[NT];            // the lane's row's position (pad rows: as far as any)
+  int t[NT];            // the lane's row's position; of rows that are not there or see nothing: behind every key
+  uint32_t none;        // rows (bit 16 i + c) whose position is outside the cache: zeros
   int tmin, tmax;       // of the wavefront's rows
   int seen;             // values past this position count as zeros
   uint4 q[NT][C::KS];
@@ -195,6 +196,7 @@ struct Share {
     vb = (const TA_GLOBAL T*)p.v + (p.ptab ? 0 : b * p.vsb + h * p.vsh);
     tab = p.ptab ? p.ptab + b * p.pt_sb + h * p.pt_sh : nullptr;
     int lo = 0x7fffffff, hi = -1;
+    none = 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int r = row0 + kRows * i + c;
@@ -204,11 +206,14 @@ struct Share {
       int tt = 0x7fffffff;
       if (in) {
         tt = one ? last : p.tq[b * p.tq_sb + n];   // (one token: its position, checked, is known)
-        if (tt < 0 || tt >= p.Tk) tt = -1;
       }
+      // (masks would be needed for such a row's sake in every step: it goes along with the others instead)
+      const bool out = in && (tt < 0 || tt >= p.Tk);
+      none |= (uint32_t)(__ballot(out) & 0xffff) << (kRows * i);
+      if (out) tt = 0x7fffffff;
       t[i] = tt;
       lo = tt < lo ? tt : lo;
-      hi = in && tt > hi ? tt : hi;
+      hi = tt != 0x7fffffff && tt > hi ? tt : hi;
       const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + j) * p.qsh + n * p.qsn;
 #pragma unroll
       for (int s = 0; s < C::KS; ++s) {
@@ -497,7 +502,7 @@ struct Share {
 #pragma unroll 1
       for (int d = 0; d < D / 4; ++d) s = fmaf(to_f32(qr[d]), number(kr + d), s);
       s = sum_rows(s) * (p.scale * kLog2e);
-      if (key > t[i] || r >= p.R) continue;
+      if (key > t[i] || r >= p.R) continue;   // (rows that see nothing are not taken from here)
       const float mn = fmaxf(m[i], s - C::kShift);
       const float alpha = __builtin_amdgcn_exp2f(m[i] - mn), w = __builtin_amdgcn_exp2f(s - mn);
       m[i] = mn;
@@ -554,7 +559,7 @@ struct Share {
     int only = -1;
     while (true) {
       if (k0 < k1) pass(k0, k1);
-      uint32_t bad = unsound() & want, done = want & ~bad;
+      uint32_t bad = unsound() & want & ~none, done = want & ~bad;
       if (only >= 0) {
         if (bad >> only & 1) {
 #pragma unroll
@@ -564,7 +569,15 @@ struct Share {
         done = 1u << only;
       }
 #pragma unroll
-      for (int i = 0; i < NT; ++i) l[i] = sum_rows(l[i]);
+      for (int i = 0; i < NT; ++i) {
+        l[i] = sum_rows(l[i]);
+        if (none >> (kRows * i + c) & 1) {
+          m[i] = kLowest;
+          l[i] = 0.0f;
+#pragma unroll
+          for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+      }
       emit(done);
       want &= ~done;
       if (want == 0) return;
@@ -714,12 +727,17 @@ constexpr int kQuantum = 128;        // keys of one unit of work
 __device__ __forceinline__ int units_of(const Dense& p, int b0, int& n) {
   const int lane = lane_id();
   n = -1;
-  if (p.Nq <= 4) {
-    if (b0 + lane < p.B)
-      for (int i = 0; i < p.Nq; ++i) {
-        const int t = p.tq[(b0 + lane) * p.tq_sb + i];
-        n = t < p.Tk && t > n ? t : n;
+  if (p.Nq <= 64) {
+    if (b0 + lane < p.B) {
+      const int32_t* row = p.tq + (b0 + lane) * p.tq_sb;
+      for (int i0 = 0; i0 < p.Nq; i0 += 8) {   // eight loads at a time
+        int t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = row[i0 + i < p.Nq ? i0 + i : 0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n = t[i] < p.Tk && t[i] > n ? t[i] : n;
       }
+    }
   } else {
     for (int k = 0; k < kWave && b0 + k < p.B; ++k) {
       int m = -1;

@@ -1124,7 +1124,7 @@ class Decoder:
             st.repage()
         for grp in self.groups:
             grp['states'] = [st.rows(grp['b0'], grp['b1']) for st in self.states]
-        self.graph = None
+        self.graph, self.graphs = None, []
 
     # ------------------------------------------------------------------------------------------ prefill
     @torch.no_grad()

@@ -939,7 +939,8 @@ class Cache8:
     (b, h) to its page (-1: none) and may be shared by several layers.  The block being filled stands unrounded in
     tail (B, H, 2, leaf, D), in the model's type, and tail_block (B, H) int32 says which it is (-1: none); it is
     rounded into its page when its last row arrives.  tcap: positions per sequence.  The tensors are the caller's and
-    change in place (another table or pool is another Cache8); a page belongs to one block of one sequence and head.  A
+    change in place (another table or pool is another Cache8); a page that is written belongs to one block of one sequence
+    and head (whole blocks before the one being filled may be shared).  A
     new cache is pool of zeros, scale of ones, tail_block of -1."""
 
     pool, scale, table, tail, tail_block = (property(lambda self, i=i: self._tensors[i]) for i in range(5))
@@ -1164,7 +1165,9 @@ _copy_rows = L.entry('ta_copy_rows')
 def _positions(name, pos, B, N):
     """pos as int32 (N,) or (B, N) contiguous, and its sequence stride."""
     if pos.dtype != torch.int32 or not pos.is_contiguous():
-        if pos.dtype not in (torch.int32, torch.int64):
+        if pos.dtype == torch.int64:    # (what 32 bits do not hold stays outside every cache)
+            pos = pos.clamp(-2 ** 31, 2 ** 31 - 1)
+        elif pos.dtype != torch.int32:
             raise TypeError('%s: positions int32 (or int64)' % name)
         pos = pos.to(torch.int32).contiguous()
     if pos.shape == (B, N):
@@ -1200,6 +1203,8 @@ def dense_attn(q, k, v, tq, scale=None, out=None, lse=None, nsplit=1, ws=None):
         Bk, H, Dk, Tk, dt = k.B, k.H, k.D, k.tcap, k.dtype
         kt = vt = (0, 0, D)
         ka, va, pages = k.k, k.v, ctypes.byref(k.desc)
+    elif not isinstance(k, torch.Tensor):
+        raise TypeError('dense_attn: contiguous caches or a PagedCache')
     else:
         Bk, H, Tk, Dk = k.shape
         if v.shape != k.shape or v.dtype != k.dtype or k.stride(3) != 1 or v.stride(3) != 1:
@@ -1214,6 +1219,8 @@ def dense_attn(q, k, v, tq, scale=None, out=None, lse=None, nsplit=1, ws=None):
         out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dt or out.stride(3) != 1:
         raise ValueError('dense_attn: out must have the shape and dtype of q, the last dimension contiguous')
+    else:
+        _own_rows('dense_attn', q, out)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq, Nq) or not lse.is_contiguous()):
         raise ValueError('dense_attn: lse (B, Hq, Nq) float32, contiguous')
     tq, tq_sb = _positions('dense_attn', tq, B, Nq)
