@@ -764,11 +764,47 @@ __device__ __forceinline__ int prefix64(int x) {   // sum of lanes 0 .. lane
   return x + (row == 0 ? 0 : row == 1 ? a : row == 2 ? a + b : a + b + c);
 }
 
-// Workgroups of four wavefronts, each with a share of one set of 16 NT rows.  A set gets as many as its sequence is long (each
-// takes at most 1 / nwg of all units of all sets): sequences of any lengths end together, and few long ones fill the GPU.  The
-// grid has a workgroup for each of the nwg and each set, which is as many as there can be; those left over leave at once.
+// The sum of x over the wavefront, and its largest.
+__device__ __forceinline__ int sum64i(int x) { return __builtin_amdgcn_readlane(prefix64(x), kWave - 1); }
+__device__ __forceinline__ int max64i(int x) {
+  x = -min16(-x);
+  return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+             max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)((unsigned)(a + b - 1) / (unsigned)b); }
+
+// The units of every sequence, as each workgroup finds them: those of the first 64 in a lane each, of the others read again.
+struct Units {
+  const Dense& p;
+  int u0, n0;           // units and last position of sequence `lane`
+  __device__ __forceinline__ Units(const Dense& p_) : p(p_) { u0 = units_of(p, 0, n0); }
+  // f(first sequence, units, last positions) over groups of 64 sequences, until it gives false
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if (!f(0, u0, n0)) return;
+    for (int b0 = kWave; b0 < p.B; b0 += kWave) {
+      int n;
+      const int u = units_of(p, b0, n);
+      if (!f(b0, u, n)) return;
+    }
+  }
+  // workgroups of one set of every sequence, at `most` units each
+  __device__ __forceinline__ int parts(int most) const {
+    int s = 0;
+    each([&](int, int u, int) {
+      s += sum64i(ceil_div(u, most));
+      return true;
+    });
+    return s;
+  }
+};
+
+// Workgroups of four wavefronts, each with a share of one set of 16 NT rows.  A set gets as many as its sequence is long, so that
+// sequences of any lengths end together and few long ones fill the GPU: the fewest units a workgroup with which all sets together
+// need at most nwg of them (as many as run at once: one more costs a round of its own), and a set at most `top` (what joins them
+// is one workgroup).  The grid has nwg or as many as there are sets; those that are left over leave at once.
 template <typename T, int D, bool WIDE, int NT, bool STREAM>
-__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg) {
+__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg, int top) {
   extern __shared__ __align__(16) float smem[];
   constexpr int KEYS = Tile<T, D>::KEYS;
   constexpr int kSet = kRows * NT;
@@ -776,52 +812,51 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   const int sets = (p.R + kSet - 1) / kSet;      // of a (sequence, key head)
   const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
   const int per = p.H * sets;                    // sets of a sequence (all units: fewer than 2^31)
-  int all = 0;
-  int u0 = 0, n0 = -1;                           // lane i: units of a set of sequence i of the first 64, its last position
-  for (int b0 = 0; b0 < p.B; b0 += kWave) {
-    int n;
-    const int u = units_of(p, b0, n);
-    if (b0 == 0) {
-      u0 = u;
-      n0 = n;
+  const Units units(p);
+  int all = 0, longest = 0;
+  units.each([&](int, int u, int) {
+    all += sum64i(u);
+    longest = max(longest, max64i(u));
+    return true;
+  });
+  const int share = nwg / (per * p.B) < 1 ? 1 : nwg / (per * p.B);   // workgroups that every set can have
+  int most = ceil_div(longest, share);
+  if (p.B > 1 && share < longest) {
+    // sequences shorter than the longest leave workgroups to the others
+    int least = ceil_div(all * per, nwg);
+    for (int i = 0; i < 6 && least < most; ++i) {
+      const int half = (least + most) >> 1;
+      if (units.parts(half) * per <= nwg) most = half;
+      else least = half + 1;
     }
-    all += __builtin_amdgcn_readlane(prefix64(u), kWave - 1);
   }
-  all *= per;
-  const int most = (int)(((unsigned)all + nwg - 1) / nwg);       // units of a workgroup
+  if (ceil_div(longest, most) > top) most = ceil_div(longest, top);
   int wg = blockIdx.x;
   if (sets > 1) {
     // sets of one key head share its keys: the workgroups in use next to each other are those of one XCD (they go round robin
     // over the 8; the grid is a multiple of 8)
-    int used = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kWave) {
-      int n;
-      const int u = b0 == 0 ? u0 : units_of(p, b0, n);
-      used += __builtin_amdgcn_readlane(prefix64((int)((unsigned)(u + most - 1) / (unsigned)most)), kWave - 1);
-    }
-    const int share = (used * per + 7) / 8;
-    if (wg / 8 >= share) return;
-    wg = wg % 8 * share + wg / 8;
+    const int each = ceil_div(units.parts(most) * per, 8);
+    if (wg / 8 >= each) return;
+    wg = wg % 8 * each + wg / 8;
   }
   // its sequence, and the workgroups of that one's sets
   int b = -1, ub = 0, count = 0, start = 0, last = -1;
-  for (int b0 = 0; b0 < p.B; b0 += kWave) {
-    int t = n0;
-    const int u = b0 == 0 ? u0 : units_of(p, b0, t);
-    const int n = (int)((unsigned)(u + most - 1) / (unsigned)most);
+  units.each([&](int b0, int u, int t) {
+    const int n = ceil_div(u, most);
     const int sum = prefix64(n);
     const uint64_t past = __ballot(start + sum * per > wg);
-    if (past != 0) {
-      const int i = __ffsll((unsigned long long)past) - 1;
-      b = b0 + i;
-      ub = __builtin_amdgcn_readlane(u, i);
-      count = __builtin_amdgcn_readlane(n, i);
-      last = __builtin_amdgcn_readlane(t, i);
-      start += (__builtin_amdgcn_readlane(sum, i) - count) * per;
-      break;
+    if (past == 0) {
+      start += __builtin_amdgcn_readlane(sum, kWave - 1) * per;
+      return true;
     }
-    start += __builtin_amdgcn_readlane(sum, kWave - 1) * per;
-  }
+    const int i = __ffsll((unsigned long long)past) - 1;
+    b = b0 + i;
+    ub = __builtin_amdgcn_readlane(u, i);
+    count = __builtin_amdgcn_readlane(n, i);
+    last = __builtin_amdgcn_readlane(t, i);
+    start += (__builtin_amdgcn_readlane(sum, i) - count) * per;
+    return false;
+  });
   if (b < 0) return;
   const int in = (wg - start) / count;           // set of the sequence
   const int part = wg - start - in * count;
@@ -910,16 +945,18 @@ int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const int rows = p.R < kRows * NT ? p.R : kRows * NT;
   const size_t stage = kWaves * Tile<T, D>::LSTEP, parts = (size_t)kWaves * rows * (D + 2), join = 3 * kWaves * kWave;
   const int nwg = nsplit / kWaves;
-  const int64_t wgs = nwg == 1 ? sets : nwg + sets;
+  const int64_t wgs = nwg < sets ? sets : nwg;
+  // (rows of 64, one set of 131000 keys: a row 128 parts 17.6 us, 256 parts 19.5; eight rows 64 parts 32 us, 256 parts 57)
+  const int top = rows > 10 ? 24 : 256 / rows;
   const dim3 grid((unsigned)(per > 1 ? (wgs + 7) / 8 * 8 : wgs));
   const size_t lds = stage + (parts > join ? parts : join) * sizeof(float);
   if constexpr (NT == 1) {
     if (per == 1 && (int64_t)p.BH * p.Tk * 2 * D * (int64_t)sizeof(T) >= kOnce) {
-      hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, 1, true>), grid, blk, lds, st, p, nwg);
+      hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, 1, true>), grid, blk, lds, st, p, nwg, top);
       return check_launch("dense_split_kernel");
     }
   }
-  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT, false>), grid, blk, lds, st, p, nwg);
+  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT, false>), grid, blk, lds, st, p, nwg, top);
   return check_launch("dense_split_kernel");
 }
 

@@ -586,20 +586,25 @@ def decode_nsplit8(B, H, Nq, wl, leaf):
 
 def decode_nsplit_dense(B, H, rows, keys, D=64):
     """dense_attn's nsplit for B * H (sequence, key head) pairs of `rows` query rows (query heads of a key head times tokens)
-    over up to `keys` keys: four wavefronts for each of the workgroups that the units of 128 keys are dealt to.
+    over up to `keys` keys: 1, a wavefront a set of rows, or four wavefronts for each of the workgroups that there may be at most.
 
-    A set of rows gets a whole number of workgroups, so those in use are up to one a set more than that; all at once on the 256
-    compute units they should be: 12 queries over 131000 keys of 64 take 66 us with 244 and 74 with 256 (264 in use), 32 sets of
-    4 x 128 over 6001 keys 23.2 and 25.4.  From 192 sets on, two workgroups a compute unit (384 sets over 32768 keys 491 us with
-    512, 516 with 256), and from 4096 a wavefront a set; of 32 rows, as prompts have, from 1024 (16 heads of 128 x 4096 tokens
-    275 us so, 379 with a workgroup a set; 12 heads of 64 x 1024 tokens, 384 sets, 31 and 23)."""
+    Few sets: a workgroup for each of the 256 compute units, where whole workgroups a set come near that (96 sets over 16000 keys
+    of 64, 192 workgroups 67 us and 256, some of them two to a unit, 87).  Else about 768, so that what the units have left
+    over at the end is little (144 sets 92 us with 720 and 126 with 144, 192 sets 118 and 132, 384 sets over 32768 keys 439 and
+    521), where each has 16 units of 128 keys or more (384 sets over 500 keys 14 us with 384 and 21 with 768).  Rows of prompts,
+    more than 16: at most 512 (192 sets of 32 rows over 8000 keys 58 us with 384, 66 with 192, 70 with 576), and from 1024 sets on
+    a wavefront a set (16 heads of 128 x 4096 tokens 275 us so, 379 with a workgroup a set)."""
     sets = max(1, B * H * ((rows + 31) // 32 if rows > 16 else 1))
     units = (max(1, keys) + 127) // 128
     if sets >= (1024 if rows > 16 else 4096):
         return 1
-    if units == 1:
-        return 4
-    return 4 * min(256 - sets if sets <= 192 else 512, sets * units)
+    if sets <= 256 and 256 // sets * sets >= 218:
+        parts = 256 // sets
+    else:
+        parts = max(1, 512 // sets) if rows > 16 else -(-768 // sets)
+        if units < 16 * parts:
+            parts = max(1, 256 // sets)
+    return 4 if parts == 1 or units == 1 else 4 * parts * sets
 
 
 def _budget_weights(state, pw):
