@@ -7,12 +7,17 @@
 //
 // Angles: t reaches 10^6, so t * w_i in 32 bits would be off by up to 0.06; w_i comes as turns (w_i / 2 pi) in 64 bits,
 // the product is taken modulo one turn in 64 bits, and only the rest, at most half a turn, goes to a 32-bit sine and
-// cosine.  For float32 rows those are the library's (2^-23 of it); 16-bit rows take the hardware's sine, whose error
-// (measured 2^-21 absolute) is far below half a step of the result (2^-12 and 2^-9 of it).
+// cosine.  For float32 rows those are the library's (off by at most 2^-24.2 over 2^24 arguments of that range); 16-bit rows
+// take the hardware's sine, off by 2^-22.9 there, half a step of their results being 2^-11 and 2^-8 of them.
 //
-// Bound by bytes: each element is read and written once.  A thread holds one unit, 16 bytes of each half of some pairs
-// (single elements where rows are not whole 16-byte pieces), and takes it through several heads of its token, which share
-// its sines: with one head a thread the sines cost more than the bytes.
+// Bound by bytes: each element is read and written once.  A thread takes one unit of one row, two pieces of 16 bytes that lie
+// half the turned part apart (single elements where rows are not whole such pieces), so that the threads of a row read and
+// write whole runs of it.  The sines again for every head cost nothing beside the bytes: four heads of a token a thread, which
+// share them, took 113 and 130 us for the sizes below, eight 116 and 144.  Stores are ordinary ones: what is written is read
+// next.
+//
+// 30001 positions of 20 heads of 128 in float32, 614 MB: 106 us, 5.8 TB/s.  Prompts of 8 x 8191 tokens, 12 heads of 64, into
+// pages of 64 rows in bfloat16 (queries turned too), 604 MB: 121 us, 5.0 TB/s.  One token of 32 sequences: 3.6 us, a launch.
 //
 // The reference has learned positions only (model.py:54, 74); it stores keys and values at engine.py:41-55.
 #include "common.hpp"
@@ -52,7 +57,7 @@ __device__ __forceinline__ void turn_of(const Rope& r, int pair, int pos, float&
   s = sn * (r.amp * r.sign);
 }
 
-// A unit of a row: NE elements at a and NE at b, as pairs (a[i], b[i]) (half) or (a[2i], a[2i + 1]), then b's (interleaved);
+// A unit of a row: NE elements at a and NE at b, as pairs (a[i], b[i]) (half) or (a[2i], a[2i + 1]) and b's (interleaved);
 // NE = 16 bytes' worth with VEC, else one element.
 template <typename T, bool VEC> struct Unit {
   static constexpr int NE = VEC ? vec_elems<T>() : 1;
@@ -87,18 +92,23 @@ __device__ __forceinline__ void turn_pair(T& x, T& y, float c, float s) {
   x = from_f32<T>(fmaf(a, c, -(b * s)));
   y = from_f32<T>(fmaf(a, s, b * c));
 }
+// Unit u, turned: its pairs' angles from the position.
 template <typename T, bool VEC, bool INTER>
-__device__ __forceinline__ void unit_turn(Unit<T, VEC>& u, const float* c, const float* s) {
+__device__ __forceinline__ void unit_turn(Unit<T, VEC>& e, const Rope& r, int u, int pos) {
   constexpr int NE = Unit<T, VEC>::NE;
-  if constexpr (INTER && VEC) {
 #pragma unroll
-    for (int i = 0; i < NE / 2; ++i) {
-      turn_pair<T>(u.a[2 * i], u.a[2 * i + 1], c[i], s[i]);
-      turn_pair<T>(u.b[2 * i], u.b[2 * i + 1], c[NE / 2 + i], s[NE / 2 + i]);
+  for (int i = 0; i < NE; ++i) {
+    float c, s;
+    if constexpr (INTER && VEC) {
+      const bool second = i >= NE / 2;
+      const int k = i % (NE / 2);
+      turn_of<T>(r, (second ? r.rot / 4 : 0) + u * (NE / 2) + k, pos, c, s);
+      T* x = second ? e.b : e.a;
+      turn_pair<T>(x[2 * k], x[2 * k + 1], c, s);
+    } else {
+      turn_of<T>(r, u * NE + i, pos, c, s);
+      turn_pair<T>(e.a[i], e.b[i], c, s);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NE; ++i) turn_pair<T>(u.a[i], u.b[i], c[i], s[i]);
   }
 }
 
@@ -106,20 +116,19 @@ __device__ __forceinline__ void unit_turn(Unit<T, VEC>& u, const float* c, const
 template <typename T, bool VEC, bool INTER>
 struct RowUnits {
   static constexpr int NE = Unit<T, VEC>::NE;
-  int turned, rest, ia, ib;   // rest: pieces past the turned part
-  bool turn, two;
+  int ia, ib;
+  bool turn;
   __device__ __forceinline__ RowUnits(int u, int rot, int D) {
-    turned = rot / (2 * NE);
+    const int turned = rot / (2 * NE);
     turn = u < turned;
-    two = true;
     if (turn) {
-      ia = INTER ? u * 2 * NE : u * NE;
-      ib = INTER ? ia + NE : ia + rot / 2;
+      ia = INTER && !VEC ? 2 * u : u * NE;
+      ib = INTER && !VEC ? ia + 1 : ia + rot / 2;
     } else {
-      ia = rot + (u - turned) * 2 * NE;
-      ib = ia + NE;
-      two = ib < D;
-      if (!two) ib = ia;
+      const int units = ((D - rot) / NE + 1) / 2;
+      ia = rot + (u - turned) * NE;
+      ib = ia + units * NE;
+      if (ib >= D) ib = ia;
     }
   }
 };
@@ -129,47 +138,28 @@ struct RopeArgs {
   RowsOf x;
   void* y;
   int64_t ysb, ysh, yst;
-  int H, T, D, units, groups;   // groups of heads a token
-  int64_t n;                    // threads' worth of work
+  int H, T, D, units;
+  int64_t n;            // units in all
   Rope r;
   const int32_t* pos;
   int64_t pos_sb;
 };
 
-// HPT heads of one token a thread, the same unit of each.
-template <typename T, bool VEC, bool INTER, int HPT>
+template <typename T, bool VEC, bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs p) {
-  using U = Unit<T, VEC>;
   const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (at >= p.n) return;
   const int u = (int)(at % p.units);
   const int64_t rest = at / p.units;
-  const int g = (int)(rest % p.groups);
-  const int64_t tok = rest / p.groups;
+  const int h = (int)(rest % p.H);
+  const int64_t tok = rest / p.H;
   const int t = (int)(tok % p.T);
   const int64_t b = tok / p.T;
   const RowUnits<T, VEC, INTER> w(u, p.r.rot, p.D);
-  const T* x = reinterpret_cast<const T*>(p.x.p) + b * p.x.sb + t * p.x.st;
-  T* y = reinterpret_cast<T*>(p.y) + b * p.ysb + t * p.yst;
-  U e[HPT];
-#pragma unroll
-  for (int j = 0; j < HPT; ++j) {
-    const int h = g + j * p.groups;
-    if (h < p.H) unit_load<T, VEC>(x + h * p.x.sh, w.ia, w.ib, e[j]);
-  }
-  if (w.turn) {
-    float c[U::NE], s[U::NE];
-    const int pos = p.pos[b * p.pos_sb + t];
-#pragma unroll
-    for (int i = 0; i < U::NE; ++i) turn_of<T>(p.r, u * U::NE + i, pos, c[i], s[i]);
-#pragma unroll
-    for (int j = 0; j < HPT; ++j) unit_turn<T, VEC, INTER>(e[j], c, s);
-  }
-#pragma unroll
-  for (int j = 0; j < HPT; ++j) {
-    const int h = g + j * p.groups;
-    if (h < p.H) unit_store<T, VEC>(y + h * p.ysh, w.ia, w.ib, e[j]);
-  }
+  Unit<T, VEC> e;
+  unit_load<T, VEC>(reinterpret_cast<const T*>(p.x.p) + b * p.x.sb + h * p.x.sh + t * p.x.st, w.ia, w.ib, e);
+  if (w.turn) unit_turn<T, VEC, INTER>(e, p.r, u, p.pos[b * p.pos_sb + t]);
+  unit_store<T, VEC>(reinterpret_cast<T*>(p.y) + b * p.ysb + h * p.ysh + t * p.yst, w.ia, w.ib, e);
 }
 
 struct StoreArgs {
@@ -182,7 +172,7 @@ struct StoreArgs {
   const int32_t* ptab;
   int64_t pt_sb, pt_sh, pstride, npages;
   int blog2;
-  int Hq, H, N, D, Tcap, units, groups;
+  int Hq, H, N, D, Tcap, units;
   int64_t n;
   Rope r;
   const int32_t* pos;
@@ -191,61 +181,40 @@ struct StoreArgs {
 
 // As rope_kernel over the Hq query heads, the H key heads and the H value heads of a token; keys and values go to the row
 // of the token's position in the cache (nowhere when it is outside the cache or its block has no page).
-template <typename T, bool VEC, bool INTER, int HPT>
+template <typename T, bool VEC, bool INTER>
 __global__ __launch_bounds__(kThreads) void kv_store_kernel(StoreArgs p) {
-  using U = Unit<T, VEC>;
   const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (at >= p.n) return;
   const int u = (int)(at % p.units);
   const int64_t rest = at / p.units;
-  const int g = (int)(rest % p.groups);
-  const int64_t tok = rest / p.groups;
+  const int heads = p.Hq + 2 * p.H, h = (int)(rest % heads);
+  const int64_t tok = rest / heads;
   const int t = (int)(tok % p.N);
   const int64_t b = tok / p.N;
   const RowUnits<T, VEC, INTER> w(u, p.r.rot, p.D);
   const int pos = p.pos[b * p.pos_sb + t];
-  const bool in = pos >= 0 && pos < p.Tcap;
-  const int heads = p.Hq + 2 * p.H;
-  U e[HPT];
-  int64_t to[HPT];     // the row's place in the cache, -1: none
-#pragma unroll
-  for (int j = 0; j < HPT; ++j) {
-    const int h = g + j * p.groups;
-    to[j] = -1;
-    if (h >= heads) continue;
-    const RowsOf& src = h < p.Hq ? p.q : (h < p.Hq + p.H ? p.k : p.v);
-    const int hh = h < p.Hq ? h : (h - p.Hq) % p.H;
-    unit_load<T, VEC>(reinterpret_cast<const T*>(src.p) + b * src.sb + hh * src.sh + t * src.st, w.ia, w.ib, e[j]);
-    if (h >= p.Hq && in) {
-      if (p.ptab == nullptr) {
-        to[j] = b * p.csb + hh * p.csh + pos * p.cst;
-      } else {
-        const int pg = p.ptab[b * p.pt_sb + hh * p.pt_sh + (pos >> p.blog2)];
-        if (pg >= 0 && pg < p.npages) to[j] = pg * p.pstride + (pos & ((1 << p.blog2) - 1)) * p.cst;
-      }
+  const bool query = h < p.Hq, value = h >= p.Hq + p.H;
+  const int hh = query ? h : h - p.Hq - (value ? p.H : 0);
+  const RowsOf& src = query ? p.q : value ? p.v : p.k;
+  Unit<T, VEC> e;
+  unit_load<T, VEC>(reinterpret_cast<const T*>(src.p) + b * src.sb + hh * src.sh + t * src.st, w.ia, w.ib, e);
+  T* to;
+  if (query) {
+    to = reinterpret_cast<T*>(p.qo) + b * p.osb + hh * p.osh + t * p.ost;
+  } else {
+    if (pos < 0 || pos >= p.Tcap) return;
+    to = reinterpret_cast<T*>(value ? p.Vc : p.Kc);
+    if (p.ptab == nullptr) {
+      to += b * p.csb + hh * p.csh + pos * p.cst;
+    } else {
+      const int pg = p.ptab[b * p.pt_sb + hh * p.pt_sh + (pos >> p.blog2)];
+      if (pg < 0 || pg >= p.npages) return;
+      to += pg * p.pstride + (pos & ((1 << p.blog2) - 1)) * p.cst;
     }
   }
-  if (w.turn) {
-    float c[U::NE], s[U::NE];
-#pragma unroll
-    for (int i = 0; i < U::NE; ++i) turn_of<T>(p.r, u * U::NE + i, pos, c[i], s[i]);
-#pragma unroll
-    for (int j = 0; j < HPT; ++j)
-      if (g + j * p.groups < p.Hq + p.H) unit_turn<T, VEC, INTER>(e[j], c, s);
-  }
-#pragma unroll
-  for (int j = 0; j < HPT; ++j) {
-    const int h = g + j * p.groups;
-    if (h < p.Hq)
-      unit_store<T, VEC>(reinterpret_cast<T*>(p.qo) + b * p.osb + h * p.osh + t * p.ost, w.ia, w.ib, e[j]);
-    else if (to[j] >= 0)
-      unit_store<T, VEC>(reinterpret_cast<T*>(h < p.Hq + p.H ? p.Kc : p.Vc) + to[j], w.ia, w.ib, e[j]);
-  }
+  if (w.turn && !value) unit_turn<T, VEC, INTER>(e, p.r, u, pos);
+  unit_store<T, VEC>(to, w.ia, w.ib, e);
 }
-
-// Heads a thread: four where that leaves enough threads for the whole GPU, else one (the sines again for every head).
-constexpr int kHeads = 4;
-constexpr int64_t kEnough = (int64_t)1 << 19;
 
 bool pieces(int sz, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
   for (const void* p : ptrs)
@@ -268,19 +237,14 @@ int check_rope(const char* who, int dtype, int D, int rot, const double* turns, 
   return TA_OK;
 }
 
-template <typename F>
-int grid_of(const char* who, int64_t tokens, int heads, int units, int& groups, int64_t& n, bool& many, F f) {
-  const int64_t one = tokens * heads;
-  many = one * units >= kEnough * kHeads;
-  groups = many ? (heads + kHeads - 1) / kHeads : heads;
-  n = tokens * groups * units;
+// Workgroups for `n` units; 0 (and the error set): too many.
+unsigned grid_of(const char* who, int64_t n) {
   const int64_t blocks = (n + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffffLL) {
     set_error(std::string(who) + ": too large");
-    return TA_ERR_UNSUPPORTED;
+    return 0;
   }
-  f((unsigned)blocks);
-  return check_launch(who);
+  return (unsigned)blocks;
 }
 
 }  // namespace
@@ -301,15 +265,13 @@ extern "C" int ta_rope(const void* x, int dtype, int64_t xsb, int64_t xsh, int64
   const int sz = dtype == TA_F32 ? 4 : 2;
   const int ne = 16 / sz;
   const bool vec = rot % (2 * ne) == 0 && D % ne == 0 && pieces(sz, {x, y}, {xsb, xsh, xst, ysb, ysh, yst});
-  RopeArgs p{{x, xsb, xsh, xst}, y, ysb, ysh, yst, H, T, D, row_units(vec ? ne : 1, rot, D), 0, 0,
+  RopeArgs p{{x, xsb, xsh, xst}, y, ysb, ysh, yst, H, T, D, row_units(vec ? ne : 1, rot, D), 0,
              {rot, turns, amp, inverse ? -1.0f : 1.0f}, pos, pos_sb};
-  bool many;
-  return grid_of("ta_rope", (int64_t)B * T, H, p.units, p.groups, p.n, many, [&](unsigned blocks) {
-#define TA_ROPE(TT, V, I)                                                                                              \
-  do {                                                                                                                 \
-    if (many) hipLaunchKernelGGL((rope_kernel<TT, V, I, kHeads>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, p); \
-    else hipLaunchKernelGGL((rope_kernel<TT, V, I, 1>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, p);       \
-  } while (0)
+  p.n = (int64_t)B * T * H * p.units;
+  const unsigned blocks = grid_of("ta_rope", p.n);
+  if (!blocks) return TA_ERR_UNSUPPORTED;
+#define TA_ROPE(TT, V, I) \
+  hipLaunchKernelGGL((rope_kernel<TT, V, I>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, p)
 #define TA_ROPE_T(TT)                                          \
   do {                                                         \
     if (vec && interleaved) TA_ROPE(TT, true, true);           \
@@ -317,14 +279,14 @@ extern "C" int ta_rope(const void* x, int dtype, int64_t xsb, int64_t xsh, int64
     else if (interleaved) TA_ROPE(TT, false, true);            \
     else TA_ROPE(TT, false, false);                            \
   } while (0)
-    switch (dtype) {
-      case TA_F32: TA_ROPE_T(float); break;
-      case TA_F16: TA_ROPE_T(f16_t); break;
-      default: TA_ROPE_T(bf16_t); break;
-    }
+  switch (dtype) {
+    case TA_F32: TA_ROPE_T(float); break;
+    case TA_F16: TA_ROPE_T(f16_t); break;
+    default: TA_ROPE_T(bf16_t); break;
+  }
 #undef TA_ROPE
 #undef TA_ROPE_T
-  });
+  return check_launch("rope_kernel");
 }
 
 extern "C" int ta_kv_store(const void* k, const void* v, int dtype, int64_t ksb, int64_t ksh, int64_t kst, int64_t vsb,
@@ -351,7 +313,7 @@ extern "C" int ta_kv_store(const void* k, const void* v, int dtype, int64_t ksb,
              (Hq == 0 || pieces(sz, {q, q_out}, {qsb, qsh, qst, osb, osh, ost})) &&
              (pages ? pieces(sz, {}, {pages->page_stride}) : pieces(sz, {}, {csb, csh}));
   StoreArgs p{{q, qsb, qsh, qst}, {k, ksb, ksh, kst}, {v, vsb, vsh, vst}, q_out, osb, osh, ost, Kc, Vc, csb, csh, cst,
-              nullptr, 0, 0, 0, 0, 0, Hq, H, N, D, Tcap, row_units(vec ? ne : 1, rot, D), 0, 0,
+              nullptr, 0, 0, 0, 0, 0, Hq, H, N, D, Tcap, row_units(vec ? ne : 1, rot, D), 0,
               {rot, turns, amp, 1.0f}, pos, pos_sb};
   if (pages) {
     p.ptab = pages->table;
@@ -361,15 +323,11 @@ extern "C" int ta_kv_store(const void* k, const void* v, int dtype, int64_t ksb,
     p.npages = pages->num_pages;
     p.blog2 = pages->block_log2;
   }
-  bool many;
-  return grid_of("ta_kv_store", (int64_t)B * N, Hq + 2 * H, p.units, p.groups, p.n, many, [&](unsigned blocks) {
-#define TA_STORE(TT, V, I)                                                                                          \
-  do {                                                                                                              \
-    if (many)                                                                                                       \
-      hipLaunchKernelGGL((kv_store_kernel<TT, V, I, kHeads>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, p); \
-    else                                                                                                            \
-      hipLaunchKernelGGL((kv_store_kernel<TT, V, I, 1>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, p);  \
-  } while (0)
+  p.n = (int64_t)B * N * (Hq + 2 * H) * p.units;
+  const unsigned blocks = grid_of("ta_kv_store", p.n);
+  if (!blocks) return TA_ERR_UNSUPPORTED;
+#define TA_STORE(TT, V, I) \
+  hipLaunchKernelGGL((kv_store_kernel<TT, V, I>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, p)
 #define TA_STORE_T(TT)                                         \
   do {                                                         \
     if (vec && interleaved) TA_STORE(TT, true, true);          \
@@ -377,12 +335,12 @@ extern "C" int ta_kv_store(const void* k, const void* v, int dtype, int64_t ksb,
     else if (interleaved) TA_STORE(TT, false, true);           \
     else TA_STORE(TT, false, false);                           \
   } while (0)
-    switch (dtype) {
-      case TA_F32: TA_STORE_T(float); break;
-      case TA_F16: TA_STORE_T(f16_t); break;
-      default: TA_STORE_T(bf16_t); break;
-    }
+  switch (dtype) {
+    case TA_F32: TA_STORE_T(float); break;
+    case TA_F16: TA_STORE_T(f16_t); break;
+    default: TA_STORE_T(bf16_t); break;
+  }
 #undef TA_STORE
 #undef TA_STORE_T
-  });
+  return check_launch("kv_store_kernel");
 }
