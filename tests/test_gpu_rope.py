@@ -259,3 +259,17 @@ def test_refusals():
             bad()
     assert K.kv_store(k[:, :, :0], k[:, :, :0], c, None, pos[:0]) is None
     assert K.rope(x[:, :, :0], pos[:0], r).shape == (2, 3, 0, 64)
+
+
+def test_store_without_a_position():
+    """A cache that holds no position stores nothing; its queries are turned all the same."""
+    k = torch.randn(2, 3, 5, 64, device=DEV)
+    q = torch.randn(2, 6, 5, 64, device=DEV)
+    pos = torch.arange(5, dtype=torch.int32, device=DEV)
+    r = K.Rope(P.rope_frequencies(64)[0], DEV)
+    none = torch.zeros(2, 3, 0, 64, device=DEV)
+    assert torch.equal(K.kv_store(k, k, none, none, pos, q=q, rope=r), K.rope(q, pos, r))
+    assert torch.equal(K.kv_store(k, k, none, none, pos, q=q), q)
+    for bad in (lambda: K.kv_store(k, k, none, None, pos), lambda: K.dense_attn(q, k, None, pos)):
+        with pytest.raises(TypeError):
+            bad()

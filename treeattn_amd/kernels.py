@@ -1190,9 +1190,10 @@ def dense_attn(q, k, v, tq, scale=None, out=None, lse=None, nsplit=1, ws=None):
     """Attention over the whole cache: q (B,Hq,Nq,D) at positions tq ((Nq,) or (B,Nq)) over every key 0 .. tq of k, v
     (B,H,Tk,D) or of a PagedCache (as k; v None), Hq a multiple of H (query head h reads key head h // (Hq // H)).  Keys of a
     block without a page do not count; a query without any key, or at a position outside [0, Tk), gives zeros and lse -1e30.
-    lse: None, or (B,Hq,Nq) float32 to receive the log-sum-exp.  nsplit: wavefronts that share the keys of 16 query rows, 1 or
-    a multiple of 4 up to 1024 (engine.decode_nsplit_dense chooses); past 4 with a workspace (dense_attn_workspace).  Returns
-    (out in q's dtype, lse)."""
+    lse: None, or (B,Hq,Nq) float32 to receive the log-sum-exp.  nsplit: 1, a wavefront for each set of 16 or 32 rows, or a
+    multiple of 4 up to 8192, four wavefronts for each of nsplit / 4 workgroups that the sets share by their sequences' lengths
+    (engine.decode_nsplit_dense chooses); past 4 with a workspace (dense_attn_workspace; None: a new one).  Returns (out in q's
+    dtype, lse)."""
     dev = L.device_index(q)
     B, Hq, Nq, D = shape = q.shape
     qt = q.stride()
@@ -1203,7 +1204,7 @@ def dense_attn(q, k, v, tq, scale=None, out=None, lse=None, nsplit=1, ws=None):
         Bk, H, Dk, Tk, dt = k.B, k.H, k.D, k.tcap, k.dtype
         kt = vt = (0, 0, D)
         ka, va, pages = k.k, k.v, ctypes.byref(k.desc)
-    elif not isinstance(k, torch.Tensor):
+    elif not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
         raise TypeError('dense_attn: contiguous caches or a PagedCache')
     else:
         Bk, H, Tk, Dk = k.shape
@@ -1280,6 +1281,9 @@ def rope(x, pos, rope, out=None, inverse=False):
     return out
 
 
+_turned = rope     # (kv_store's argument has its name)
+
+
 def _own_rows(name, x, out):
     """out is written row by row while x is read: it repeats no row of its own, and where it starts at x it is x."""
     if any(s > 1 and t == 0 for s, t in zip(out.shape, out.stride())):
@@ -1300,7 +1304,7 @@ def kv_store(k, v, Kc, Vc, pos, q=None, rope=None, q_out=None):
             raise ValueError('kv_store: Vc is None with a PagedCache')
         want, dt, Ka, Va = (Kc.B, Kc.H, Kc.D), Kc.dtype, Kc.k, Kc.v
         ct, tcap, pages = (0, 0, D), Kc.tcap, ctypes.byref(Kc.desc)
-    elif isinstance(Kc, torch.Tensor):
+    elif isinstance(Kc, torch.Tensor) and isinstance(Vc, torch.Tensor):
         if Kc.shape != Vc.shape or Kc.stride() != Vc.stride() or Kc.dtype != Vc.dtype or Kc.stride(3) != 1:
             raise ValueError('kv_store: K and V caches (B, H, Tcap, D) need one dtype, the same strides and contiguous rows')
         want, dt, Ka, Va = (Kc.shape[0], Kc.shape[1], Kc.shape[3]), Kc.dtype, Kc, Vc
@@ -1336,7 +1340,10 @@ def kv_store(k, v, Kc, Vc, pos, q=None, rope=None, q_out=None):
         raise ValueError('kv_store: q_out without q')
     pos, pos_sb = _positions('kv_store', pos, B, N)
     _on('kv_store', dev, v, Ka, Va, pos, q, q_out)
-    if tcap and k.numel():
+    if not tcap:
+        if q is not None:
+            q_out.copy_(q) if rope is None else _turned(q, pos, rope, out=q_out)
+    elif k.numel():
         _kv_store(dev, k.data_ptr(), v.data_ptr(), L.dtype_code(k), kt[0], kt[1], kt[2], vt[0], vt[1], vt[2], qp, qt[0], qt[1],
                   qt[2], op, ot[0], ot[1], ot[2], Hq, Ka.data_ptr(), Va.data_ptr(), ct[0], ct[1], ct[2], B, H, N, D, tcap,
                   pos.data_ptr(), pos_sb, rot, turns, inter, amp, pages)
