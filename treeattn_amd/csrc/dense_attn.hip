@@ -336,8 +336,8 @@ struct Share {
   }
 
   // The step's keys from the lanes that loaded them to the lanes whose operand they are: lane (c, g) takes piece g of row c.
-  // (Loaded in that order, each 16 bytes would be an access of their own to the first cache: 371 accesses a step of 32 keys of
-  // 64, now 180, which a piece of a prompt is bound by.)
+  // (Loaded in that order, each 16 bytes would be an access of their own to the first cache, which a piece of a prompt was
+  // bound by: 371 accesses a step of 32 keys of 64 by a counter, now some 190.)
   __device__ __forceinline__ void turn(Step<T, D>& x) const {
     wave_sync();
 #pragma unroll

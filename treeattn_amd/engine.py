@@ -1096,7 +1096,8 @@ class Decoder:
     def fork(self, src, dst, t):
         """Sequence dst goes on from the first t positions of src (at most those that src holds), as after the same tokens: whole
         pages of the caches are shared (read only; a step that goes back into one gets a copy), the rows behind them and the
-        tree's state copied.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] and g_t[dst] too.
+        tree's state copied.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] and g_t[dst] too
+        (a replay hands out no copies: before one that goes back behind t, reserve(t_end, start) does).
         With the budget head's global pool the running sum of keys is that of the cache's rows."""
         t = int(t)
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
