@@ -359,3 +359,114 @@ def test_refusals():
     empty = torch.zeros(2, 2, 0, 64, device=DEV, dtype=BF16)
     assert not K.dense_attn(torch.ones_like(q), empty, empty, tq)[0].any()
     assert K.dense_attn(q[:, :, :0], k, k, tq[:, :0])[0].shape == (2, 4, 0, 64)
+
+
+def some_rows(out, lse, q, k, v, tq, scale, pairs, dtype, at, have=None):
+    """Rows `at` of the (sequence, query head) pairs against float64."""
+    G = q.shape[1] // k.shape[1]
+    for b, h in pairs:
+        g = h // G
+        want, wl, tol = want64(q[b:b + 1, h:h + 1, at], k[b:b + 1, g:g + 1], v[b:b + 1, g:g + 1], tq[b:b + 1, at], scale,
+                               None if have is None else have[b:b + 1, g:g + 1])
+        close(out[b:b + 1, h:h + 1, at], want, tol, dtype)
+        if lse is not None:
+            got = lse[b, h, at].cpu()
+            assert torch.equal(got == -1e30, wl[0, 0] == -1e30)
+            ok = wl[0, 0] > -1e29
+            assert bool(((got.double() - wl[0, 0]).abs()[ok] <= (tol[0, 0, :, 0][ok] / 2 + 1e-6 * (1 + wl[0, 0][ok].abs())) + 1e-5).all())
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('D,leaf,H,G,N,T', [(64, 64, 12, 1, 1000, 1003), (128, 32, 8, 3, 500, 513), (32, 128, 12, 1, 1024, 1024),
+                                            (64, 0, 12, 1, 901, 929), (128, 0, 12, 1, 1000, 1001), (32, 0, 3, 65, 63, 640),
+                                            (64, 64, 96, 1, 65, 577)])
+def test_many_rows(dtype, D, leaf, H, G, N, T):
+    """Prompts and pieces of them, their positions in any order, some outside the cache; contiguous caches that end inside a
+    tile; last sets with wavefronts that have no rows."""
+    B = 2
+    k, v = rnd(B, H, T, D, seed=31, dtype=dtype), rnd(B, H, T, D, seed=32, dtype=dtype)
+    q = rnd(B, G * H, N, D, seed=33, dtype=dtype)
+    g = torch.Generator().manual_seed(34)
+    tq = rows([T, T - 3], N)
+    mixed = torch.randint(-2, T + 2, (N,), generator=g, dtype=torch.int32)
+    tq[1, N // 2:] = mixed[N // 2:]
+    have = None
+    if leaf:
+        missing = [(0, 0, 1), (1, H - 1, 0), (1, H - 1, 3)]
+        have = torch.ones(B, H, T, dtype=torch.bool)
+        for b, h, j in missing:
+            have[b, h, j * leaf:(j + 1) * leaf] = False
+        c = paged(k, v, leaf, seed=D, fill=float('nan'), missing=missing), None
+    else:   # strides of a larger cache, whose other rows are NaN
+        wide = [torch.full((B, H, T + 70, D), float('nan'), dtype=dtype, device=DEV)[:, :, :T] for _ in range(2)]
+        c = wide[0].copy_(k), wide[1].copy_(v)
+    scale = 1 / math.sqrt(D)
+    lse = torch.empty(B, G * H, N, device=DEV)
+    out, _ = K.dense_attn(q.to(DEV), *c, tq.to(DEV), scale, lse=lse, nsplit=1)
+    at = torch.unique(torch.cat([torch.arange(0, N, max(1, N // 12)), torch.tensor([N - 1, N - 2]),
+                                 torch.randint(0, N, (8,), generator=g)]))
+    some_rows(out, lse, q, k, v, tq, scale, [(0, 0), (1, G * H - 1), (1, G)], dtype, at, have)
+    # the same whatever the other rows are: each sequence by itself, with other tokens before and after
+    same, _ = K.dense_attn(q.to(DEV).flip(2), *c, tq.to(DEV).flip(1), scale, nsplit=1)
+    far = (torch.arange(B * G * H * N * D) % 7 == 0).view(B, G * H, N, D)
+    a, b = out.cpu()[far].double(), same.flip(2).cpu()[far].double()
+    assert bool(((a - b).abs() <= 2 * torch.finfo(dtype).eps * a.abs() + 1e-3).all())
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('D', [64, 128])
+def test_many_rows_what_is_masked(dtype, D):
+    """A value that some rows of a tile see and others do not: only those that see it show it, the others' bits stay; also
+    where it is the key."""
+    B, H, N, T = 4, 12, 500, 600
+    k, v = rnd(B, H, T, D, seed=41, dtype=dtype).to(DEV), rnd(B, H, T, D, seed=42, dtype=dtype).to(DEV)
+    q = rnd(B, H, N, D, seed=43, dtype=dtype).to(DEV)
+    tq = rows([T, T, T - 7, N], N).to(DEV)
+    clean, _ = K.dense_attn(q, k, v, tq, nsplit=1)
+    for bad in (float('inf'), float('nan'), torch.finfo(dtype).min):
+        for which in (0, 1):
+            x = [k.clone(), v.clone()]
+            for b, h, t in ((0, 0, T - 5), (1, 3, 330), (2, 11, T - 1), (3, 0, 70)):
+                x[which][b, h, t, 5] = bad
+            got, _ = K.dense_attn(q, *x, tq, nsplit=1)
+            for b, h, t in ((0, 0, T - 5), (1, 3, 330), (2, 11, T - 1), (3, 0, 70)):
+                blind = tq[b] < t
+                assert torch.equal(got[b, h, blind], clean[b, h, blind]), (bad, which, b)
+                if math.isnan(bad):
+                    seen = got[b, h, ~blind]
+                    assert bool(torch.isnan(seen if which == 0 else seen[:, 5]).all())
+                if which == 1 and math.isinf(bad):
+                    assert bool((got[b, h, ~blind][:, 5] == bad).all())
+                    assert torch.equal(got[b, h, ~blind][:, 6:].isfinite(), torch.ones_like(got[b, h, ~blind][:, 6:]).bool())
+            other = torch.ones(B, H, dtype=torch.bool)
+            other[[0, 1, 2, 3], [0, 3, 11, 0]] = False
+            assert torch.equal(got[other], clean[other])
+
+
+def test_many_rows_extreme_scores_and_replays():
+    B, H, N, T, D = 4, 12, 512, 640, 64
+    k, v, q = [rnd(B, H, n, D, seed=50 + n, dtype=BF16).to(DEV) for n in (T, T, N)]
+    tq = rows([T, 600, N, 513], N).to(DEV)
+    for scale in (0.0, -0.125, 30.0):
+        out, _ = K.dense_attn(q, k, v, tq, scale, nsplit=1)
+        at = torch.tensor([0, 1, 127, 128, 300, 511])
+        if scale < 0:
+            some_rows(out, None, -q.cpu(), k.cpu(), v.cpu(), tq.cpu(), -scale, [(0, 0), (3, 11)], BF16, at)
+        else:
+            some_rows(out, None, q.cpu(), k.cpu(), v.cpu(), tq.cpu(), scale, [(0, 0), (3, 11)], BF16, at)
+    out = torch.empty_like(q)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        K.dense_attn(q, k, v, tq, out=out, nsplit=1)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        K.dense_attn(q, k, v, tq, out=out, nsplit=1)
+    for i in range(3):
+        q.copy_(rnd(B, H, N, D, seed=60 + i, dtype=BF16).to(DEV))
+        tq.copy_(rows([T - i, 600, N, 513 + i], N).to(DEV))
+        g.replay()
+        want, _ = K.dense_attn(q, k, v, tq, nsplit=1)
+        assert torch.equal(out, want)
+        torch.cuda.synchronize()

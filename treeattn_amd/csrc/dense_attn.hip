@@ -18,7 +18,11 @@
 // than kSlack: until then weights are at most 2^kSlack.
 //
 // Bound by bytes, 2 D a key and key head, where rows are few; the keys of a sequence are split over wavefronts and
-// workgroups, whose partial results the last workgroup to arrive joins.
+// workgroups, whose partial results the last workgroup to arrive joins.  32 x 12 queries over 32768 keys of 64: 440 us, 6.4 TB/s;
+// one sequence of 131000: 62 us, 5.6 TB/s.  Rows of prompts, by the hundred, share their keys through LDS (Block).
+//
+// Phase marks (trace.hpp): 0 start, 1 its part and queries are known, 2 its keys are done, 3 its part is written, 4 it is counted
+// in, 5 the set is joined.
 //
 // Reference functions replaced: engine.py:74-81 (DenseState.attend).
 #include "attn.hpp"
@@ -65,11 +69,11 @@ constexpr int kRows = 16;            // query rows of a tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <typename T, int D> struct Tile {
+template <typename T, int D, bool MANY = false> struct Tile {
   static constexpr int EB = (int)sizeof(T);
   // Tiles of 16 keys a step.  Heads of 128 take one: two steps of 32 keys in registers leave no room for two wavefronts on a
-  // SIMD (256 registers and spills).
-  static constexpr int KT = D == 128 ? 1 : 2;
+  // SIMD (256 registers and spills).  MANY: the steps stand in LDS.
+  static constexpr int KT = MANY ? 4 : D == 128 ? 1 : 2;
   static constexpr int KEYS = 16 * KT;
   static constexpr int KS = EB == 2 ? (D + 31) / 32 : D / 16;   // 16-byte pieces of a key row a lane
   static constexpr int DJ = D / 16;                             // columns of V a lane holds
@@ -85,9 +89,10 @@ template <typename T, int D> struct Tile {
 
 // The keys and values of one step, in a lane: K rows 16 i + lane / 4 at pieces lane % 4 (four lanes next to each other read 64
 // bytes of a row); V rows 16 i + 4 (lane / 16) + u at columns DJ (lane % 16) ...
-template <typename T, int D> struct Step {
-  uint4 k[Tile<T, D>::KT][Tile<T, D>::KS];
-  uint32_t v[Tile<T, D>::KT * 4][Tile<T, D>::VW];
+template <typename T, int D, bool MANY = false> struct Step {
+  using C = Tile<T, D, MANY>;
+  uint4 k[C::KT][C::KS];
+  uint32_t v[MANY ? 1 : C::KT * 4][C::VW];
   uint32_t have;     // bit 4 i + u: key 16 i + 4 (lane / 16) + u has a page
   int key0;
 };
@@ -127,6 +132,23 @@ template <typename T>
 __device__ __forceinline__ float unpack_hi(uint32_t x) {
   if constexpr (__is_same(T, f16_t)) return (float)__builtin_bit_cast(_Float16, (uint16_t)(x >> 16));
   else return __uint_as_float(x & 0xffff0000u);
+}
+
+// What is left of two weights once their two halves of hi are taken off.
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
+  if constexpr (__is_same(T, f16_t)) {
+    return pack2<T>(a - unpack_lo<T>(hi), b - unpack_hi<T>(hi));
+  } else {
+    // a - 1 x one half - 0 x the other, exact (weights are finite); the factors from registers, since as an inline constant the
+    // compiler's -1 of the lower half is the instruction's of the upper one
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 h = __builtin_bit_cast(bf16x2, hi);
+    uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+    asm("" : "+s"(first), "+s"(second));
+    return pack2<T>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), a, false),
+                    __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), b, false));
+  }
 }
 
 // The larger / the sum of x over the four lanes that share lane % 16.
@@ -172,9 +194,9 @@ __device__ __forceinline__ V once(const TA_GLOBAL V* p) {
 }
 
 // One wavefront's share: keys [k0, k1) for NT tiles of 16 query rows of one (sequence, key head).
-template <typename T, int D, bool WIDE, int NT, bool STREAM>
+template <typename T, int D, bool WIDE, int NT, bool STREAM, bool MANY = false>
 struct Share {
-  using C = Tile<T, D>;
+  using C = Tile<T, D, MANY>;
   const Dense& p;
   const int lane, c, g;
   const TA_GLOBAL T* kb;
@@ -354,7 +376,7 @@ struct Share {
   }
 
   // Scores of tile row set i: in lane (c, g) those of row c and keys 16 a + 4 g + u.
-  __device__ __forceinline__ void scores(const Step<T, D>& x, int i, f32x4 (&s)[C::KT]) const {
+  __device__ __forceinline__ void scores(const Step<T, D, MANY>& x, int i, f32x4 (&s)[C::KT]) const {
 #pragma unroll
     for (int a = 0; a < C::KT; ++a) {
       s[a] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -374,7 +396,7 @@ struct Share {
     }
   }
 
-  __device__ __forceinline__ bool sees(const Step<T, D>& x, int i, int a, int u) const {
+  __device__ __forceinline__ bool sees(const Step<T, D, MANY>& x, int i, int a, int u) const {
     return x.key0 + 16 * a + 4 * g + u <= t[i] && (x.have >> (4 * a + u)) & 1;
   }
 
@@ -497,7 +519,7 @@ struct Share {
         vo = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.vst;
       }
       const TA_GLOBAL T* kr = kb + ko + g * (D / 4);
-      const TA_GLOBAL T* vr = vb + vo + g * (D / 4);
+      const TA_GLOBAL T* vr = vb + vo;
       float s = 0.0f;
 #pragma unroll 1
       for (int d = 0; d < D / 4; ++d) s = fmaf(to_f32(qr[d]), number(kr + d), s);
@@ -510,7 +532,7 @@ struct Share {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int d = 0; d < C::DJ; ++d) acc[i][d][u] = fmaf(w, number(vr + u * C::DJ + d), acc[i][d][u] * alpha);
+        for (int d = 0; d < C::DJ; ++d) acc[i][d][u] = fmaf(w, number(vr + col(d, u)), acc[i][d][u] * alpha);
     }
   }
 
@@ -529,6 +551,20 @@ struct Share {
       step(x[0]);
       fetch(x[0], at(n + 2), at(n + 3), k0 + (n + 2) * C::KEYS < k1);
       if (k0 + (n + 1) * C::KEYS < k1) step(x[1]);
+    }
+  }
+
+  // The sums over a row's lanes; zeros for rows whose position is outside the cache.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      l[i] = sum_rows(l[i]);
+      if (none >> (kRows * i + c) & 1) {
+        m[i] = kLowest;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      }
     }
   }
 
@@ -568,16 +604,7 @@ struct Share {
         }
         done = 1u << only;
       }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        l[i] = sum_rows(l[i]);
-        if (none >> (kRows * i + c) & 1) {
-          m[i] = kLowest;
-          l[i] = 0.0f;
-#pragma unroll
-          for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        }
-      }
+      finish();
       emit(done);
       want &= ~done;
       if (want == 0) return;
@@ -590,7 +617,294 @@ struct Share {
   }
 
   // The column of acc[.][d][u] in a row.
-  __device__ __forceinline__ int col(int d, int u) const { return C::DJ * (4 * g + u) + d; }
+  __device__ __forceinline__ int col(int d, int u) const { return MANY ? 16 * d + 4 * g + u : C::DJ * (4 * g + u) + d; }
+};
+
+// Many rows, 16 bits: workgroups of four wavefronts with 32 rows each, which share their keys' way through LDS, 64 keys at a
+// time, the next 64 on their way there and those behind them in registers.
+//
+// Bound by instructions: for 32 rows x 32 keys some 115 of the vector units (16 of them exponentials, at a quarter of the rate)
+// beside 28 of the matrix cores, two wavefronts to a SIMD.  So what can goes to the matrix cores (the weights' sums, as a column of
+// ones) and to LDS (values turned round on the way out, where Share takes 16 permutes); scores are not kept for the branch that
+// renews a maximum but made again there; and the two parts of a weight come from one dot product each.  64 keys between two
+// branches, since their chains run beside each other (with 32, three wavefronts to a SIMD spill: 502 us in place of 389).
+//
+// 2 x 12 heads of 64 x 8192 tokens 389 us (530 TFLOP/s of the two products; a wavefront a set 540), 8 x 12 x 2048 116 (165),
+// 2 x 8 heads of 128 x 4096 188 (275; one wavefront to a SIMD, whose 512 registers it needs).
+template <typename T, int D>
+struct Block : Share<T, D, true, 2, false, true> {
+  using S = Share<T, D, true, 2, false, true>;
+  using C = typename S::C;
+  static constexpr int kKeys = 64;
+  static constexpr int PR = D * C::EB / 16;                     // 16-byte pieces of a row
+  static constexpr int NP = kKeys * PR / (kWaves * kWave);      // of K, and of V, a thread
+  static constexpr int LBUF = 2 * kKeys * C::LROW;              // LDS bytes of 64 keys and values
+  using S::acc;
+  using S::c;
+  using S::g;
+  using S::kb;
+  using S::l;
+  using S::lds;
+  using S::m;
+  using S::none;
+  using S::p;
+  f32x4 sums[2];        // the weights' sums, by the matrix cores, in every element
+  using S::seen;
+  using S::t;
+  using S::tab;
+  using S::tmax;
+  using S::tmin;
+  using S::vb;
+  struct Pieces {
+    uint4 k[NP], v[NP];
+    uint32_t ok;        // bit j: keys 32 j ... have a page
+  };
+
+  __device__ __forceinline__ Block(const Dense& p_, int b, int h, int row0, char* lds_, bool one = false, int last = -1)
+      : S(p_, b, h, row0, lds_, one, last) {
+    clear();
+  }
+  __device__ __forceinline__ void clear() { sums[0] = sums[1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f}; }
+
+  // Requests keys key0 .. key0 + 63 (those past k1 or without a page: some row's, which is not used).
+  __device__ __forceinline__ void load(Pieces& x, int key0, int k1) const {
+    const int tid = threadIdx.x;
+    x.ok = 0;
+    int64_t ko[2], vo[2];
+    uint32_t last[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int key = key0 + 32 * j < k1 ? key0 + 32 * j : key0;   // (what stands past k1 no row of the workgroup sees)
+      if (tab) {
+        const int page = tab[key >> p.blog2];
+        const bool ok = page >= 0 && page < p.npages;
+        const int64_t to = (ok ? page : 0) * p.pstride;
+        const int r = key & ((1 << p.blog2) - 1);
+        x.ok |= ok ? 1u << j : 0u;
+        ko[j] = to + r * p.kst;
+        vo[j] = to + r * p.vst;
+        last[j] = 31;
+      } else {
+        x.ok |= 1u << j;
+        ko[j] = key * p.kst;
+        vo[j] = key * p.vst;
+        last[j] = p.Tk - 1 - key < 31 ? p.Tk - 1 - key : 31;
+      }
+    }
+    const uint32_t ks = (uint32_t)p.kst * C::EB, vs = (uint32_t)p.vst * C::EB;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int at = tid + kWaves * kWave * i, row = at / PR;
+      // (32 rows are 32 PR pieces: a wavefront's are of one half)
+      const int j = PR >= 8 ? kWaves * kWave * i / (32 * PR) : __builtin_amdgcn_readfirstlane(row >> 5);
+      const uint32_t r = row & 31, rr = r < last[j] ? r : last[j], o = 16 * (at % PR);
+      x.k[i] = ldg_piece((const TA_GLOBAL char*)(kb + ko[j]) + (rr * ks + o));
+      x.v[i] = ldg_piece((const TA_GLOBAL char*)(vb + vo[j]) + (rr * vs + o));
+    }
+  }
+  static __device__ __forceinline__ uint4 ldg_piece(const TA_GLOBAL char* at) {
+    const u32x4_t r = *(const TA_GLOBAL u32x4_t*)at;
+    return make_uint4(r.x, r.y, r.z, r.w);
+  }
+  __device__ __forceinline__ void put(const Pieces& x, char* buf) const {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int at = threadIdx.x + kWaves * kWave * i;
+      char* to = buf + at / PR * C::LROW + 16 * (at % PR);
+      *reinterpret_cast<uint4*>(to) = x.k[i];
+      *reinterpret_cast<uint4*>(to + kKeys * C::LROW) = x.v[i];
+    }
+  }
+
+  // The weights of all row sets in place of their scores (0 where masked), a row's running maximum renewed when one of its
+  // scores passes it by more than kSlack.  One branch for all sets, so that their products and exponentials stand in one run of
+  // instructions.
+  // again(i, s) gives the scores of set i anew, for that branch.
+  template <bool MASKED, typename F>
+  __device__ __forceinline__ void weights(const Step<T, D, true>& x, f32x4 (&s)[2][C::KT], F again) {
+    const float f = fabsf(p.scale) * kLog2e;   // (a negative scale turns q round: the largest score is the largest product)
+    constexpr float kPast = C::kShift + C::kSlack;
+    float top[2];
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = -INFINITY;
+#pragma unroll
+      for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          s[i][a][u] = fmaf(s[i][a][u], f, -m[i]);   // the exponent; masked: -inf
+          if (MASKED && !this->sees(x, i, a, u)) s[i][a][u] = -INFINITY;
+          top[i] = fmaxf(top[i], s[i][a][u]);
+        }
+      some |= top[i] > kPast;
+    }
+    if (__ballot(some) != 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // only the rows that need it: what a row gives does not depend on the others
+        float mx = kLowest;
+        f32x4 r[C::KT];
+        again(i, r);
+#pragma unroll
+        for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx = s[i][a][u] != -INFINITY ? fmaxf(mx, r[a][u] * f) : mx;
+        mx = max_rows(mx);
+        const float mn = max_rows(top[i]) > kPast ? mx - C::kShift : m[i];
+        const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
+        m[i] = mn;
+        sums[i] *= alpha;
+#pragma unroll
+        for (int d = 0; d < C::DJ; ++d) acc[i][d] *= alpha;
+#pragma unroll
+        for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[i][a][u] = s[i][a][u] != -INFINITY ? fmaf(r[a][u], f, -mn) : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[i][a][u] = __builtin_amdgcn_exp2f(s[i][a][u]);
+  }
+
+  // 64 keys from LDS; bit j of ok: keys 32 j ... have a page.
+  template <bool MASKED>
+  __device__ __forceinline__ void tile(int key0, uint32_t ok, const char* kl, const char* vl) {
+    typedef short s16x4_t __attribute__((ext_vector_type(4)));
+    Step<T, D, true> x;
+    x.key0 = key0;
+    x.have = (ok & 1 ? 0xffu : 0u) | (ok & 2 ? 0xff00u : 0u);
+    auto keys = [&]() {
+#pragma unroll
+      for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+        for (int e = 0; e < C::KS; ++e)
+          x.k[a][e] = *reinterpret_cast<const uint4*>(kl + (16 * a + c) * C::LROW + 64 * e + 16 * g);
+    };
+    keys();
+    f32x4 s[2][C::KT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) this->scores(x, i, s[i]);
+    weights<MASKED>(x, s, [&](int i, f32x4 (&r)[C::KT]) {
+      keys();
+      this->scores(x, i, r);
+    });
+    const char* vrow = vl + (4 * g + (c >> 2)) * C::LROW + 8 * (c & 3);
+#pragma unroll
+    for (int half = 0; half < C::KT / 2; ++half) {
+      uint4 hi[2], lo[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t hw[4], lw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float w0 = s[i][2 * half + e / 2][2 * (e % 2)], w1 = s[i][2 * half + e / 2][2 * (e % 2) + 1];
+          hw[e] = pack2<T>(w0, w1);
+          lw[e] = rest2<T>(w0, w1, hw[e]);
+        }
+        hi[i] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+        lo[i] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+      }
+      // four keys' values of column 16 d + c: four rows of 16 columns, turned round on their way from LDS
+      // (the weights' sums with them: ones in place of values)
+      const uint32_t one = __is_same(T, f16_t) ? 0x3c003c00u : 0x3f803f80u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sums[i] = mfma32<T>(make_uint4(one, one, one, one), hi[i], sums[i]);
+        sums[i] = mfma32<T>(make_uint4(one, one, one, one), lo[i], sums[i]);
+      }
+#pragma unroll
+      for (int d = 0; d < C::DJ; ++d) {
+        uint32_t v[4];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4_t*)(vrow + (32 * half + 16 * a) * C::LROW + 32 * d)));
+          v[2 * a] = r.x;
+          v[2 * a + 1] = r.y;
+        }
+        if constexpr (MASKED) {
+          // values that no query sees count as zeros (0 times what stands there need not be 0)
+          const int end = ok >> half & 1 ? seen : -1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 32 * half + 16 * (e / 2) + 4 * g + 2 * (e % 2);
+            v[e] = key + 1 <= end ? v[e] : key <= end ? v[e] & 0xffffu : 0u;
+          }
+        }
+        const uint4 va = make_uint4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][d] = mfma32<T>(va, hi[i], acc[i][d]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][d] = mfma32<T>(va, lo[i], acc[i][d]);
+      }
+    }
+  }
+
+  // Keys [k0, k1) for the whole workgroup; a wavefront without rows brings its pieces and goes along.
+  __device__ __forceinline__ void pass(int k0, int k1, bool work) {
+    if (k0 >= k1) return;
+    const int n = (k1 - k0 + kKeys - 1) / kKeys;
+    Pieces x;
+    load(x, k0, k1);
+    put(x, lds);
+    uint32_t ok = x.ok;
+    if (n > 1) load(x, k0 + kKeys, k1);
+    lds_barrier();
+    for (int i = 0; i < n; ++i) {
+      const int key0 = k0 + kKeys * i;
+      const char* buf = lds + (i & 1) * LBUF;
+      if (work && key0 <= tmax) {
+        if (ok == 3 && key0 + kKeys - 1 <= (tmin < seen ? tmin : seen)) tile<false>(key0, ok, buf, buf + kKeys * C::LROW);
+        else tile<true>(key0, ok, buf, buf + kKeys * C::LROW);
+      }
+      if (i + 1 < n) {
+        put(x, lds + ((i + 1) & 1) * LBUF);
+        ok = x.ok;
+        if (i + 2 < n) load(x, key0 + 2 * kKeys, k1);
+      }
+      lds_barrier();
+    }
+  }
+
+  // As Share::run, by the whole workgroup until none of its rows is left.
+  template <typename Emit>
+  __device__ __forceinline__ void run(int row0, int b, int h, int k0, int k1, uint32_t want, Emit emit) {
+    int only = -1;
+    while (true) {
+      pass(k0, k1, want != 0);
+      if (want != 0) {
+        uint32_t bad = this->unsound() & want & ~none, done = want & ~bad;
+        // (a lane's part of a sum: the whole of it, in one lane of the row)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) l[i] = g == 0 ? sums[i][0] : 0.0f;
+        if (only >= 0) {
+          if (bad >> only & 1) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (only / kRows == i) this->careful(i, row0, b, h, k0, k1);
+          }
+          done = 1u << only;
+        }
+        this->finish();
+        emit(done);
+        want &= ~done;
+      }
+      if (!__syncthreads_or(want != 0)) return;
+      if (want != 0) {
+        only = __ffs(want) - 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (only / kRows == i) seen = __builtin_amdgcn_readlane(t[i], only % kRows);
+        this->reset();
+        clear();
+      }
+    }
+  }
 };
 
 __device__ __forceinline__ void row_place(const Dense& p, int b, int h, int r, int64_t& out, int64_t& lse) {
@@ -799,18 +1113,17 @@ struct Units {
   }
 };
 
-// Workgroups of four wavefronts, each with a share of one set of 16 NT rows.  A set gets as many as its sequence is long, so that
-// sequences of any lengths end together and few long ones fill the GPU: the fewest units a workgroup with which all sets together
-// need at most nwg of them (as many as run at once: one more costs a round of its own), and a set at most `top` (what joins them
-// is one workgroup).  The grid has nwg or as many as there are sets; those that are left over leave at once.
-template <typename T, int D, bool WIDE, int NT, bool STREAM>
-__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg, int top) {
-  extern __shared__ __align__(16) float smem[];
-  constexpr int KEYS = Tile<T, D>::KEYS;
-  constexpr int kSet = kRows * NT;
-  TA_DMARK(0);
-  const int sets = (p.R + kSet - 1) / kSet;      // of a (sequence, key head)
-  const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
+// A workgroup's part: keys [k0, k1) (before the end that its rows see) of set `set` of (b, h), part `part` of `count`; wg: its
+// place among all, in: the set's among those of its sequence; last: the sequence's last position.
+struct Part {
+  int b, h, set, in, part, count, wg, last, k0, k1;
+};
+
+// A set gets as many workgroups as its sequence is long, so that sequences of any lengths end together and few long ones fill
+// the GPU: the fewest units a workgroup with which all sets together need at most nwg of them (as many as run at once: one
+// more costs a round of its own), and a set at most `top` (what joins them is one workgroup).  The grid has nwg or as many as
+// there are sets; those that are left over leave at once (false).  sets: of a (sequence, key head).
+__device__ __forceinline__ bool find_part(const Dense& p, int sets, int nwg, int top, Part& r) {
   const int per = p.H * sets;                    // sets of a sequence (all units: fewer than 2^31)
   const Units units(p);
   int all = 0, longest = 0;
@@ -836,7 +1149,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
     // sets of one key head share its keys: the workgroups in use next to each other are those of one XCD (they go round robin
     // over the 8; the grid is a multiple of 8)
     const int each = ceil_div(units.parts(most) * per, 8);
-    if (wg / 8 >= each) return;
+    if (wg / 8 >= each) return false;
     wg = wg % 8 * each + wg / 8;
   }
   // its sequence, and the workgroups of that one's sets
@@ -857,19 +1170,39 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
     start += (__builtin_amdgcn_readlane(sum, i) - count) * per;
     return false;
   });
-  if (b < 0) return;
-  const int in = (wg - start) / count;           // set of the sequence
-  const int part = wg - start - in * count;
-  const int h = sets > 1 ? in / sets : in, row0 = sets > 1 ? (in - h * sets) * kSet : 0;
+  if (b < 0) return false;
+  r.b = b;
+  r.count = count;
+  r.wg = wg;
+  r.last = last;
+  r.in = (wg - start) / count;
+  r.part = wg - start - r.in * count;
+  r.h = sets > 1 ? r.in / sets : r.in;
+  r.set = sets > 1 ? r.in - r.h * sets : 0;
+  const int mine = (int)((unsigned)ub / (unsigned)count), more = ub - mine * count;
+  const int first = r.part * mine + (r.part < more ? r.part : more);
+  r.k0 = first * kQuantum;
+  r.k1 = (first + mine + (r.part < more ? 1 : 0)) * kQuantum;
+  return true;
+}
+
+// Workgroups of four wavefronts, each with a share of one set of 16 NT rows (find_part).
+template <typename T, int D, bool WIDE, int NT, bool STREAM>
+__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg, int top) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int KEYS = Tile<T, D>::KEYS;
+  constexpr int kSet = kRows * NT;
+  TA_DMARK(0);
+  const int sets = (p.R + kSet - 1) / kSet;      // of a (sequence, key head)
+  const int w = __builtin_amdgcn_readfirstlane(wave_id()), tid = threadIdx.x;
+  Part at;
+  if (!find_part(p, sets, nwg, top, at)) return;
+  const int b = at.b, h = at.h, row0 = at.set * kSet;
   const int rows = p.R - row0 < kSet ? p.R - row0 : kSet;
-  Share<T, D, WIDE, NT, STREAM> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, last);
+  Share<T, D, WIDE, NT, STREAM> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, at.last);
   // its keys, and the equal runs of whole steps of its wavefronts
   const int nkeys = s.tmax + 1;
-  const int mine = (int)((unsigned)ub / (unsigned)count), more = ub - mine * count;
-  const int first = part * mine + (part < more ? part : more);
-  int k0 = first * kQuantum, k1 = (first + mine + (part < more ? 1 : 0)) * kQuantum;
-  k0 = k0 < nkeys ? k0 : nkeys;
-  k1 = k1 < nkeys ? k1 : nkeys;
+  const int k0 = at.k0 < nkeys ? at.k0 : nkeys, k1 = at.k1 < nkeys ? at.k1 : nkeys;
   int run = (k1 - k0 + kWaves - 1) / kWaves + KEYS - 1;
   run -= run % KEYS;
   const int from = k0 + w * run < k1 ? k0 + w * run : k1, to = from + run < k1 ? from + run : k1;
@@ -893,7 +1226,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   });
   TA_DMARK(2);
   __syncthreads();
-  float* ws = p.ws + (int64_t)wg * kSet * (D + 2);
+  float* ws = p.ws + (int64_t)at.wg * kSet * (D + 2);
   for (int i = tid; i < rows * D; i += kWaves * kWave) {
     const int r = i / D, d = i % D;
     float M = kLowest, L = 0.0f, a = 0.0f;
@@ -911,10 +1244,10 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
         a = fmaf(q[2 + d], f, a);
       }
     }
-    if (count == 1) {
-      int64_t at, le;
-      row_place(p, b, h, row0 + r, at, le);
-      reinterpret_cast<T*>(p.out)[at + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
+    if (at.count == 1) {
+      int64_t to, le;
+      row_place(p, b, h, row0 + r, to, le);
+      reinterpret_cast<T*>(p.out)[to + d] = from_f32<T>(L != 0.0f ? a / L : 0.0f);
       if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
     } else {
       stgf_dc(ws + r * (D + 2) + 2 + d, a);
@@ -924,7 +1257,44 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
       }
     }
   }
-  if (count > 1) join_parts<T, D, kSet>(p, b, h, row0, rows, b * per + in, wg - part, count, smem);
+  if (at.count > 1) join_parts<T, D, kSet>(p, b, h, row0, rows, b * p.H * sets + at.in, at.wg - at.part, at.count, smem);
+}
+
+// A workgroup a set of 128 rows, four wavefronts with 32 rows each over the same keys (Block), no split.  The longest sets
+// first: 2 x 12 heads x 8192 tokens 403 us so, 470 a key head at a time.
+constexpr int kBlock = kWaves * 2 * kRows;
+template <typename T, int D>
+__global__ __launch_bounds__(kWaves * kWave, D == 128 ? 1 : 2) void dense_block_kernel(Dense p) {
+  using S = Block<T, D>;
+  __shared__ __align__(16) char smem[2 * S::LBUF];
+  // (the last rows of a prompt see the most; the sets of a key head go to one XCD where there are a multiple of 8 of these)
+  const int sets = (p.R + kBlock - 1) / kBlock, rank = blockIdx.x / p.BH, bh = blockIdx.x - rank * p.BH;
+  const int b = bh / p.H, h = bh - b * p.H, w = __builtin_amdgcn_readfirstlane(wave_id());
+  const int row0 = (sets - 1 - rank) * kBlock + w * 2 * kRows;
+  S s(p, b, h, row0, smem);
+  int* const ends = reinterpret_cast<int*>(smem);
+  if (s.lane == 0) ends[w] = s.tmax + 1;
+  __syncthreads();
+  const int nkeys = __builtin_amdgcn_readfirstlane(max(max(ends[0], ends[1]), max(ends[2], ends[3])));
+  __syncthreads();
+  const int left = p.R - row0;
+  const uint32_t want = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1 : 0u;
+  s.run(row0, b, h, 0, nkeys, want, [&](uint32_t done) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = kRows * i + s.c;
+      if (!(done >> r & 1)) continue;
+      int64_t at, le;
+      row_place(p, b, h, row0 + r, at, le);
+      T* o = reinterpret_cast<T*>(p.out) + at;
+      const float inv = s.l[i] != 0.0f ? 1.0f / s.l[i] : 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[s.col(d, u)] = from_f32<T>(s.acc[i][d][u] * inv);
+      if (s.g == 0 && p.lse) p.lse[le] = lse_of(s.m[i], s.l[i]);
+    }
+  });
 }
 
 // Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level cache
@@ -965,8 +1335,20 @@ int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
 template <typename T, int D>
 constexpr int two_tiles() { return sizeof(T) == 2 && D < 128 ? 2 : 1; }
 
+template <typename T, int D>
+int block_dense(const Dense& p, hipStream_t st) {
+  const int64_t wgs = p.BH * ((p.R + kBlock - 1) / kBlock);
+  hipLaunchKernelGGL((dense_block_kernel<T, D>), dim3((unsigned)wgs), dim3(kWaves * kWave), 0, st, p);
+  return check_launch("dense_block_kernel");
+}
+
 template <typename T, int D, bool WIDE>
 int rows_dense(const Dense& p, int nsplit, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && WIDE && D >= 32)
+    // (a workgroup a set of 128 rows; 24 heads x 1024 tokens, 192 workgroups, 28.8 us and 31.1 a wavefront a set, 8 heads of
+    // 128 x 2048, 128 of them, 89 and 78; caches of 128 keys 12.8 and 10.7, of 512 20.0 and 24.0; 64 rows over 4000 keys 94 and 114)
+    if (nsplit == 1 && p.R >= 64 && p.Tk >= 512 && p.BH * (((int64_t)p.R + kBlock - 1) / kBlock) >= 192)
+      return block_dense<T, D>(p, st);
   if constexpr (two_tiles<T, D>() == 2)
     if (p.R > kRows) return launch_dense<T, D, WIDE, 2>(p, nsplit, st);
   return launch_dense<T, D, WIDE, 1>(p, nsplit, st);

@@ -593,10 +593,11 @@ def decode_nsplit_dense(B, H, rows, keys, D=64):
     over at the end is little (144 sets 92 us with 720 and 126 with 144, 192 sets 118 and 132, 384 sets over 32768 keys 439 and
     521), where each has 16 units of 128 keys or more (384 sets over 500 keys 14 us with 384 and 21 with 768).  Rows of prompts,
     more than 16: at most 512 (192 sets of 32 rows over 8000 keys 58 us with 384, 66 with 192, 70 with 576), and from 1024 sets on
-    a wavefront a set (16 heads of 128 x 4096 tokens 275 us so, 379 with a workgroup a set)."""
+    no split (16 heads of 128 x 4096 tokens 188 us so, 379 with four wavefronts a set); from 768 on where the rows see about half
+    of the keys (24 heads x 1024 tokens 29 us so, 41 with four wavefronts a set; 256 rows behind 8000 tokens 186 and 150)."""
     sets = max(1, B * H * ((rows + 31) // 32 if rows > 16 else 1))
     units = (max(1, keys) + 127) // 128
-    if sets >= (1024 if rows > 16 else 4096):
+    if sets >= (1024 if rows > 16 else 4096) or (rows > 16 and sets >= 768 and keys <= 2 * rows):
         return 1
     if sets <= 256 and 256 // sets * sets >= 218:
         parts = 256 // sets
