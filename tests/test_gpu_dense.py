@@ -379,8 +379,9 @@ def some_rows(out, lse, q, k, v, tq, scale, pairs, dtype, at, have=None):
 @pytest.mark.parametrize('dtype', [F16, BF16])
 @pytest.mark.parametrize('D,leaf,H,G,N,T', [(64, 64, 12, 1, 1000, 1003), (128, 32, 8, 3, 500, 513), (32, 128, 12, 1, 1024, 1024),
                                             (64, 0, 12, 1, 901, 929), (128, 0, 12, 1, 1000, 1001), (32, 0, 3, 65, 63, 640),
-                                            (64, 64, 96, 1, 65, 577)])
-def test_many_rows(dtype, D, leaf, H, G, N, T):
+                                            (64, 64, 96, 1, 100, 577)])
+@pytest.mark.parametrize('nsplit', [1, 132, 1024, 2600])
+def test_many_rows(dtype, D, leaf, H, G, N, T, nsplit):
     """Prompts and pieces of them, their positions in any order, some outside the cache; contiguous caches that end inside a
     tile; last sets with wavefronts that have no rows."""
     B = 2
@@ -402,12 +403,12 @@ def test_many_rows(dtype, D, leaf, H, G, N, T):
         c = wide[0].copy_(k), wide[1].copy_(v)
     scale = 1 / math.sqrt(D)
     lse = torch.empty(B, G * H, N, device=DEV)
-    out, _ = K.dense_attn(q.to(DEV), *c, tq.to(DEV), scale, lse=lse, nsplit=1)
+    out, _ = K.dense_attn(q.to(DEV), *c, tq.to(DEV), scale, lse=lse, nsplit=nsplit)
     at = torch.unique(torch.cat([torch.arange(0, N, max(1, N // 12)), torch.tensor([N - 1, N - 2]),
                                  torch.randint(0, N, (8,), generator=g)]))
     some_rows(out, lse, q, k, v, tq, scale, [(0, 0), (1, G * H - 1), (1, G)], dtype, at, have)
     # the same whatever the other rows are: each sequence by itself, with other tokens before and after
-    same, _ = K.dense_attn(q.to(DEV).flip(2), *c, tq.to(DEV).flip(1), scale, nsplit=1)
+    same, _ = K.dense_attn(q.to(DEV).flip(2), *c, tq.to(DEV).flip(1), scale, nsplit=nsplit)
     far = (torch.arange(B * G * H * N * D) % 7 == 0).view(B, G * H, N, D)
     a, b = out.cpu()[far].double(), same.flip(2).cpu()[far].double()
     assert bool(((a - b).abs() <= 2 * torch.finfo(dtype).eps * a.abs() + 1e-3).all())
@@ -415,20 +416,21 @@ def test_many_rows(dtype, D, leaf, H, G, N, T):
 
 @pytest.mark.parametrize('dtype', [F16, BF16])
 @pytest.mark.parametrize('D', [64, 128])
-def test_many_rows_what_is_masked(dtype, D):
+@pytest.mark.parametrize('nsplit', [1, 1600])
+def test_many_rows_what_is_masked(dtype, D, nsplit):
     """A value that some rows of a tile see and others do not: only those that see it show it, the others' bits stay; also
     where it is the key."""
     B, H, N, T = 4, 12, 500, 600
     k, v = rnd(B, H, T, D, seed=41, dtype=dtype).to(DEV), rnd(B, H, T, D, seed=42, dtype=dtype).to(DEV)
     q = rnd(B, H, N, D, seed=43, dtype=dtype).to(DEV)
     tq = rows([T, T, T - 7, N], N).to(DEV)
-    clean, _ = K.dense_attn(q, k, v, tq, nsplit=1)
+    clean, _ = K.dense_attn(q, k, v, tq, nsplit=nsplit)
     for bad in (float('inf'), float('nan'), torch.finfo(dtype).min):
         for which in (0, 1):
             x = [k.clone(), v.clone()]
             for b, h, t in ((0, 0, T - 5), (1, 3, 330), (2, 11, T - 1), (3, 0, 70)):
                 x[which][b, h, t, 5] = bad
-            got, _ = K.dense_attn(q, *x, tq, nsplit=1)
+            got, _ = K.dense_attn(q, *x, tq, nsplit=nsplit)
             for b, h, t in ((0, 0, T - 5), (1, 3, 330), (2, 11, T - 1), (3, 0, 70)):
                 blind = tq[b] < t
                 assert torch.equal(got[b, h, blind], clean[b, h, blind]), (bad, which, b)
@@ -454,19 +456,27 @@ def test_many_rows_extreme_scores_and_replays():
             some_rows(out, None, -q.cpu(), k.cpu(), v.cpu(), tq.cpu(), -scale, [(0, 0), (3, 11)], BF16, at)
         else:
             some_rows(out, None, q.cpu(), k.cpu(), v.cpu(), tq.cpu(), scale, [(0, 0), (3, 11)], BF16, at)
-    out = torch.empty_like(q)
-    s = torch.cuda.Stream()
-    s.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(s):
-        K.dense_attn(q, k, v, tq, out=out, nsplit=1)
-    torch.cuda.current_stream().wait_stream(s)
-    g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g, stream=s):
-        K.dense_attn(q, k, v, tq, out=out, nsplit=1)
-    for i in range(3):
-        q.copy_(rnd(B, H, N, D, seed=60 + i, dtype=BF16).to(DEV))
-        tq.copy_(rows([T - i, 600, N, 513 + i], N).to(DEV))
-        g.replay()
-        want, _ = K.dense_attn(q, k, v, tq, nsplit=1)
-        assert torch.equal(out, want)
-        torch.cuda.synchronize()
+    # one workspace for two calls of a graph and for eager ones between its replays, also of another cache's kind
+    small = paged(k[:, :, :400].cpu(), v[:, :, :400].cpu(), 8)
+    for nsplit in (1, 1024):
+        ws = K.dense_attn_workspace(B, H, N, D, nsplit, DEV, H)
+        out, two = torch.empty_like(q), torch.empty_like(q)
+
+        def calls():
+            K.dense_attn(q, k, v, tq, out=out, nsplit=nsplit, ws=ws)
+            K.dense_attn(q, small, None, tq, out=two, nsplit=nsplit, ws=ws)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            calls()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            calls()
+        for i in range(3):
+            q.copy_(rnd(B, H, N, D, seed=60 + i, dtype=BF16).to(DEV))
+            tq.copy_(rows([T - i, 600, N, 513 + i], N).to(DEV))
+            g.replay()
+            assert torch.equal(out, K.dense_attn(q, k, v, tq, nsplit=nsplit, ws=ws)[0])
+            assert torch.equal(two, K.dense_attn(q, small, None, tq, nsplit=nsplit)[0])
+            torch.cuda.synchronize()

@@ -55,6 +55,7 @@ struct Dense {
   int B;
   float* ws;            // parts (workgroup, row, D + 2) and
   uint32_t* cnt;        // arrival counters of the sets (zero between calls)
+  int2* heads;          // of many rows' sets: the first part, and how many
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -1260,41 +1261,112 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   if (at.count > 1) join_parts<T, D, kSet>(p, b, h, row0, rows, b * p.H * sets + at.in, at.wg - at.part, at.count, smem);
 }
 
-// A workgroup a set of 128 rows, four wavefronts with 32 rows each over the same keys (Block), no split.  The longest sets
-// first: 2 x 12 heads x 8192 tokens 403 us so, 470 a key head at a time.
+// Workgroups of four wavefronts with 32 rows each of a set of 128, all over the same keys (Block).  nwg 0: one a set, the longest
+// sets first: 2 x 12 heads x 8192 tokens 403 us so, 470 a key head at a time.  Else a set's keys are split (find_part) and its
+// parts joined by a launch of its own (dense_join_kernel): 128 rows are too many for the workgroup that comes last.  2 x 12 heads
+// x 256 rows over 8000 keys 50 us (60 by sets of 32 rows; 88 and more with the last workgroup's join).
 constexpr int kBlock = kWaves * 2 * kRows;
+constexpr int kManyRows = 96;
 template <typename T, int D>
-__global__ __launch_bounds__(kWaves * kWave, D == 128 ? 1 : 2) void dense_block_kernel(Dense p) {
+__global__ __launch_bounds__(kWaves * kWave, D == 128 ? 1 : 2) void dense_block_kernel(Dense p, int nwg) {
   using S = Block<T, D>;
   __shared__ __align__(16) char smem[2 * S::LBUF];
-  // (the last rows of a prompt see the most; the sets of a key head go to one XCD where there are a multiple of 8 of these)
-  const int sets = (p.R + kBlock - 1) / kBlock, rank = blockIdx.x / p.BH, bh = blockIdx.x - rank * p.BH;
-  const int b = bh / p.H, h = bh - b * p.H, w = __builtin_amdgcn_readfirstlane(wave_id());
-  const int row0 = (sets - 1 - rank) * kBlock + w * 2 * kRows;
+  const int sets = (p.R + kBlock - 1) / kBlock, w = __builtin_amdgcn_readfirstlane(wave_id());
+  Part at;
+  if (nwg > 0) {
+    if (!find_part(p, sets, nwg, 1 << 20, at)) return;
+    if (at.part == 0 && threadIdx.x == 0) {
+      p.heads[(int64_t)at.b * p.H * sets + at.in] = make_int2(at.wg, at.count);
+    }
+  } else {
+    // (the last rows of a prompt see the most; the sets of a key head go to one XCD where there are a multiple of 8 of these)
+    const int rank = blockIdx.x / p.BH, bh = blockIdx.x - rank * p.BH, b = bh / p.H;
+    at = Part{b, bh - b * p.H, sets - 1 - rank, 0, 0, 1, 0, -1, 0, 0x7fffffff};
+  }
+  const int b = at.b, h = at.h, row0 = at.set * kBlock + w * 2 * kRows;
   S s(p, b, h, row0, smem);
   int* const ends = reinterpret_cast<int*>(smem);
   if (s.lane == 0) ends[w] = s.tmax + 1;
   __syncthreads();
   const int nkeys = __builtin_amdgcn_readfirstlane(max(max(ends[0], ends[1]), max(ends[2], ends[3])));
   __syncthreads();
+  const int k0 = at.k0 < nkeys ? at.k0 : nkeys, k1 = at.k1 < nkeys ? at.k1 : nkeys;
   const int left = p.R - row0;
   const uint32_t want = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1 : 0u;
-  s.run(row0, b, h, 0, nkeys, want, [&](uint32_t done) {
+  const bool whole = at.count == 1;
+  float* const part = p.ws + ((int64_t)at.wg * kBlock + w * 2 * kRows) * (D + 4);
+  s.run(row0, b, h, k0, k1, want, [&](uint32_t done) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = kRows * i + s.c;
       if (!(done >> r & 1)) continue;
-      int64_t at, le;
-      row_place(p, b, h, row0 + r, at, le);
-      T* o = reinterpret_cast<T*>(p.out) + at;
-      const float inv = s.l[i] != 0.0f ? 1.0f / s.l[i] : 0.0f;
+      if (whole) {
+        int64_t to, le;
+        row_place(p, b, h, row0 + r, to, le);
+        T* o = reinterpret_cast<T*>(p.out) + to;
+        const float inv = s.l[i] != 0.0f ? 1.0f / s.l[i] : 0.0f;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d)
+        for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) o[s.col(d, u)] = from_f32<T>(s.acc[i][d][u] * inv);
-      if (s.g == 0 && p.lse) p.lse[le] = lse_of(s.m[i], s.l[i]);
+          for (int u = 0; u < 4; ++u) o[s.col(d, u)] = from_f32<T>(s.acc[i][d][u] * inv);
+        if (s.g == 0 && p.lse) p.lse[le] = lse_of(s.m[i], s.l[i]);
+      } else {
+        float* o = part + r * (D + 4);
+        if (s.g == 0) *reinterpret_cast<float2*>(o) = make_float2(s.m[i], s.l[i]);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(o + 4 + s.col(d, 0)) = s.acc[i][d];
+      }
     }
   });
+}
+
+// The parts of dense_block_kernel's rows joined, D / 4 threads a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dense_join_kernel(Dense p) {
+  constexpr int kPer = 256 / (D / 4);            // rows a workgroup
+  const int sets = (p.R + kBlock - 1) / kBlock;
+  const int per = (p.R + kPer - 1) / kPer;
+  const int bh = blockIdx.x / per, row = (blockIdx.x - bh * per) * kPer + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  if (row >= p.R) return;
+  const int b = bh / p.H, h = bh - b * p.H, set = row / kBlock;
+  const int2 head = p.heads[(int64_t)bh * sets + set];
+  if (head.y == 1) return;                       // (written by its only workgroup)
+  const float* q = p.ws + ((int64_t)head.x * kBlock + row - set * kBlock) * (D + 4);
+  const int64_t step = (int64_t)kBlock * (D + 4);
+  float M = kLowest, L = 0.0f;
+  f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = 0; k0 < head.y; k0 += 8) {
+    float2 ml[8];
+    f32x4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float* x = q + (k0 + k < head.y ? k0 + k : 0) * step;
+      ml[k] = *reinterpret_cast<const float2*>(x);
+      v[k] = *reinterpret_cast<const f32x4*>(x + 4 + d);
+      if (k0 + k >= head.y) ml[k].y = 0.0f;
+    }
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mn = ml[k].y != 0.0f ? fmaxf(mn, ml[k].x) : mn;
+    const float alpha = __builtin_amdgcn_exp2f(M - mn);
+    M = mn;
+    L *= alpha;
+    a *= alpha;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (ml[k].y != 0.0f) {
+        const float f = __builtin_amdgcn_exp2f(ml[k].x - M);
+        L = fmaf(ml[k].y, f, L);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a[u] = fmaf(v[k][u], f, a[u]);
+      }
+    }
+  }
+  int64_t at, le;
+  row_place(p, b, h, row, at, le);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) reinterpret_cast<T*>(p.out)[at + d + u] = from_f32<T>(L != 0.0f ? a[u] / L : 0.0f);
+  if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
 }
 
 // Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level cache
@@ -1336,10 +1408,17 @@ template <typename T, int D>
 constexpr int two_tiles() { return sizeof(T) == 2 && D < 128 ? 2 : 1; }
 
 template <typename T, int D>
-int block_dense(const Dense& p, hipStream_t st) {
-  const int64_t wgs = p.BH * ((p.R + kBlock - 1) / kBlock);
-  hipLaunchKernelGGL((dense_block_kernel<T, D>), dim3((unsigned)wgs), dim3(kWaves * kWave), 0, st, p);
-  return check_launch("dense_block_kernel");
+int block_dense(const Dense& p, int nsplit, hipStream_t st) {
+  const int64_t sets = p.BH * (((int64_t)p.R + kBlock - 1) / kBlock);
+  const int nwg = nsplit > kWaves ? nsplit / kWaves : 0;
+  const int64_t wgs = nwg < sets ? sets : nwg;
+  hipLaunchKernelGGL((dense_block_kernel<T, D>), dim3((unsigned)(nwg > 0 ? (wgs + 7) / 8 * 8 : wgs)), dim3(kWaves * kWave), 0, st, p,
+                     nwg);
+  const int rc = check_launch("dense_block_kernel");
+  if (rc != TA_OK || nwg <= sets) return rc;     // (no set has more than one)
+  constexpr int kPer = 256 / (D / 4);
+  hipLaunchKernelGGL((dense_join_kernel<T, D>), dim3((unsigned)(p.BH * (((int64_t)p.R + kPer - 1) / kPer))), dim3(256), 0, st, p);
+  return check_launch("dense_join_kernel");
 }
 
 template <typename T, int D, bool WIDE>
@@ -1347,8 +1426,9 @@ int rows_dense(const Dense& p, int nsplit, hipStream_t st) {
   if constexpr (sizeof(T) == 2 && WIDE && D >= 32)
     // (a workgroup a set of 128 rows; 24 heads x 1024 tokens, 192 workgroups, 28.8 us and 31.1 a wavefront a set, 8 heads of
     // 128 x 2048, 128 of them, 89 and 78; caches of 128 keys 12.8 and 10.7, of 512 20.0 and 24.0; 64 rows over 4000 keys 94 and 114)
-    if (nsplit == 1 && p.R >= 64 && p.Tk >= 512 && p.BH * (((int64_t)p.R + kBlock - 1) / kBlock) >= 192)
-      return block_dense<T, D>(p, st);
+    if (nsplit != kWaves && p.R >= kManyRows && p.Tk >= 512 &&
+        (nsplit > 1 || p.BH * (((int64_t)p.R + kBlock - 1) / kBlock) >= 192))
+      return block_dense<T, D>(p, nsplit, st);
   if constexpr (two_tiles<T, D>() == 2)
     if (p.R > kRows) return launch_dense<T, D, WIDE, 2>(p, nsplit, st);
   return launch_dense<T, D, WIDE, 1>(p, nsplit, st);
@@ -1379,14 +1459,18 @@ int64_t dense_sets(int B, int Hq, int H, int Nq) {
   const int64_t R = (int64_t)(Hq / H) * Nq;
   return (int64_t)B * H * (R <= 16 ? 1 : (R + 31) / 32 * 2);
 }
+// Bytes of the counters, and of the heads of a quarter as many sets or fewer behind them.
+int64_t counter_bytes(int64_t sets) { return (sets * 4 + 255) / 256 * 256 * 2; }
 }  // namespace
 }  // namespace ta
 
 extern "C" int64_t ta_dense_attn_workspace_size(int B, int Hq, int H, int Nq, int D, int nsplit) {
   if (B <= 0 || H <= 0 || Hq <= 0 || Nq <= 0 || nsplit <= 4) return 0;
   const int64_t sets = dense_sets(B, Hq, H, Nq);
-  // a part for each workgroup and each set, of 16 rows, or of 32 for half as many sets
-  return (sets * 4 + 255) / 256 * 256 + (sets + nsplit / 2) * 16 * (D + 2) * 4;
+  // counters; heads; a part for each workgroup and each set, of 16 rows, or of 32 or 128 for fewer sets
+  const int64_t R = (int64_t)(Hq / H) * Nq, rows = R < kManyRows ? 32 : kBlock;
+  const int64_t all = R < kManyRows ? sets * 16 : (int64_t)B * H * ((R + kBlock - 1) / kBlock * kBlock);
+  return counter_bytes(sets) + (all + nsplit / 4 * rows) * (D + 4) * 4;
 }
 
 extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, int dtype, int64_t qsb, int64_t qsh,
@@ -1457,7 +1541,8 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
   p.B = B;
   if (need > 0) {
     p.cnt = reinterpret_cast<uint32_t*>(ws);
-    p.ws = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + (sets * 4 + 255) / 256 * 256);
+    p.heads = reinterpret_cast<int2*>(reinterpret_cast<char*>(ws) + counter_bytes(sets) / 2);
+    p.ws = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + counter_bytes(sets));
   }
   hipStream_t st = (hipStream_t)stream;
   if (dtype == TA_F32) return dispatch_dense<float>(p, nsplit, st);

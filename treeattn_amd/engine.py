@@ -592,12 +592,17 @@ def decode_nsplit_dense(B, H, rows, keys, D=64):
     of 64, 192 workgroups 67 us and 256, some of them two to a unit, 87).  Else about 768, so that what the units have left
     over at the end is little (144 sets 92 us with 720 and 126 with 144, 192 sets 118 and 132, 384 sets over 32768 keys 439 and
     521), where each has 16 units of 128 keys or more (384 sets over 500 keys 14 us with 384 and 21 with 768).  Rows of prompts,
-    more than 16: at most 512 (192 sets of 32 rows over 8000 keys 58 us with 384, 66 with 192, 70 with 576), and from 1024 sets on
-    no split (16 heads of 128 x 4096 tokens 188 us so, 379 with four wavefronts a set); from 768 on where the rows see about half
-    of the keys (24 heads x 1024 tokens 29 us so, 41 with four wavefronts a set; 256 rows behind 8000 tokens 186 and 150)."""
+    more than 16: at most 512, and from 1024 sets of 32 rows on no split (16 heads of 128 x 4096 tokens 188 us so, 379 with four
+    wavefronts a set); from 768 on where the rows see about half of the keys (24 heads x 1024 tokens 29 us so, 41 with four
+    wavefronts a set).
+
+    From 96 rows on a workgroup takes 128 of them (16 bits): as many as run at once, two to a compute unit (one with heads of 128),
+    with four units each or more, or as few as give 192 workgroups (24 heads x 256 rows behind 8000 tokens 46 us with 480, 54 with
+    240; 12 heads x 128 behind 1000 16.5 with 108, 20.4 with 48).  256 sets of 32 rows over fewer than 32 units: four wavefronts a
+    set (12 heads x 1024 rows behind 1000 tokens 34 us so, 36 with 480 workgroups)."""
     sets = max(1, B * H * ((rows + 31) // 32 if rows > 16 else 1))
     units = (max(1, keys) + 127) // 128
-    if sets >= (1024 if rows > 16 else 4096) or (rows > 16 and sets >= 768 and keys <= 2 * rows):
+    if sets >= (1024 if rows > 16 else 4096) or (rows > 16 and sets >= 768 and keys <= rows):
         return 1
     if sets <= 256 and 256 // sets * sets >= 218:
         parts = 256 // sets
@@ -605,7 +610,12 @@ def decode_nsplit_dense(B, H, rows, keys, D=64):
         parts = max(1, 512 // sets) if rows > 16 else -(-768 // sets)
         if units < 16 * parts:
             parts = max(1, 256 // sets)
-    return 4 if parts == 1 or units == 1 else 4 * parts * sets
+    n = 4 if parts == 1 or units == 1 else 4 * parts * sets
+    if rows >= 96 and not (sets >= 256 and units < 32):
+        many = B * H * ((rows + 127) // 128)
+        parts = min((256 if D == 128 else 512) // many, max(units // 4, min(units, 192 // many)))
+        n = max(n, 4 * parts * many) if parts > 1 else n
+    return n
 
 
 def _budget_weights(state, pw):
