@@ -18,11 +18,11 @@
 // than kSlack: until then weights are at most 2^kSlack.
 //
 // Bound by bytes, 2 D a key and key head, where rows are few; the keys of a sequence are split over wavefronts and
-// workgroups, whose partial results the last workgroup to arrive joins.  32 x 12 queries over 32768 keys of 64: 440 us, 6.4 TB/s;
-// one sequence of 131000: 62 us, 5.6 TB/s.  Rows of prompts, by the hundred, share their keys through LDS (Block).
+// workgroups, whose partial results the last workgroup to arrive joins.  32 x 12 queries over 32768 keys of 64: 440 us, 6.4
+// TB/s; one sequence of 131000: 62 us, 5.6 TB/s.  Rows of prompts, by the hundred, share their keys through LDS (Block).
 //
-// Phase marks (trace.hpp): 0 start, 1 its part and queries are known, 2 its keys are done, 3 its part is written, 4 it is counted
-// in, 5 the set is joined.
+// Phase marks (trace.hpp): 0 start, 1 its part and queries are known, 2 its keys are done, 3 its part is written, 4 it is
+// counted in, 5 the set is joined.
 //
 // Reference functions replaced: engine.py:74-81 (DenseState.attend).
 #include "attn.hpp"
@@ -587,10 +587,10 @@ struct Share {
 
   // Keys [k0, k1) for the rows of `want`; emit(mask) takes the results of some rows at a time.
   //
-  // A value that is infinite or NaN reaches, in the matrix instructions, rows that do not see its key (as 0 times it), and comes
-  // as a sum of two products (which may be inf - inf).  So a row whose result is not finite goes through its keys again by
-  // itself, values that it does not see taken as zeros (the same sums as if they had been finite); one that is still not finite
-  // goes through them without matrix instructions.
+  // A value that is infinite or NaN reaches, in the matrix instructions, rows that do not see its key (as 0 times it), and
+  // comes as a sum of two products (which may be inf - inf).  So a row whose result is not finite goes through its keys again
+  // by itself, values that it does not see taken as zeros (the same sums as if they had been finite); one that is still not
+  // finite goes through them without matrix instructions.
   template <typename Emit>
   __device__ __forceinline__ void run(int row0, int b, int h, int k0, int k1, uint32_t want, Emit emit) {
     int only = -1;
@@ -625,10 +625,11 @@ struct Share {
 // time, the next 64 on their way there and those behind them in registers.
 //
 // Bound by instructions: for 32 rows x 32 keys some 115 of the vector units (16 of them exponentials, at a quarter of the rate)
-// beside 28 of the matrix cores, two wavefronts to a SIMD.  So what can goes to the matrix cores (the weights' sums, as a column of
-// ones) and to LDS (values turned round on the way out, where Share takes 16 permutes); scores are not kept for the branch that
-// renews a maximum but made again there; and the two parts of a weight come from one dot product each.  64 keys between two
-// branches, since their chains run beside each other (with 32, three wavefronts to a SIMD spill: 502 us in place of 389).
+// beside 28 of the matrix cores, two wavefronts to a SIMD.  So what can goes to the matrix cores (the weights' sums, as a
+// column of ones) and to LDS (values turned round on the way out, where Share takes 16 permutes); scores are not kept for the
+// branch that renews a maximum but made again there; and the two parts of a weight come from one dot product each.  64 keys
+// between two branches, since their chains run beside each other (with 32, three wavefronts to a SIMD spill: 502 us in place
+// of 389).
 //
 // 2 x 12 heads of 64 x 8192 tokens 389 us (530 TFLOP/s of the two products; a wavefront a set 540), 8 x 12 x 2048 116 (165),
 // 2 x 8 heads of 128 x 4096 188 (275; one wavefront to a SIMD, whose 512 registers it needs).
@@ -1261,10 +1262,10 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   if (at.count > 1) join_parts<T, D, kSet>(p, b, h, row0, rows, b * p.H * sets + at.in, at.wg - at.part, at.count, smem);
 }
 
-// Workgroups of four wavefronts with 32 rows each of a set of 128, all over the same keys (Block).  nwg 0: one a set, the longest
-// sets first: 2 x 12 heads x 8192 tokens 403 us so, 470 a key head at a time.  Else a set's keys are split (find_part) and its
-// parts joined by a launch of its own (dense_join_kernel): 128 rows are too many for the workgroup that comes last.  2 x 12 heads
-// x 256 rows over 8000 keys 50 us (60 by sets of 32 rows; 88 and more with the last workgroup's join).
+// Workgroups of four wavefronts with 32 rows each of a set of 128, all over the same keys (Block).  nwg 0: one a set, the
+// longest sets first: 2 x 12 heads x 8192 tokens 403 us so, 470 a key head at a time.  Else a set's keys are split (find_part)
+// and its parts joined by a launch of its own (dense_join_kernel): 128 rows are too many for the workgroup that comes last.  2
+// x 12 heads x 256 rows over 8000 keys 50 us (60 by sets of 32 rows; 88 and more with the last workgroup's join).
 constexpr int kBlock = kWaves * 2 * kRows;
 constexpr int kManyRows = 96;
 template <typename T, int D>
@@ -1369,10 +1370,10 @@ __global__ __launch_bounds__(256) void dense_join_kernel(Dense p) {
   if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
 }
 
-// Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level cache
-// (256 MiB) is not there any more at the next call, and its reads get in each other's way.  Of 32 x 12 queries over 32768 keys of
-// 64 (2.8 GB) 489 us with ordinary loads and 439 with these, one stream of 131000 (352 MB) 71.7 and 64.9; three caches of 86 MB
-// in turns 23.8 and 25.3.  Only where one set reads a key: several share them in the second cache.
+// Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level
+// cache (256 MiB) is not there any more at the next call, and its reads get in each other's way.  Of 32 x 12 queries over
+// 32768 keys of 64 (2.8 GB) 489 us with ordinary loads and 439 with these, one stream of 131000 (352 MB) 71.7 and 64.9; three
+// caches of 86 MB in turns 23.8 and 25.3.  Only where one set reads a key: several share them in the second cache.
 constexpr int64_t kOnce = (int64_t)256 << 20;
 
 template <typename T, int D, bool WIDE, int NT>
@@ -1412,12 +1413,13 @@ int block_dense(const Dense& p, int nsplit, hipStream_t st) {
   const int64_t sets = p.BH * (((int64_t)p.R + kBlock - 1) / kBlock);
   const int nwg = nsplit > kWaves ? nsplit / kWaves : 0;
   const int64_t wgs = nwg < sets ? sets : nwg;
-  hipLaunchKernelGGL((dense_block_kernel<T, D>), dim3((unsigned)(nwg > 0 ? (wgs + 7) / 8 * 8 : wgs)), dim3(kWaves * kWave), 0, st, p,
-                     nwg);
+  const dim3 grid((unsigned)(nwg > 0 ? (wgs + 7) / 8 * 8 : wgs)), blk(kWaves * kWave);
+  hipLaunchKernelGGL((dense_block_kernel<T, D>), grid, blk, 0, st, p, nwg);
   const int rc = check_launch("dense_block_kernel");
   if (rc != TA_OK || nwg <= sets) return rc;     // (no set has more than one)
   constexpr int kPer = 256 / (D / 4);
-  hipLaunchKernelGGL((dense_join_kernel<T, D>), dim3((unsigned)(p.BH * (((int64_t)p.R + kPer - 1) / kPer))), dim3(256), 0, st, p);
+  const int64_t joins = p.BH * (((int64_t)p.R + kPer - 1) / kPer);
+  hipLaunchKernelGGL((dense_join_kernel<T, D>), dim3((unsigned)joins), dim3(256), 0, st, p);
   return check_launch("dense_join_kernel");
 }
 
@@ -1425,7 +1427,8 @@ template <typename T, int D, bool WIDE>
 int rows_dense(const Dense& p, int nsplit, hipStream_t st) {
   if constexpr (sizeof(T) == 2 && WIDE && D >= 32)
     // (a workgroup a set of 128 rows; 24 heads x 1024 tokens, 192 workgroups, 28.8 us and 31.1 a wavefront a set, 8 heads of
-    // 128 x 2048, 128 of them, 89 and 78; caches of 128 keys 12.8 and 10.7, of 512 20.0 and 24.0; 64 rows over 4000 keys 94 and 114)
+    // 128 x 2048, 128 of them, 89 and 78; caches of 128 keys 12.8 and 10.7, of 512 20.0 and 24.0; 64 rows over 4000 keys 94
+    // and 114)
     if (nsplit != kWaves && p.R >= kManyRows && p.Tk >= 512 &&
         (nsplit > 1 || p.BH * (((int64_t)p.R + kBlock - 1) / kBlock) >= 192))
       return block_dense<T, D>(p, nsplit, st);
