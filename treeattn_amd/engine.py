@@ -1175,8 +1175,10 @@ class Decoder:
                 qkv = _product(x, L['c_attn'], L['ln1'], bits)
                 q, k, v = [a.view(nb, T0, H, dh).transpose(1, 2) for a in qkv.split(C, -1)]
                 if self.mode == 'dense':
-                    ns = decode_nsplit_dense(nb, H, T0, T0, dh)
-                    out = st.rows(b0, b1).attend(q, k, v, tq, ns, None).transpose(1, 2)
+                    if i == 0:
+                        ns = decode_nsplit_dense(nb, H, T0, T0, dh)
+                        dws = K.dense_attn_workspace(nb, H, T0, dh, ns, self.dev, H)
+                    out = st.rows(b0, b1).attend(q, k, v, tq, ns, dws).transpose(1, 2)
                     x = _product(out.reshape(nb, T0, C), L['c_proj'], bits=bits, residual=x)
                     x = _product(_product(x, L['c_fc'], L['ln2'], bits, gelu=True), L['c_mlp'], bits=bits, residual=x)
                     continue
