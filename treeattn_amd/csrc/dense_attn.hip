@@ -7,8 +7,8 @@
 //
 // One pass over the keys with a running maximum and sum, on the matrix cores even for a single query: the 16 rows of a tile
 // are the query heads of a key head times the new tokens, and what a lone row wastes of the instructions is less than the
-// vector units would take (32 keys of 64: 12 instructions of 16 cycles, against some 150 of 4).  Nothing passes through
-// LDS: with S^T = K Q^T a lane holds four scores of one query row, which are what the next product, O^T = V^T P^T, takes as
+// vector units would take (32 keys of 64: 12 instructions of 16 cycles, against some 150 of 4).  Scores and weights
+// stay in registers: with S^T = K Q^T a lane holds four scores of one query row, which are what the next product, O^T = V^T P^T, takes as
 // its B operand when that product counts the keys in the order the first leaves them in; V^T's operand is a lane's eight
 // keys at its own columns, turned round in registers; the running maximum, the sum and their corrections are then one
 // number a lane.
@@ -627,7 +627,7 @@ struct Share {
 // Bound by instructions: for 32 rows x 32 keys some 115 of the vector units (16 of them exponentials, at a quarter of the rate)
 // beside 28 of the matrix cores, two wavefronts to a SIMD.  So what can goes to the matrix cores (the weights' sums, as a
 // column of ones) and to LDS (values turned round on the way out, where Share takes 16 permutes); scores are not kept for the
-// branch that renews a maximum but made again there; and the two parts of a weight come from one dot product each.  64 keys
+// branch that renews a maximum but made again there; and what the first part of a weight leaves is one dot product.  64 keys
 // between two branches, since their chains run beside each other (with 32, three wavefronts to a SIMD spill: 502 us in place
 // of 389).
 //
