@@ -8,6 +8,7 @@ their projection gives (heads), the decoder what it stores and asks with.
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import kernels as K
 
@@ -43,27 +44,35 @@ def rope_frequencies(rot, base=10000.0, scaling='', factor=1.0, trained=0, low=1
 
 
 class _Rotate(torch.autograd.Function):
-    """The turn; its gradient is the turn back."""
+    """The turn, linear in x: its gradient is the turn back, its forward derivative the turn of the tangent."""
 
     @staticmethod
     def forward(ctx, x, pos, rope, inverse):
         ctx.save_for_backward(pos)
+        ctx.save_for_forward(pos)
         ctx.rope, ctx.inverse = rope, inverse
         return K.rope(x if x.stride(-1) == 1 else x.contiguous(), pos, rope, inverse=inverse)
 
     @staticmethod
     def backward(ctx, dy):
-        pos, = ctx.saved_tensors
-        if torch.is_grad_enabled():     # a gradient that is to be differentiated itself
-            return _Rotate.apply(dy, pos, ctx.rope, not ctx.inverse), None, None, None
-        return K.rope(dy if dy.stride(-1) == 1 else dy.contiguous(), pos, ctx.rope, inverse=not ctx.inverse), None, None, None
+        return _turn(dy, ctx.saved_tensors[0], ctx.rope, not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        return _turn(dx, ctx.saved_tensors[0], ctx.rope, ctx.inverse)
+
+
+def _turn(x, pos, rope, inverse):
+    # (outside a level of forward_ad no tensor has a tangent, and the second question costs nothing)
+    if (torch.is_grad_enabled() and x.requires_grad) or forward_ad.unpack_dual(x).tangent is not None:
+        return _Rotate.apply(x, pos, rope, inverse)
+    return K.rope(x if x.stride(-1) == 1 else x.contiguous(), pos, rope, inverse=inverse)
 
 
 def rotate(x, pos, rope):
-    """x (B,H,T,D), each row turned by the angles of its position (pos (T,) or (B,T)); differentiable in x."""
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Rotate.apply(x, pos, rope, False)
-    return K.rope(x if x.stride(-1) == 1 else x.contiguous(), pos, rope)
+    """x (B,H,T,D), each row turned by the angles of its position (pos (T,) or (B,T)); differentiable in x, backwards and
+    forwards."""
+    return _turn(x, pos, rope, False)
 
 
 def rope_of(cfg, device):
