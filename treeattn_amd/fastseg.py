@@ -11,6 +11,7 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import kernels as K
@@ -89,13 +90,19 @@ class _SparseAttnFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
+def differentiated(*tensors):
+    """Whether a derivative is asked for through any of the tensors: a gradient, or a forward-mode tangent."""
+    return ((torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+            or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+
+
 def sparse_attn(q, k, v, cand, scale, causal=False):
     """cand: (b,H,T,K) int, -1 = unused slot (fastseg.py:173-177).  Differentiable in q, k, v; the gradients
     of k and v are summed in a fixed order (bit-reproducible) up to 131072 queries and keys, with atomic adds past that
     (kernels.SORTED_MAX_POSITIONS).  causal (no counterpart in the reference): every candidate position is at most its
-    query's position."""
+    query's position.  There is no forward-mode derivative: tensors with a tangent raise."""
     _use_fast(q)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if differentiated(q, k, v):
         return _SparseAttnFn.apply(q, k, v, cand, scale, causal)
     return K.sparse_attn_fwd(q, k, v, cand, scale)[0]
 

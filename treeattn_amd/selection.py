@@ -209,7 +209,8 @@ def attend(q, k, v, lhat, cfg, scale=None, want_sel=True):
     dyn = getattr(cfg, 'attn', 'seg') == 'dyn'
     # gradients wanted (training): the candidate-list kernels, whose backward is built (the structural kernel
     # attends the same key set, forward only)
-    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
+    from .fastseg import differentiated
+    grad = differentiated(q, k, v)
     if dyn:   # the LaneTree selection (attention_dyn.py:74-75)
         from .dyntree import select_keys
         leaf = 2
