@@ -75,6 +75,12 @@ def rotate(x, pos, rope):
     return _turn(x, pos, rope, False)
 
 
+def _settings(cfg, device):
+    """What a Rope of rope_of is made from."""
+    return (cfg.rope, cfg.rope_dim, cfg.rope_base, cfg.rope_scaling, cfg.rope_factor, cfg.rope_trained, cfg.seq_len, cfg.n_embd,
+            cfg.n_head, device)
+
+
 def rope_of(cfg, device):
     """The Rope of a model configuration on `device`, None when its positions are learned."""
     if not getattr(cfg, 'rope', ''):
@@ -94,9 +100,11 @@ def heads(module, qkv):
     C, H = C3 // 3, module.H
     if not getattr(module.cfg, 'rope', ''):
         return [t.view(b, T, H, C // H).transpose(1, 2) for t in qkv.split(C, dim=2)]
-    r = module.__dict__.get('_rope')
-    if r is None or r.turns.device != qkv.device:
-        r = module.__dict__['_rope'] = rope_of(module.cfg, qkv.device)
+    made, r = module.__dict__.get('_rope', (None, None))
+    now = _settings(module.cfg, qkv.device)
+    if made != now:
+        r = rope_of(module.cfg, qkv.device)
+        module.__dict__['_rope'] = now, r
     qk, v = qkv.split((2 * C, C), dim=2)
     pos = torch.arange(T, device=qkv.device, dtype=torch.int32)
     qk = rotate(qk.view(b, T, 2 * H, C // H).transpose(1, 2), pos, r)
