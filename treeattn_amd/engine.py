@@ -74,6 +74,7 @@ class PagePool:
         self.table = torch.full((B, H, nblk), -1, dtype=torch.int32, device=dev)
         self.host = torch.full((B, H, nblk), -1, dtype=torch.int32)
         self.nblk = [0] * B                        # leaf blocks of each sequence that have pages
+        self.tokens = [None] * B                   # positions of each that have been written (wrote); None: nobody said
         self.free = list(range(self.P - 1, -1, -1))   # pages handed out in increasing order
         self.refs = [0] * self.P                   # sequences that use a page
         self.n_shared = 0                          # pages that more than one uses
@@ -176,30 +177,41 @@ class PagePool:
         self._copy(old, ids)
         self._show(b, b + 1, j0, j1)
 
-    def fork(self, src, dst, t):
-        """Sequence dst takes the first t positions of src (at most those that src holds; what dst had is released): whole blocks
-        share src's pages, the rows of a block that t ends inside are copied into pages of dst's own."""
+    def wrote(self, t_end, seqs=None):
+        """Positions < t_end of the given sequences (all by default) have been written: fork takes no others from there on."""
+        for b in range(self.B) if seqs is None else seqs:
+            self.tokens[b] = max(self.tokens[b] or 0, min(int(t_end), self.Tcap))
+
+    def fork(self, src, dst, t, ahead=None):
+        """Sequence dst takes the first t positions of src (what dst had is released): whole blocks share src's pages, the rows
+        of a block that t ends inside are copied into pages of dst's own.  t: at most the positions of src that have been
+        written (wrote), or, where nobody said, that have pages.  ahead: the position from which src is written without
+        ensure being told (a captured step's); blocks from there on are copied too."""
         t = int(t)
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
             raise ValueError('PagePool.fork: two different sequences of %d' % self.B)
-        if not 0 <= t <= min(self.nblk[src] * self.leaf, self.Tcap):
+        held = min(self.nblk[src] * self.leaf, self.Tcap)
+        if self.tokens[src] is not None:
+            held = min(held, self.tokens[src])
+        if not 0 <= t <= held:
             raise ValueError('PagePool.fork: sequence %d holds no %d positions' % (src, t))
-        whole, part = divmod(t, self.leaf)
+        whole, need = t // self.leaf, (t + self.leaf - 1) // self.leaf
+        if ahead is not None:
+            whole = min(whole, max(0, int(ahead)) // self.leaf)
         back = sum(self.refs[int(p)] == 1 for p in self.host[dst, :, :self.nblk[dst]].reshape(-1).tolist())
-        if part and self.H > len(self.free) + back:
+        if (need - whole) * self.H > len(self.free) + back:
             raise RuntimeError('PagePool: out of pages (%d needed, %d free of %d): raise max_tokens'
-                               % (self.H, len(self.free) + back, self.P))
+                               % ((need - whole) * self.H, len(self.free) + back, self.P))
         had = self.nblk[dst]
         self._forget(dst)
         for p in self.host[src, :, :whole].reshape(-1).tolist():
             self._use(p)
         self.host[dst, :, :whole] = self.host[src, :, :whole]
-        self.nblk[dst] = whole
-        if part:
-            ids = self._take(self.H)
-            self.host[dst, :, whole] = torch.tensor(ids, dtype=torch.int32)
-            self.nblk[dst] = whole + 1
-            self._copy(self.host[src, :, whole].tolist(), ids)
+        self.nblk[dst], self.tokens[dst] = need, None if self.tokens[src] is None else t
+        if need > whole:
+            ids = self._take((need - whole) * self.H)
+            self.host[dst, :, whole:need] = torch.tensor(ids, dtype=torch.int32).view(self.H, need - whole)
+            self._copy(self.host[src, :, whole:need].reshape(-1).tolist(), ids)
         if max(had, self.nblk[dst]):
             self._show(dst, dst + 1, 0, max(had, self.nblk[dst]))
 
@@ -210,7 +222,7 @@ class PagePool:
             for p in self.host[b, h, :n].flip(0).tolist():
                 self._drop(int(p))
         self.host[b, :, :n] = -1
-        self.nblk[b] = 0
+        self.nblk[b], self.tokens[b] = 0, None
 
     def release(self, b):
         """Return sequence b's pages (its cache rows are forgotten, those of the block an 8-bit cache's tail holds too); a page
@@ -450,6 +462,8 @@ class SegState:
         if self.pages is not None:
             self.pages.ensure(T, start=[0] * self.B)
         self.write_rows(0, K_, V_)
+        if self.pages is not None:
+            self.pages.wrote(T)
         t_end = T if t_end is None else t_end
         kd = K_.to(self.dtype)
         SEL.build_pyramid(kd, self.shape, t_end=t_end, out=self.levels)
@@ -1089,6 +1103,9 @@ class Decoder:
             at = t.reshape(-1).tolist() if torch.is_tensor(t) else [int(t)] * self.B
             self.reserve(max(at) + 1, at)
         logits = self._forward_step(tk, tp)
+        if self.pool is not None:
+            for b, x in enumerate(at):
+                self.pool.wrote(x + 1, (b,))
         keys = self.keys_read()
         if scalar and self.B == 1:
             return logits[0], float(keys[0])
@@ -1103,12 +1120,23 @@ class Decoder:
             self.pool.ensure(t_end, start=start)
 
     # ------------------------------------------------------------------------------------------ sequences
+    def _replayed(self):
+        """The positions of a captured step's next replay (read from the device), [] without one: what is before them has been
+        written, which the page pool is told."""
+        if self.graph is None or self.pool is None:
+            return []
+        at = self.g_t.tolist()
+        for b, t in enumerate(at):
+            self.pool.wrote(t, (b,))
+        return at
+
     @torch.no_grad()
     def fork(self, src, dst, t):
-        """Sequence dst goes on from the first t positions of src (at most those that src holds), as after the same tokens: whole
-        pages of the caches are shared (read only; a step that goes back into one gets a copy), the rows behind them and the
-        tree's state copied.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] and g_t[dst] too
-        (a replay hands out no copies: before one that goes back behind t, reserve(t_end, start) does).
+        """Sequence dst goes on from the first t positions of src, as after the same tokens: whole pages of the caches are
+        shared (read only; a step that goes back into one gets a copy), the rows behind them and the tree's state copied.  t: at
+        most the positions of src that a prompt, a step or a replay (by g_t) has written; with contiguous caches this is not
+        known, and t at most Tcap.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] too (g_t[dst]
+        becomes t; a replay hands out no copies: before one that goes back behind t, reserve(t_end, start) does).
         With the budget head's global pool the running sum of keys is that of the cache's rows."""
         t = int(t)
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
@@ -1118,9 +1146,12 @@ class Decoder:
         if self.mode != 'seg' and not self.paged:
             raise NotImplementedError('dense comparison mode is batch 1')
         if self.pool is not None:
-            self.pool.fork(src, dst, t)
+            at = self._replayed()
+            self.pool.fork(src, dst, t, at[src] if at else None)
             if self.graph is not None and self._t_host is not None:
                 self.pool.ensure(self._reserved)
+        if self.graph is not None:
+            self.g_t[dst] = t
         ids = torch.tensor([[src], [dst]], dtype=torch.int32).to(self.dev)
         K.copy_rows([x for st in self.states for x in st.sequence_tensors()], ids[0], ids[1])
         for st in self.states:
@@ -1136,6 +1167,7 @@ class Decoder:
         """Page pools of num_pages pages for the caches (PagePool.resize).  A captured step is captured again after it."""
         if self.pool is None:
             raise ValueError('Decoder.resize: paged caches')
+        self._replayed()
         self.pool.resize(num_pages)
         for st in self.states:
             st.repage()
@@ -1234,6 +1266,8 @@ class Decoder:
                 if cfg.global_pool:
                     st.ksum[b0:b1] = k.float().sum(2)
             last.append(F.linear(_ln(x[:, -1], W['ln_f']), W['wte']))
+        if self.pool is not None:
+            self.pool.wrote(T0)
         return torch.cat(last, 0)
 
     # ------------------------------------------------------------------------------------------ graphs
@@ -1245,6 +1279,7 @@ class Decoder:
         so the groups' steps run concurrently."""
         B = self.B
         V = self.W['wte'].shape[0]
+        self._replayed()
         self.g_tok = tok.to(self.dev).long().clone()
         self.g_t = (t.to(self.dev).long() if torch.is_tensor(t) else
                     torch.full((B,), int(t), device=self.dev, dtype=torch.long)).clone()
