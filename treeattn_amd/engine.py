@@ -182,11 +182,12 @@ class PagePool:
         for b in range(self.B) if seqs is None else seqs:
             self.tokens[b] = max(self.tokens[b] or 0, min(int(t_end), self.Tcap))
 
-    def fork(self, src, dst, t, ahead=None):
+    def fork(self, src, dst, t, ahead=None, t_end=0):
         """Sequence dst takes the first t positions of src (what dst had is released): whole blocks share src's pages, the rows
         of a block that t ends inside are copied into pages of dst's own.  t: at most the positions of src that have been
         written (wrote), or, where nobody said, that have pages.  ahead: the position from which src is written without
-        ensure being told (a captured step's); blocks from there on are copied too."""
+        ensure being told (a captured step's); blocks from there on are copied too.  t_end: dst gets pages for positions < t_end
+        as ensure gives them.  Out of pages: nothing is changed."""
         t = int(t)
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
             raise ValueError('PagePool.fork: two different sequences of %d' % self.B)
@@ -198,10 +199,11 @@ class PagePool:
         whole, need = t // self.leaf, (t + self.leaf - 1) // self.leaf
         if ahead is not None:
             whole = min(whole, max(0, int(ahead)) // self.leaf)
+        end = max(need, (min(int(t_end), self.Tcap) + self.leaf - 1) // self.leaf)
         back = sum(self.refs[int(p)] == 1 for p in self.host[dst, :, :self.nblk[dst]].reshape(-1).tolist())
-        if (need - whole) * self.H > len(self.free) + back:
+        if (end - whole) * self.H > len(self.free) + back:
             raise RuntimeError('PagePool: out of pages (%d needed, %d free of %d): raise max_tokens'
-                               % ((need - whole) * self.H, len(self.free) + back, self.P))
+                               % ((end - whole) * self.H, len(self.free) + back, self.P))
         had = self.nblk[dst]
         self._forget(dst)
         for p in self.host[src, :, :whole].reshape(-1).tolist():
@@ -214,6 +216,7 @@ class PagePool:
             self._copy(self.host[src, :, whole:need].reshape(-1).tolist(), ids)
         if max(had, self.nblk[dst]):
             self._show(dst, dst + 1, 0, max(had, self.nblk[dst]))
+        self.ensure(t_end, (dst,))
 
     def _forget(self, b):
         """Sequence b's pages back, in the host's table."""
@@ -1147,9 +1150,8 @@ class Decoder:
             raise NotImplementedError('dense comparison mode is batch 1')
         if self.pool is not None:
             at = self._replayed()
-            self.pool.fork(src, dst, t, at[src] if at else None)
-            if self.graph is not None and self._t_host is not None:
-                self.pool.ensure(self._reserved)
+            # (captured: with the pages of the replays to come, in one call that either does all of it or nothing)
+            self.pool.fork(src, dst, t, at[src] if at else None, self._reserved if at else 0)
         if self.graph is not None:
             self.g_t[dst] = t
         ids = torch.tensor([[src], [dst]], dtype=torch.int32).to(self.dev)
@@ -1280,17 +1282,19 @@ class Decoder:
         B = self.B
         V = self.W['wte'].shape[0]
         self._replayed()
-        self.g_tok = tok.to(self.dev).long().clone()
-        self.g_t = (t.to(self.dev).long() if torch.is_tensor(t) else
-                    torch.full((B,), int(t), device=self.dev, dtype=torch.long)).clone()
+        g_tok = tok.to(self.dev).long().clone()
+        g_t = (t.to(self.dev).long() if torch.is_tensor(t) else
+               torch.full((B,), int(t), device=self.dev, dtype=torch.long)).clone()
         # the replays' positions, followed on the host so pages can be handed out ahead of them without a sync
-        self._t_host = int(self.g_t.max()) if torch.is_tensor(t) else int(t)
-        self._reserved = self._t_host + 1 + self.reserve_ahead
-        self.reserve(self._reserved, self.g_t.tolist() if self.pool is not None and self.pool.n_shared else None)
+        t_host = int(g_t.max()) if torch.is_tensor(t) else int(t)
+        end = t_host + 1 + self.reserve_ahead
+        self.reserve(end, g_t.tolist() if self.pool is not None and self.pool.n_shared else None)
+        # (out of pages: the step that was captured before is as it was; from here on there is only the new one)
+        self.graph, self.graphs = None, []
+        self.g_tok, self.g_t, self._t_host, self._reserved = g_tok, g_t, t_host, end
         self.g_logits = torch.empty(B, V, device=self.dev, dtype=torch.bfloat16 if self.fused else torch.float32)
         main = torch.cuda.current_stream()
         groups = self.groups if (self.fused and len(self.groups) > 1) else [None]
-        self.graphs = []
         for grp in groups:
             s = grp['stream'] if grp is not None else torch.cuda.Stream(device=self.dev)
             b0, b1 = (grp['b0'], grp['b1']) if grp is not None else (0, B)
@@ -1344,8 +1348,9 @@ class Decoder:
             raise RuntimeError('Decoder.replay: no captured step (capture; again after reset and resize)')
         if self.pool is not None and self._t_host is not None:
             if self._t_host + 1 >= self._reserved:
-                self._reserved = self._t_host + 1 + self.reserve_ahead
-                self.reserve(self._reserved)
+                end = self._t_host + 1 + self.reserve_ahead
+                self.reserve(end)          # (out of pages: the next replay asks again)
+                self._reserved = end
             self._t_host += 1
         main = torch.cuda.current_stream()
         for g, s in self.graphs:
