@@ -102,3 +102,16 @@ def test_a_decoder_forks_what_its_steps_wrote():
         assert all(d.pool.refs[int(p)] == 1 for p in d.pool.host[0, :, j])
     d.resize(d.pool.P + 1)                    # (no captured step any more: what its replays wrote stays known)
     assert d.graph is None and d.pool.tokens == [140, 140, 130]
+
+
+def test_a_fork_forgets_the_tail_of_its_target():
+    """The unrounded rows of an 8-bit cache's last block belong to what the target held before."""
+    pool = new(cache='e4m3')
+    held = [torch.tensor([[2, 2], [1, 1], [0, 0]], dtype=torch.int32) for _ in range(2)]
+    pool.held += held
+    pool.ensure(12)
+    pool.fork(0, 1, 8)
+    assert all(x.tolist() == [[2, 2], [-1, -1], [0, 0]] for x in held)
+    with pytest.raises(ValueError):
+        pool.fork(0, 2, 13)
+    assert all(x.tolist() == [[2, 2], [-1, -1], [0, 0]] for x in held)

@@ -187,7 +187,8 @@ class PagePool:
         of a block that t ends inside are copied into pages of dst's own.  t: at most the positions of src that have been
         written (wrote), or, where nobody said, that have pages.  ahead: the position from which src is written without
         ensure being told (a captured step's); blocks from there on are copied too.  t_end: dst gets pages for positions < t_end
-        as ensure gives them.  Out of pages: nothing is changed."""
+        as ensure gives them.  Out of pages: nothing is changed.  8-bit caches: dst's tail is forgotten, as release does; rows
+        of src that are still in its tail only are for the caller to copy (Decoder.fork)."""
         t = int(t)
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
             raise ValueError('PagePool.fork: two different sequences of %d' % self.B)
@@ -217,6 +218,8 @@ class PagePool:
         if max(had, self.nblk[dst]):
             self._show(dst, dst + 1, 0, max(had, self.nblk[dst]))
         self.ensure(t_end, (dst,))
+        for held in self.held:
+            held[dst].fill_(-1)
 
     def _forget(self, b):
         """Sequence b's pages back, in the host's table."""
