@@ -304,6 +304,7 @@ class SegState:
         self.shape = SEL.cfg_shape(cfg, Tcap)
         self.Lm = self.shape.blevels[-1] if self.shape.n_levels else 0
         self.pages, self.layer = pages, layer
+        self.b0 = 0                                # the pool's sequence that this state's first is (rows)
         self.cache8 = None
         if pages is not None and pages.scales is not None:
             self.cache8 = pages.cache8(layer, dtype)
@@ -448,7 +449,7 @@ class SegState:
         """A view of sequences b0..b1-1 of this cache (the tensors are shared, not copied)."""
         v = object.__new__(SegState)
         v.__dict__.update(self.__dict__)
-        v.B = b1 - b0
+        v.B, v.b0 = b1 - b0, self.b0 + b0
         for name in ('K', 'V', 'st_leaf', 'st_score', 'st_ok', 'ksum'):
             if hasattr(self, name):
                 setattr(v, name, getattr(self, name)[b0:b1])
@@ -466,10 +467,11 @@ class SegState:
         """Load a whole context (engine.py:57-71).  K_, V_: (B,H,T,dh) with T <= Tcap."""
         T = K_.shape[2]
         if self.pages is not None:
-            self.pages.ensure(T, start=[0] * self.B)
+            seqs = range(self.b0, self.b0 + self.B)
+            self.pages.ensure(T, seqs, start=[0] * self.B)
         self.write_rows(0, K_, V_)
         if self.pages is not None:
-            self.pages.wrote(T)
+            self.pages.wrote(T, seqs)
         t_end = T if t_end is None else t_end
         kd = K_.to(self.dtype)
         SEL.build_pyramid(kd, self.shape, t_end=t_end, out=self.levels)
