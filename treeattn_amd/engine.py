@@ -136,15 +136,16 @@ class PagePool:
         if self.refs[p] == 0:
             self.free.append(p)
 
-    def ensure(self, t_end, seqs=None, start=None):
+    def ensure(self, t_end, seqs=None, start=None, stop=None):
         """Pages for positions < t_end (at most Tcap) of the given sequences (all by default): a sequence's
         blocks get consecutive pages, head by head.  start: the first position of each of these sequences that will be written
-        (blocks from there on that are shared get pages of their own); None: only positions that no page holds yet."""
+        (blocks from there on, up to the position stop of each, by default t_end, that are shared get pages of their own);
+        None: only positions that no page holds yet."""
         need = (min(int(t_end), self.Tcap) + self.leaf - 1) // self.leaf
         seqs = range(self.B) if seqs is None else seqs
         if start is not None and self.n_shared:
-            for b, t in zip(seqs, start):
-                self.own(b, t, t_end)
+            for i, (b, t) in enumerate(zip(seqs, start)):
+                self.own(b, t, t_end if stop is None else stop[i])
         todo = [b for b in seqs if self.nblk[b] < need]
         if not todo:
             return
@@ -164,16 +165,19 @@ class PagePool:
     def own(self, b, t, t_end=None):
         """Pages of its own for the blocks of sequence b that hold positions t .. t_end-1 (default: to the last) and that it
         shares: copies of what they hold."""
-        j0 = int(t) // self.leaf
+        j0 = max(0, int(t)) // self.leaf
         j1 = self.nblk[b] if t_end is None else min(self.nblk[b], (int(t_end) + self.leaf - 1) // self.leaf)
-        todo = [(h, j) for j in range(max(0, j0), j1) for h in range(self.H) if self.refs[int(self.host[b, h, j])] > 1]
-        if not todo:
+        if j0 >= j1 or (t_end is not None and t_end <= max(0, int(t))):
             return
-        ids = self._take(len(todo))
-        old = [int(self.host[b, h, j]) for h, j in todo]
-        for (h, j), p, q in zip(todo, ids, old):
-            self.host[b, h, j] = p
-            self._drop(q)
+        mine = self.host[b, :, j0:j1].reshape(-1).tolist()
+        old = [p for p in mine if self.refs[p] > 1]
+        if not old:
+            return
+        ids = self._take(len(old))
+        new = dict(zip(old, ids))                  # (a page is one block of a sequence)
+        self.host[b, :, j0:j1] = torch.tensor([new.get(p, p) for p in mine], dtype=torch.int32).view(self.H, j1 - j0)
+        for p in old:
+            self._drop(p)
         self._copy(old, ids)
         self._show(b, b + 1, j0, j1)
 
@@ -1109,7 +1113,7 @@ class Decoder:
               torch.full((self.B,), int(t), device=self.dev, dtype=torch.long))
         if self.pool is not None:
             at = t.reshape(-1).tolist() if torch.is_tensor(t) else [int(t)] * self.B
-            self.reserve(max(at) + 1, at)
+            self.reserve(max(at) + 1, at, [x + 1 for x in at])
         logits = self._forward_step(tk, tp)
         if self.pool is not None:
             for b, x in enumerate(at):
@@ -1119,13 +1123,14 @@ class Decoder:
             return logits[0], float(keys[0])
         return logits, keys
 
-    def reserve(self, t_end, start=None):
+    def reserve(self, t_end, start=None, stop=None):
         """Pages for positions < t_end of every sequence (paged caches; host side, not inside a captured step).  start: the
-        position that each sequence goes on from (its pages from there on are its own then); None: behind all it holds."""
+        position that each sequence goes on from (its pages from there on, or up to the position stop of each, are its own then);
+        None: behind all it holds."""
         if self.pool is not None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('Decoder.reserve: pages are handed out outside graph capture')
-            self.pool.ensure(t_end, start=start)
+            self.pool.ensure(t_end, start=start, stop=stop)
 
     # ------------------------------------------------------------------------------------------ sequences
     def _replayed(self):
