@@ -893,7 +893,7 @@ class Decoder:
         self.cache = cache
         # the whole step as one launch (ta_decode_step): bf16, head_dim 64, up to 32 sequences, the structural
         # key set (no neighbour borrowing, fixed budget) and one sequence group
-        # attn_split: workgroups per query of the per-op decode attention (default: decode_nsplit's choice)
+        # attn_split: workgroups per query of the per-op decode attention (default: the choice of decode_nsplit and its like)
         self.attn_split = attn_split
         can = (self.fused and mode == 'seg' and self.rope is None and self.dh == 64 and batch <= 32 and not groups
                and not cfg.neighbors and cfg.beam_mode != 'pred' and n_layer <= 64 and not SEL.gate_on(cfg) and not self.mx4)
@@ -954,7 +954,9 @@ class Decoder:
             self.pool = PagePool(B, H, dh, DENSE_PAGE, self.Tcap, npages, self.nl, self.dtype, self.dev)
             self.states = [PagedState(self.pool, i, self.rope) for i in range(self.nl)]
             self.scratch = sc = _Scratch(B, H, dh, 0, self.dev, 1, self.nl)
-            ns = decode_nsplit_dense(B, H, 1, self.max_tokens, dh) if not self.attn_split else 4 * int(self.attn_split)
+            # (dense_attn's nsplit counts the wavefronts of all queries together)
+            ns = (min(8192, 4 * int(self.attn_split) * B * H if self.attn_split > 1 else 4) if self.attn_split else
+                  decode_nsplit_dense(B, H, 1, self.max_tokens, dh))
             sc.dense = ns, K.dense_attn_workspace(B, H, 1, dh, ns, self.dev, H)
             sc.rowvec = B <= ROWVEC_MAX_ROWS
             self.groups = [dict(b0=0, b1=B, states=self.states, scratch=sc, stream=None,
