@@ -67,6 +67,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kRows = 16;            // query rows of a tile
+constexpr float kLittle = -24.0f;    // log2 of the largest weight where sums would pass the range of a float
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -166,11 +167,26 @@ __device__ __forceinline__ float sum_rows(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// One element in device memory.
-__device__ __forceinline__ float number(const TA_GLOBAL float* p) { return *p; }
-__device__ __forceinline__ float number(const TA_GLOBAL f16_t* p) { return (float)*p; }
-__device__ __forceinline__ float number(const TA_GLOBAL bf16_t* p) {
-  return __uint_as_float((uint32_t) * (const TA_GLOBAL uint16_t*)p << 16);
+// What a pass over the keys takes for values: what is there; with a weight of 1 for every key that a row sees, ones where it is
+// infinite with the sign or NaN and zeros elsewhere (kUp, kDown); zeros where it is infinite or NaN (kFinite, and kSmall, whose
+// weights are at most 2^-24).
+enum Values { kAll, kUp, kDown, kFinite, kSmall };
+
+// Those values in place of x's two 16-bit ones (one of 32 bits).
+template <typename T>
+__device__ __forceinline__ uint32_t stand_in(uint32_t x, Values values) {
+  constexpr bool wide = sizeof(T) == 4;
+  constexpr uint32_t kExp = wide ? 0x7f800000u : __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t kOne = wide ? 0x3f800000u : __is_same(T, f16_t) ? 0x3c00u : 0x3f80u;
+  constexpr uint32_t kAbs = wide ? 0x7fffffffu : 0x7fffu;
+  auto one = [&](uint32_t h) {
+    const bool not_finite = (h & kExp) == kExp;
+    if (values >= kFinite) return not_finite ? 0u : h;
+    const bool sign = values == kUp ? h <= kAbs : h > kAbs;
+    return not_finite && (sign || (h & kAbs) != kExp) ? kOne : 0u;
+  };
+  if constexpr (wide) return one(x);
+  else return one(x & 0xffffu) | one(x >> 16) << 16;
 }
 
 // Row r of a key head's query rows: query head j of its group, token n.
@@ -205,8 +221,7 @@ struct Share {
   const int32_t* tab;
   int t[NT];            // the lane's row's position; of rows that are not there or see nothing: behind every key
   uint32_t none;        // rows (bit 16 i + c) whose position is outside the cache: zeros
-  int tmin, tmax;       // of the wavefront's rows
-  int seen;             // values past this position count as zeros
+  int tmin, tmax;       // of the wavefront's rows; values past the last count as zeros
   uint4 q[NT][C::KS];
   f32x4 acc[NT][C::DJ];
   float m[NT], l[NT];   // the reference of the weights (max - kShift), and the lane's part of their sum
@@ -256,7 +271,6 @@ struct Share {
     hi = -min16(-hi);
     tmin = __builtin_amdgcn_readfirstlane(lo);
     tmax = __builtin_amdgcn_readfirstlane(hi);
-    seen = tmax;
   }
 
   __device__ __forceinline__ int page_of(int key0) const {
@@ -402,9 +416,18 @@ struct Share {
   }
 
   // The weights of row set i in place of its scores (0 where masked), the running maximum renewed when one passes it by more
-  // than kSlack.
-  template <bool MASKED>
-  __device__ __forceinline__ void weights(const Step<T, D>& x, int i, f32x4 (&s)[C::KT]) {
+  // than kSlack.  AGAIN: for the values of `values`.
+  template <bool MASKED, bool AGAIN>
+  __device__ __forceinline__ void weights(const Step<T, D>& x, int i, f32x4 (&s)[C::KT], Values values) {
+    if (AGAIN && values <= kDown) {
+#pragma unroll
+      for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[a][u] = sees(x, i, a, u) ? 1.0f : 0.0f;
+      return;
+    }
+    const float shift = AGAIN && values == kSmall ? kLittle : C::kShift;
+    const float past = AGAIN && values == kSmall ? kLittle : C::kShift + C::kSlack;
     const float f = fabsf(p.scale) * kLog2e;   // (a negative scale turns q round: the largest score is the largest product)
     float top = kLowest;
 #pragma unroll
@@ -413,10 +436,10 @@ struct Share {
       for (int u = 0; u < 4; ++u)
         if (!MASKED || sees(x, i, a, u)) top = fmaxf(top, s[a][u]);
     top = top > kLowest ? top * f : kLowest;   // (a scale of zero, and products below the range, as others)
-    if (__ballot(top > m[i] + (C::kShift + C::kSlack)) != 0) {
+    if (__ballot(top > m[i] + past) != 0) {
       // only the rows that need it: what a row gives does not depend on the others
       const float mx = max_rows(top);
-      const float mn = mx > m[i] + (C::kShift + C::kSlack) ? mx - C::kShift : m[i];
+      const float mn = mx > m[i] + past ? mx - shift : m[i];
       const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
       m[i] = mn;
       l[i] *= alpha;
@@ -433,22 +456,22 @@ struct Share {
       }
   }
 
-  template <bool MASKED>
-  __device__ __forceinline__ void consume(Step<T, D>& x) {
+  template <bool MASKED, bool AGAIN>
+  __device__ __forceinline__ void consume(Step<T, D>& x, Values values) {
     if constexpr (MASKED) {
       // values that no query sees count as zeros (0 times what stands there need not be 0)
 #pragma unroll
       for (int e = 0; e < C::KT * 4; ++e) {
-        const bool ok = x.key0 + 16 * (e / 4) + 4 * g + e % 4 <= seen && (x.have >> e) & 1;
+        const bool ok = x.key0 + 16 * (e / 4) + 4 * g + e % 4 <= tmax && (x.have >> e) & 1;
 #pragma unroll
-        for (int w = 0; w < C::VW; ++w) x.v[e][w] = ok ? x.v[e][w] : 0u;
+        for (int w = 0; w < C::VW; ++w) x.v[e][w] = !ok ? 0u : AGAIN ? stand_in<T>(x.v[e][w], values) : x.v[e][w];
       }
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       f32x4 s[C::KT];
       scores(x, i, s);
-      weights<MASKED>(x, i, s);
+      weights<MASKED, AGAIN>(x, i, s, values);
       if constexpr (C::EB == 2) {
         uint32_t hi[2 * C::KT], lo[2 * C::KT];
 #pragma unroll
@@ -482,12 +505,17 @@ struct Share {
       }
     }
   }
-  __device__ __forceinline__ void step(Step<T, D>& x) {
+  template <bool AGAIN>
+  __device__ __forceinline__ void step(Step<T, D>& x, Values values) {
     turn(x);
-    const bool full = x.key0 + C::KEYS - 1 <= (tmin < seen ? tmin : seen) &&
-                      __ballot((x.have & ((1u << (4 * C::KT)) - 1)) != (1u << (4 * C::KT)) - 1) == 0;
-    if (full) consume<false>(x);
-    else consume<true>(x);
+    if constexpr (AGAIN) {
+      consume<true, true>(x, values);
+    } else {
+      const bool full = x.key0 + C::KEYS - 1 <= tmin &&
+                        __ballot((x.have & ((1u << (4 * C::KT)) - 1)) != (1u << (4 * C::KT)) - 1) == 0;
+      if (full) consume<false, false>(x, kAll);
+      else consume<true, false>(x, kAll);
+    }
   }
 
   __device__ __forceinline__ void reset() {
@@ -500,44 +528,8 @@ struct Share {
     }
   }
 
-  // Keys [k0, k1) of row set i, key by key without matrix instructions: each weight times each value of the keys the row sees,
-  // nothing else.  Lane (c, g) takes a quarter of row c.
-  __device__ __forceinline__ void careful(int i, int row0, int b, int h, int k0, int k1) {
-    m[i] = kLowest;
-    l[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < C::DJ; ++d) acc[i][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    const int r = row0 + kRows * i + c;
-    int j = 0, n = 0;
-    if (r < p.R) head_token(p, r, j, n);
-    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + j) * p.qsh + n * p.qsn + g * (D / 4);
-    for (int key = k0; key < k1; ++key) {
-      int64_t ko = key * p.kst, vo = key * p.vst;
-      if (tab) {
-        const int page = tab[key >> p.blog2];
-        if (page < 0 || page >= p.npages) continue;
-        ko = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.kst;
-        vo = page * p.pstride + (key & ((1 << p.blog2) - 1)) * p.vst;
-      }
-      const TA_GLOBAL T* kr = kb + ko + g * (D / 4);
-      const TA_GLOBAL T* vr = vb + vo;
-      float s = 0.0f;
-#pragma unroll 1
-      for (int d = 0; d < D / 4; ++d) s = fmaf(to_f32(qr[d]), number(kr + d), s);
-      s = sum_rows(s) * (p.scale * kLog2e);
-      if (key > t[i] || r >= p.R) continue;   // (rows that see nothing are not taken from here)
-      const float mn = fmaxf(m[i], s - C::kShift);
-      const float alpha = __builtin_amdgcn_exp2f(m[i] - mn), w = __builtin_amdgcn_exp2f(s - mn);
-      m[i] = mn;
-      l[i] = l[i] * alpha + (g == 0 ? w : 0.0f);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int d = 0; d < C::DJ; ++d) acc[i][d][u] = fmaf(w, number(vr + col(d, u)), acc[i][d][u] * alpha);
-    }
-  }
-
-  __device__ __forceinline__ void pass(int k0, int k1) {
+  template <bool AGAIN = false>
+  __device__ __forceinline__ void pass(int k0, int k1, Values values = kAll) {
     const int last = k0 + (k1 - 1 - k0) / C::KEYS * C::KEYS;   // the last step's first key
     auto at = [&](int n) {
       const int key = k0 + n * C::KEYS;
@@ -549,9 +541,9 @@ struct Share {
     fetch(x[0], at(0), at(1), true);
     for (int n = 0; k0 + n * C::KEYS < k1; n += 2) {
       fetch(x[1], at(n + 1), at(n + 2), k0 + (n + 1) * C::KEYS < k1);
-      step(x[0]);
+      step<AGAIN>(x[0], values);
       fetch(x[0], at(n + 2), at(n + 3), k0 + (n + 2) * C::KEYS < k1);
-      if (k0 + (n + 1) * C::KEYS < k1) step(x[1]);
+      if (k0 + (n + 1) * C::KEYS < k1) step<AGAIN>(x[1], values);
     }
   }
 
@@ -569,7 +561,8 @@ struct Share {
     }
   }
 
-  // The rows (bit 16 i + c) whose accumulators are not finite.
+  // The rows (bit 16 i + c) whose accumulators are not finite, though the sum of their weights is: where that is not, nor is
+  // a weight, and the whole row is NaN.
   __device__ __forceinline__ uint32_t unsound() const {
     uint32_t rows = 0;
 #pragma unroll
@@ -579,41 +572,68 @@ struct Share {
       for (int d = 0; d < C::DJ; ++d)
 #pragma unroll
         for (int u = 0; u < 4; ++u) bad |= !(fabsf(acc[i][d][u]) < INFINITY);
-      const uint64_t w = __ballot(bad);
-      rows |= (uint32_t)((w | w >> 16 | w >> 32 | w >> 48) & 0xffff) << (16 * i);
+      const uint64_t w = __ballot(bad), n = __ballot(!(fabsf(l[i]) < INFINITY));
+      const uint64_t ww = w | w >> 32, nn = n | n >> 32;
+      rows |= (uint32_t)((ww | ww >> 16) & ~(nn | nn >> 16) & 0xffff) << (16 * i);
     }
     return rows;
+  }
+
+  // The elements of acc (bit 4 d + u of row set i) that are not zero.
+  __device__ __forceinline__ void marks(uint32_t (&bits)[NT]) const {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      bits[i] = 0;
+#pragma unroll
+      for (int d = 0; d < C::DJ; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) bits[i] |= acc[i][d][u] != 0.0f ? 1u << (4 * d + u) : 0u;
+    }
+  }
+  // Infinities and NaN in the elements that see them.
+  __device__ __forceinline__ void mark(const uint32_t (&up)[NT], const uint32_t (&down)[NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int d = 0; d < C::DJ; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const bool a = up[i] >> (4 * d + u) & 1, b = down[i] >> (4 * d + u) & 1;
+          acc[i][d][u] = a && b ? NAN : a ? INFINITY : b ? -INFINITY : acc[i][d][u];
+        }
   }
 
   // Keys [k0, k1) for the rows of `want`; emit(mask) takes the results of some rows at a time.
   //
   // A value that is infinite or NaN reaches, in the matrix instructions, rows that do not see its key (as 0 times it), and
-  // comes as a sum of two products (which may be inf - inf).  So a row whose result is not finite goes through its keys again
-  // by itself, values that it does not see taken as zeros (the same sums as if they had been finite); one that is still not
-  // finite goes through them without matrix instructions.
+  // comes as a sum of two products (which may be inf - inf).  So where a row's result is not finite, its wavefront goes
+  // through the keys again: twice with ones for such values and for the weights of what a row sees, which says which elements
+  // see +inf, -inf or NaN, and once with zeros for such values (the same sums as if they had been finite).  What is still
+  // not finite has passed the range of a float on the way (not float16 values): once more, with weights of at most 2^-24.  Five
+  // passes at most, whatever the values are, and the rows that none of it reaches keep their bits.
   template <typename Emit>
-  __device__ __forceinline__ void run(int row0, int b, int h, int k0, int k1, uint32_t want, Emit emit) {
-    int only = -1;
-    while (true) {
-      if (k0 < k1) pass(k0, k1);
-      uint32_t bad = unsound() & want & ~none, done = want & ~bad;
-      if (only >= 0) {
-        if (bad >> only & 1) {
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-            if (only / kRows == i) careful(i, row0, b, h, k0, k1);
-        }
-        done = 1u << only;
-      }
-      finish();
-      emit(done);
-      want &= ~done;
-      if (want == 0) return;
-      only = __ffs(want) - 1;
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-        if (only / kRows == i) seen = __builtin_amdgcn_readlane(t[i], only % kRows);
+  __device__ __forceinline__ void run(int k0, int k1, uint32_t want, Emit emit) {
+    if (k0 < k1) pass(k0, k1);
+    const uint32_t bad = unsound() & want & ~none;
+    finish();
+    emit(want & ~bad);
+    if (bad == 0) return;
+    uint32_t left = bad, up[NT], down[NT];
+#pragma unroll 1
+    for (int n = kUp; n <= kSmall; ++n) {
       reset();
+      pass<true>(k0, k1, (Values)n);
+      if (n <= kDown) {
+        if (n == kUp) marks(up);
+        else marks(down);
+        continue;
+      }
+      const uint32_t most = n == kFinite ? unsound() & left : 0;
+      finish();
+      mark(up, down);
+      emit(left & ~most);
+      left = most;
+      if (left == 0) return;
     }
   }
 
@@ -651,7 +671,6 @@ struct Block : Share<T, D, true, 2, false, true> {
   using S::none;
   using S::p;
   f32x4 sums[2];        // the weights' sums, by the matrix cores, in every element
-  using S::seen;
   using S::t;
   using S::tab;
   using S::tmax;
@@ -722,10 +741,20 @@ struct Block : Share<T, D, true, 2, false, true> {
   // scores passes it by more than kSlack.  One branch for all sets, so that their products and exponentials stand in one run of
   // instructions.
   // again(i, s) gives the scores of set i anew, for that branch.
-  template <bool MASKED, typename F>
-  __device__ __forceinline__ void weights(const Step<T, D, true>& x, f32x4 (&s)[2][C::KT], F again) {
+  template <bool MASKED, bool AGAIN, typename F>
+  __device__ __forceinline__ void weights(const Step<T, D, true>& x, f32x4 (&s)[2][C::KT], Values values, F again) {
+    if (AGAIN && values <= kDown) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int a = 0; a < C::KT; ++a)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[i][a][u] = this->sees(x, i, a, u) ? 1.0f : 0.0f;
+      return;
+    }
+    const float shift = AGAIN && values == kSmall ? kLittle : C::kShift;
+    const float past = AGAIN && values == kSmall ? kLittle : C::kShift + C::kSlack;
     const float f = fabsf(p.scale) * kLog2e;   // (a negative scale turns q round: the largest score is the largest product)
-    constexpr float kPast = C::kShift + C::kSlack;
     float top[2];
     bool some = false;
 #pragma unroll
@@ -739,7 +768,7 @@ struct Block : Share<T, D, true, 2, false, true> {
           if (MASKED && !this->sees(x, i, a, u)) s[i][a][u] = -INFINITY;
           top[i] = fmaxf(top[i], s[i][a][u]);
         }
-      some |= top[i] > kPast;
+      some |= top[i] > past;
     }
     if (__ballot(some) != 0) {
 #pragma unroll
@@ -753,7 +782,7 @@ struct Block : Share<T, D, true, 2, false, true> {
 #pragma unroll
           for (int u = 0; u < 4; ++u) mx = s[i][a][u] != -INFINITY ? fmaxf(mx, r[a][u] * f) : mx;
         mx = max_rows(mx);
-        const float mn = max_rows(top[i]) > kPast ? mx - C::kShift : m[i];
+        const float mn = max_rows(top[i]) > past ? mx - shift : m[i];
         const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
         m[i] = mn;
         sums[i] *= alpha;
@@ -774,8 +803,8 @@ struct Block : Share<T, D, true, 2, false, true> {
   }
 
   // 64 keys from LDS; bit j of ok: keys 32 j ... have a page.
-  template <bool MASKED>
-  __device__ __forceinline__ void tile(int key0, uint32_t ok, const char* kl, const char* vl) {
+  template <bool MASKED, bool AGAIN>
+  __device__ __forceinline__ void tile(int key0, uint32_t ok, const char* kl, const char* vl, Values values) {
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     Step<T, D, true> x;
     x.key0 = key0;
@@ -791,7 +820,7 @@ struct Block : Share<T, D, true, 2, false, true> {
     f32x4 s[2][C::KT];
 #pragma unroll
     for (int i = 0; i < 2; ++i) this->scores(x, i, s[i]);
-    weights<MASKED>(x, s, [&](int i, f32x4 (&r)[C::KT]) {
+    weights<MASKED, AGAIN>(x, s, values, [&](int i, f32x4 (&r)[C::KT]) {
       keys();
       this->scores(x, i, r);
     });
@@ -831,11 +860,12 @@ struct Block : Share<T, D, true, 2, false, true> {
         }
         if constexpr (MASKED) {
           // values that no query sees count as zeros (0 times what stands there need not be 0)
-          const int end = ok >> half & 1 ? seen : -1;
+          const int end = ok >> half & 1 ? tmax : -1;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + 32 * half + 16 * (e / 2) + 4 * g + 2 * (e % 2);
             v[e] = key + 1 <= end ? v[e] : key <= end ? v[e] & 0xffffu : 0u;
+            if (AGAIN) v[e] = stand_in<T>(v[e], values);
           }
         }
         const uint4 va = make_uint4(v[0], v[1], v[2], v[3]);
@@ -848,10 +878,23 @@ struct Block : Share<T, D, true, 2, false, true> {
   }
 
   // Keys [k0, k1) for the whole workgroup; a wavefront without rows brings its pieces and goes along.
-  __device__ __forceinline__ void pass(int k0, int k1, bool work) {
+  template <bool AGAIN = false>
+  __device__ __forceinline__ void pass(int k0, int k1, bool work, Values values = kAll) {
     if (k0 >= k1) return;
     const int n = (k1 - k0 + kKeys - 1) / kKeys;
     Pieces x;
+    if constexpr (AGAIN) {   // (rare: one buffer, and no register for what comes next)
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int key0 = k0 + kKeys * i;
+        load(x, key0, k1);
+        put(x, lds);
+        lds_barrier();
+        if (work && key0 <= tmax) tile<true, true>(key0, x.ok, lds, lds + kKeys * C::LROW, values);
+        lds_barrier();
+      }
+      return;
+    }
     load(x, k0, k1);
     put(x, lds);
     uint32_t ok = x.ok;
@@ -861,8 +904,9 @@ struct Block : Share<T, D, true, 2, false, true> {
       const int key0 = k0 + kKeys * i;
       const char* buf = lds + (i & 1) * LBUF;
       if (work && key0 <= tmax) {
-        if (ok == 3 && key0 + kKeys - 1 <= (tmin < seen ? tmin : seen)) tile<false>(key0, ok, buf, buf + kKeys * C::LROW);
-        else tile<true>(key0, ok, buf, buf + kKeys * C::LROW);
+        const char* vals = buf + kKeys * C::LROW;
+        if (ok == 3 && key0 + kKeys - 1 <= tmin) tile<false, false>(key0, ok, buf, vals, kAll);
+        else tile<true, false>(key0, ok, buf, vals, kAll);
       }
       if (i + 1 < n) {
         put(x, lds + ((i + 1) & 1) * LBUF);
@@ -873,39 +917,39 @@ struct Block : Share<T, D, true, 2, false, true> {
     }
   }
 
-  // As Share::run, by the whole workgroup until none of its rows is left.
+  // As Share::run, by the whole workgroup for any of its rows.
   template <typename Emit>
-  __device__ __forceinline__ void run(int row0, int b, int h, int k0, int k1, uint32_t want, Emit emit) {
-    int only = -1;
-    while (true) {
-      pass(k0, k1, want != 0);
-      if (want != 0) {
-        uint32_t bad = this->unsound() & want & ~none, done = want & ~bad;
-        // (a lane's part of a sum: the whole of it, in one lane of the row)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) l[i] = g == 0 ? sums[i][0] : 0.0f;
-        if (only >= 0) {
-          if (bad >> only & 1) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (only / kRows == i) this->careful(i, row0, b, h, k0, k1);
-          }
-          done = 1u << only;
-        }
-        this->finish();
-        emit(done);
-        want &= ~done;
+  __device__ __forceinline__ void run(int k0, int k1, uint32_t want, Emit emit) {
+    pass(k0, k1, want != 0);
+    sum();
+    const uint32_t bad = this->unsound() & want & ~none;
+    this->finish();
+    emit(want & ~bad);
+    if (!__syncthreads_or(bad != 0)) return;
+    uint32_t left = bad, up[2], down[2];
+#pragma unroll 1
+    for (int n = kUp; n <= kSmall; ++n) {
+      this->reset();
+      clear();
+      pass<true>(k0, k1, left != 0, (Values)n);
+      if (n <= kDown) {
+        if (n == kUp) this->marks(up);
+        else this->marks(down);
+        continue;
       }
-      if (!__syncthreads_or(want != 0)) return;
-      if (want != 0) {
-        only = __ffs(want) - 1;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (only / kRows == i) seen = __builtin_amdgcn_readlane(t[i], only % kRows);
-        this->reset();
-        clear();
-      }
+      sum();
+      const uint32_t most = n == kFinite ? this->unsound() & left : 0;
+      this->finish();
+      this->mark(up, down);
+      emit(left & ~most);
+      left = most;
+      if (!__syncthreads_or(left != 0)) return;
     }
+  }
+  // (a lane's part of a sum: the whole of it, in one lane of the row)
+  __device__ __forceinline__ void sum() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) l[i] = g == 0 ? sums[i][0] : 0.0f;
   }
 };
 
@@ -931,7 +975,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   __shared__ __align__(16) char stage[kWaves * Tile<T, D>::LSTEP];
   Share<T, D, WIDE, NT, false> s(p, b, h, row0, stage + wave_id() * Tile<T, D>::LSTEP);
   const int left = p.R - row0;
-  s.run(row0, b, h, 0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1,
+  s.run(0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1,
         [&](uint32_t done) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -1211,7 +1255,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   TA_DMARK(1);
   // the four wavefronts' parts, behind their keys: [4][rows][D + 2], first the reference and the sum
   float* const parts = smem + kWaves * Tile<T, D>::LSTEP / 4;
-  s.run(row0, b, h, from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, [&](uint32_t done) {
+  s.run(from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, [&](uint32_t done) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (!(done >> (kRows * i + s.c) & 1)) continue;
@@ -1268,8 +1312,10 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
 // x 12 heads x 256 rows over 8000 keys 50 us (60 by sets of 32 rows; 88 and more with the last workgroup's join).
 constexpr int kBlock = kWaves * 2 * kRows;
 constexpr int kManyRows = 96;
+// (Heads of 32: three wavefronts to a SIMD, 2 x 12 heads x 8192 tokens 276 us; two 329.  What spills for it is in the passes
+// after the first.)
 template <typename T, int D>
-__global__ __launch_bounds__(kWaves * kWave, D == 128 ? 1 : 2) void dense_block_kernel(Dense p, int nwg) {
+__global__ __launch_bounds__(kWaves * kWave, D == 128 ? 1 : D == 64 ? 2 : 3) void dense_block_kernel(Dense p, int nwg) {
   using S = Block<T, D>;
   __shared__ __align__(16) char smem[2 * S::LBUF];
   const int sets = (p.R + kBlock - 1) / kBlock, w = __builtin_amdgcn_readfirstlane(wave_id());
@@ -1296,7 +1342,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 ? 1 : 2) void dense_block_
   const uint32_t want = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1 : 0u;
   const bool whole = at.count == 1;
   float* const part = p.ws + ((int64_t)at.wg * kBlock + w * 2 * kRows) * (D + 4);
-  s.run(row0, b, h, k0, k1, want, [&](uint32_t done) {
+  s.run(k0, k1, want, [&](uint32_t done) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = kRows * i + s.c;
