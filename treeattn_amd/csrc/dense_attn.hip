@@ -211,7 +211,7 @@ __device__ __forceinline__ V once(const TA_GLOBAL V* p) {
 }
 
 // One wavefront's share: keys [k0, k1) for NT tiles of 16 query rows of one (sequence, key head).
-template <typename T, int D, bool WIDE, int NT, bool STREAM, bool MANY = false>
+template <typename T, int D, bool WIDE, int NT, bool MANY = false>
 struct Share {
   using C = Tile<T, D, MANY>;
   const Dense& p;
@@ -282,6 +282,7 @@ struct Share {
   // Requests step x's rows (keys key0 ...) from the pages in pg, and before them the pages of the step at next0.  A step that
   // is not needed (past the last one; loads are not left out, so that what is waited for is a fixed number of loads) reads one
   // row of its first key.
+  template <bool STREAM>
   __device__ __forceinline__ void fetch(Step<T, D>& x, int key0, int next0, bool live) {
     x.key0 = key0;
     const int mine = pg;
@@ -528,8 +529,8 @@ struct Share {
     }
   }
 
-  template <bool AGAIN = false>
-  __device__ __forceinline__ void pass(int k0, int k1, Values values = kAll) {
+  template <bool AGAIN, bool STREAM>
+  __device__ __forceinline__ void pass(int k0, int k1, Values values) {
     const int last = k0 + (k1 - 1 - k0) / C::KEYS * C::KEYS;   // the last step's first key
     auto at = [&](int n) {
       const int key = k0 + n * C::KEYS;
@@ -538,11 +539,11 @@ struct Share {
     pg = page_of(k0);
     // two steps in registers: one arrives while the other is used
     Step<T, D> x[2];
-    fetch(x[0], at(0), at(1), true);
+    fetch<STREAM>(x[0], at(0), at(1), true);
     for (int n = 0; k0 + n * C::KEYS < k1; n += 2) {
-      fetch(x[1], at(n + 1), at(n + 2), k0 + (n + 1) * C::KEYS < k1);
+      fetch<STREAM>(x[1], at(n + 1), at(n + 2), k0 + (n + 1) * C::KEYS < k1);
       step<AGAIN>(x[0], values);
-      fetch(x[0], at(n + 2), at(n + 3), k0 + (n + 2) * C::KEYS < k1);
+      fetch<STREAM>(x[0], at(n + 2), at(n + 3), k0 + (n + 2) * C::KEYS < k1);
       if (k0 + (n + 1) * C::KEYS < k1) step<AGAIN>(x[1], values);
     }
   }
@@ -603,7 +604,8 @@ struct Share {
         }
   }
 
-  // Keys [k0, k1) for the rows of `want`; emit(mask) takes the results of some rows at a time.
+  // Keys [k0, k1) for the rows of `want`; emit(mask) takes the results of some rows at a time.  stream (one set of rows): by
+  // loads that the caches need not keep.
   //
   // A value that is infinite or NaN reaches, in the matrix instructions, rows that do not see its key (as 0 times it), and
   // comes as a sum of two products (which may be inf - inf).  So where a row's result is not finite, its wavefront goes
@@ -612,8 +614,11 @@ struct Share {
   // not finite has passed the range of a float on the way (not float16 values): once more, with weights of at most 2^-24.  Five
   // passes at most, whatever the values are, and the rows that none of it reaches keep their bits.
   template <typename Emit>
-  __device__ __forceinline__ void run(int k0, int k1, uint32_t want, Emit emit) {
-    if (k0 < k1) pass(k0, k1);
+  __device__ __forceinline__ void run(int k0, int k1, uint32_t want, bool stream, Emit emit) {
+    if (k0 < k1) {
+      if (NT == 1 && stream) pass<false, NT == 1>(k0, k1, kAll);
+      else pass<false, false>(k0, k1, kAll);
+    }
     const uint32_t bad = unsound() & want & ~none;
     finish();
     emit(want & ~bad);
@@ -622,7 +627,7 @@ struct Share {
 #pragma unroll 1
     for (int n = kUp; n <= kSmall; ++n) {
       reset();
-      pass<true>(k0, k1, (Values)n);
+      pass<true, false>(k0, k1, (Values)n);
       if (n <= kDown) {
         if (n == kUp) marks(up);
         else marks(down);
@@ -654,8 +659,8 @@ struct Share {
 // 2 x 12 heads of 64 x 8192 tokens 389 us (530 TFLOP/s of the two products; a wavefront a set 540), 8 x 12 x 2048 116 (165),
 // 2 x 8 heads of 128 x 4096 188 (275; one wavefront to a SIMD, whose 512 registers it needs).
 template <typename T, int D>
-struct Block : Share<T, D, true, 2, false, true> {
-  using S = Share<T, D, true, 2, false, true>;
+struct Block : Share<T, D, true, 2, true> {
+  using S = Share<T, D, true, 2, true>;
   using C = typename S::C;
   static constexpr int kKeys = 64;
   static constexpr int PR = D * C::EB / 16;                     // 16-byte pieces of a row
@@ -973,9 +978,9 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   const int bh = (int)(id / per), row0 = (int)(id % per) * kRows * NT;
   const int b = bh / p.H, h = bh % p.H;
   __shared__ __align__(16) char stage[kWaves * Tile<T, D>::LSTEP];
-  Share<T, D, WIDE, NT, false> s(p, b, h, row0, stage + wave_id() * Tile<T, D>::LSTEP);
+  Share<T, D, WIDE, NT> s(p, b, h, row0, stage + wave_id() * Tile<T, D>::LSTEP);
   const int left = p.R - row0;
-  s.run(0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1,
+  s.run(0, s.tmax + 1, left >= kRows * NT ? (uint32_t)((1ull << (kRows * NT)) - 1) : (1u << left) - 1, false,
         [&](uint32_t done) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -1160,9 +1165,9 @@ struct Units {
 };
 
 // A workgroup's part: keys [k0, k1) (before the end that its rows see) of set `set` of (b, h), part `part` of `count`; wg: its
-// place among all, in: the set's among those of its sequence; last: the sequence's last position.
+// place among all, in: the set's among those of its sequence; last: the sequence's last position; units: of all sequences.
 struct Part {
-  int b, h, set, in, part, count, wg, last, k0, k1;
+  int b, h, set, in, part, count, wg, last, k0, k1, units;
 };
 
 // A set gets as many workgroups as its sequence is long, so that sequences of any lengths end together and few long ones fill
@@ -1221,6 +1226,7 @@ __device__ __forceinline__ bool find_part(const Dense& p, int sets, int nwg, int
   r.count = count;
   r.wg = wg;
   r.last = last;
+  r.units = all;
   r.in = (wg - start) / count;
   r.part = wg - start - r.in * count;
   r.h = sets > 1 ? r.in / sets : r.in;
@@ -1232,9 +1238,17 @@ __device__ __forceinline__ bool find_part(const Dense& p, int sets, int nwg, int
   return true;
 }
 
-// Workgroups of four wavefronts, each with a share of one set of 16 NT rows (find_part).
-template <typename T, int D, bool WIDE, int NT, bool STREAM>
-__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg, int top) {
+// Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level
+// cache (256 MiB) is not there any more at the next call, and its reads get in each other's way.  Of 32 x 12 queries over
+// 32768 keys of 64 (2.8 GB) 489 us with ordinary loads and 439 with these, one stream of 131000 (352 MB) 71.7 and 64.9; three
+// caches of 86 MB in turns 23.8 and 25.3.  By what the sequences hold, and at most what the pages or the contiguous cache are:
+// 32 x 12 queries over 2000 keys of caches for 65536 (197 MB read) 41.5 us, 50.0 with these.
+// Only where one set reads a key: several share them in the second cache.
+constexpr int64_t kOnce = (int64_t)256 << 20;
+
+// Workgroups of four wavefronts, each with a share of one set of 16 NT rows (find_part).  once: the cache is of kOnce bytes.
+template <typename T, int D, bool WIDE, int NT>
+__global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void dense_split_kernel(Dense p, int nwg, int top, bool once) {
   extern __shared__ __align__(16) float smem[];
   constexpr int KEYS = Tile<T, D>::KEYS;
   constexpr int kSet = kRows * NT;
@@ -1245,7 +1259,7 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   if (!find_part(p, sets, nwg, top, at)) return;
   const int b = at.b, h = at.h, row0 = at.set * kSet;
   const int rows = p.R - row0 < kSet ? p.R - row0 : kSet;
-  Share<T, D, WIDE, NT, STREAM> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, at.last);
+  Share<T, D, WIDE, NT> s(p, b, h, row0, reinterpret_cast<char*>(smem) + w * Tile<T, D>::LSTEP, p.Nq == 1, at.last);
   // its keys, and the equal runs of whole steps of its wavefronts
   const int nkeys = s.tmax + 1;
   const int k0 = at.k0 < nkeys ? at.k0 : nkeys, k1 = at.k1 < nkeys ? at.k1 : nkeys;
@@ -1255,7 +1269,8 @@ __global__ __launch_bounds__(kWaves * kWave, sizeof(T) * D >= 512 ? 1 : 2) void 
   TA_DMARK(1);
   // the four wavefronts' parts, behind their keys: [4][rows][D + 2], first the reference and the sum
   float* const parts = smem + kWaves * Tile<T, D>::LSTEP / 4;
-  s.run(from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, [&](uint32_t done) {
+  const bool stream = once && (int64_t)at.units * p.H * (kQuantum * 2 * D * (int)sizeof(T)) >= kOnce;
+  s.run(from, to, rows == 32 ? 0xffffffffu : (1u << rows) - 1, stream, [&](uint32_t done) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (!(done >> (kRows * i + s.c) & 1)) continue;
@@ -1416,12 +1431,6 @@ __global__ __launch_bounds__(256) void dense_join_kernel(Dense p) {
   if (d == 0 && p.lse) p.lse[le] = lse_of(M, L);
 }
 
-// Bytes of a cache from which its rows are read by loads that the caches need not keep: what is larger than the last-level
-// cache (256 MiB) is not there any more at the next call, and its reads get in each other's way.  Of 32 x 12 queries over
-// 32768 keys of 64 (2.8 GB) 489 us with ordinary loads and 439 with these, one stream of 131000 (352 MB) 71.7 and 64.9; three
-// caches of 86 MB in turns 23.8 and 25.3.  Only where one set reads a key: several share them in the second cache.
-constexpr int64_t kOnce = (int64_t)256 << 20;
-
 template <typename T, int D, bool WIDE, int NT>
 int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const dim3 blk(kWaves * kWave);
@@ -1439,13 +1448,9 @@ int launch_dense(const Dense& p, int nsplit, hipStream_t st) {
   const int top = rows > 10 ? 24 : 256 / rows;
   const dim3 grid((unsigned)(per > 1 ? (wgs + 7) / 8 * 8 : wgs));
   const size_t lds = stage + (parts > join ? parts : join) * sizeof(float);
-  if constexpr (NT == 1) {
-    if (per == 1 && (int64_t)p.BH * p.Tk * 2 * D * (int64_t)sizeof(T) >= kOnce) {
-      hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, 1, true>), grid, blk, lds, st, p, nwg, top);
-      return check_launch("dense_split_kernel");
-    }
-  }
-  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT, false>), grid, blk, lds, st, p, nwg, top);
+  const int64_t bytes = (int64_t)sizeof(T) * (p.ptab ? p.npages * p.pstride : (int64_t)p.BH * p.Tk * 2 * D);
+  const bool once = NT == 1 && per == 1 && bytes >= kOnce;
+  hipLaunchKernelGGL((dense_split_kernel<T, D, WIDE, NT>), grid, blk, lds, st, p, nwg, top, once);
   return check_launch("dense_split_kernel");
 }
 
