@@ -515,9 +515,11 @@ class PagedState:
     def dense_kv(self, b, t_end=None):
         return self.cache.dense(b, t_end)
 
-    def rows(self, b0, b1):
-        v = object.__new__(PagedState)
-        v.__dict__.update(self.__dict__, cache=self.cache.rows(b0, b1))
+    def rows(self, b0, b1, t_end=None):
+        """The state of sequences b0 .. b1-1, seen up to position t_end (all by default)."""
+        c, v = self.cache, object.__new__(PagedState)
+        cache = K.PagedCache(c.pool, c.table[b0:b1], c.tcap if t_end is None else min(int(t_end), c.tcap))
+        v.__dict__.update(self.__dict__, cache=cache)
         return v
 
     def attend(self, q, k, v, tpos, nsplit, ws):
@@ -1224,7 +1226,8 @@ class Decoder:
                     if i == 0:
                         ns = decode_nsplit_dense(nb, H, T0, T0, dh)
                         dws = K.dense_attn_workspace(nb, H, T0, dh, ns, self.dev, H)
-                    out = st.rows(b0, b1).attend(q, k, v, tq, ns, dws).transpose(1, 2)
+                    # (up to the prompt's end: dense_attn's choices go by the positions that the cache is given for)
+                    out = st.rows(b0, b1, T0).attend(q, k, v, tq, ns, dws).transpose(1, 2)
                     x = _product(out.reshape(nb, T0, C), L['c_proj'], bits=bits, residual=x)
                     x = _product(_product(x, L['c_fc'], L['ln2'], bits, gelu=True), L['c_mlp'], bits=bits, residual=x)
                     continue
