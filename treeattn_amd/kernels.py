@@ -70,6 +70,8 @@ class PagedCache:
             raise ValueError('PagedCache: pool (P, 2, leaf, D) contiguous and an int32 contiguous table')
         if table.shape[2] * leaf < tcap:
             raise ValueError('PagedCache: the table does not cover tcap positions')
+        if table.device != pool.device:      # (the kernels read both)
+            raise ValueError('PagedCache: pool on %s, table on %s' % (pool.device, table.device))
         self.pool, self.table, self.tcap = pool, table, int(tcap)
         self.leaf, self.D, self.dtype, self.device = leaf, D, pool.dtype, pool.device
         self.B, self.H = table.shape[0], table.shape[1]
