@@ -1557,6 +1557,12 @@ extern "C" int ta_dense_attn_fwd(const void* q, const void* k, const void* v, in
     set_error("ta_dense_attn_fwd: a missing pointer");
     return TA_ERR_ARG;
   }
+  // (a stride of a dimension of one is never a step)
+  if (B == 1) qsb = ksb = vsb = 0;
+  if (Hq == 1) qsh = 0;
+  if (H == 1) ksh = vsh = 0;
+  if (Nq == 1) qsn = 0;
+  if (Tk == 1 && !pages) kst = vst = 0;
   const int sz = dtype == TA_F32 ? 4 : 2;
   const int64_t bits = (int64_t)((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) | (qsb | qsh | qsn | kst | vst) * sz |
                        (pages ? pages->page_stride * sz : (ksb | ksh | vsb | vsh) * sz);

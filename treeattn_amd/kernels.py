@@ -1190,7 +1190,8 @@ def dense_attn_workspace(B, Hq, Nq, D, nsplit, device, kv_heads=None):
 
 def dense_attn(q, k, v, tq, scale=None, out=None, lse=None, nsplit=1, ws=None):
     """Attention over the whole cache: q (B,Hq,Nq,D) at positions tq ((Nq,) or (B,Nq)) over every key 0 .. tq of k, v
-    (B,H,Tk,D) or of a PagedCache (as k; v None), Hq a multiple of H (query head h reads key head h // (Hq // H)).  Keys of a
+    (B,H,Tk,D) or of a PagedCache (as k; v None), Hq a multiple of H (query head h reads key head h // (Hq // H)), all rows
+    16-byte aligned.  Keys of a
     block without a page do not count; a query without any key, or at a position outside [0, Tk), gives zeros and lse -1e30.
     lse: None, or (B,Hq,Nq) float32 to receive the log-sum-exp.  nsplit: 1, a wavefront for each set of 16 or 32 rows (a
     workgroup for 128 where there are many), or a multiple of 4 up to 8192, four wavefronts for each of
