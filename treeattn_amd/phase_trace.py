@@ -10,6 +10,8 @@ launch follows a 1 GiB read, so its caches are as cold as inside a decode step.
     python -m treeattn_amd.build --trace lanetree.hip
     python -m treeattn_amd.phase_trace lanetree-walk    # the LaneTree walk of bench_speed's layer (T=512), one position
     python -m treeattn_amd.phase_trace lanetree-tail    # the LaneTree build's window launch (T=4096), per level
+    python -m treeattn_amd.build --trace dense_attn.hip
+    python -m treeattn_amd.phase_trace whole-cache      # dense_split_kernel: one sequence, shared key heads, some tokens
 
 Marks: the descent's 0 (set-up: position, query row, first level's node rows), 1 + 2k / 2 + 2k (level k scored /
 ranked); the layer attention's 12 (start), 13 (descent done), 14 (attention start), 15 (done); the descent
@@ -17,7 +19,8 @@ kernel's 12 (start), 13 (cache append done), 14 (descent done); the LaneTree wal
 0 (start), 1 (neighbours scored and counted), 2 (first occurrences counted), 3 (search started), 4 + l (level l + 1
 ranked), 12 (outputs written), 13 (insertion started), 14 (insertion done), 15 (position done); the LaneTree
 build's window launch (lanetree_tail_kernel), 0 (start) and for its k-th level 1 + 3k (statistics exchanged), 2 + 3k
-(Lloyd iterations done), 3 + 3k (laid out).
+(Lloyd iterations done), 3 + 3k (laid out); attention over a whole cache (dense_split_kernel), 0 (start), 1 (its part and
+queries known), 2 (its keys done), 3 (its part written), 4 (counted in), 5 (the set joined; its last workgroup only).
 """
 import argparse
 import ctypes
@@ -201,15 +204,54 @@ def lanetree_tail(reps, T=4096, D=64, H=6, chunk=64):
             flush=True)
 
 
+def whole_cache(reps):
+    """dense_split_kernel over pages of normal random rows: 12 heads, one query over 131000 keys (bf16); 4 sequences of 6001
+    keys, 8 key heads of 128 for 4 queries each (float16, pages of 16); 8 sequences of 2500 keys, 12 heads x 5 tokens (float32,
+    pages of 8).  The join's figures are those of the workgroups that came last."""
+    lib = _load('dense_attn.hip')
+    from . import kernels as K
+    from .engine import decode_nsplit_dense
+    names = {0: 'start', 1: 'part known', 2: 'keys done', 3: 'written', 4: 'counted', 5: 'joined'}
+    buf = (ctypes.c_ulonglong * (4096 * 16))()
+    flush = torch.ones(1 << 28, dtype=torch.float32, device='cuda')
+    for B, H, G, N, T, D, leaf, dtype in ((1, 12, 1, 1, 131000, 64, 64, torch.bfloat16), (4, 8, 4, 1, 6001, 128, 16, torch.float16),
+                                          (8, 12, 1, 5, 2500, 64, 8, torch.float32)):
+        nb = (T + leaf - 1) // leaf
+        pool = torch.empty(B * H * nb, 2, leaf, D, device='cuda', dtype=dtype).normal_()
+        cache = K.PagedCache(pool, torch.randperm(B * H * nb, device='cuda').to(torch.int32).view(B, H, nb), T)
+        q = torch.randn(B, G * H, N, D, device='cuda').to(dtype)
+        tq = torch.arange(T - N, T, device='cuda', dtype=torch.int32)
+        ns = decode_nsplit_dense(B, H, G * N, T, D)
+        ws = K.dense_attn_workspace(B, G * H, N, D, ns, 'cuda', H)
+        print('%d x %d key heads of %d, %d rows each, %d keys, %s, pages of %d:' % (B, H, D, G * N, T, dtype, leaf))
+        for rep in range(reps + 2):
+            flush.sum()
+            torch.cuda.synchronize()
+            lib.ta_trace_clear()
+            K.dense_attn(q, cache, None, tq, nsplit=ns, ws=ws)
+            torch.cuda.synchronize()
+            lib.ta_trace_read(buf)
+            tr = torch.tensor(list(buf), dtype=torch.float64).view(4096, 16)
+            tr = tr[tr[:, 0] > 0]
+            if rep < 2:
+                continue
+            parts = []
+            for m in range(6):
+                v = (tr[:, m][tr[:, m] > 0] - tr[:, 0].min()) / 100.0
+                if len(v):
+                    parts.append('%s %.1f/%.1f/%.1f' % (names[m], v.min(), v.median(), v.max()))
+            print('launch %d (%d workgroups): %s' % (rep - 2, len(tr), ' | '.join(parts)), flush=True)
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument('workload', choices=('layer-attention', 'descent-append', 'lanetree-walk', 'lanetree-tail'))
+    ap.add_argument('workload', choices=('layer-attention', 'descent-append', 'lanetree-walk', 'lanetree-tail', 'whole-cache'))
     ap.add_argument('--reps', type=int, default=5)
     args = ap.parse_args()
     if not torch.cuda.is_available():
         raise SystemExit('phase_trace needs a GPU')
     {'layer-attention': layer_attention, 'descent-append': descent_append,
-     'lanetree-walk': lanetree_walk, 'lanetree-tail': lanetree_tail}[args.workload](args.reps)
+     'lanetree-walk': lanetree_walk, 'lanetree-tail': lanetree_tail, 'whole-cache': whole_cache}[args.workload](args.reps)
 
 
 if __name__ == '__main__':
