@@ -7,8 +7,8 @@
 // fit such a piece.  A pair with an id outside its tensor copies nothing.
 //
 // Loads and stores that the caches need not keep: what the stores leave in the second caches is written back when the kernel
-// ends (96 pages of 16 KiB in 12 layers 20.5 us so, 8.6 us with nontemporal ones, 4.4 TB/s; eight pages of one layer 4.3 and
-// 2.5).  6143 8-bit pages of 12 layers 234 us, 5.2 TB/s.
+// ends (in one session 96 pages of 16 KiB in 12 layers 20.5 us so and 8.6 us with nontemporal ones, eight pages of one layer 4.3
+// and 2.5; three sets of pools in turns 10.1, 3.7 TB/s).  6143 8-bit pages of 12 layers 228 us, 5.3 TB/s.
 //
 // The reference keeps one contiguous cache a sequence (engine.py:26-27) and has no counterpart.
 #include "common.hpp"

@@ -18,8 +18,9 @@
 // than kSlack: until then weights are at most 2^kSlack.
 //
 // Bound by bytes, 2 D a key and key head, where rows are few; the keys of a sequence are split over wavefronts and
-// workgroups, whose partial results the last workgroup to arrive joins.  32 x 12 queries over 32768 keys of 64: 440 us, 6.4
-// TB/s; one sequence of 131000: 62 us, 5.6 TB/s.  Rows of prompts, by the hundred, share their keys through LDS (Block).
+// workgroups, whose partial results the last workgroup to arrive joins.  32 x 12 queries over 32768 keys of 64: 441 us, 6.4
+// TB/s; one sequence of 131000: 59 us, 5.9 TB/s.  Rows of prompts, by the hundred, share their keys through LDS (Block).
+// (Times beside a choice are of one session, both sides; the same call differs by up to 10 % between sessions.)
 //
 // Phase marks (trace.hpp): 0 start, 1 its part and queries are known, 2 its keys are done, 3 its part is written, 4 it is
 // counted in, 5 the set is joined.
@@ -656,8 +657,8 @@ struct Share {
 // between two branches, since their chains run beside each other (with 32, three wavefronts to a SIMD spill: 502 us in place
 // of 389).
 //
-// 2 x 12 heads of 64 x 8192 tokens 389 us (530 TFLOP/s of the two products; a wavefront a set 540), 8 x 12 x 2048 116 (165),
-// 2 x 8 heads of 128 x 4096 188 (275; one wavefront to a SIMD, whose 512 registers it needs).
+// 2 x 12 heads of 64 x 8192 tokens 418 us (493 TFLOP/s of the two products), 8 x 12 x 2048 128, 2 x 8 heads of 128 x 4096 192 (one
+// wavefront to a SIMD, whose 512 registers it needs).  In one session 389, 116 and 188 us; 540, 165 and 275 a wavefront a set.
 template <typename T, int D>
 struct Block : Share<T, D, true, 2, true> {
   using S = Share<T, D, true, 2, true>;

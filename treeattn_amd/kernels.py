@@ -1262,8 +1262,9 @@ class Rope:
 
 
 def rope(x, pos, rope, out=None, inverse=False):
-    """x (B,H,T,D) with every row turned by its position's angles (pos (T,) or (B,T)); inverse: turned back (the gradient: the
-    amplitude is applied again, not taken back).  out: None, x itself (in place) or a tensor that does not overlap it."""
+    """x (B,H,T,D) with every row turned by its position's angles (pos (T,) or (B,T), within 32 bits: int64 ones past them count
+    as the last that fits); inverse: turned back (the gradient: the amplitude is applied again, not taken back).  out: None, x
+    itself (in place) or a tensor that does not overlap it."""
     dev = L.device_index(x)
     B, H, T, D = shape = x.shape
     xt = x.stride()

@@ -1,4 +1,5 @@
-"""Rotary positions of queries and keys (no counterpart in the reference, whose positions are learned: model.py:54, 74).
+"""Rotary positions of queries and keys (Su et al. 2021, arXiv:2104.09864; no counterpart in the reference, whose positions are
+learned: model.py:54, 74).
 
 A Rope (kernels.Rope) holds the angle of each pair of a head's elements for one position; rotate() turns queries and keys by
 their positions' angles, differentiably.  rope_frequencies() gives the angles, also those of a model stretched past the
@@ -18,10 +19,13 @@ SCALINGS = ('', 'linear', 'ntk', 'bands')
 def rope_frequencies(rot, base=10000.0, scaling='', factor=1.0, trained=0, low=1.0, high=32.0):
     """(inv_freq, amplitude) for rot turned elements of a head: inv_freq[i] = base^(-2i / rot) radians a position, and for a
     context `factor` times the trained one
-      'linear'  every angle divided by factor (positions pressed together);
-      'ntk'     the base raised to base * factor^(rot / (rot - 2)): the slowest pair slowed by factor, the fastest not at all;
+      'linear'  every angle divided by factor (positions pressed together: position interpolation, Chen et al. 2023,
+                arXiv:2306.15595);
+      'ntk'     the base raised to base * factor^(rot / (rot - 2)): the slowest pair slowed by factor, the fastest not at all (the
+                "NTK-aware" change of base, as Peng et al. 2023, arXiv:2309.00071, section 3.1, give it);
       'bands'   pairs that turn less than `low` times in the `trained` length slowed by factor, those that turn more than `high`
-                times left, in between by parts; the amplitude is 0.1 ln(factor) + 1."""
+                times left, in between by parts; the amplitude is 0.1 ln(factor) + 1 (by parts and with that factor on queries
+                and keys both: the same paper, sections 3.2 to 3.4)."""
     if rot < 2 or rot % 2 or not base > 0 or not factor >= 1:
         raise ValueError('rope_frequencies: an even number of elements, a positive base and a factor of at least 1')
     if scaling not in SCALINGS:
