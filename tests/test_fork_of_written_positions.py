@@ -87,11 +87,19 @@ def test_a_decoder_forks_what_its_steps_wrote():
         with pytest.raises(ValueError, match='holds no'):
             d.fork(*bad)
         sound(d.pool)
-    d.fork(1, 2, 25)
-    assert d.g_t.tolist() == [40, 25, 25]
+    d.fork(1, 2, 12)
+    assert d.g_t.tolist() == [40, 25, 12]     # (the caller's)
+    d.fork(0, 1, 20)
+    with pytest.raises(ValueError, match='holds no'):
+        d.fork(1, 2, 21)                      # g_t still says 25, which sequence 1 had before
+    sound(d.pool)
+    d.g_t[1] = 20
     d.g_t += 100                              # replays
     d.fork(0, 1, 140)
-    assert d.pool.n_shared == 140 // 64 * 2 and d.g_t.tolist() == [140, 140, 125]
+    d.g_t[1] = 140
+    assert d.pool.n_shared == 140 // 64 * 2
+    d.fork(0, 2, 125)
+    d.g_t[2] = 125
     d.g_t[0] = 70                             # sequence 0 goes back: its next replays write blocks 1 and 2
     d.pool.own(0, 70)
     with pytest.raises(ValueError, match='holds no'):
@@ -101,7 +109,7 @@ def test_a_decoder_forks_what_its_steps_wrote():
     for j in (1, 2):
         assert all(d.pool.refs[int(p)] == 1 for p in d.pool.host[0, :, j])
     d.resize(d.pool.P + 1)                    # (no captured step any more: what its replays wrote stays known)
-    assert d.graph is None and d.pool.tokens == [140, 140, 130]
+    assert d.graph is None and d.pool.tokens[:2] == [140, 140]
 
 
 def test_a_fork_forgets_the_tail_of_its_target():

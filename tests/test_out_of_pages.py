@@ -26,7 +26,7 @@ def test_a_fork_with_the_pages_of_replays_to_come():
     sound(d.pool)
     d.fork(0, 1, 130)                         # 2 blocks shared, 2 of its own
     sound(d.pool)
-    assert d.pool.nblk == [3, 4, 3] and d.g_t.tolist() == [130, 130, 20]
+    assert d.pool.nblk == [3, 4, 3] and d.pool.tokens == [130, 130, 20]
 
 
 def test_pool_forks_are_whole_or_nothing():

@@ -921,6 +921,7 @@ class Decoder:
         B, H, dh = self.B, self.H, self.dh
         self.pool = None
         self._t_host = None      # largest position a step has used (host copy; None when unknown)
+        self._stale = {}         # g_t of forks' targets when they were forked (_replayed)
         if self.mode == 'seg':
             if self.paged:
                 leaf = SEL.cfg_shape(self.cfg, self.Tcap).leaf
@@ -1139,12 +1140,14 @@ class Decoder:
     # ------------------------------------------------------------------------------------------ sequences
     def _replayed(self):
         """The positions of a captured step's next replay (read from the device), [] without one: what is before them has been
-        written, which the page pool is told."""
+        written, which the page pool is told.  The position of a fork's target says nothing while it is what it was then."""
         if self.graph is None or self.pool is None:
             return []
         at = self.g_t.tolist()
         for b, t in enumerate(at):
-            self.pool.wrote(t, (b,))
+            if self._stale.get(b) != t:
+                self._stale.pop(b, None)
+                self.pool.wrote(t, (b,))
         return at
 
     @torch.no_grad()
@@ -1152,8 +1155,8 @@ class Decoder:
         """Sequence dst goes on from the first t positions of src, as after the same tokens: whole pages of the caches are
         shared (read only; a step that goes back into one gets a copy), the rows behind them and the tree's state copied.  t: at
         most the positions of src that a prompt, a step or a replay (by g_t) has written; with contiguous caches this is not
-        known, and t at most Tcap.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] too (g_t[dst]
-        becomes t; a replay hands out no copies: before one that goes back behind t, reserve(t_end, start) does).
+        known, and t at most Tcap.  What dst held is dropped.  Between the replays of a captured step: set g_tok[dst] and g_t[dst] too
+        (a replay hands out no copies: before one that goes back behind t, reserve(t_end, start) does).
         With the budget head's global pool the running sum of keys is that of the cache's rows."""
         t = int(t)
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
@@ -1166,8 +1169,8 @@ class Decoder:
             at = self._replayed()
             # (captured: with the pages of the replays to come, in one call that either does all of it or nothing)
             self.pool.fork(src, dst, t, at[src] if at else None, self._reserved if at else 0)
-        if self.graph is not None:
-            self.g_t[dst] = t
+            if at:
+                self._stale[dst] = at[dst]
         ids = torch.tensor([[src], [dst]], dtype=torch.int32).to(self.dev)
         K.copy_rows([x for st in self.states for x in st.sequence_tensors()], ids[0], ids[1])
         for st in self.states:
@@ -1306,7 +1309,7 @@ class Decoder:
         self.reserve(end, g_t.tolist() if self.pool is not None and self.pool.n_shared else None)
         # (out of pages: the step that was captured before is as it was; from here on there is only the new one)
         self.graph, self.graphs = None, []
-        self.g_tok, self.g_t, self._t_host, self._reserved = g_tok, g_t, t_host, end
+        self.g_tok, self.g_t, self._t_host, self._reserved, self._stale = g_tok, g_t, t_host, end, {}
         self.g_logits = torch.empty(B, V, device=self.dev, dtype=torch.bfloat16 if self.fused else torch.float32)
         main = torch.cuda.current_stream()
         groups = self.groups if (self.fused and len(self.groups) > 1) else [None]

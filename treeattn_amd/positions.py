@@ -104,11 +104,11 @@ def heads(module, qkv):
     C, H = C3 // 3, module.H
     if not getattr(module.cfg, 'rope', ''):
         return [t.view(b, T, H, C // H).transpose(1, 2) for t in qkv.split(C, dim=2)]
-    made, r = module.__dict__.get('_rope', (None, None))
+    made, r = module.__dict__.get('_rope_made', (None, None))
     now = _settings(module.cfg, qkv.device)
     if made != now:
         r = rope_of(module.cfg, qkv.device)
-        module.__dict__['_rope'] = now, r
+        module.__dict__['_rope_made'] = now, r
     qk, v = qkv.split((2 * C, C), dim=2)
     pos = torch.arange(T, device=qkv.device, dtype=torch.int32)
     qk = rotate(qk.view(b, T, 2 * H, C // H).transpose(1, 2), pos, r)
