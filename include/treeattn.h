@@ -155,8 +155,9 @@ int ta_seg_attn8_fwd(const void* q, int dtype, int64_t qsb, int64_t qsh, int64_t
  * page do not count; a query at a position outside [0, Tk), or without a key, gives zeros and lse -1e30.  What stands in
  * rows past a query's position has no effect on it, whatever it is.  A value that is infinite or NaN and that a query sees makes
  * its column so; a NaN or +inf score the whole row NaN.  Rows that share their way through the keys (up to 128) with one whose
- * result such a value reaches take up to five passes over them in place of one.  D 16, 32, 64 or 128; q, K and V rows 16-byte
- * aligned, their row strides from 0 to 64 MiB (strides of dimensions of one: any); pages of 2 rows or more.
+ * result such a value reaches take up to five passes over them in place of one, up to ten times the time (the later passes have
+ * less in flight).  D 16, 32, 64 or 128; q, K and V rows 16-byte aligned, their row strides from 0 to 64 MiB (strides of
+ * dimensions of one: any); pages of 2 rows or more.
  * nsplit: 1, a wavefront for each set of 16 or 32 query rows of one key head (the Hq / H heads times Nq; for many rows a
  * workgroup for each 128), or a multiple of 4 up to 8192: four wavefronts for each of nsplit / 4 workgroups, of which a
  * sequence's sets get as many as it is long (each set at least one; 4: one each); past 4 it needs ws, 256-byte aligned, of
